@@ -195,8 +195,8 @@ def _run_own(s):
         r = cb.token_logprobs(s["logits"], s["targets"], mask=s["mask"], temperature=s["temperature"])
         if not s["backward"]:
             return {"logprobs": r.logprobs, "lse": r.lse}
-        grad = cb.token_logprobs_backward(s["upstream"], s["logits"], s["targets"], r.lse, mask=s["mask"],
-                                          temperature=s["temperature"])
+        grad = cb.token_logprobs_backward(s["upstream"], s["logits"], s["targets"], r.logprobs, r.lse,
+                                          mask=s["mask"], temperature=s["temperature"])
         return {"logprobs": r.logprobs, "lse": r.lse, "grad": grad}
     if s["op"] == "distill":
         r = cb.distill_loss(s["logits"], s["teacher"], s["index"], teacher_lse=s["lse"], weights=s["weights"],
