@@ -5,9 +5,23 @@ of that ABI:
   * ctorch_plugin/cuda_backend.cpp — the C++ drop-in for ctorch itself: it defines ctorch's four
     CUDA registration hooks and fills every CUDA dispatch slot;
   * this package — the same ops for torch CUDA tensors (ops.py mirrors ctorch's public API and
-    error types), plus the row-sharded multi-GPU workload (sharded.py).
+    error types), the losses over logits rows with their gradients (losses.py), plus the
+    row-sharded multi-GPU workload (sharded.py).
 """
 from .errors import AliasError, CommTimeoutError, DeviceError, DTypeError, Error, ShapeError  # noqa: F401
+from .losses import (  # noqa: F401
+    DistillLoss,
+    PolicyLoss,
+    PreferenceLoss,
+    TokenLogprobs,
+    check_index_status,
+    distill_loss,
+    index_status,
+    policy_loss,
+    preference_loss,
+    token_logprobs,
+    token_logprobs_backward,
+)
 from .ops import (  # noqa: F401
     ValuesIndices,
     abs,

@@ -288,6 +288,91 @@ CTB_API int ctb_minmax_combine(int op, const ctb_view* values, const ctb_view* i
                                const int64_t* d_row_offsets, const ctb_view* out_values,
                                const ctb_view* out_indices, ctb_stream stream);
 
+/* ---- losses over the rows of a logits matrix, with their gradients ---- */
+
+/* Common to the entry points of this section. logits is [..., V]: any leading dims and strides, the
+ * vocabulary last, float32, float64 or bfloat16 (the one section of this ABI that takes bfloat16);
+ * a "row" is one position of the leading dims, z = logits / temperature, p = softmax(z) over the
+ * row. Numbers a row (targets, weights, ...) are views that broadcast (right-aligned) to the leading
+ * dims, integers int32 or int64, reals float32 or float64; results a row have exactly the leading
+ * shape and float32 elements (float64 for float64 logits). Row statistics and sums are float32 (float64
+ * for float64 logits), what is computed once a row is float64, the scalar loss is summed in float64 in
+ * a fixed order and rounded once: equal calls give equal bits.
+ * A row whose mask or weight is 0 does not count: its logits, targets and other operands are not looked
+ * at (they may hold anything), its results are 0 and its gradient row is 0. Logits of -inf have
+ * probability 0; a row with +inf or NaN, or of -inf alone, gives NaN in its own results. A row of the
+ * type's lowest finite value is uniform.
+ * grad has the logits' shape and dtype; it may be the logits' own view (the gradient then replaces the
+ * logits) and must not overlap them otherwise. Rows of unit stride are read and written fastest where
+ * logits and grad start their rows at the same offset from a 16-byte boundary.
+ * An index outside [0, V) in a row that counts makes that row's results NaN. When d_status is not NULL
+ * it is also recorded there: 16 bytes of device memory on an 8-byte boundary, an int32 flag at byte 0
+ * and, at byte 8, an int64 offending index, written only when an index is bad, so the caller zeroes
+ * it once and reads it when it likes. No ctorch counterpart (ctorch has no losses). */
+
+/* logprobs = log p[target] and, unless NULL, lse = log sum exp z, one of each a row. */
+CTB_API int ctb_token_logprobs(const ctb_view* logits, const ctb_view* targets, const ctb_view* mask,
+                               double temperature, const ctb_view* logprobs, const ctb_view* lse,
+                               int32_t* d_status, ctb_stream stream);
+
+/* grad = the gradient of sum(grad_logprobs * logprobs): grad_logprobs / T * (1[target] - p). logprobs,
+ * lse, mask and temperature are those of the forward call. Rows with a zero grad_logprobs are not read. */
+CTB_API int ctb_token_logprobs_backward(const ctb_view* grad_logprobs, const ctb_view* logits,
+                                        const ctb_view* targets, const ctb_view* logprobs, const ctb_view* lse,
+                                        const ctb_view* mask, double temperature, const ctb_view* grad,
+                                        int32_t* d_status, ctb_stream stream);
+
+/* Scratch bytes of the losses below (8-byte aligned): pairs = 0 for ctb_distill_loss and
+ * ctb_policy_loss (needed there only when `loss` is wanted). */
+CTB_API size_t ctb_loss_scratch_bytes(const ctb_view* logits, int64_t pairs);
+
+/* Distillation from a teacher's top entries: teacher_logits [..., K] (also bfloat16) and their
+ * vocabulary indices [..., K], K up to 2048, V up to 2^20. An entry of -inf is padding: its index is
+ * not looked at, and a row of nothing else does not count. An index that occurs twice among a row's
+ * entries is a bad index. With teacher_lse NULL the entries are renormalised, q = softmax(teacher / T):
+ *     row_loss = sum_k q_k (log q_k - log p[index_k])
+ * With teacher_lse = the log-sum-exp of the teacher's whole row of logits / T, q_k = exp(teacher_k / T -
+ * teacher_lse), and the mass outside the entries, q' = max(0, 1 - sum q) and p' = 1 - sum p[index_k],
+ * is one more event: row_loss += q' (log q' - log p'). (With an entry for every logit there is none.)
+ * loss = sum of weight_scale * weights * row_loss (weights NULL: 1), grad = its gradient. loss,
+ * row_loss and grad may each be NULL. */
+CTB_API int ctb_distill_loss(const ctb_view* logits, const ctb_view* teacher_logits,
+                             const ctb_view* teacher_indices, const ctb_view* teacher_lse,
+                             const ctb_view* weights, double weight_scale, double temperature,
+                             const ctb_view* loss, const ctb_view* row_loss, const ctb_view* grad,
+                             int32_t* d_status, void* scratch, size_t scratch_bytes, ctb_stream stream);
+
+/* The clipped policy loss with a KL term. With logp = log p[target], r = exp(logp - old_logprobs),
+ * A = advantages and d = ref_logprobs - logp:
+ *     row_loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - 1 - d)
+ * (the gradient goes through r A where the two are equal). loss and grad as in ctb_distill_loss.
+ * kl = exp(d) - 1 - d (0 without ref_logprobs). ref_logprobs may be NULL when kl_coef is 0; loss,
+ * row_loss, logprobs, kl and grad may each be NULL. */
+CTB_API int ctb_policy_loss(const ctb_view* logits, const ctb_view* targets, const ctb_view* old_logprobs,
+                            const ctb_view* advantages, const ctb_view* ref_logprobs, const ctb_view* weights,
+                            double weight_scale, double clip_low, double clip_high, double kl_coef,
+                            double temperature, const ctb_view* loss, const ctb_view* row_loss,
+                            const ctb_view* logprobs, const ctb_view* kl, const ctb_view* grad,
+                            int32_t* d_status, void* scratch, size_t scratch_bytes, ctb_stream stream);
+
+/* The preference loss on pairs of sequences. The rows are 2 * pairs sequences, the chosen ones first
+ * (pair i is sequences i and pairs + i): equal shares of the leading dims' rows, or, for [rows, V]
+ * logits, rows offsets[s] to offsets[s + 1] of sequence s (offsets [2 * pairs + 1], device; rows of no
+ * sequence do not count; offsets that fall or point outside the rows are a bad index and make every
+ * result NaN). Over a sequence's rows with mask, S = sum (logp - ref_logprobs) (ref NULL: 0),
+ * divided by their number when `average`; rewards = beta S, h = rewards of the chosen less the rejected:
+ *     pair_loss = -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h)
+ * loss = sum of weight_scale * weights * pair_loss (weights [pairs], NULL: 1), grad = its gradient.
+ * loss, pair_loss [pairs], rewards [2 * pairs], logprobs and grad may each be NULL; scratch is always
+ * needed. */
+CTB_API int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets, int64_t pairs,
+                                const ctb_view* offsets, const ctb_view* ref_logprobs, const ctb_view* mask,
+                                const ctb_view* weights, double weight_scale, double beta,
+                                double label_smoothing, int average, const ctb_view* loss,
+                                const ctb_view* pair_loss, const ctb_view* rewards, const ctb_view* logprobs,
+                                const ctb_view* grad, int32_t* d_status, void* scratch, size_t scratch_bytes,
+                                ctb_stream stream);
+
 /* ---- synthetic inputs ---- */
 
 /* Fills a contiguous view with a counter-based pseudo-random sequence (splitmix64 of
