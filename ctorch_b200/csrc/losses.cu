@@ -1,6 +1,7 @@
 // losses.cu — the entry points of the losses over logits rows (include/ctb/ctb.h): checks, the plan of a
 // call (its rows and where each operand of a row lies), the choice of kernel, and the two small
 // kernels around the row kernels: the sum of the weighted losses, and the preference loss's pairs.
+#include <cmath>
 #include <exception>
 #include <initializer_list>
 #include <string>
@@ -210,6 +211,11 @@ struct Builder {
         p.temp = temperature;
         p.inv_temp = 1.0 / temperature;
         p.c2 = static_cast<float>(1.4426950408889634 * p.inv_temp);
+        const double c2 = 1.4426950408889634 * p.inv_temp;
+        float down = static_cast<float>(c2);
+        if (static_cast<double>(down) > c2) down = std::nextafterf(down, 0.0f);
+        p.c2_down = down;
+        p.c2_rest = std::fmax(static_cast<float>((c2 - down) / down), 1e-30f);
         p.scale = 1.0;
         p.status = status;
         p.ptr[kLrX] = x->data;
@@ -345,7 +351,10 @@ int check_status(const int32_t* status) {
                                                    : CTB_OK;
 }
 
-int run_rows(const LossPlan& p, int* ctas, cudaStream_t st) { return loss_rows_general(p, ctas, st); }
+int run_rows(const LossPlan& p, int* ctas, cudaStream_t st) {
+    if (p.op != kLossToken && loss_rows_fit(p)) return loss_rows_fast(p, ctas, st);
+    return loss_rows_general(p, ctas, st);
+}
 int run_backward(const LossArgs& a, cudaStream_t st) { return loss_backward_general(a, st); }
 
 int run_total(const double* partials, int n, const ctb_view* out, cudaStream_t st) {
@@ -360,6 +369,7 @@ int run_loss(Builder& b, const ctb_view* loss, void* scratch, size_t scratch_byt
     if (int rc = check_scratch(scratch, scratch_bytes, need)) return rc;
     b.finish();
     b.a().partials = loss ? static_cast<double*>(scratch) : nullptr;
+    b.a().timeouts = wait_timeout_counter();
     int ctas = 0;
     if (!b.plan.empty)
         if (int rc = run_rows(b.plan, &ctas, st)) return rc;

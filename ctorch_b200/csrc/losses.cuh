@@ -57,6 +57,7 @@ struct LossArgs {
     int tail;             // distill: the mass outside the top entries is one more event
     double temp, inv_temp;
     float c2;             // log2(e) / T
+    float c2_down, c2_rest;  // the same rounded down, and what that leaves: c2_down (1 + c2_rest), at least 1e-30
     double scale;         // multiplies every weight
     double clip_lo, clip_hi, kl_coef;
     const void* offsets;  // preference, packed rows: rows before the first offset or from the last one on
@@ -186,9 +187,8 @@ template <class Acc> struct RowSum {
 // one row's arithmetic
 
 struct RowGrad {
-    double a;          // g_j = a * exp((x_j - m) / T)
-    double at_target;  // the target's own value (policy)
-    double loss;       // before its weight
+    double a;     // g_j = a * exp((x_j - m) / T)
+    double loss;  // before its weight
 };
 
 // Log-probability of a target from the row's statistics: (x_t - m) / T - log s.
@@ -196,35 +196,29 @@ __device__ __forceinline__ double target_logp(const LossArgs& a, double xt, doub
     return (xt - m) * a.inv_temp - log(s);
 }
 
-// The clipped policy loss of one row and its gradient's numbers; with r = exp(logp - old),
-//     loss = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef (exp(d) - 1 - d),  d = ref - logp
-//     dloss/dlogp = (r A <= clip(r) A ? -r A : 0) + kl_coef (1 - exp(d))
+// The clipped policy loss of one row; with r = exp(logp - old), d = ref - logp and ed = exp(d) - 1,
+//     loss = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl_coef (ed - d)
+//     dloss/dlogp = (r A <= clip(r) A ? -r A : 0) - kl_coef ed
 // and dlogp/dx_j = (1[j = t] - p_j) / T. Comparisons are written so that a NaN stays one.
-__device__ __forceinline__ RowGrad policy_row(const LossArgs& a, int64_t row, double w, double logp, double s) {
-    const double old = row_real(a, kLrOld, row), adv = row_real(a, kLrAdv, row);
-    const double r = exp(logp - old);
+struct PolicyTerms {
+    double loss, kl;
+    double g;  // w / T dloss/dlogp
+};
+
+__device__ __forceinline__ PolicyTerms policy_terms(const LossArgs& a, double w, double adv, double r, double d, double ed) {
     const double lo = 1.0 - a.clip_lo, hi = 1.0 + a.clip_hi;
     const double u = r * adv, c = (r < lo ? lo : r > hi ? hi : r) * adv;
     const bool free = !(u > c);
-    double loss = free ? -u : -c, slope = free ? -u : 0.0;
-    if (a.ptr[kLrRef]) {
-        const double d = row_real(a, kLrRef, row) - logp, e = expm1(d);
-        put_row(a, kLrKl, row, e - d);
-        if (a.kl_coef != 0.0) {
-            loss += a.kl_coef * (e - d);
-            slope -= a.kl_coef * e;
-        }
-    } else {
-        put_row(a, kLrKl, row, 0.0);
+    PolicyTerms t;
+    t.loss = free ? -u : -c;
+    t.kl = a.ptr[kLrRef] ? ed - d : 0.0;
+    double slope = free ? -u : 0.0;
+    if (a.kl_coef != 0.0) {
+        t.loss += a.kl_coef * t.kl;
+        slope -= a.kl_coef * ed;
     }
-    put_row(a, kLrLogp, row, logp);
-    put_row(a, kLrRowLoss, row, loss);
-    const double g = w * slope * a.inv_temp;
-    RowGrad o;
-    o.a = -g / s;
-    o.at_target = -g * expm1(logp);  // g (1 - p_t)
-    o.loss = loss;
-    return o;
+    t.g = w * slope * a.inv_temp;
+    return t;
 }
 
 // Outputs of a row that does not count.
@@ -255,7 +249,6 @@ __device__ __forceinline__ RowGrad distill_row(const LossArgs& a, double w, doub
     } else {
         o.a = w * a.inv_temp / s;
     }
-    o.at_target = 0.0;
     o.loss = loss;
     return o;
 }
@@ -333,6 +326,8 @@ constexpr int64_t kLossMaxDistillCols = int64_t(1) << 20;  // columns of a disti
 // the scratch query.
 constexpr int kLossMaxCtas = 148 * 16;
 
+bool loss_rows_fit(const LossPlan& p);                                        // losses_rows.cu
+int loss_rows_fast(const LossPlan& p, int* parts, cudaStream_t st);           // losses_rows.cu
 int loss_rows_general(const LossPlan& p, int* ctas, cudaStream_t st);      // losses_general.cu
 int loss_backward_general(const LossArgs& a, cudaStream_t st);              // losses_general.cu
 

@@ -152,10 +152,15 @@ template <class T, int OP> __global__ void __launch_bounds__(kThreads) loss_rows
                     put_row(a, kLrLogp, row, logp);
                     put_row(a, kLrLse, row, m * a.inv_temp + log(s));
                 } else {
-                    const RowGrad o = policy_row(a, row, w, logp, s);
+                    const double d = a.ptr[kLrRef] ? row_real(a, kLrRef, row) - logp : 0.0;
+                    const PolicyTerms o = policy_terms(a, w, row_real(a, kLrAdv, row),
+                                                       exp(logp - row_real(a, kLrOld, row)), d, expm1(d));
+                    put_row(a, kLrLogp, row, logp);
+                    put_row(a, kLrRowLoss, row, o.loss);
+                    put_row(a, kLrKl, row, o.kl);
                     total += w * o.loss;
-                    sh[0] = o.a;
-                    sh[1] = o.at_target;
+                    sh[0] = -o.g / s;
+                    sh[1] = -o.g * expm1(logp);  // g (1 - p_t)
                     if (!ok) target = -1;
                 }
             }

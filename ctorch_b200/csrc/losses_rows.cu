@@ -1,0 +1,905 @@
+// losses_rows.cu — the losses over rows of unit stride, float32 and bfloat16: each logit is read from
+// memory once and each gradient element written once.
+//
+// A row belongs to a thread-block cluster of C CTAs (C = 1 for rows that one CTA can hold), a CTA to a
+// contiguous slice of the row's 16-byte packs. Clusters are persistent: cluster c takes rows c, c + n,
+// c + 2n, ... A CTA has eight consumer warps and two helpers:
+//   * the producer warp streams the slices of the coming rows into a ring of shared-memory stages with
+//     bulk asynchronous copies (async_copy.cuh) and reads the rows' small operands ahead, 32 rows a time;
+//   * the consumers take a slice out of the ring into registers, find the warp's maximum, turn the
+//     logits into e = exp((x - m_w) / T) and send each warp's (m_w, sum e) to every CTA of the cluster
+//     (st.async into its mailbox, completion counted on its mbarrier: no cluster-wide barrier);
+//   * the row warp joins the C * 8 partial sums, does the row's own arithmetic in float64 and publishes
+//     the row's coefficient A; the consumers then write g = e * A exp((m_w - m) / T) from registers.
+// So a logit costs one exponential, not two, and the exchange of one cluster hides behind the other
+// clusters of the SM and behind the copies of the next rows.
+//
+// Accuracy of the sum. The hardware's 2^t is low by 5.0e-8 on average (measured over t in [-30, -1] on
+// B200; at most 1.5e-7 off), which a sum of thousands does not average out; log2(e)/T as one float32 is
+// off by up to 6e-8 relative, and so is every t. Sums of log-probabilities over a sequence show both. t is
+// therefore corrected with the rest of log2(e)/T (one fused multiply-add), and the joined sum by the mean.
+#include <map>
+#include <mutex>
+#include <string>
+#include <tuple>
+
+#include "async_copy.cuh"
+#include "losses.cuh"
+
+namespace ctb {
+
+namespace {
+
+constexpr int kConsWarps = 8;
+constexpr int kCons = kConsWarps * 32;
+constexpr int kProducer = kConsWarps;  // warp numbers
+constexpr int kRowWarp = kConsWarps + 1;
+constexpr int kThreads = kCons + 64;
+constexpr int kMaxCluster = 8;
+constexpr int kBatch = 32;  // rows whose operands the producer reads together, one a lane
+constexpr double kExp2Low = 5.0e-8;
+constexpr int kMaxSmem = 227 * 1024;
+
+// ------------------------------------------------------------------------------------------------
+// pairs of floats (one instruction for two elements on sm_100)
+
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void un(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// The largest of the warp's values (NaN loses against any number).
+__device__ __forceinline__ float warp_max(float x) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
+// A 16-byte pack as pairs of floats, its maximum, and back (rounded to nearest even).
+template <class T> struct PackOf;
+template <> struct PackOf<float> {
+    static constexpr int VE = 4;
+    __device__ static __forceinline__ float max(const uint4& p) {
+        return fmaxf(fmaxf(__uint_as_float(p.x), __uint_as_float(p.y)), fmaxf(__uint_as_float(p.z), __uint_as_float(p.w)));
+    }
+    __device__ static __forceinline__ void up(const uint4& p, F2* o) {
+        o[0] = f2(__uint_as_float(p.x), __uint_as_float(p.y));
+        o[1] = f2(__uint_as_float(p.z), __uint_as_float(p.w));
+    }
+    __device__ static __forceinline__ uint4 down(const F2* e) {
+        float a, b, c, d;
+        un(e[0], a, b);
+        un(e[1], c, d);
+        return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+    }
+    __device__ static __forceinline__ uint4 lowest() {
+        return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);  // -inf
+    }
+};
+template <> struct PackOf<__nv_bfloat16> {
+    static constexpr int VE = 8;
+    __device__ static __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    __device__ static __forceinline__ float max(const uint4& p) {
+        const uint32_t m = max2(max2(p.x, p.y), max2(p.z, p.w));
+        return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    }
+    __device__ static __forceinline__ F2 pair(uint32_t w) { return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    __device__ static __forceinline__ void up(const uint4& p, F2* o) {
+        o[0] = pair(p.x);
+        o[1] = pair(p.y);
+        o[2] = pair(p.z);
+        o[3] = pair(p.w);
+    }
+    __device__ static __forceinline__ uint32_t two(F2 e) {
+        float a, b;
+        un(e, a, b);
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));  // first operand in the upper half
+        return r;
+    }
+    __device__ static __forceinline__ uint4 down(const F2* e) { return make_uint4(two(e[0]), two(e[1]), two(e[2]), two(e[3])); }
+    __device__ static __forceinline__ uint4 lowest() {
+        return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+    }
+};
+
+// exp of pairs: t = d c + d c rho with c = log2(e)/T rounded down and rho >= 1e-30 its rest, so that
+// d = -inf stays -inf.
+struct ExpConst {
+    F2 c, rho;
+};
+__device__ __forceinline__ ExpConst exp_const(const LossArgs& a) {
+    ExpConst k;
+    k.c = f2(a.c2_down, a.c2_down);
+    k.rho = f2(a.c2_rest, a.c2_rest);
+    return k;
+}
+__device__ __forceinline__ F2 exp_pair(F2 x, F2 minus_m, const ExpConst& k) {
+    const F2 d = mul2(add2(x, minus_m), k.c);
+    const F2 t = fma2(d, k.rho, d);
+    float a, b;
+    un(t, a, b);
+    return f2(exp2_fast(a), exp2_fast(b));
+}
+__device__ __forceinline__ float exp_one(const LossArgs& a, float x, float m) {
+    const float d = (x - m) * a.c2_down;
+    return exp2_fast(fmaf(d, a.c2_rest, d));
+}
+
+// ------------------------------------------------------------------------------------------------
+// clusters
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+// Every thread of every CTA of the cluster. Used at the start (barriers are initialised before anyone
+// sends to them) and at the end (no CTA leaves while another may still send to its memory).
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Stores 8 bytes to the same place in CTA `cta` of the cluster and counts them on its barrier.
+__device__ __forceinline__ void send8(const void* local, uint64_t* local_bar, uint32_t cta, uint64_t v) {
+    asm volatile(
+        "{\n\t.reg .b32 ra, rb;\n\t"
+        "mapa.shared::cluster.u32 ra, %0, %2;\n\t"
+        "mapa.shared::cluster.u32 rb, %1, %2;\n\t"
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [ra], %3, [rb];\n\t}" ::"r"(smem_addr(local)),
+        "r"(smem_addr(local_bar)), "r"(cta), "l"(v)
+        : "memory");
+}
+
+// The end of every warp's work. After a wait that ran out, another CTA may have sent what this one no longer
+// waits for: it stays for a millisecond more, a thousand times what a store takes.
+__device__ __forceinline__ void leave_cluster(bool ok) {
+    __syncwarp();
+    cluster_sync();
+    if (!ok) {
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 1000000ull) {
+        }
+    }
+}
+
+// Waits for a phase that threads of other CTAs of the cluster contribute to.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint64_t t0 = 0;
+    for (int i = 0;; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (i % 32 == 0) {
+            if (t0 == 0) t0 = global_ns();
+            else if (global_ns() - t0 > kWaitLimitNs) return false;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// shared memory
+
+// What the producer knows of a row before its logits arrive.
+struct RowMeta {
+    double w;            // 0: the row does not count
+    double xt;           // target's logit
+    double old, adv, ref;
+    long long row, g_off;
+    int target;          // -1: bad
+    int head, packs;     // elements before the first whole 16-byte pack, whole packs
+    int pad_;
+};
+
+// What the producer knows of a teacher's list.
+struct ListInfo {
+    double q_logq, q_x, ref, mass;  // sums of q log q, q (x - ref) and q over the entries
+    float x_max;
+    int count, bad;
+    uint32_t edge_named;  // which of the 16 edge elements the teacher names
+};
+
+struct Coef {
+    float a, m, at_target, pad_;
+};
+
+template <class T, int E, int CP, int NS> struct Layout {
+    static constexpr int VE = PackOf<T>::VE;
+    static constexpr int RP = E / VE;        // packs a consumer thread holds
+    static constexpr int NCH = RP / CP;      // stages a slice takes
+    static constexpr int kChunkPacks = CP * kCons;
+    static constexpr size_t kStage = static_cast<size_t>(kChunkPacks) * 16;
+    static constexpr size_t kMail = NS * kStage;                       // uint64 [2][kMaxCluster * kConsWarps]
+    static constexpr size_t kMeta = kMail + 2 * kMaxCluster * kConsWarps * 8;  // RowMeta [2][kBatch]
+    static constexpr size_t kEdge = kMeta + 2 * kBatch * sizeof(RowMeta);      // float [2][kBatch][16]
+    static constexpr size_t kCoef = kEdge + 2 * kBatch * 16 * sizeof(float);   // Coef [2]
+    static constexpr size_t kBars = kCoef + 2 * sizeof(Coef);
+    static constexpr int kNumBars = 2 * NS + 2 + 2 + 2 + 2 + 2 + 2;
+    static constexpr size_t kList = kBars + kNumBars * 8;              // ListInfo [2]
+    static constexpr size_t kBits = (kList + 2 * sizeof(ListInfo) + 15) / 16 * 16;  // bytes [2][kCons * RP]
+    static constexpr size_t kEntries = kBits + 2 * kCons * RP;         // per side: int idx[K], float x[K], float q[K]
+    static constexpr size_t bytes(int op, int top) {
+        return op == kLossDistill ? kEntries + static_cast<size_t>(2) * 12 * top : kList;
+    }
+};
+
+// The barriers of a CTA.
+template <int NS> struct Bars {
+    uint64_t full[NS], empty[NS];
+    uint64_t meta_full[2], meta_empty[2];
+    uint64_t list_full[2], list_empty[2];
+    uint64_t mail[2], coef[2];
+};
+
+// Rank r's share of a row's packs.
+__device__ __forceinline__ void slice_of(int packs, int rank, int size, int& first, int& count) {
+    first = static_cast<int>(static_cast<int64_t>(packs) * rank / size);
+    count = static_cast<int>(static_cast<int64_t>(packs) * (rank + 1) / size) - first;
+}
+
+// ------------------------------------------------------------------------------------------------
+// the producer's reads
+
+template <class T, int OP> __device__ __forceinline__ RowMeta read_meta(const LossArgs& a, int64_t row, int64_t& x_off) {
+    RowMeta r;
+    const T* X = static_cast<const T*>(a.ptr[kLrX]);
+    r.row = row;
+    r.w = row_weight(a, row);
+    x_off = loss_offset(a, kLrX, row);
+    r.g_off = a.ptr[kLrGrad] ? loss_offset(a, kLrGrad, row) : 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(X + x_off);
+    const int64_t head = ((16 - (at & 15)) & 15) / sizeof(T);
+    r.head = static_cast<int>(head < a.cols ? head : a.cols);
+    r.packs = static_cast<int>((a.cols - r.head) / PackOf<T>::VE);
+    r.target = -1;
+    r.xt = r.old = r.adv = r.ref = 0.0;
+    if (OP != kLossDistill && r.w != 0.0) {
+        const int64_t t = load_index(a.ptr[kLrTarget], a.dtype[kLrTarget], loss_offset(a, kLrTarget, row));
+        if (OP == kLossPolicy) {
+            r.old = row_real(a, kLrOld, row);
+            r.adv = row_real(a, kLrAdv, row);
+            if (a.ptr[kLrRef]) r.ref = row_real(a, kLrRef, row);
+        }
+        if (t >= 0 && t < a.cols) {
+            r.target = static_cast<int>(t);
+            r.xt = LossElem<T>::up(X[x_off + t]);
+        } else {
+            note_bad_index(a, t);
+        }
+    }
+    return r;
+}
+
+// The elements around the whole packs: 0..7 before them, 8..15 behind them; -1 where there is none.
+__device__ __forceinline__ int64_t edge_position(const LossArgs& a, int head, int packs, int ve, int l) {
+    const int64_t behind = head + static_cast<int64_t>(packs) * ve;
+    if (l < 8) return l < head ? l : -1;
+    return behind + (l - 8) < a.cols ? behind + (l - 8) : -1;
+}
+
+// ------------------------------------------------------------------------------------------------
+// losses with their gradient (policy, distill)
+
+template <class T, int OP, int E, int CP, int NS, int PER_SM>
+__global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_constant__ LossArgs a) {
+    using L = Layout<T, E, CP, NS>;
+    using P = PackOf<T>;
+    constexpr int VE = L::VE, RP = L::RP;
+    extern __shared__ __align__(128) unsigned char sm[];
+    Bars<NS>& bars = *reinterpret_cast<Bars<NS>*>(sm + L::kBars);
+    uint64_t* mail = reinterpret_cast<uint64_t*>(sm + L::kMail);
+    RowMeta* metas = reinterpret_cast<RowMeta*>(sm + L::kMeta);
+    float* edges = reinterpret_cast<float*>(sm + L::kEdge);
+    Coef* coefs = reinterpret_cast<Coef*>(sm + L::kCoef);
+    ListInfo* lists = reinterpret_cast<ListInfo*>(sm + L::kList);
+    unsigned char* bits = sm + L::kBits;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_rank()), size = static_cast<int>(cluster_size());
+    const uint32_t mail_bytes = static_cast<uint32_t>(size) * kConsWarps * 8;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&bars.full[i], 1);
+            mbar_init(&bars.empty[i], kConsWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.meta_full[i], 1);
+            mbar_init(&bars.meta_empty[i], kConsWarps + 1);
+            mbar_init(&bars.list_full[i], 1);
+            mbar_init(&bars.list_empty[i], kConsWarps + 1);
+            mbar_init(&bars.mail[i], 1);
+            mbar_init(&bars.coef[i], 1);
+        }
+        mbar_fence_init();
+        for (int i = 0; i < 2; ++i) mbar_arrive_expect_tx(&bars.mail[i], mail_bytes);
+    }
+    __syncthreads();
+    cluster_sync();
+    dependent_wait();  // the previous kernel in the stream has completed and its writes are visible
+
+    const int64_t cluster = blockIdx.x / size, clusters = gridDim.x / size;
+    const int64_t my_rows = cluster < a.rows ? (a.rows - cluster + clusters - 1) / clusters : 0;
+    bool ok = true;
+
+    if (warp == kProducer) {
+        uint32_t g = 0;     // stages filled
+        uint32_t live = 0;  // rows that count
+        auto issue = [&](int64_t x_off, int head, int packs) {
+            int first, count;
+            slice_of(packs, rank, size, first, count);
+            const T* src = static_cast<const T*>(a.ptr[kLrX]) + x_off + head + static_cast<int64_t>(first) * VE;
+            for (int p = 0; p < count && ok; p += L::kChunkPacks, ++g) {
+                const int slot = static_cast<int>(g % NS);
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[slot], ((g / NS) & 1u) ^ 1u));
+                if (!ok) break;
+                const int n = min(L::kChunkPacks, count - p);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&bars.full[slot], static_cast<uint32_t>(n) * 16u);
+                    bulk_load(sm + static_cast<size_t>(slot) * L::kStage, src + static_cast<int64_t>(p) * VE,
+                              static_cast<uint32_t>(n) * 16u, &bars.full[slot]);
+                }
+                __syncwarp();
+            }
+        };
+        auto read_list = [&](int64_t row, int64_t x_off, int head, int packs, double w) {
+            (void)w;
+            const int side = static_cast<int>(live & 1u);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.list_empty[side], ((live >> 1) & 1u) ^ 1u));
+            if (!ok) return;
+            int* e_idx = reinterpret_cast<int*>(sm + L::kEntries + static_cast<size_t>(side) * 12 * a.top);
+            float* e_x = reinterpret_cast<float*>(e_idx + a.top);
+            float* e_q = e_x + a.top;
+            uint4* b16 = reinterpret_cast<uint4*>(bits + side * kCons * RP);
+            for (int i = lane; i < kCons * RP / 16; i += 32) b16[i] = make_uint4(0u, 0u, 0u, 0u);
+            ListInfo& li = lists[side];
+            if (lane == 0) li.edge_named = 0u;
+            __syncwarp();
+            int first, count;
+            slice_of(packs, rank, size, first, count);
+            const T* x = static_cast<const T*>(a.ptr[kLrX]) + x_off;
+            const int64_t t_off = loss_offset(a, kLrTeacher, row), ti_off = loss_offset(a, kLrTeacherIdx, row);
+            auto scaled = [&](int k) {
+                return load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
+            };
+            double mx = -INFINITY;
+            float x_max = -INFINITY;
+            int entries = 0, bad = 0;
+            for (int k = lane; k < a.top; k += 32) {
+                const double z = scaled(k);
+                int j = -1;
+                float xk = -INFINITY;
+                if (z != -INFINITY) {
+                    ++entries;
+                    mx = fmax(mx, z);
+                    const int64_t at = load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in);
+                    if (at < 0 || at >= a.cols) {
+                        bad = 1;
+                        if (rank == 0) note_bad_index(a, at);
+                    } else {
+                        j = static_cast<int>(at);
+                        xk = LossElem<T>::up(x[j]);
+                        x_max = fmaxf(x_max, xk);
+                        const int b = j - head;
+                        uint32_t was = 0u, bit = 1u;
+                        if (b >= 0 && b < packs * VE) {
+                            const int p = b / VE - first;
+                            if (p >= 0 && p < count) {
+                                bit = 1u << ((p & 3) * 8 + b % VE);
+                                was = atomicOr(reinterpret_cast<uint32_t*>(bits + side * kCons * RP) + (p >> 2), bit);
+                            }
+                        } else if (rank == 0) {
+                            bit = 1u << (b < 0 ? j : 8 + b - packs * VE);
+                            was = atomicOr(&li.edge_named, bit);
+                        }
+                        if (was & bit) {
+                            bad = 1;
+                            note_bad_index(a, at);
+                        }
+                    }
+                }
+                e_idx[k] = j;
+                e_x[k] = xk;
+            }
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            x_max = warp_max(x_max);
+            entries = __reduce_add_sync(0xffffffffu, entries);
+            bad = __any_sync(0xffffffffu, bad);
+            double lse = 0.0;
+            if (a.tail) {
+                lse = entries ? row_real(a, kLrTeacherLse, row) : 0.0;
+            } else if (entries) {
+                double s = 0.0;
+                for (int k = lane; k < a.top; k += 32) s += exp(scaled(k) - mx);
+                lse = mx + log(warp_sum(s));
+            }
+            const double ref = x_max == -INFINITY ? 0.0 : static_cast<double>(x_max);
+            double mass = 0.0, q_logq = 0.0, q_x = 0.0;
+            for (int k = lane; k < a.top; k += 32) {
+                const double z = scaled(k), q = z == -INFINITY ? 0.0 : exp(z - lse);
+                if (q != 0.0) {
+                    mass += q;
+                    q_logq += q * (z - lse);
+                    q_x += q * (static_cast<double>(e_x[k]) - ref);
+                }
+                e_q[k] = static_cast<float>(q);
+            }
+            mass = warp_sum(mass);
+            q_logq = warp_sum(q_logq);
+            q_x = warp_sum(q_x);
+            __syncwarp();
+            if (lane == 0) {
+                li.q_logq = q_logq;
+                li.q_x = q_x;
+                li.ref = ref;
+                li.mass = mass;
+                li.x_max = x_max;
+                li.count = entries;
+                li.bad = bad;
+                mbar_arrive(&bars.list_full[side]);
+            }
+            __syncwarp();
+        };
+        for (int64_t b = 0; b * kBatch < my_rows && ok; ++b) {
+            const int side = static_cast<int>(b & 1);
+            const int n = static_cast<int>(min(static_cast<int64_t>(kBatch), my_rows - b * kBatch));
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.meta_empty[side], ((b >> 1) & 1) ^ 1));
+            if (!ok) break;
+            int64_t x_off = 0;
+            RowMeta r{};
+            if (lane < n) {
+                r = read_meta<T, OP>(a, cluster + (b * kBatch + lane) * clusters, x_off);
+                metas[side * kBatch + lane] = r;
+            }
+            if (rank == 0) {
+                for (int i = 0; i < n; ++i) {
+                    const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
+                    const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
+                    const bool counts = __shfl_sync(0xffffffffu, r.w != 0.0, i);
+                    if (lane < 16) {
+                        const int64_t at = edge_position(a, head, packs, VE, lane);
+                        edges[(side * kBatch + i) * 16 + lane] =
+                            at >= 0 && counts ? LossElem<T>::up(static_cast<const T*>(a.ptr[kLrX])[off + at]) : -INFINITY;
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.meta_full[side]);
+            for (int i = 0; i < n && ok; ++i) {
+                const double w = __shfl_sync(0xffffffffu, r.w, i);
+                if (w == 0.0) continue;
+                const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
+                const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
+                issue(off, head, packs);
+                if (OP == kLossDistill && ok) read_list(__shfl_sync(0xffffffffu, r.row, i), off, head, packs, w);
+                ++live;
+            }
+        }
+        if (!ok) {
+            if (lane == 0) note_timeout(a.timeouts);
+            // the copies in flight land before the CTA's memory goes away
+            for (uint32_t i = g > static_cast<uint32_t>(NS) ? g - NS : 0u; i < g; ++i)
+                mbar_wait(&bars.full[i % NS], (i / NS) & 1u);
+        }
+    } else if (warp == kRowWarp) {
+        uint32_t live = 0;
+        double total = 0.0;
+        for (int64_t i = 0; i < my_rows && ok; ++i) {
+            const int64_t b = i / kBatch;
+            const int side = static_cast<int>(b & 1);
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.meta_full[side], (b >> 1) & 1));
+            if (!ok) break;
+            const RowMeta& r = metas[side * kBatch + i % kBatch];
+            const int64_t row = r.row;
+            if (r.w == 0.0) {
+                if (rank == 0 && lane == 0) put_empty_row(a, row);
+            } else {
+                const int par = static_cast<int>(live & 1u);
+                const uint32_t phase = (live >> 1) & 1u;
+                ok = mbar_wait_cluster(&bars.mail[par], phase);
+                if (OP == kLossDistill) ok = ok && mbar_wait(&bars.list_full[par], phase);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                // the partial sums, joined in float64
+                const int parts = size * kConsWarps;
+                float pm[2], ps[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint64_t v = lane + 32 * k < parts ? mail[par * kMaxCluster * kConsWarps + lane + 32 * k] : 0xff800000ull;
+                    pm[k] = __uint_as_float(static_cast<uint32_t>(v));
+                    ps[k] = __uint_as_float(static_cast<uint32_t>(v >> 32));
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&bars.mail[par], mail_bytes);  // for the row after the next
+                float mf = warp_max(fmaxf(pm[0], pm[1]));
+                const ListInfo* li = &lists[par];
+                if (OP == kLossDistill) mf = fmaxf(mf, li->x_max);
+                double s = 0.0;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (pm[k] != -INFINITY)
+                        s += (ps[k] + kExp2Low * (static_cast<double>(ps[k]) - 1.0)) *
+                             (pm[k] == mf ? 1.0 : exp((static_cast<double>(pm[k]) - mf) * a.inv_temp));
+                    else
+                        s += ps[k];  // 0, or the NaN of a bad index
+                }
+                s = warp_sum(s);
+                if (mf == INFINITY) s = quiet_nan();
+                const double m = mf;
+                Coef c;
+                c.m = mf;
+                c.at_target = c.pad_ = 0.f;
+                double loss = 0.0;
+                bool counts = true;
+                if (OP == kLossPolicy) {
+                    const double logp = r.target >= 0 ? (r.xt - m) * a.inv_temp - log(s) : quiet_nan();
+                    // three exponentials of the row, one a lane
+                    const double v = expm1(lane == 0 ? logp - r.old : lane == 1 ? r.ref - logp : logp);
+                    const double e_old = __shfl_sync(0xffffffffu, v, 0), e_ref = __shfl_sync(0xffffffffu, v, 1),
+                                 e_logp = __shfl_sync(0xffffffffu, v, 2);
+                    PolicyTerms t = policy_terms(a, r.w, r.adv, 1.0 + e_old, r.ref - logp, e_ref);
+                    c.a = static_cast<float>(-t.g / s);
+                    c.at_target = static_cast<float>(-t.g * e_logp);
+                    loss = t.loss;
+                    if (rank == 0 && lane == 0) {
+                        put_row(a, kLrLogp, row, logp);
+                        put_row(a, kLrKl, row, t.kl);
+                    }
+                } else {
+                    const int* e_idx = reinterpret_cast<const int*>(sm + L::kEntries + static_cast<size_t>(par) * 12 * a.top);
+                    const float* e_x = reinterpret_cast<const float*>(e_idx + a.top);
+                    const float* e_q = e_x + a.top;
+                    counts = li->count > 0;
+                    const double s_rest = s;
+                    float named = 0.f;
+                    for (int k = lane; k < a.top; k += 32)
+                        if (e_idx[k] >= 0) named += exp_one(a, e_x[k], mf);
+                    s = s_rest + warp_sum(static_cast<double>(named));
+                    const double log_s = log(s);
+                    const double cross = li->q_logq - a.inv_temp * (li->q_x + (li->ref - m) * li->mass) + li->mass * log_s;
+                    double big_q;
+                    RowGrad o = distill_row(a, r.w, s, s_rest, cross, li->mass, li->count == a.cols, big_q);
+                    if (!(s > 0.0)) o.a = o.loss = quiet_nan();
+                    c.a = counts ? static_cast<float>(o.a) : 0.f;
+                    loss = counts ? o.loss : 0.0;
+                    T* G = static_cast<T*>(a.ptr[kLrGrad]);
+                    if (G && counts) {
+                        T* gr = G + r.g_off;
+                        int first, count;
+                        slice_of(r.packs, rank, size, first, count);
+                        const float scale = static_cast<float>(r.w * a.inv_temp), p_scale = static_cast<float>(big_q / s);
+                        // a bad row is NaN throughout: its named columns too, whoever found it
+                        const float poison = c.a == c.a ? 0.f : c.a;
+                        for (int k = lane; k < a.top; k += 32) {
+                            const int j = e_idx[k];
+                            if (j < 0) continue;
+                            const int body = j - r.head;
+                            const bool mine = body >= 0 && body < r.packs * VE ? body / VE >= first && body / VE < first + count
+                                                                               : rank == 0;
+                            if (mine) gr[j * a.g_in] = LossElem<T>::down(scale * (exp_one(a, e_x[k], mf) * p_scale - e_q[k]) + poison);
+                        }
+                    }
+                }
+                if (lane == 0) {
+                    coefs[par] = c;
+                    mbar_arrive(&bars.coef[par]);
+                }
+                if (rank == 0 && lane == 0) {
+                    put_row(a, kLrRowLoss, row, loss);
+                    if (counts) total += r.w * loss;
+                }
+                __syncwarp();
+                if (OP == kLossDistill && lane == 0) mbar_arrive(&bars.list_empty[par]);
+                ++live;
+            }
+            __syncwarp();
+            if (lane == 0 && (i % kBatch == kBatch - 1 || i + 1 == my_rows)) mbar_arrive(&bars.meta_empty[side]);
+        }
+        if (!ok && lane == 0) note_timeout(a.timeouts);
+        if (a.partials && rank == 0 && lane == 0) a.partials[cluster] = total;
+    } else {
+        // ---- consumers
+        const int t = threadIdx.x;
+        const ExpConst kc = exp_const(a);
+        uint32_t g = 0, live = 0;
+        for (int64_t i = 0; i < my_rows && ok; ++i) {
+            const int64_t b = i / kBatch;
+            const int side = static_cast<int>(b & 1);
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.meta_full[side], (b >> 1) & 1));
+            if (!ok) break;
+            const RowMeta& r = metas[side * kBatch + i % kBatch];
+            int first, count;
+            slice_of(r.packs, rank, size, first, count);
+            T* gr = a.ptr[kLrGrad] ? static_cast<T*>(a.ptr[kLrGrad]) + r.g_off : nullptr;
+            // Packs are stored whole where the gradient's rows are aligned like the logits', element by element
+            // elsewhere (which costs eight times the store instructions, and takes any stride).
+            T* gs = gr + (r.head + static_cast<int64_t>(first) * VE) * a.g_in;
+            const bool whole = a.g_in == 1 && (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
+            auto put_pack = [&](int p, const uint4& o, uint32_t skip) {
+                if (whole && skip == 0u) {
+                    reinterpret_cast<uint4*>(gs)[p] = o;
+                } else {
+                    const T* ov = reinterpret_cast<const T*>(&o);
+                    T* dst = gs + static_cast<int64_t>(p) * VE * a.g_in;
+#pragma unroll
+                    for (int k = 0; k < VE; ++k)
+                        if (!(skip >> k & 1u)) dst[k * a.g_in] = ov[k];
+                }
+            };
+            const bool edge = rank == 0 && t < 16;
+            const int64_t edge_at = edge ? edge_position(a, r.head, r.packs, VE, t) : -1;
+            auto zeros = [&]() {
+                if (!gr) return;
+                for (int p = t; p < count; p += kCons) put_pack(p, make_uint4(0u, 0u, 0u, 0u), 0u);
+                if (edge_at >= 0) gr[edge_at * a.g_in] = LossElem<T>::down(0.f);
+            };
+            if (r.w == 0.0) {
+                zeros();
+            } else {
+                const int par = static_cast<int>(live & 1u);
+                const uint32_t phase = (live >> 1) & 1u;
+                if (OP == kLossDistill) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.list_full[par], phase));
+                    if (!ok) break;
+                }
+                const unsigned char* named = bits + par * kCons * RP;
+                // the slice, out of the ring
+                uint4 raw[RP];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int ch = 0; ch < L::NCH; ++ch) {
+                    if (ch * L::kChunkPacks < count) {
+                        const int slot = static_cast<int>(g % NS);
+                        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars.full[slot], (g / NS) & 1u));
+                        const uint4* st = reinterpret_cast<const uint4*>(sm + static_cast<size_t>(slot) * L::kStage);
+#pragma unroll
+                        for (int u = 0; u < CP; ++u) {
+                            const int p = ch * L::kChunkPacks + u * kCons + t;
+                            raw[ch * CP + u] = ok && p < count ? st[u * kCons + t] : P::lowest();
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars.empty[slot]);
+                        ++g;
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < CP; ++u) raw[ch * CP + u] = P::lowest();
+                    }
+                }
+                if (!ok) break;
+                uint32_t mark = 0u;  // packs of mine with a named element
+                if (OP == kLossDistill) {
+#pragma unroll
+                    for (int p = 0; p < RP; ++p) {
+                        const uint32_t by = p * kCons + t < count ? named[p * kCons + t] : 0u;
+                        if (by) {
+                            mark |= 1u << p;
+                            uint32_t* w = reinterpret_cast<uint32_t*>(&raw[p]);
+#pragma unroll
+                            for (int e = 0; e < VE; ++e)
+                                if (by >> e & 1u) {
+                                    if (VE == 4) w[e] = 0xff800000u;
+                                    else w[e >> 1] = e & 1 ? (w[e >> 1] & 0x0000ffffu) | 0xff800000u : (w[e >> 1] & 0xffff0000u) | 0x0000ff80u;
+                                }
+                        }
+                    }
+                }
+                float xe = -INFINITY;
+                if (edge_at >= 0 && !(OP == kLossDistill && (lists[par].edge_named >> t & 1u)))
+                    xe = edges[(side * kBatch + i % kBatch) * 16 + t];
+#pragma unroll
+                for (int p = 0; p < RP; ++p) mx = fmaxf(mx, P::max(raw[p]));
+                const float mw = warp_max(fmaxf(mx, xe));
+                const float at = mw == -INFINITY ? 0.f : mw;
+                const F2 minus = f2(-at, -at);
+                F2 e[RP][VE / 2];
+                F2 acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
+#pragma unroll
+                for (int p = 0; p < RP; ++p) {
+                    P::up(raw[p], e[p]);
+#pragma unroll
+                    for (int h = 0; h < VE / 2; ++h) {
+                        e[p][h] = exp_pair(e[p][h], minus, kc);
+                        if (h & 1) acc1 = add2(acc1, e[p][h]);
+                        else acc0 = add2(acc0, e[p][h]);
+                    }
+                }
+                const float ee = exp_one(a, xe, at);
+                float s0, s1;
+                un(add2(acc0, acc1), s0, s1);
+                float s = warp_sum(s0 + s1 + ee);
+                if (OP == kLossDistill && warp == 0 && lists[par].bad) s = NAN;
+                if (lane < size)
+                    send8(&mail[par * kMaxCluster * kConsWarps + rank * kConsWarps + warp], &bars.mail[par], lane,
+                          static_cast<uint64_t>(__float_as_uint(mw)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.coef[par], phase));
+                if (!ok) break;
+                const Coef c = coefs[par];
+                if (OP == kLossDistill && lists[par].count == 0) {
+                    zeros();
+                } else if (gr) {
+                    const float f = c.a * exp_one(a, mw, c.m);
+                    const F2 ff = f2(f, f);
+                    const int tb = r.target - r.head;  // the target among the whole packs
+                    const int tp = OP == kLossPolicy && tb >= 0 && r.target >= 0 ? tb / VE - first : -1;
+#pragma unroll
+                    for (int p = 0; p < RP; ++p) {
+                        const int pk = p * kCons + t;
+                        if (pk < count) {
+#pragma unroll
+                            for (int h = 0; h < VE / 2; ++h) e[p][h] = mul2(e[p][h], ff);
+                            if (OP == kLossPolicy && pk == tp) {
+#pragma unroll
+                                for (int h = 0; h < VE / 2; ++h) {
+                                    float x0, x1;
+                                    un(e[p][h], x0, x1);
+                                    if (tb % VE == 2 * h) x0 = c.at_target;
+                                    if (tb % VE == 2 * h + 1) x1 = c.at_target;
+                                    e[p][h] = f2(x0, x1);
+                                }
+                            }
+                            // the row warp writes the named elements
+                            put_pack(pk, P::down(e[p]), OP == kLossDistill && (mark >> p & 1u) ? named[pk] : 0u);
+                        }
+                    }
+                    if (edge_at >= 0 && !(OP == kLossDistill && (lists[par].edge_named >> t & 1u)))
+                        gr[edge_at * a.g_in] = LossElem<T>::down(OP == kLossPolicy && r.target == edge_at ? c.at_target : ee * f);
+                }
+                if (OP == kLossDistill) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.list_empty[par]);
+                }
+                ++live;
+            }
+            __syncwarp();
+            if (lane == 0 && (i % kBatch == kBatch - 1 || i + 1 == my_rows)) mbar_arrive(&bars.meta_empty[side]);
+        }
+        if (!ok && lane == 0) note_timeout(a.timeouts);
+    }
+    allow_dependents();
+    leave_cluster(ok);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+
+template <class... Ps> int launch_cluster(void (*fn)(Ps...), unsigned grid, int cluster, size_t smem, cudaStream_t st,
+                                          const LossArgs& a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, a);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(CTB_ERR_CUDA, std::string("loss rows: ") + cudaGetErrorString(e));
+    }
+    count_launch();
+    return CTB_OK;
+}
+
+// How many clusters of `cluster` CTAs are resident at once on the current device (cached). Also opts the
+// kernel in to its shared memory there.
+int resident_clusters(const void* fn, int cluster, size_t smem, int* out) {
+    static std::mutex mu;
+    static std::map<std::tuple<const void*, int, int, size_t>, int> cache;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("loss rows device");
+    const auto key = std::make_tuple(fn, dev, cluster, smem);
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = cache.find(key);
+    if (it == cache.end()) {
+        // the largest size any call asks for: a smaller one later must not lower it under a concurrent launch
+        if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
+            return check_launch("loss rows smem attribute");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(cluster));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) return check_launch("loss rows occupancy");
+        it = cache.emplace(key, n < 1 ? 1 : n).first;
+    }
+    *out = it->second;
+    return CTB_OK;
+}
+
+template <class T, int OP, int E, int CP, int NS, int PER_SM> int hold_typed(const LossArgs& a, int cluster, int* parts, cudaStream_t st) {
+    using L = Layout<T, E, CP, NS>;
+    const size_t smem = L::bytes(OP, a.top);
+    auto fn = loss_hold<T, OP, E, CP, NS, PER_SM>;
+    int n = 0;
+    if (int rc = resident_clusters(reinterpret_cast<const void*>(fn), cluster, smem, &n)) return rc;
+    int64_t clusters = n < a.rows ? n : a.rows;
+    if (clusters > kLossMaxCtas) clusters = kLossMaxCtas;
+    *parts = static_cast<int>(clusters);
+    return launch_cluster(fn, static_cast<unsigned>(clusters * cluster), cluster, smem, st, a);
+}
+
+template <class T, int OP> int hold_sized(const LossArgs& a, int* parts, cudaStream_t st) {
+    constexpr int VE = PackOf<T>::VE;
+    const int64_t packs = a.cols / VE;
+    auto need = [&](int e) { return static_cast<int>((packs + static_cast<int64_t>(kCons) * (e / VE) - 1) / (static_cast<int64_t>(kCons) * (e / VE))); };
+    if (need(16) <= 1) return hold_typed<T, OP, 16, 16 / VE, 4, 4>(a, 1, parts, st);
+    int c = need(64);
+    return hold_typed<T, OP, 64, 4, 6, 2>(a, c, parts, st);
+}
+
+}  // namespace
+
+// Whether the kernels of this file take the call: float32 or bfloat16 rows of unit stride that a cluster
+// can hold.
+bool loss_rows_fit(const LossPlan& p) {
+    const LossArgs& a = p.args;
+    if (a.dtype[kLrX] != CTB_FLOAT32 && a.dtype[kLrX] != CTB_BFLOAT16) return false;
+    if (a.cols > 1 && a.x_in != 1) return false;
+    return a.cols <= static_cast<int64_t>(kMaxCluster) * kCons * 64;
+}
+
+int loss_rows_fast(const LossPlan& p, int* parts, cudaStream_t st) {
+    const LossArgs& a = p.args;
+    const bool bf = a.dtype[kLrX] == CTB_BFLOAT16;
+    if (p.op == kLossPolicy)
+        return bf ? hold_sized<__nv_bfloat16, kLossPolicy>(a, parts, st) : hold_sized<float, kLossPolicy>(a, parts, st);
+    return bf ? hold_sized<__nv_bfloat16, kLossDistill>(a, parts, st) : hold_sized<float, kLossDistill>(a, parts, st);
+}
+
+}  // namespace ctb
