@@ -295,7 +295,11 @@ struct Builder {
             r = 1;
         }
         p.rank = r;
-        for (int d = 0; d < r; ++d) p.div[d] = FastDiv(static_cast<uint64_t>(ext[d] > 0 ? ext[d] : 1));
+        for (int d = 0; d < r; ++d) {
+            p.ext[d] = ext[d];
+            p.div[d] = FastDiv(static_cast<uint64_t>(ext[d] > 0 ? ext[d] : 1));
+        }
+        p.timeouts = wait_timeout_counter();
     }
 };
 
@@ -352,10 +356,12 @@ int check_status(const int32_t* status) {
 }
 
 int run_rows(const LossPlan& p, int* ctas, cudaStream_t st) {
-    if (p.op != kLossToken && loss_rows_fit(p)) return loss_rows_fast(p, ctas, st);
+    if (loss_rows_fit(p.args, p.op != kLossToken)) return loss_rows_fast(p, ctas, st);
     return loss_rows_general(p, ctas, st);
 }
-int run_backward(const LossArgs& a, cudaStream_t st) { return loss_backward_general(a, st); }
+int run_backward(const LossArgs& a, cudaStream_t st) {
+    return loss_rows_fit(a, false) ? loss_backward_fast(a, st) : loss_backward_general(a, st);
+}
 
 int run_total(const double* partials, int n, const ctb_view* out, cudaStream_t st) {
     launch_dependent(loss_total, 1, 256, 0, st, partials, n, out->data, out->dtype);
@@ -369,7 +375,6 @@ int run_loss(Builder& b, const ctb_view* loss, void* scratch, size_t scratch_byt
     if (int rc = check_scratch(scratch, scratch_bytes, need)) return rc;
     b.finish();
     b.a().partials = loss ? static_cast<double*>(scratch) : nullptr;
-    b.a().timeouts = wait_timeout_counter();
     int ctas = 0;
     if (!b.plan.empty)
         if (int rc = run_rows(b.plan, &ctas, st)) return rc;
@@ -590,7 +595,7 @@ int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets, int64_t
             int64_t step = 1;
             for (int d = f.rank - 1; d >= 0; --d) {
                 f.stride[slot][d] = step;
-                step *= static_cast<int64_t>(f.div[d].d);
+                step *= f.ext[d];
             }
         };
         by_row(forward.args, kLrLogp, logp);

@@ -49,7 +49,8 @@ struct LossArgs {
     int32_t dtype[kLossRowViews];
     int64_t stride[kLossRowViews][kMaxDims];  // over the collapsed leading dims
     int rank;                                 // of the collapsed leading dims, >= 1
-    FastDiv div[kMaxDims];                    // divisors = their extents
+    int64_t ext[kMaxDims];                    // their extents
+    FastDiv div[kMaxDims];                    // divisors = the extents
     int64_t rows, cols;
     int64_t x_in, g_in;   // strides along the vocabulary
     int64_t t_in, ti_in;  // strides along the teacher's entries
@@ -326,7 +327,8 @@ constexpr int64_t kLossMaxDistillCols = int64_t(1) << 20;  // columns of a disti
 // the scratch query.
 constexpr int kLossMaxCtas = 148 * 16;
 
-bool loss_rows_fit(const LossPlan& p);                                        // losses_rows.cu
+bool loss_rows_fit(const LossArgs& a, bool held);                             // losses_rows.cu
+int loss_backward_fast(const LossArgs& a, cudaStream_t st);                   // losses_rows.cu
 int loss_rows_fast(const LossPlan& p, int* parts, cudaStream_t st);           // losses_rows.cu
 int loss_rows_general(const LossPlan& p, int* ctas, cudaStream_t st);      // losses_general.cu
 int loss_backward_general(const LossArgs& a, cudaStream_t st);              // losses_general.cu

@@ -14,10 +14,12 @@
 // So a logit costs one exponential, not two, and the exchange of one cluster hides behind the other
 // clusters of the SM and behind the copies of the next rows.
 //
-// Accuracy of the sum. The hardware's 2^t is low by 5.0e-8 on average (measured over t in [-30, -1] on
-// B200; at most 1.5e-7 off), which a sum of thousands does not average out; log2(e)/T as one float32 is
-// off by up to 6e-8 relative, and so is every t. Sums of log-probabilities over a sequence show both. t is
-// therefore corrected with the rest of log2(e)/T (one fused multiply-add), and the joined sum by the mean.
+// Accuracy of the sum. log2(e)/T as one float32 is off by up to 6e-8 relative, and so is every t = d log2(e)/T
+// and with it, one-sidedly, the sum; a sequence's log-probabilities add that up. t is therefore corrected
+// with the rest of log2(e)/T, one fused multiply-add (log-probabilities on B200, [8192, 32768] bfloat16: mean
+// error -6e-9, of the order of the hardware's 2^t). Long sums are taken in two levels, a stage's share of a
+// thread and then the stages, so that small terms are not lost against a grown sum ([2048, 131072] logits of
+// standard deviation 4 in one level: 1.7e-7 low on average).
 #include <map>
 #include <mutex>
 #include <string>
@@ -37,7 +39,6 @@ constexpr int kRowWarp = kConsWarps + 1;
 constexpr int kThreads = kCons + 64;
 constexpr int kMaxCluster = 8;
 constexpr int kBatch = 32;  // rows whose operands the producer reads together, one a lane
-constexpr double kExp2Low = 5.0e-8;
 constexpr int kMaxSmem = 227 * 1024;
 
 // ------------------------------------------------------------------------------------------------
@@ -159,6 +160,15 @@ __device__ __forceinline__ F2 exp_pair(F2 x, F2 minus_m, const ExpConst& k) {
 __device__ __forceinline__ float exp_one(const LossArgs& a, float x, float m) {
     const float d = (x - m) * a.c2_down;
     return exp2_fast(fmaf(d, a.c2_rest, d));
+}
+
+// Gives a stage back after the warp's reads of it. The reads may still be in flight when the next copy is
+// allowed to start, and that copy belongs to another proxy: without the fence, a refill was seen to
+// overtake them (a few packs at the start of a stage, once in some ten thousand stages).
+__device__ __forceinline__ void release_stage(uint64_t* empty, int lane) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -323,10 +333,10 @@ __device__ __forceinline__ int64_t edge_position(const LossArgs& a, int head, in
 }
 
 // ------------------------------------------------------------------------------------------------
-// losses with their gradient (policy, distill)
+// forward passes: log-probabilities alone (token), losses with their gradient (policy, distill)
 
 template <class T, int OP, int E, int CP, int NS, int PER_SM>
-__global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_constant__ LossArgs a) {
+__global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __grid_constant__ LossArgs a) {
     using L = Layout<T, E, CP, NS>;
     using P = PackOf<T>;
     constexpr int VE = L::VE, RP = L::RP;
@@ -562,8 +572,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_const
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     if (pm[k] != -INFINITY)
-                        s += (ps[k] + kExp2Low * (static_cast<double>(ps[k]) - 1.0)) *
-                             (pm[k] == mf ? 1.0 : exp((static_cast<double>(pm[k]) - mf) * a.inv_temp));
+                        s += ps[k] * (pm[k] == mf ? 1.0 : exp((static_cast<double>(pm[k]) - mf) * a.inv_temp));
                     else
                         s += ps[k];  // 0, or the NaN of a bad index
                 }
@@ -575,7 +584,13 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_const
                 c.at_target = c.pad_ = 0.f;
                 double loss = 0.0;
                 bool counts = true;
-                if (OP == kLossPolicy) {
+                if (OP == kLossToken) {
+                    if (rank == 0 && lane == 0) {
+                        const double log_s = log(s);
+                        put_row(a, kLrLogp, row, r.target >= 0 ? (r.xt - m) * a.inv_temp - log_s : quiet_nan());
+                        put_row(a, kLrLse, row, m * a.inv_temp + log_s);
+                    }
+                } else if (OP == kLossPolicy) {
                     const double logp = r.target >= 0 ? (r.xt - m) * a.inv_temp - log(s) : quiet_nan();
                     // three exponentials of the row, one a lane
                     const double v = expm1(lane == 0 ? logp - r.old : lane == 1 ? r.ref - logp : logp);
@@ -628,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_const
                     coefs[par] = c;
                     mbar_arrive(&bars.coef[par]);
                 }
-                if (rank == 0 && lane == 0) {
+                if (OP != kLossToken && rank == 0 && lane == 0) {
                     put_row(a, kLrRowLoss, row, loss);
                     if (counts) total += r.w * loss;
                 }
@@ -679,6 +694,57 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_const
             };
             if (r.w == 0.0) {
                 zeros();
+            } else if constexpr (OP == kLossToken) {
+                // Nothing is written back, so the slice is folded stage by stage, whatever its length: the warp
+                // keeps one maximum, and its sum is brought down to a new one when that grows (a few times a row).
+                float m = warp_max(edge_at >= 0 ? edges[(side * kBatch + i % kBatch) * 16 + t] : -INFINITY);
+                F2 sum = f2(edge_at >= 0 ? exp_one(a, edges[(side * kBatch + i % kBatch) * 16 + t], m == -INFINITY ? 0.f : m) : 0.f, 0.f);
+                for (int p0 = 0; p0 < count; p0 += L::kChunkPacks, ++g) {
+                    const int slot = static_cast<int>(g % NS);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.full[slot], (g / NS) & 1u));
+                    if (!ok) break;
+                    const uint4* st = reinterpret_cast<const uint4*>(sm + static_cast<size_t>(slot) * L::kStage);
+                    uint4 raw[CP];
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < CP; ++u) {
+                        raw[u] = p0 + u * kCons + t < count ? st[u * kCons + t] : P::lowest();
+                        mx = fmaxf(mx, P::max(raw[u]));
+                    }
+                    release_stage(&bars.empty[slot], lane);
+                    mx = warp_max(mx);
+                    if (mx > m) {
+                        const float down = exp_one(a, m, mx);
+                        sum = mul2(sum, f2(down, down));
+                        m = mx;
+                    }
+                    const float at = m == -INFINITY ? 0.f : m;
+                    const F2 minus = f2(-at, -at);
+                    F2 acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
+#pragma unroll
+                    for (int u = 0; u < CP; ++u) {
+                        F2 e[VE / 2];
+                        P::up(raw[u], e);
+#pragma unroll
+                        for (int h = 0; h < VE / 2; h += 2) {
+                            acc0 = add2(acc0, exp_pair(e[h], minus, kc));
+                            acc1 = add2(acc1, exp_pair(e[h + 1], minus, kc));
+                        }
+                    }
+                    sum = add2(sum, add2(acc0, acc1));
+                }
+                float s0, s1;
+                un(sum, s0, s1);
+                const float s = warp_sum(s0 + s1);
+                // the mailbox has two sides: the row before the last one must have been read, everywhere
+                if (ok && live > 0)
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.coef[(live - 1) & 1u], ((live - 1) >> 1) & 1u));
+                if (!ok) break;
+                const int par = static_cast<int>(live & 1u);
+                if (lane < size)
+                    send8(&mail[par * kMaxCluster * kConsWarps + rank * kConsWarps + warp], &bars.mail[par], lane,
+                          static_cast<uint64_t>(__float_as_uint(m)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
+                ++live;
             } else {
                 const int par = static_cast<int>(live & 1u);
                 const uint32_t phase = (live >> 1) & 1u;
@@ -701,8 +767,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_const
                             const int p = ch * L::kChunkPacks + u * kCons + t;
                             raw[ch * CP + u] = ok && p < count ? st[u * kCons + t] : P::lowest();
                         }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bars.empty[slot]);
+                        release_stage(&bars.empty[slot], lane);
                         ++g;
                     } else {
 #pragma unroll
@@ -804,6 +869,197 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_hold(const __grid_const
 }
 
 // ------------------------------------------------------------------------------------------------
+// the backward pass of the log-probabilities
+
+struct PullMeta {
+    long long g_off;
+    float at, shift, a, at_target;  // backward_row
+    int target, zero;
+    int head, packs;
+};
+
+template <class T, int CP, int NS> struct PullLayout {
+    static constexpr int kChunkPacks = CP * kCons;
+    static constexpr size_t kStage = static_cast<size_t>(kChunkPacks) * 16;
+    static constexpr size_t kMeta = NS * kStage;  // PullMeta [2][kBatch]
+    static constexpr size_t kEdge = kMeta + 2 * kBatch * sizeof(PullMeta);
+    static constexpr size_t kBars = kEdge + 2 * kBatch * 16 * sizeof(float);
+    static constexpr size_t kBytes = kBars + (2 * NS + 4) * 8;
+};
+
+// g_j = a exp((x_j - at) / T) 2^shift with numbers that are known when the row begins, so a row is a stream:
+// out of the ring, through one exponential, to memory. CTA (row group, part): the parts of a row are
+// independent. One producer warp, eight consumer warps; bound by the memory.
+template <class T, int CP, int NS, int PER_SM>
+__global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __grid_constant__ LossArgs a, int parts) {
+    using L = PullLayout<T, CP, NS>;
+    using P = PackOf<T>;
+    constexpr int VE = P::VE;
+    extern __shared__ __align__(128) unsigned char sm[];
+    PullMeta* metas = reinterpret_cast<PullMeta*>(sm + L::kMeta);
+    float* edges = reinterpret_cast<float*>(sm + L::kEdge);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::kBars);
+    uint64_t* empty = full + NS;
+    uint64_t* meta_full = empty + NS;
+    uint64_t* meta_empty = meta_full + 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kConsWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&meta_full[i], 1);
+            mbar_init(&meta_empty[i], kConsWarps);
+        }
+        mbar_fence_init();
+    }
+    __syncthreads();
+    dependent_wait();
+    const int rank = static_cast<int>(blockIdx.x) % parts;
+    const int64_t group = blockIdx.x / parts, groups = gridDim.x / parts;
+    const int64_t my_rows = group < a.rows ? (a.rows - group + groups - 1) / groups : 0;
+    const T* X = static_cast<const T*>(a.ptr[kLrX]);
+    bool ok = true;
+    uint32_t g = 0;
+    if (warp == kProducer) {
+        for (int64_t b = 0; b * kBatch < my_rows && ok; ++b) {
+            const int side = static_cast<int>(b & 1);
+            const int n = static_cast<int>(min(static_cast<int64_t>(kBatch), my_rows - b * kBatch));
+            ok = __all_sync(0xffffffffu, mbar_wait(&meta_empty[side], ((b >> 1) & 1) ^ 1));
+            if (!ok) break;
+            int64_t x_off = 0;
+            PullMeta r{};
+            if (lane < n) {
+                const int64_t row = group + (b * kBatch + lane) * groups;
+                x_off = loss_offset(a, kLrX, row);
+                r.g_off = loss_offset(a, kLrGrad, row);
+                const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(X + x_off) & 15)) & 15) / sizeof(T);
+                r.head = static_cast<int>(head < a.cols ? head : a.cols);
+                r.packs = static_cast<int>((a.cols - r.head) / VE);
+                const BackwardRow<float> c = backward_row<T>(a, row, X + x_off);
+                r.at = c.at;
+                r.shift = c.shift;
+                r.a = c.a;
+                r.at_target = c.at_target;
+                r.target = static_cast<int>(c.target);
+                r.zero = c.zero;
+                metas[side * kBatch + lane] = r;
+            }
+            if (rank == 0) {
+                for (int i = 0; i < n; ++i) {
+                    const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
+                    const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
+                    const bool zero = __shfl_sync(0xffffffffu, r.zero, i);
+                    if (lane < 16) {
+                        const int64_t at = edge_position(a, head, packs, VE, lane);
+                        if (at >= 0 && !zero) edges[(side * kBatch + i) * 16 + lane] = LossElem<T>::up(X[off + at]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&meta_full[side]);
+            for (int i = 0; i < n && ok; ++i) {
+                const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
+                const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
+                if (__shfl_sync(0xffffffffu, r.zero, i)) continue;
+                int first, count;
+                slice_of(packs, rank, parts, first, count);
+                const T* src = X + off + head + static_cast<int64_t>(first) * VE;
+                for (int p = 0; p < count; p += L::kChunkPacks, ++g) {
+                    const int slot = static_cast<int>(g % NS);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], ((g / NS) & 1u) ^ 1u));
+                    if (!ok) break;
+                    const uint32_t bytes = static_cast<uint32_t>(min(L::kChunkPacks, count - p)) * 16u;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&full[slot], bytes);
+                        bulk_load(sm + static_cast<size_t>(slot) * L::kStage, src + static_cast<int64_t>(p) * VE, bytes, &full[slot]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (!ok) {
+            if (lane == 0) note_timeout(a.timeouts);
+            for (uint32_t i = g > static_cast<uint32_t>(NS) ? g - NS : 0u; i < g; ++i)
+                mbar_wait(&full[i % NS], (i / NS) & 1u);
+        }
+        return;
+    }
+    const int t = threadIdx.x;
+    const F2 c2 = f2(a.c2, a.c2);
+    for (int64_t i = 0; i < my_rows; ++i) {
+        const int64_t b = i / kBatch;
+        const int side = static_cast<int>(b & 1);
+        if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&meta_full[side], (b >> 1) & 1));
+        if (!ok) break;
+        const PullMeta r = metas[side * kBatch + i % kBatch];
+        int first, count;
+        slice_of(r.packs, rank, parts, first, count);
+        T* gr = static_cast<T*>(a.ptr[kLrGrad]) + r.g_off;
+        T* gs = gr + (r.head + static_cast<int64_t>(first) * VE) * a.g_in;
+        const bool whole = a.g_in == 1 && (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
+        auto put_pack = [&](int p, const uint4& o) {
+            if (whole) {
+                reinterpret_cast<uint4*>(gs)[p] = o;
+            } else {
+                const T* ov = reinterpret_cast<const T*>(&o);
+                T* dst = gs + static_cast<int64_t>(p) * VE * a.g_in;
+#pragma unroll
+                for (int k = 0; k < VE; ++k) dst[k * a.g_in] = ov[k];
+            }
+        };
+        const int64_t edge_at = rank == 0 && t < 16 ? edge_position(a, r.head, r.packs, VE, t) : -1;
+        if (edge_at >= 0) {
+            const float x = edges[(side * kBatch + i % kBatch) * 16 + t];
+            const float v = r.zero ? 0.f : r.target == edge_at ? r.at_target : r.a * row_exp_shifted(a, x, r.at, r.shift);
+            gr[edge_at * a.g_in] = LossElem<T>::down(v);
+        }
+        if (r.zero) {
+            for (int p = t; p < count; p += kCons) put_pack(p, make_uint4(0u, 0u, 0u, 0u));
+        } else {
+            const F2 minus = f2(-r.at, -r.at), shift = f2(r.shift, r.shift), ga = f2(r.a, r.a);
+            const int tb = r.target - r.head;
+            const int tp = r.target >= 0 && tb >= 0 ? tb / VE - first : -1;
+            for (int p0 = 0; p0 < count; p0 += L::kChunkPacks, ++g) {
+                const int slot = static_cast<int>(g % NS);
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (g / NS) & 1u));
+                if (!ok) break;
+                const uint4* st = reinterpret_cast<const uint4*>(sm + static_cast<size_t>(slot) * L::kStage);
+                uint4 raw[CP];
+#pragma unroll
+                for (int u = 0; u < CP; ++u) raw[u] = p0 + u * kCons + t < count ? st[u * kCons + t] : P::lowest();
+                release_stage(&empty[slot], lane);
+#pragma unroll
+                for (int u = 0; u < CP; ++u) {
+                    const int pk = p0 + u * kCons + t;
+                    if (pk >= count) continue;
+                    F2 e[VE / 2];
+                    P::up(raw[u], e);
+#pragma unroll
+                    for (int h = 0; h < VE / 2; ++h) {
+                        float x0, x1;
+                        un(fma2(add2(e[h], minus), c2, shift), x0, x1);
+                        un(mul2(f2(exp2_fast(x0), exp2_fast(x1)), ga), x0, x1);
+                        if (pk == tp) {
+                            if (tb % VE == 2 * h) x0 = r.at_target;
+                            if (tb % VE == 2 * h + 1) x1 = r.at_target;
+                        }
+                        e[h] = f2(x0, x1);
+                    }
+                    put_pack(pk, P::down(e));
+                }
+            }
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0 && (i % kBatch == kBatch - 1 || i + 1 == my_rows)) mbar_arrive(&meta_empty[side]);
+    }
+    if (!ok && lane == 0) note_timeout(a.timeouts);
+    allow_dependents();
+}
+
+// ------------------------------------------------------------------------------------------------
 // host side
 
 template <class... Ps> int launch_cluster(void (*fn)(Ps...), unsigned grid, int cluster, size_t smem, cudaStream_t st,
@@ -832,7 +1088,7 @@ template <class... Ps> int launch_cluster(void (*fn)(Ps...), unsigned grid, int 
 
 // How many clusters of `cluster` CTAs are resident at once on the current device (cached). Also opts the
 // kernel in to its shared memory there.
-int resident_clusters(const void* fn, int cluster, size_t smem, int* out) {
+int resident_blocks(const void* fn, int threads, int cluster, size_t smem, int* out) {
     static std::mutex mu;
     static std::map<std::tuple<const void*, int, int, size_t>, int> cache;
     int dev = 0;
@@ -841,12 +1097,12 @@ int resident_clusters(const void* fn, int cluster, size_t smem, int* out) {
     std::lock_guard<std::mutex> lock(mu);
     auto it = cache.find(key);
     if (it == cache.end()) {
-        // the largest size any call asks for: a smaller one later must not lower it under a concurrent launch
+        // the most that any call may ask for, so that no later call lowers it under a concurrent launch
         if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
             return check_launch("loss rows smem attribute");
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(cluster));
-        cfg.blockDim = dim3(kThreads);
+        cfg.blockDim = dim3(static_cast<unsigned>(threads));
         cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -865,9 +1121,9 @@ int resident_clusters(const void* fn, int cluster, size_t smem, int* out) {
 template <class T, int OP, int E, int CP, int NS, int PER_SM> int hold_typed(const LossArgs& a, int cluster, int* parts, cudaStream_t st) {
     using L = Layout<T, E, CP, NS>;
     const size_t smem = L::bytes(OP, a.top);
-    auto fn = loss_hold<T, OP, E, CP, NS, PER_SM>;
+    auto fn = loss_rows_kernel<T, OP, E, CP, NS, PER_SM>;
     int n = 0;
-    if (int rc = resident_clusters(reinterpret_cast<const void*>(fn), cluster, smem, &n)) return rc;
+    if (int rc = resident_blocks(reinterpret_cast<const void*>(fn), kThreads, cluster, smem, &n)) return rc;
     int64_t clusters = n < a.rows ? n : a.rows;
     if (clusters > kLossMaxCtas) clusters = kLossMaxCtas;
     *parts = static_cast<int>(clusters);
@@ -879,24 +1135,76 @@ template <class T, int OP> int hold_sized(const LossArgs& a, int* parts, cudaStr
     const int64_t packs = a.cols / VE;
     auto need = [&](int e) { return static_cast<int>((packs + static_cast<int64_t>(kCons) * (e / VE) - 1) / (static_cast<int64_t>(kCons) * (e / VE))); };
     if (need(16) <= 1) return hold_typed<T, OP, 16, 16 / VE, 4, 4>(a, 1, parts, st);
-    int c = need(64);
+    const int c = need(64);
     return hold_typed<T, OP, 64, 4, 6, 2>(a, c, parts, st);
+}
+
+// Log-probabilities: a CTA streams a row of any length, so rows are split only where there are too few of
+// them to give every SM two, and never below a stage a CTA.
+template <class T> int stream_sized(const LossArgs& a, int* parts, cudaStream_t st) {
+    const int64_t want = (2 * static_cast<int64_t>(sm_count()) + a.rows - 1) / a.rows;
+    const int64_t stages = a.cols / PackOf<T>::VE / (4 * kCons);
+    int64_t c = want < stages ? want : stages;
+    c = c < 1 ? 1 : c > kMaxCluster ? kMaxCluster : c;
+    return hold_typed<T, kLossToken, 4 * PackOf<T>::VE, 4, 6, 2>(a, static_cast<int>(c), parts, st);
+}
+
+// Whether the gradient lies over the logits: a row's parts then must not run apart, because each of them
+// reads the target's logit, and one of them overwrites it.
+bool in_place(const LossArgs& a) {
+    auto range = [&](int view, int64_t inner, uintptr_t& lo, uintptr_t& hi) {
+        const int64_t size = static_cast<int64_t>(dtype_size(a.dtype[kLrX]));
+        int64_t down = inner < 0 ? (a.cols - 1) * inner : 0, up = inner > 0 ? (a.cols - 1) * inner : 0;
+        for (int d = 0; d < a.rank; ++d) {
+            const int64_t reach = (static_cast<int64_t>(a.ext[d]) - 1) * a.stride[view][d];
+            (reach < 0 ? down : up) += reach;
+        }
+        lo = reinterpret_cast<uintptr_t>(a.ptr[view]) + down * size;
+        hi = reinterpret_cast<uintptr_t>(a.ptr[view]) + (up + 1) * size;
+    };
+    uintptr_t xl, xh, gl, gh;
+    range(kLrX, a.x_in, xl, xh);
+    range(kLrGrad, a.g_in, gl, gh);
+    return xl < gh && gl < xh;
+}
+
+template <class T> int pull_typed(const LossArgs& a, cudaStream_t st) {
+    constexpr int CP = 4, NS = 6, PER_SM = 2;
+    using L = PullLayout<T, CP, NS>;
+    auto fn = loss_pull_kernel<T, CP, NS, PER_SM>;
+    int resident = 0;
+    if (int rc = resident_blocks(reinterpret_cast<const void*>(fn), kCons + 32, 1, L::kBytes, &resident)) return rc;
+    // Parts of a row: stages enough that one CTA's last row is a small share of its work.
+    const int64_t stages = (a.cols / PackOf<T>::VE + L::kChunkPacks - 1) / L::kChunkPacks;
+    int64_t parts = 1;
+    if (!in_place(a)) {
+        while (parts < 16 && parts * 2 <= stages && (parts * 4 < stages || a.rows * parts < 8 * static_cast<int64_t>(resident))) parts *= 2;
+    }
+    int64_t groups = (resident + parts - 1) / parts;
+    if (groups > a.rows) groups = a.rows;
+    launch_dependent(fn, static_cast<unsigned>(groups * parts), kCons + 32, L::kBytes, st, a, static_cast<int>(parts));
+    count_launch();
+    return check_launch("loss backward");
 }
 
 }  // namespace
 
-// Whether the kernels of this file take the call: float32 or bfloat16 rows of unit stride that a cluster
-// can hold.
-bool loss_rows_fit(const LossPlan& p) {
-    const LossArgs& a = p.args;
+// Whether the kernels of this file take the call: float32 or bfloat16 rows of unit stride; for a loss with
+// its gradient, rows that a cluster can hold.
+bool loss_rows_fit(const LossArgs& a, bool held) {
     if (a.dtype[kLrX] != CTB_FLOAT32 && a.dtype[kLrX] != CTB_BFLOAT16) return false;
     if (a.cols > 1 && a.x_in != 1) return false;
-    return a.cols <= static_cast<int64_t>(kMaxCluster) * kCons * 64;
+    return !held || a.cols <= static_cast<int64_t>(kMaxCluster) * kCons * 64;
+}
+
+int loss_backward_fast(const LossArgs& a, cudaStream_t st) {
+    return a.dtype[kLrX] == CTB_BFLOAT16 ? pull_typed<__nv_bfloat16>(a, st) : pull_typed<float>(a, st);
 }
 
 int loss_rows_fast(const LossPlan& p, int* parts, cudaStream_t st) {
     const LossArgs& a = p.args;
     const bool bf = a.dtype[kLrX] == CTB_BFLOAT16;
+    if (p.op == kLossToken) return bf ? stream_sized<__nv_bfloat16>(a, parts, st) : stream_sized<float>(a, parts, st);
     if (p.op == kLossPolicy)
         return bf ? hold_sized<__nv_bfloat16, kLossPolicy>(a, parts, st) : hold_sized<float, kLossPolicy>(a, parts, st);
     return bf ? hold_sized<__nv_bfloat16, kLossDistill>(a, parts, st) : hold_sized<float, kLossDistill>(a, parts, st);

@@ -119,9 +119,12 @@ def test_leading_dims_and_broadcast_operands():
     # permuted leading dims of rank 3, and target strides of their own
     p = dev(rng.normal(0, 2, (2, 3, 4, 65)), torch.float32).permute(2, 0, 1, 3)
     tp = dev(rng.integers(0, 65, (3, 4, 2))).permute(1, 2, 0)
-    got = cb().token_logprobs(p, tp)
-    want = cb().token_logprobs(p.contiguous(), tp.contiguous())
-    assert torch.equal(got.logprobs, want.logprobs)
+    # (rows that start elsewhere on a 16-byte boundary are added in another order: equal within the bound)
+    logp, lt, lse, st = O.token(host(p).reshape(-1, 65), tp.cpu().numpy().reshape(-1), np.ones(24, bool), 1.0, "f32")
+    for q, tq in ((p, tp), (p.contiguous(), tp.contiguous())):
+        got = cb().token_logprobs(q, tq)
+        check(got.logprobs.reshape(-1), (logp, lt), "logprobs")
+        check(got.lse.reshape(-1), (lse, st), "lse")
 
 
 @pytest.mark.parametrize("kind", list(KIND))
@@ -523,6 +526,39 @@ def test_run_together_repeated_on_streams_and_captured(rows, v, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want[k], out))
+
+
+@pytest.mark.parametrize("v,dtype", [(50021, torch.float32), (32768, torch.float32), (100003, torch.bfloat16)])
+def test_every_element_of_many_rows(v, dtype):
+    """Enough rows for every stage of the kernels' rings to be refilled many times: every gradient element
+    against float64, so that one pack read from the wrong copy shows. A pack of another row is off by a
+    factor; the bound is 2^-15 of each element (64 roundings of float32 and more, see losses_oracle), and half a
+    step of bfloat16."""
+    rows = 2000
+    g = torch.Generator(device="cuda")
+    g.manual_seed(v)
+    x = (2 * torch.randn(rows, v, generator=g, device="cuda")).to(dtype)
+    t = torch.randint(v, (rows,), generator=g, device="cuda")
+    up = torch.ones(rows, device="cuda")
+    r = cb().token_logprobs(x, t)
+    pull = cb().token_logprobs_backward(up, x, t, r.logprobs, r.lse)
+    old = r.logprobs.clone()
+    held = cb().policy_loss(x, t, old, -up, weights=up).grad  # ratio r = 1, A = -1: loss r, gradient r (1[t] - p)
+    index = (torch.arange(4, device="cuda") * (v // 4)).expand(rows, 4)
+    top = cb().distill_loss(x, torch.zeros(rows, 4, device="cuda"), index, weights=up).grad
+    half = 2.0 ** -9 if dtype == torch.bfloat16 else 0.0
+    for i in range(0, rows, 200):
+        b = slice(i, i + 200)
+        p = torch.softmax(x[b].double(), -1)
+        want = -p
+        want.scatter_add_(1, t[b, None], torch.ones(200, 1, dtype=torch.float64, device="cuda"))
+        bound = (2.0 ** -15 + 2 * half) * want.abs() + 1e-30
+        assert ((pull[b].double() - want).abs() <= bound).all()
+        assert ((held[b].double() - want).abs() <= bound).all()
+        p[:, index[0]] -= 0.25
+        bound = (2.0 ** -15 + 2 * half) * p.abs() + 1e-30
+        bound[:, index[0]] += 2.0 ** -20
+        assert ((top[b].double() - p).abs() <= bound).all()
 
 
 def test_rows_far_apart():
