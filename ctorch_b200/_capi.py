@@ -56,7 +56,7 @@ def _load() -> ctypes.CDLL:
     P = ctypes.POINTER(View)
     vp, sz, i32, i64, u32, u64 = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64,
                                   ctypes.c_uint32, ctypes.c_uint64)
-    f64 = ctypes.c_double
+    f64, V = ctypes.c_double, ctypes.c_void_p
     sigs = {
         "ctb_abi_version": (i32, []),
         "ctb_last_error": (ctypes.c_char_p, []),
@@ -87,12 +87,13 @@ def _load() -> ctypes.CDLL:
         "ctb_peer_status": (i32, [vp, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)]),
         "ctb_peer_trace": (i32, [vp, ctypes.POINTER(ctypes.c_uint64)]),
         "ctb_chain_rows_allsum": (i32, [i32, i32, P, P, P, P, i32, P, vp, vp, i32, i32, u64, P, vp, u64, vp]),
-        "ctb_loss_scratch_bytes": (sz, [P, i64]),
-        "ctb_token_logprobs": (i32, [P, P, P, f64, P, P, vp, vp]),
-        "ctb_token_logprobs_backward": (i32, [P, P, P, P, P, P, f64, P, vp, vp]),
-        "ctb_distill_loss": (i32, [P, P, P, P, P, f64, f64, P, P, P, vp, vp, sz, vp]),
-        "ctb_policy_loss": (i32, [P, P, P, P, P, P, f64, f64, f64, f64, f64, P, P, P, P, P, vp, vp, sz, vp]),
-        "ctb_preference_loss": (i32, [P, P, i64, P, P, P, P, f64, f64, f64, i32, P, P, P, P, P, vp, vp, sz, vp]),
+        # the losses take their views as packed bytes too (losses.py), so these arguments are untyped pointers
+        "ctb_loss_scratch_bytes": (sz, [V, i64]),
+        "ctb_token_logprobs": (i32, [V, V, V, f64, V, V, vp, vp]),
+        "ctb_token_logprobs_backward": (i32, [V, V, V, V, V, V, f64, V, vp, vp]),
+        "ctb_distill_loss": (i32, [V, V, V, V, V, f64, f64, V, V, V, vp, vp, sz, vp]),
+        "ctb_policy_loss": (i32, [V, V, V, V, V, V, f64, f64, f64, f64, f64, V, V, V, V, V, vp, vp, sz, vp]),
+        "ctb_preference_loss": (i32, [V, V, i64, V, V, V, V, f64, f64, f64, i32, V, V, V, V, V, vp, vp, sz, vp]),
         "ctb_fill_random": (i32, [P, i32, u64, u64, i64, ctypes.c_double, ctypes.c_double, vp]),
         "ctb_debug_plan_elementwise": (i32, [P, ctypes.POINTER(P), i32, i32, ctypes.c_char_p, i32,
                                              ctypes.POINTER(ctypes.c_int),
@@ -150,6 +151,14 @@ def view(t: torch.Tensor | None) -> View | None:
 
 def stream_handle(device: torch.device | None = None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(device: torch.device) -> int:
+    """The current stream of `device` as an integer, without building a torch.cuda.Stream for it (2 us)."""
+    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
 def wait_timeouts() -> int:

@@ -18,37 +18,78 @@ synchronisation is affordable (check_index_status()).
 """
 from __future__ import annotations
 
+import struct
 from collections import namedtuple
+from math import prod
 
 import torch
 
 from . import _capi as C
 from .errors import AliasError, DTypeError, ShapeError
-from .ops import _call, _cuda, _same_view, _scratch, may_overlap
+from .ops import _call, _cuda, _same_view, may_overlap
 
 TokenLogprobs = namedtuple("TokenLogprobs", ["logprobs", "lse"])
 DistillLoss = namedtuple("DistillLoss", ["loss", "row_loss", "grad"])
 PolicyLoss = namedtuple("PolicyLoss", ["loss", "row_loss", "logprobs", "kl", "grad"])
 PreferenceLoss = namedtuple("PreferenceLoss", ["loss", "pair_loss", "rewards", "logprobs", "grad"])
 
-_LOGITS = (torch.float32, torch.float64, torch.bfloat16)
+_SIZE = {torch.float32: 4, torch.float64: 8, torch.bfloat16: 2}
+
+# A loss of a few rows takes the GPU less time than it takes Python to describe its operands, so the views
+# are packed in one go (ctb_view as bytes) and the results of a call share one allocation.
+_VIEW = [struct.Struct(f"<Qii{n}q{8 * (C.MAX_DIMS - n)}x{n}q{8 * (C.MAX_DIMS - n)}x") for n in range(C.MAX_DIMS + 1)]
+
+
+def _view(t):
+    if t is None:
+        return None
+    n = t.dim()
+    if n > C.MAX_DIMS:
+        raise ShapeError(f"ctorch: tensor rank exceeds kMaxRank (got {n})")
+    return _VIEW[n].pack(t.data_ptr(), C.CODE_OF_TORCH[t.dtype], n, *t.shape, *t.stride())
 
 
 def _check(name, logits, *others):
     """Device and dtype checks shared by the losses; returns the device."""
-    dev = _cuda(name, logits, *(t for t in others if t is not None))
-    if logits.dtype not in _LOGITS:
+    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":
+        _cuda(name, logits)  # raises
+    dev = logits.device
+    if logits.dtype not in _SIZE:
         raise DTypeError(f"ctorch::{name}: logits must be float32, float64 or bfloat16 (got {logits.dtype})")
     for t in others:
-        if t is not None and t.dtype not in C.CODE_OF_TORCH:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"ctorch::{name}: expected a tensor")
+        if t.device != dev:
+            _cuda(name, logits, t)  # raises
+        if t.dtype not in C.CODE_OF_TORCH:
             raise DTypeError(f"ctorch::{name}: {t.dtype} is not supported")
     if logits.dim() == 0:
         raise ShapeError(f"ctorch::{name}: logits must have at least one dim (the vocabulary, last)")
     return dev
 
 
-def _result_dtype(logits):
-    return torch.float64 if logits.dtype == torch.float64 else torch.float32
+def _run(name, dev, fn, *args):
+    """fn(*args, stream) on the current stream of the operands' device."""
+    if dev.index == torch.cuda.current_device():
+        _call(fn(*args, C.raw_stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            _call(fn(*args, C.raw_stream(dev)), name)
+
+
+def _results(logits, dev, sizes, scratch=0):
+    """One allocation for scratch (bytes, first) and results of `sizes` elements in the type of a row's
+    results; returns the scratch's address and the results."""
+    dt = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    lead = -(-scratch // (8 if dt == torch.float64 else 4))
+    flat = torch.empty(lead + sum(sizes), dtype=dt, device=dev)
+    return flat.data_ptr(), flat.split_with_sizes([lead, *sizes])[1:]
+
+
+def _shaped(t, rows):
+    return t if len(rows) == 1 else t.view(rows)
 
 
 def _grad_for(name, logits, out, dev):
@@ -64,16 +105,14 @@ def _grad_for(name, logits, out, dev):
         if may_overlap(out, logits) and not _same_view(out, logits):
             raise AliasError(f"ctorch::{name}: the gradient overlaps the logits without being the same view")
         return out
-    shape, size, v = logits.shape, logits.element_size(), logits.shape[-1]
+    if logits.is_contiguous():
+        return torch.empty_like(logits)
+    shape, size, v = logits.shape, _SIZE[logits.dtype], logits.shape[-1]
     if v * size % 16 and logits.dim() > 1 and logits.data_ptr() % 16 == 0 and \
             all(st * size % 16 == 0 for s, st in zip(shape[:-1], logits.stride()) if s > 1):
         pitch = -(-v * size // 128) * 128 // size
         return torch.empty((*shape[:-1], pitch), dtype=logits.dtype, device=dev)[..., :v]
     return torch.empty(shape, dtype=logits.dtype, device=dev)
-
-
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
 
 
 def index_status(device="cuda") -> torch.Tensor:
@@ -102,14 +141,14 @@ def _status(name, status, dev):
 def token_logprobs(logits, targets, mask=None, temperature: float = 1.0, status=None) -> TokenLogprobs:
     """log p[target] and log-sum-exp of each row, with p = softmax(logits / temperature). Forward only:
     token_logprobs_backward() pulls a gradient back through it."""
-    dev = _check("token_logprobs", logits, targets, mask)
-    rows, dt = logits.shape[:-1], _result_dtype(logits)
-    logp = torch.empty(rows, dtype=dt, device=dev)
-    lse = torch.empty(rows, dtype=dt, device=dev)
-    with torch.cuda.device(dev):
-        _call(C.lib.ctb_token_logprobs(C.view(logits), C.view(targets), C.view(mask), temperature, C.view(logp),
-                                       C.view(lse), _status("token_logprobs", status, dev), C.stream_handle(dev)),
-              "token_logprobs")
+    name = "token_logprobs"
+    dev = _check(name, logits, targets, mask)
+    rows = logits.shape[:-1]
+    n = prod(rows)
+    _, (logp, lse) = _results(logits, dev, [n, n])
+    logp, lse = _shaped(logp, rows), _shaped(lse, rows)
+    _run(name, dev, C.lib.ctb_token_logprobs, _view(logits), _view(targets), _view(mask), temperature, _view(logp),
+         _view(lse), _status(name, status, dev))
     return TokenLogprobs(logp, lse)
 
 
@@ -121,19 +160,13 @@ def token_logprobs_backward(grad_logprobs, logits, targets, logprobs, lse, mask=
     name = "token_logprobs_backward"
     dev = _check(name, logits, grad_logprobs, targets, logprobs, lse, mask)
     grad = _grad_for(name, logits, out, dev)
-    with torch.cuda.device(dev):
-        _call(C.lib.ctb_token_logprobs_backward(C.view(grad_logprobs), C.view(logits), C.view(targets),
-                                                C.view(logprobs), C.view(lse), C.view(mask), temperature,
-                                                C.view(grad), _status(name, status, dev), C.stream_handle(dev)), name)
+    _run(name, dev, C.lib.ctb_token_logprobs_backward, _view(grad_logprobs), _view(logits), _view(targets),
+         _view(logprobs), _view(lse), _view(mask), temperature, _view(grad), _status(name, status, dev))
     return grad
 
 
 def _scale(weights, n):
     return 1.0 if weights is not None else 1.0 / max(n, 1)
-
-
-def _rows(logits):
-    return logits.numel() // logits.shape[-1] if logits.shape[-1] else 0
 
 
 def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weights=None, temperature: float = 1.0,
@@ -148,18 +181,16 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weig
     loss, None when grad=False."""
     name = "distill_loss"
     dev = _check(name, logits, teacher_logits, teacher_indices, teacher_lse, weights)
-    dt = _result_dtype(logits)
-    row_loss = torch.empty(logits.shape[:-1], dtype=dt, device=dev)
-    loss = torch.empty((), dtype=dt, device=dev)
+    rows = logits.shape[:-1]
+    n = prod(rows)
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
-    with torch.cuda.device(dev):
-        vx = C.view(logits)
-        need = C.lib.ctb_loss_scratch_bytes(vx, 0)
-        scratch = _scratch(need, dev)
-        _call(C.lib.ctb_distill_loss(vx, C.view(teacher_logits), C.view(teacher_indices), C.view(teacher_lse),
-                                     C.view(weights), _scale(weights, _rows(logits)), temperature, C.view(loss),
-                                     C.view(row_loss), C.view(g), _status(name, status, dev), _ptr(scratch), need,
-                                     C.stream_handle(dev)), name)
+    vx = _view(logits)
+    need = C.lib.ctb_loss_scratch_bytes(vx, 0)
+    scratch, (row_loss, loss) = _results(logits, dev, [n, 1], need)
+    row_loss, loss = _shaped(row_loss, rows), loss.view(())
+    _run(name, dev, C.lib.ctb_distill_loss, vx, _view(teacher_logits), _view(teacher_indices), _view(teacher_lse),
+         _view(weights), _scale(weights, n), temperature, _view(loss), _view(row_loss), _view(g),
+         _status(name, status, dev), scratch, need)
     return DistillLoss(loss, row_loss, g)
 
 
@@ -175,19 +206,16 @@ def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, we
     without ref_logprobs; grad = the gradient of loss, None when grad=False."""
     name = "policy_loss"
     dev = _check(name, logits, targets, old_logprobs, advantages, ref_logprobs, weights)
-    dt, rows = _result_dtype(logits), logits.shape[:-1]
-    row_loss, logp, kl = (torch.empty(rows, dtype=dt, device=dev) for _ in range(3))
-    loss = torch.empty((), dtype=dt, device=dev)
+    rows = logits.shape[:-1]
+    n = prod(rows)
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
-    with torch.cuda.device(dev):
-        vx = C.view(logits)
-        need = C.lib.ctb_loss_scratch_bytes(vx, 0)
-        scratch = _scratch(need, dev)
-        _call(C.lib.ctb_policy_loss(vx, C.view(targets), C.view(old_logprobs), C.view(advantages),
-                                    C.view(ref_logprobs), C.view(weights), _scale(weights, _rows(logits)), clip_low,
-                                    clip_high, kl_coef, temperature, C.view(loss), C.view(row_loss), C.view(logp),
-                                    C.view(kl), C.view(g), _status(name, status, dev), _ptr(scratch), need,
-                                    C.stream_handle(dev)), name)
+    vx = _view(logits)
+    need = C.lib.ctb_loss_scratch_bytes(vx, 0)
+    scratch, (row_loss, logp, kl, loss) = _results(logits, dev, [n, n, n, 1], need)
+    row_loss, logp, kl, loss = _shaped(row_loss, rows), _shaped(logp, rows), _shaped(kl, rows), loss.view(())
+    _run(name, dev, C.lib.ctb_policy_loss, vx, _view(targets), _view(old_logprobs), _view(advantages),
+         _view(ref_logprobs), _view(weights), _scale(weights, n), clip_low, clip_high, kl_coef, temperature,
+         _view(loss), _view(row_loss), _view(logp), _view(kl), _view(g), _status(name, status, dev), scratch, need)
     return PolicyLoss(loss, row_loss, logp, kl, g)
 
 
@@ -208,21 +236,15 @@ def preference_loss(logits, targets, pairs: int, ref_logprobs=None, mask=None, o
     logits are read twice."""
     name = "preference_loss"
     dev = _check(name, logits, targets, ref_logprobs, mask, offsets, weights)
-    dt = _result_dtype(logits)
     if pairs < 1:
         raise ValueError(f"ctorch::{name}: pairs must be at least 1")
-    pair_loss = torch.empty(pairs, dtype=dt, device=dev)
-    rewards = torch.empty(2 * pairs, dtype=dt, device=dev)
-    logp = torch.empty(logits.shape[:-1], dtype=dt, device=dev)
-    loss = torch.empty((), dtype=dt, device=dev)
+    rows = logits.shape[:-1]
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
-    with torch.cuda.device(dev):
-        vx = C.view(logits)
-        need = C.lib.ctb_loss_scratch_bytes(vx, pairs)
-        scratch = _scratch(need, dev)
-        _call(C.lib.ctb_preference_loss(vx, C.view(targets), pairs, C.view(offsets), C.view(ref_logprobs),
-                                        C.view(mask), C.view(weights), _scale(weights, pairs), beta, label_smoothing,
-                                        int(average), C.view(loss), C.view(pair_loss), C.view(rewards), C.view(logp),
-                                        C.view(g), _status(name, status, dev), _ptr(scratch), need,
-                                        C.stream_handle(dev)), name)
+    vx = _view(logits)
+    need = C.lib.ctb_loss_scratch_bytes(vx, pairs)
+    scratch, (logp, pair_loss, rewards, loss) = _results(logits, dev, [prod(rows), pairs, 2 * pairs, 1], need)
+    logp, loss = _shaped(logp, rows), loss.view(())
+    _run(name, dev, C.lib.ctb_preference_loss, vx, _view(targets), pairs, _view(offsets), _view(ref_logprobs),
+         _view(mask), _view(weights), _scale(weights, pairs), beta, label_smoothing, int(average), _view(loss),
+         _view(pair_loss), _view(rewards), _view(logp), _view(g), _status(name, status, dev), scratch, need)
     return PreferenceLoss(loss, pair_loss, rewards, logp, g)
