@@ -187,11 +187,6 @@ template <class Acc> struct RowSum {
 // ------------------------------------------------------------------------------------------------
 // one row's arithmetic
 
-struct RowGrad {
-    double a;     // g_j = a * exp((x_j - m) / T)
-    double loss;  // before its weight
-};
-
 // Log-probability of a target from the row's statistics: (x_t - m) / T - log s.
 __device__ __forceinline__ double target_logp(const LossArgs& a, double xt, double m, double s) {
     return (xt - m) * a.inv_temp - log(s);
@@ -230,28 +225,30 @@ __device__ __forceinline__ void put_empty_row(const LossArgs& a, int64_t row) {
     put_row(a, kLrLse, row, 0.0);
 }
 
-// The row's loss and A, from sums over the teacher's entries: cross = sum q (log q - log p),
-// mass = sum q; s_rest is the part of s outside the entries (tail only). With Q = mass + q_rest,
-//     loss   = cross + q_rest (log q_rest - log p_rest)
-//     dl/dx_j = (Q p_j - q_j) / T on an entry, p_j (Q - q_rest / p_rest) / T elsewhere;
-// renormalised entries have Q = 1 and no rest.
-__device__ __forceinline__ RowGrad distill_row(const LossArgs& a, double w, double s, double s_rest, double cross,
-                                               double mass, bool every_column, double& big_q) {
-    double q_rest = 0.0, loss = cross;
-    big_q = 1.0;
-    RowGrad o;
-    if (a.tail) {
-        if (!every_column && mass < 1.0) q_rest = 1.0 - mass;
-        if (mass != mass) q_rest = mass;
-        big_q = mass + q_rest;
-        if (q_rest != 0.0) loss += q_rest * (log(q_rest) - (log(s_rest) - log(s)));
-        // with no mass outside the entries every other p_j is 0 and so is its gradient
-        o.a = s_rest > 0.0 ? w * a.inv_temp * (big_q / s - q_rest / s_rest) : s_rest == 0.0 ? 0.0 : s_rest;
-    } else {
-        o.a = w * a.inv_temp / s;
-    }
-    o.loss = loss;
-    return o;
+// The loss and A of a distilled row, from sums over the teacher's entries: cross = sum q (log q - log p),
+// mass = sum q; s_rest is the part of s outside the entries. With q' = 1 - mass the rest's share under the
+// teacher, p' = s_rest / s under the student (tail only, else q' = 0) and Q = mass + q',
+//     loss    = cross + q' (log q' - log p')
+//     dl/dx_j = (Q p_j - q_j) / T on an entry, p_j (Q - q' / p') / T elsewhere;
+// renormalised entries have Q = 1.
+__device__ __forceinline__ double rest_of_teacher(const LossArgs& a, double mass, bool every_column) {
+    if (!a.tail || every_column) return 0.0;
+    return mass < 1.0 ? 1.0 - mass : mass == mass ? 0.0 : mass;
+}
+
+__device__ __forceinline__ double distill_slope(const LossArgs& a, double w, double s, double s_rest, double mass,
+                                                bool every_column, double& big_q) {
+    const double q_rest = rest_of_teacher(a, mass, every_column);
+    big_q = a.tail ? mass + q_rest : 1.0;
+    if (!a.tail) return w * a.inv_temp / s;
+    // with no mass outside the entries every other p_j is 0 and so is its gradient
+    return s_rest > 0.0 ? w * a.inv_temp * (big_q / s - q_rest / s_rest) : s_rest == 0.0 ? 0.0 : s_rest;
+}
+
+__device__ __forceinline__ double distill_loss_of(const LossArgs& a, double s, double s_rest, double cross, double mass,
+                                                  bool every_column) {
+    const double q_rest = rest_of_teacher(a, mass, every_column);
+    return q_rest == 0.0 ? cross : cross + q_rest * (log(q_rest) - (log(s_rest) - log(s)));
 }
 
 // What the backward pass needs of a row: p_j = exp((x_j - at) / T) 2^shift, g_j = a p_j.

@@ -179,8 +179,9 @@ template <class T, int OP> __global__ void __launch_bounds__(kThreads) loss_rows
             cross = cta_sum(cross, sm_d);
             mass = cta_sum(mass, sm_d);
             double big_q;
-            RowGrad o = distill_row(a, w, s, s_rest, cross, mass, entries == a.cols, big_q);
-            if (bad || !(s > 0.0)) o.a = o.loss = quiet_nan();
+            double slope = distill_slope(a, w, s, s_rest, mass, entries == a.cols, big_q);
+            double loss = distill_loss_of(a, s, s_rest, cross, mass, entries == a.cols);
+            if (bad || !(s > 0.0)) slope = loss = quiet_nan();
             for (int k = threadIdx.x; k < a.top; k += kThreads) {
                 const double z = load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
                 if (z == -INFINITY || bad) continue;
@@ -188,9 +189,9 @@ template <class T, int OP> __global__ void __launch_bounds__(kThreads) loss_rows
                 fix[k] = static_cast<Acc>(w * a.inv_temp * (big_q * exp(target_logp(a, E::up(x[j * a.x_in]), m, s)) - exp(z - tl)));
             }
             if (threadIdx.x == 0) {
-                put_row(a, kLrRowLoss, row, o.loss);
-                total += w * o.loss;
-                sh[0] = o.a;
+                put_row(a, kLrRowLoss, row, loss);
+                total += w * loss;
+                sh[0] = slope;
             }
         }
         if (!g && OP != kLossDistill) {

@@ -38,6 +38,7 @@ constexpr int kProducer = kConsWarps;  // warp numbers
 constexpr int kRowWarp = kConsWarps + 1;
 constexpr int kThreads = kCons + 64;
 constexpr int kMaxCluster = 8;
+constexpr int kAhead = 4;   // teacher entries a lane of the producer fetches a row ahead
 constexpr int kBatch = 32;  // rows whose operands the producer reads together, one a lane
 constexpr int kMaxSmem = 227 * 1024;
 
@@ -165,9 +166,12 @@ __device__ __forceinline__ float exp_one(const LossArgs& a, float x, float m) {
 // Gives a stage back after the warp's reads of it. The reads may still be in flight when the next copy is
 // allowed to start, and that copy belongs to another proxy: without the fence, a refill was seen to
 // overtake them (a few packs at the start of a stage, once in some ten thousand stages).
-__device__ __forceinline__ void release_stage(uint64_t* empty, int lane) {
+__device__ __forceinline__ void release_fence() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
+}
+__device__ __forceinline__ void release_stage(uint64_t* empty, int lane) {
+    release_fence();
     if (lane == 0) mbar_arrive(empty);
 }
 
@@ -240,6 +244,7 @@ struct RowMeta {
     double w;            // 0: the row does not count
     double xt;           // target's logit
     double old, adv, ref;
+    double exp_old, exp_ref;  // exp(-old), exp(ref)
     long long row, g_off;
     int target;          // -1: bad
     int head, packs;     // elements before the first whole 16-byte pack, whole packs
@@ -249,9 +254,10 @@ struct RowMeta {
 // What the producer knows of a teacher's list.
 struct ListInfo {
     double q_logq, q_x, ref, mass;  // sums of q log q, q (x - ref) and q over the entries
+    double named;                   // sum of exp((x - x_max) / T) over them
     float x_max;
     int count, bad;
-    uint32_t edge_named;  // which of the 16 edge elements the teacher names
+    uint32_t edge_named;  // which of the 16 edge elements the teacher names (the producer's own)
 };
 
 struct Coef {
@@ -269,10 +275,10 @@ template <class T, int E, int CP, int NS> struct Layout {
     static constexpr size_t kEdge = kMeta + 2 * kBatch * sizeof(RowMeta);      // float [2][kBatch][16]
     static constexpr size_t kCoef = kEdge + 2 * kBatch * 16 * sizeof(float);   // Coef [2]
     static constexpr size_t kBars = kCoef + 2 * sizeof(Coef);
-    static constexpr int kNumBars = 2 * NS + 2 + 2 + 2 + 2 + 2 + 2;
+    static constexpr int kNumBars = 2 * NS + 14;
     static constexpr size_t kList = kBars + kNumBars * 8;              // ListInfo [2]
-    static constexpr size_t kBits = (kList + 2 * sizeof(ListInfo) + 15) / 16 * 16;  // bytes [2][kCons * RP]
-    static constexpr size_t kEntries = kBits + 2 * kCons * RP;         // per side: int idx[K], float x[K], float q[K]
+    static constexpr size_t kBits = (kList + 2 * sizeof(ListInfo) + 15) / 16 * 16;  // bytes [kCons * RP]
+    static constexpr size_t kEntries = kBits + kCons * RP;         // per side: int idx[K], float x[K], float q[K]
     static constexpr size_t bytes(int op, int top) {
         return op == kLossDistill ? kEntries + static_cast<size_t>(2) * 12 * top : kList;
     }
@@ -284,6 +290,7 @@ template <int NS> struct Bars {
     uint64_t meta_full[2], meta_empty[2];
     uint64_t list_full[2], list_empty[2];
     uint64_t mail[2], coef[2];
+    uint64_t done[2];  // the consumers have written the row's slice
 };
 
 // Rank r's share of a row's packs.
@@ -307,13 +314,17 @@ template <class T, int OP> __device__ __forceinline__ RowMeta read_meta(const Lo
     r.head = static_cast<int>(head < a.cols ? head : a.cols);
     r.packs = static_cast<int>((a.cols - r.head) / PackOf<T>::VE);
     r.target = -1;
-    r.xt = r.old = r.adv = r.ref = 0.0;
+    r.xt = r.old = r.adv = r.ref = r.exp_old = r.exp_ref = 0.0;
     if (OP != kLossDistill && r.w != 0.0) {
         const int64_t t = load_index(a.ptr[kLrTarget], a.dtype[kLrTarget], loss_offset(a, kLrTarget, row));
         if (OP == kLossPolicy) {
             r.old = row_real(a, kLrOld, row);
             r.adv = row_real(a, kLrAdv, row);
-            if (a.ptr[kLrRef]) r.ref = row_real(a, kLrRef, row);
+            r.exp_old = exp(-r.old);
+            if (a.ptr[kLrRef]) {
+                r.ref = row_real(a, kLrRef, row);
+                r.exp_ref = exp(r.ref);
+            }
         }
         if (t >= 0 && t < a.cols) {
             r.target = static_cast<int>(t);
@@ -363,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             mbar_init(&bars.list_empty[i], kConsWarps + 1);
             mbar_init(&bars.mail[i], 1);
             mbar_init(&bars.coef[i], 1);
+            mbar_init(&bars.done[i], kConsWarps);
         }
         mbar_fence_init();
         for (int i = 0; i < 2; ++i) mbar_arrive_expect_tx(&bars.mail[i], mail_bytes);
@@ -395,62 +407,78 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 __syncwarp();
             }
         };
-        auto read_list = [&](int64_t row, int64_t x_off, int head, int packs, double w) {
-            (void)w;
+        // The teacher's list of one row. Entries lane, lane + 32, ... of the first kAhead * 32 are fetched a row
+        // ahead into registers (z, at); longer lists are read in place.
+        double z[kAhead];
+        int64_t at[kAhead];
+        auto scaled = [&](int64_t t_off, int k) {
+            return load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
+        };
+        auto fetch_list = [&](int64_t row) {
+            const int64_t t_off = loss_offset(a, kLrTeacher, row), ti_off = loss_offset(a, kLrTeacherIdx, row);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int k = lane + 32 * u;
+                z[u] = k < a.top ? scaled(t_off, k) : -INFINITY;
+                at[u] = k < a.top ? load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in) : -1;
+            }
+        };
+        // Joins the list of the row whose stages are g0 to g1 with the row's logits: sums for the row warp, and -inf
+        // in place of the named logits, so that the consumers' sum is that of the others. `next`: the row to
+        // fetch ahead, or -1.
+        auto read_list = [&](int64_t row, int64_t next, int64_t x_off, int head, int packs, uint32_t g0, uint32_t g1,
+                             float* edge) {
             const int side = static_cast<int>(live & 1u);
             ok = __all_sync(0xffffffffu, mbar_wait(&bars.list_empty[side], ((live >> 1) & 1u) ^ 1u));
             if (!ok) return;
             int* e_idx = reinterpret_cast<int*>(sm + L::kEntries + static_cast<size_t>(side) * 12 * a.top);
             float* e_x = reinterpret_cast<float*>(e_idx + a.top);
             float* e_q = e_x + a.top;
-            uint4* b16 = reinterpret_cast<uint4*>(bits + side * kCons * RP);
-            for (int i = lane; i < kCons * RP / 16; i += 32) b16[i] = make_uint4(0u, 0u, 0u, 0u);
-            ListInfo& li = lists[side];
-            if (lane == 0) li.edge_named = 0u;
-            __syncwarp();
-            int first, count;
-            slice_of(packs, rank, size, first, count);
             const T* x = static_cast<const T*>(a.ptr[kLrX]) + x_off;
             const int64_t t_off = loss_offset(a, kLrTeacher, row), ti_off = loss_offset(a, kLrTeacherIdx, row);
-            auto scaled = [&](int k) {
-                return load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
+            double zr[kAhead];
+            int jr[kAhead];
+            float xr[kAhead];
+            int bad = 0;
+            // a valid entry's column, -1 for padding and for an index outside the row
+            auto column = [&](double zk, int64_t k) -> int {
+                if (zk == -INFINITY) return -1;
+                if (k >= 0 && k < a.cols) return static_cast<int>(k);
+                bad = 1;
+                if (rank == 0) note_bad_index(a, k);
+                return -1;
             };
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                zr[u] = z[u];
+                jr[u] = column(zr[u], at[u]);
+                xr[u] = jr[u] >= 0 ? LossElem<T>::up(x[jr[u]]) : -INFINITY;
+            }
+            if (next >= 0) fetch_list(next);
+            // which columns of this CTA's slice are named already
+            uint4* b16 = reinterpret_cast<uint4*>(bits);
+            for (int i = lane; i < kCons * RP / 16; i += 32) b16[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (lane == 0) lists[side].edge_named = 0u;
             double mx = -INFINITY;
             float x_max = -INFINITY;
-            int entries = 0, bad = 0;
-            for (int k = lane; k < a.top; k += 32) {
-                const double z = scaled(k);
-                int j = -1;
-                float xk = -INFINITY;
-                if (z != -INFINITY) {
-                    ++entries;
-                    mx = fmax(mx, z);
-                    const int64_t at = load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in);
-                    if (at < 0 || at >= a.cols) {
-                        bad = 1;
-                        if (rank == 0) note_bad_index(a, at);
-                    } else {
-                        j = static_cast<int>(at);
-                        xk = LossElem<T>::up(x[j]);
-                        x_max = fmaxf(x_max, xk);
-                        const int b = j - head;
-                        uint32_t was = 0u, bit = 1u;
-                        if (b >= 0 && b < packs * VE) {
-                            const int p = b / VE - first;
-                            if (p >= 0 && p < count) {
-                                bit = 1u << ((p & 3) * 8 + b % VE);
-                                was = atomicOr(reinterpret_cast<uint32_t*>(bits + side * kCons * RP) + (p >> 2), bit);
-                            }
-                        } else if (rank == 0) {
-                            bit = 1u << (b < 0 ? j : 8 + b - packs * VE);
-                            was = atomicOr(&li.edge_named, bit);
-                        }
-                        if (was & bit) {
-                            bad = 1;
-                            note_bad_index(a, at);
-                        }
-                    }
+            int entries = 0;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                mx = fmax(mx, zr[u]);
+                x_max = fmaxf(x_max, xr[u]);
+                entries += zr[u] != -INFINITY;
+                if (lane + 32 * u < a.top) {
+                    e_idx[lane + 32 * u] = jr[u];
+                    e_x[lane + 32 * u] = xr[u];
                 }
+            }
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
+                const double zk = scaled(t_off, k);
+                const int j = column(zk, load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in));
+                const float xk = j >= 0 ? LossElem<T>::up(x[j]) : -INFINITY;
+                mx = fmax(mx, zk);
+                x_max = fmaxf(x_max, xk);
+                entries += zk != -INFINITY;
                 e_idx[k] = j;
                 e_x[k] = xk;
             }
@@ -458,35 +486,84 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             for (int d = 16; d >= 1; d >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             x_max = warp_max(x_max);
             entries = __reduce_add_sync(0xffffffffu, entries);
-            bad = __any_sync(0xffffffffu, bad);
-            double lse = 0.0;
-            if (a.tail) {
-                lse = entries ? row_real(a, kLrTeacherLse, row) : 0.0;
-            } else if (entries) {
-                double s = 0.0;
-                for (int k = lane; k < a.top; k += 32) s += exp(scaled(k) - mx);
-                lse = mx + log(warp_sum(s));
+            // q = weight * exp(z - base): weight 1 and the teacher's own log-sum-exp, or 1 / sum and the maximum
+            double base = mx, log_sum = 0.0, weight = 1.0;
+            double er[kAhead];
+            if (a.tail && entries) base = row_real(a, kLrTeacherLse, row);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) er[u] = zr[u] == -INFINITY ? 0.0 : exp(zr[u] - base);
+            if (!a.tail) {
+                double sum = 0.0;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) sum += er[u];
+                for (int k = lane + 32 * kAhead; k < a.top; k += 32) sum += exp(scaled(t_off, k) - base);
+                sum = warp_sum(sum);
+                weight = 1.0 / sum;
+                log_sum = log(sum);
             }
             const double ref = x_max == -INFINITY ? 0.0 : static_cast<double>(x_max);
-            double mass = 0.0, q_logq = 0.0, q_x = 0.0;
-            for (int k = lane; k < a.top; k += 32) {
-                const double z = scaled(k), q = z == -INFINITY ? 0.0 : exp(z - lse);
-                if (q != 0.0) {
-                    mass += q;
-                    q_logq += q * (z - lse);
-                    q_x += q * (static_cast<double>(e_x[k]) - ref);
+            double sums[4] = {0.0, 0.0, 0.0, 0.0};  // mass, q log q, q (x - ref), exp((x - x_max) / T)
+            auto add = [&](int k, double zk, double ek, int j, float xk) {
+                const double q = weight * ek;
+                if (q != 0.0) {  // NaN too
+                    sums[0] += q;
+                    sums[1] += q * (zk - base - log_sum);
+                    sums[2] += q * (static_cast<double>(xk) - ref);
                 }
+                if (j >= 0 && xk != -INFINITY) sums[3] += exp_one(a, xk, x_max);
                 e_q[k] = static_cast<float>(q);
+            };
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (lane + 32 * u < a.top) add(lane + 32 * u, zr[u], er[u], jr[u], xr[u]);
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
+                const double zk = scaled(t_off, k);
+                add(k, zk, zk == -INFINITY ? 0.0 : exp(zk - base), e_idx[k], e_x[k]);
             }
-            mass = warp_sum(mass);
-            q_logq = warp_sum(q_logq);
-            q_x = warp_sum(q_x);
-            __syncwarp();
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) sums[v] += __shfl_xor_sync(0xffffffffu, sums[v], d);
+            // the row's stages have landed: take the named logits out
+            for (uint32_t k = g0; k != g1; ++k) ok = mbar_wait(&bars.full[k % NS], (k / NS) & 1u) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            int first, count;
+            slice_of(packs, rank, size, first, count);
+            for (int k = lane; k < a.top; k += 32) {
+                const int j = e_idx[k];
+                if (j < 0) continue;
+                const int b = j - head;
+                uint32_t was = 0u, bit = 1u;
+                if (b >= 0 && b < packs * VE) {
+                    const int p = b / VE - first;
+                    if (p >= 0 && p < count) {
+                        bit = 1u << ((p & 3) * 8 + b % VE);
+                        was = atomicOr(reinterpret_cast<uint32_t*>(bits) + (p >> 2), bit);
+                        const uint32_t slot = (g0 + static_cast<uint32_t>(p / L::kChunkPacks)) % NS;
+                        T* st = reinterpret_cast<T*>(sm + slot * L::kStage) + (p % L::kChunkPacks) * VE + b % VE;
+                        *st = LossElem<T>::down(-INFINITY);
+                    }
+                } else if (rank == 0) {
+                    const int l = b < 0 ? j : 8 + b - packs * VE;
+                    bit = 1u << l;
+                    was = atomicOr(&lists[side].edge_named, bit);
+                    edge[l] = -INFINITY;
+                }
+                if (was & bit) {
+                    bad = 1;
+                    note_bad_index(a, j);
+                }
+            }
+            bad = __any_sync(0xffffffffu, bad);
+            release_fence();  // a later copy into these stages comes after these stores
             if (lane == 0) {
-                li.q_logq = q_logq;
-                li.q_x = q_x;
+                ListInfo& li = lists[side];
+                li.mass = sums[0];
+                li.q_logq = sums[1];
+                li.q_x = sums[2];
+                li.named = sums[3];
                 li.ref = ref;
-                li.mass = mass;
                 li.x_max = x_max;
                 li.count = entries;
                 li.bad = bad;
@@ -519,13 +596,35 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.meta_full[side]);
-            for (int i = 0; i < n && ok; ++i) {
-                const double w = __shfl_sync(0xffffffffu, r.w, i);
-                if (w == 0.0) continue;
+            const uint32_t counting = __ballot_sync(0xffffffffu, r.w != 0.0);
+            // A list is joined with its row once that has landed, so the next row's copies are started first,
+            // where the ring holds two rows.
+            constexpr bool kTwo = OP == kLossDistill && NS >= 2 * L::NCH;
+            uint32_t g_next = g;
+            bool issued = false;
+            for (uint32_t todo = counting; todo && ok; todo &= todo - 1) {
+                const int i = __ffs(todo) - 1;
+                const uint32_t later = todo & (todo - 1);
+                const int i2 = later ? __ffs(later) - 1 : i;
                 const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
                 const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
-                issue(off, head, packs);
-                if (OP == kLossDistill && ok) read_list(__shfl_sync(0xffffffffu, r.row, i), off, head, packs, w);
+                uint32_t g0 = g_next, g1 = g;
+                if (!issued) {
+                    g0 = g;
+                    issue(off, head, packs);
+                    g1 = g;
+                }
+                if (OP == kLossDistill && ok) {
+                    const int64_t row = __shfl_sync(0xffffffffu, r.row, i), next = __shfl_sync(0xffffffffu, r.row, i2);
+                    if (todo == counting) fetch_list(row);  // the batch's first: nobody fetched it ahead
+                    issued = kTwo && later;
+                    if (issued) {
+                        g_next = g;
+                        issue(__shfl_sync(0xffffffffu, x_off, i2), __shfl_sync(0xffffffffu, r.head, i2),
+                              __shfl_sync(0xffffffffu, r.packs, i2));
+                    }
+                    if (ok) read_list(row, later ? next : -1, off, head, packs, g0, g1, edges + (side * kBatch + i) * 16);
+                }
                 ++live;
             }
         }
@@ -568,84 +667,109 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 float mf = warp_max(fmaxf(pm[0], pm[1]));
                 const ListInfo* li = &lists[par];
                 if (OP == kLossDistill) mf = fmaxf(mf, li->x_max);
-                double s = 0.0;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (pm[k] != -INFINITY)
-                        s += ps[k] * (pm[k] == mf ? 1.0 : exp((static_cast<double>(pm[k]) - mf) * a.inv_temp));
-                    else
-                        s += ps[k];  // 0, or the NaN of a bad index
-                }
-                s = warp_sum(s);
-                if (mf == INFINITY) s = quiet_nan();
                 const double m = mf;
-                Coef c;
-                c.m = mf;
-                c.at_target = c.pad_ = 0.f;
-                double loss = 0.0;
-                bool counts = true;
-                if (OP == kLossToken) {
-                    if (rank == 0 && lane == 0) {
-                        const double log_s = log(s);
-                        put_row(a, kLrLogp, row, r.target >= 0 ? (r.xt - m) * a.inv_temp - log_s : quiet_nan());
-                        put_row(a, kLrLse, row, m * a.inv_temp + log_s);
-                    }
-                } else if (OP == kLossPolicy) {
-                    const double logp = r.target >= 0 ? (r.xt - m) * a.inv_temp - log(s) : quiet_nan();
-                    // three exponentials of the row, one a lane
-                    const double v = expm1(lane == 0 ? logp - r.old : lane == 1 ? r.ref - logp : logp);
-                    const double e_old = __shfl_sync(0xffffffffu, v, 0), e_ref = __shfl_sync(0xffffffffu, v, 1),
-                                 e_logp = __shfl_sync(0xffffffffu, v, 2);
-                    PolicyTerms t = policy_terms(a, r.w, r.adv, 1.0 + e_old, r.ref - logp, e_ref);
-                    c.a = static_cast<float>(-t.g / s);
-                    c.at_target = static_cast<float>(-t.g * e_logp);
-                    loss = t.loss;
-                    if (rank == 0 && lane == 0) {
-                        put_row(a, kLrLogp, row, logp);
-                        put_row(a, kLrKl, row, t.kl);
-                    }
-                } else {
-                    const int* e_idx = reinterpret_cast<const int*>(sm + L::kEntries + static_cast<size_t>(par) * 12 * a.top);
-                    const float* e_x = reinterpret_cast<const float*>(e_idx + a.top);
-                    const float* e_q = e_x + a.top;
-                    counts = li->count > 0;
-                    const double s_rest = s;
-                    float named = 0.f;
-                    for (int k = lane; k < a.top; k += 32)
-                        if (e_idx[k] >= 0) named += exp_one(a, e_x[k], mf);
-                    s = s_rest + warp_sum(static_cast<double>(named));
-                    const double log_s = log(s);
-                    const double cross = li->q_logq - a.inv_temp * (li->q_x + (li->ref - m) * li->mass) + li->mass * log_s;
-                    double big_q;
-                    RowGrad o = distill_row(a, r.w, s, s_rest, cross, li->mass, li->count == a.cols, big_q);
-                    if (!(s > 0.0)) o.a = o.loss = quiet_nan();
-                    c.a = counts ? static_cast<float>(o.a) : 0.f;
-                    loss = counts ? o.loss : 0.0;
-                    T* G = static_cast<T*>(a.ptr[kLrGrad]);
-                    if (G && counts) {
-                        T* gr = G + r.g_off;
-                        int first, count;
-                        slice_of(r.packs, rank, size, first, count);
-                        const float scale = static_cast<float>(r.w * a.inv_temp), p_scale = static_cast<float>(big_q / s);
-                        // a bad row is NaN throughout: its named columns too, whoever found it
-                        const float poison = c.a == c.a ? 0.f : c.a;
-                        for (int k = lane; k < a.top; k += 32) {
-                            const int j = e_idx[k];
-                            if (j < 0) continue;
-                            const int body = j - r.head;
-                            const bool mine = body >= 0 && body < r.packs * VE ? body / VE >= first && body / VE < first + count
-                                                                               : rank == 0;
-                            if (mine) gr[j * a.g_in] = LossElem<T>::down(scale * (exp_one(a, e_x[k], mf) * p_scale - e_q[k]) + poison);
+                if constexpr (OP == kLossToken) {
+                    // nobody waits for these: joined in float64
+                    double s = 0.0;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        s += pm[k] == -INFINITY ? static_cast<double>(ps[k])  // 0, or NaN
+                                                : ps[k] * (pm[k] == mf ? 1.0 : exp((static_cast<double>(pm[k]) - mf) * a.inv_temp));
+                    s = warp_sum(s);
+                    if (mf == INFINITY) s = quiet_nan();
+                    if (lane == 0) {
+                        mbar_arrive(&bars.coef[par]);
+                        if (rank == 0) {
+                            const double log_s = log(s);
+                            put_row(a, kLrLogp, row, r.target >= 0 ? (r.xt - m) * a.inv_temp - log_s : quiet_nan());
+                            put_row(a, kLrLse, row, m * a.inv_temp + log_s);
                         }
                     }
-                }
-                if (lane == 0) {
-                    coefs[par] = c;
-                    mbar_arrive(&bars.coef[par]);
-                }
-                if (OP != kLossToken && rank == 0 && lane == 0) {
-                    put_row(a, kLrRowLoss, row, loss);
-                    if (counts) total += r.w * loss;
+                } else {
+                    // Every consumer of the cluster waits from here to the coefficient, so only what it needs is
+                    // computed first: no logarithm, and the row's losses after it is published.
+                    float part = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        part += pm[k] == -INFINITY ? ps[k] : ps[k] * (pm[k] == mf ? 1.f : exp_one(a, pm[k], mf));
+                    Coef c;
+                    c.m = mf;
+                    c.at_target = c.pad_ = 0.f;
+                    auto publish = [&]() {
+                        if (lane == 0) {
+                            coefs[par] = c;
+                            mbar_arrive(&bars.coef[par]);
+                        }
+                    };
+                    if constexpr (OP == kLossPolicy) {
+                        // s relative to the target's logit instead of the maximum: r = exp(-old) / s', p_t = 1 / s'
+                        const double lift = exp((m - r.xt) * a.inv_temp);
+                        const double s = mf == INFINITY ? quiet_nan() : static_cast<double>(warp_sum(part));
+                        const double st = s * lift;
+                        double ratio = r.exp_old / st, ed = r.exp_ref * st - 1.0, rest = 1.0 - 1.0 / st, logp = 0.0;
+                        const bool far = !(st < 1e300 && r.exp_old < 1e300 && r.exp_old > 1e-300 && r.exp_ref < 1e300) || r.target < 0;
+                        if (far) {  // numbers outside these forms' range: through the logarithm
+                            logp = r.target >= 0 ? (r.xt - m) * a.inv_temp - log(s) : quiet_nan();
+                            ratio = exp(logp - r.old);
+                            ed = expm1(r.ref - logp);
+                            rest = -expm1(logp);
+                        }
+                        const double g = policy_terms(a, r.w, r.adv, ratio, 0.0, ed).g;
+                        c.a = -static_cast<float>(g) / static_cast<float>(s);
+                        c.at_target = static_cast<float>(g * rest);
+                        publish();
+                        if (rank == 0 && lane == 0) {
+                            if (!far) logp = (r.xt - m) * a.inv_temp - log(s);
+                            const double d = r.ref - logp;
+                            const PolicyTerms t = policy_terms(a, r.w, r.adv, ratio, d, a.ptr[kLrRef] ? expm1(d) : 0.0);
+                            put_row(a, kLrLogp, row, logp);
+                            put_row(a, kLrKl, row, t.kl);
+                            put_row(a, kLrRowLoss, row, t.loss);
+                            total += r.w * t.loss;
+                        }
+                    } else {
+                        const double s_rest = mf == INFINITY ? quiet_nan() : static_cast<double>(warp_sum(part));
+                        const double s = s_rest + (li->count ? li->named * exp_one(a, li->x_max, mf) : 0.0);
+                        const bool counts = li->count > 0;
+                        double big_q;
+                        c.a = static_cast<float>(distill_slope(a, r.w, s, s_rest, li->mass, li->count == a.cols, big_q));
+                        if (!(s > 0.0)) c.a = NAN;
+                        if (!counts) c.a = 0.f;
+                        publish();
+                        if (rank == 0 && lane == 0) {
+                            const double log_s = log(s);
+                            const double cross = li->q_logq - a.inv_temp * (li->q_x + (li->ref - m) * li->mass) + li->mass * log_s;
+                            double loss = distill_loss_of(a, s, s_rest, cross, li->mass, li->count == a.cols);
+                            if (!(s > 0.0)) loss = quiet_nan();
+                            if (!counts) loss = 0.0;
+                            put_row(a, kLrRowLoss, row, loss);
+                            if (counts) total += r.w * loss;
+                        }
+                        __syncwarp();
+                        // The named elements of this CTA's slice, over what the consumers have written there.
+                        T* G = static_cast<T*>(a.ptr[kLrGrad]);
+                        if (G && counts) {
+                            ok = __all_sync(0xffffffffu, mbar_wait(&bars.done[par], phase));
+                            if (!ok) break;
+                            T* gr = G + r.g_off;
+                            int first, count;
+                            slice_of(r.packs, rank, size, first, count);
+                            const int* e_idx = reinterpret_cast<const int*>(sm + L::kEntries + static_cast<size_t>(par) * 12 * a.top);
+                            const float* e_x = reinterpret_cast<const float*>(e_idx + a.top);
+                            const float* e_q = e_x + a.top;
+                            const float scale = static_cast<float>(r.w * a.inv_temp), p_scale = static_cast<float>(big_q / s);
+                            // a bad row is NaN throughout: its named columns too, whoever found it
+                            const float poison = c.a == c.a ? 0.f : c.a;
+                            for (int k = lane; k < a.top; k += 32) {
+                                const int j = e_idx[k];
+                                if (j < 0) continue;
+                                const int body = j - r.head;
+                                const bool mine = body >= 0 && body < r.packs * VE ? body / VE >= first && body / VE < first + count
+                                                                                   : rank == 0;
+                                if (mine) gr[j * a.g_in] = LossElem<T>::down(scale * (exp_one(a, e_x[k], mf) * p_scale - e_q[k]) + poison);
+                            }
+                        }
+                    }
                 }
                 __syncwarp();
                 if (OP == kLossDistill && lane == 0) mbar_arrive(&bars.list_empty[par]);
@@ -674,22 +798,21 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             // elsewhere (which costs eight times the store instructions, and takes any stride).
             T* gs = gr + (r.head + static_cast<int64_t>(first) * VE) * a.g_in;
             const bool whole = a.g_in == 1 && (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
-            auto put_pack = [&](int p, const uint4& o, uint32_t skip) {
-                if (whole && skip == 0u) {
+            auto put_pack = [&](int p, const uint4& o) {
+                if (whole) {
                     reinterpret_cast<uint4*>(gs)[p] = o;
                 } else {
                     const T* ov = reinterpret_cast<const T*>(&o);
                     T* dst = gs + static_cast<int64_t>(p) * VE * a.g_in;
 #pragma unroll
-                    for (int k = 0; k < VE; ++k)
-                        if (!(skip >> k & 1u)) dst[k * a.g_in] = ov[k];
+                    for (int k = 0; k < VE; ++k) dst[k * a.g_in] = ov[k];
                 }
             };
             const bool edge = rank == 0 && t < 16;
             const int64_t edge_at = edge ? edge_position(a, r.head, r.packs, VE, t) : -1;
             auto zeros = [&]() {
                 if (!gr) return;
-                for (int p = t; p < count; p += kCons) put_pack(p, make_uint4(0u, 0u, 0u, 0u), 0u);
+                for (int p = t; p < count; p += kCons) put_pack(p, make_uint4(0u, 0u, 0u, 0u));
                 if (edge_at >= 0) gr[edge_at * a.g_in] = LossElem<T>::down(0.f);
             };
             if (r.w == 0.0) {
@@ -752,7 +875,6 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                     ok = __all_sync(0xffffffffu, mbar_wait(&bars.list_full[par], phase));
                     if (!ok) break;
                 }
-                const unsigned char* named = bits + par * kCons * RP;
                 // the slice, out of the ring
                 uint4 raw[RP];
                 float mx = -INFINITY;
@@ -767,7 +889,6 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                             const int p = ch * L::kChunkPacks + u * kCons + t;
                             raw[ch * CP + u] = ok && p < count ? st[u * kCons + t] : P::lowest();
                         }
-                        release_stage(&bars.empty[slot], lane);
                         ++g;
                     } else {
 #pragma unroll
@@ -775,25 +896,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                     }
                 }
                 if (!ok) break;
-                uint32_t mark = 0u;  // packs of mine with a named element
-                if (OP == kLossDistill) {
-#pragma unroll
-                    for (int p = 0; p < RP; ++p) {
-                        const uint32_t by = p * kCons + t < count ? named[p * kCons + t] : 0u;
-                        if (by) {
-                            mark |= 1u << p;
-                            uint32_t* w = reinterpret_cast<uint32_t*>(&raw[p]);
-#pragma unroll
-                            for (int e = 0; e < VE; ++e)
-                                if (by >> e & 1u) {
-                                    if (VE == 4) w[e] = 0xff800000u;
-                                    else w[e >> 1] = e & 1 ? (w[e >> 1] & 0x0000ffffu) | 0xff800000u : (w[e >> 1] & 0xffff0000u) | 0x0000ff80u;
-                                }
-                        }
-                    }
-                }
                 float xe = -INFINITY;
-                if (edge_at >= 0 && !(OP == kLossDistill && (lists[par].edge_named >> t & 1u)))
+                if (edge_at >= 0)
                     xe = edges[(side * kBatch + i % kBatch) * 16 + t];
 #pragma unroll
                 for (int p = 0; p < RP; ++p) mx = fmaxf(mx, P::max(raw[p]));
@@ -816,6 +920,11 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 float s0, s1;
                 un(add2(acc0, acc1), s0, s1);
                 float s = warp_sum(s0 + s1 + ee);
+                // every lane's reads have arrived here: their values are in the sum
+                release_fence();
+                if (lane == 0)
+                    for (uint32_t k = g - static_cast<uint32_t>((count + L::kChunkPacks - 1) / L::kChunkPacks); k != g; ++k)
+                        mbar_arrive(&bars.empty[k % NS]);
                 if (OP == kLossDistill && warp == 0 && lists[par].bad) s = NAN;
                 if (lane < size)
                     send8(&mail[par * kMaxCluster * kConsWarps + rank * kConsWarps + warp], &bars.mail[par], lane,
@@ -846,16 +955,18 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                                     e[p][h] = f2(x0, x1);
                                 }
                             }
-                            // the row warp writes the named elements
-                            put_pack(pk, P::down(e[p]), OP == kLossDistill && (mark >> p & 1u) ? named[pk] : 0u);
+                            put_pack(pk, P::down(e[p]));
                         }
                     }
-                    if (edge_at >= 0 && !(OP == kLossDistill && (lists[par].edge_named >> t & 1u)))
+                    if (edge_at >= 0)
                         gr[edge_at * a.g_in] = LossElem<T>::down(OP == kLossPolicy && r.target == edge_at ? c.at_target : ee * f);
                 }
                 if (OP == kLossDistill) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.list_empty[par]);
+                    __syncwarp();  // the warp's stores are ordered before the row warp's
+                    if (lane == 0) {
+                        mbar_arrive(&bars.list_empty[par]);
+                        mbar_arrive(&bars.done[par]);
+                    }
                 }
                 ++live;
             }
@@ -1134,7 +1245,7 @@ template <class T, int OP> int hold_sized(const LossArgs& a, int* parts, cudaStr
     constexpr int VE = PackOf<T>::VE;
     const int64_t packs = a.cols / VE;
     auto need = [&](int e) { return static_cast<int>((packs + static_cast<int64_t>(kCons) * (e / VE) - 1) / (static_cast<int64_t>(kCons) * (e / VE))); };
-    if (need(16) <= 1) return hold_typed<T, OP, 16, 16 / VE, 4, 4>(a, 1, parts, st);
+    if (need(16) <= 1) return hold_typed<T, OP, 16, 16 / VE, 4, OP == kLossDistill ? 3 : 4>(a, 1, parts, st);
     const int c = need(64);
     return hold_typed<T, OP, 64, 4, 6, 2>(a, c, parts, st);
 }
