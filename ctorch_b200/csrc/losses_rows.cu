@@ -248,6 +248,7 @@ struct RowMeta {
     long long row, g_off;
     int target;          // -1: bad
     int head, packs;     // elements before the first whole 16-byte pack, whole packs
+    int first, count;    // this CTA's slice of the packs
     int pad_;
 };
 
@@ -302,7 +303,8 @@ __device__ __forceinline__ void slice_of(int packs, int rank, int size, int& fir
 // ------------------------------------------------------------------------------------------------
 // the producer's reads
 
-template <class T, int OP> __device__ __forceinline__ RowMeta read_meta(const LossArgs& a, int64_t row, int64_t& x_off) {
+template <class T, int OP>
+__device__ __forceinline__ RowMeta read_meta(const LossArgs& a, int64_t row, int rank, int size, int64_t& x_off) {
     RowMeta r;
     const T* X = static_cast<const T*>(a.ptr[kLrX]);
     r.row = row;
@@ -313,6 +315,7 @@ template <class T, int OP> __device__ __forceinline__ RowMeta read_meta(const Lo
     const int64_t head = ((16 - (at & 15)) & 15) / sizeof(T);
     r.head = static_cast<int>(head < a.cols ? head : a.cols);
     r.packs = static_cast<int>((a.cols - r.head) / PackOf<T>::VE);
+    slice_of(r.packs, rank, size, r.first, r.count);
     r.target = -1;
     r.xt = r.old = r.adv = r.ref = r.exp_old = r.exp_ref = 0.0;
     if (OP != kLossDistill && r.w != 0.0) {
@@ -390,9 +393,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
     if (warp == kProducer) {
         uint32_t g = 0;     // stages filled
         uint32_t live = 0;  // rows that count
-        auto issue = [&](int64_t x_off, int head, int packs) {
-            int first, count;
-            slice_of(packs, rank, size, first, count);
+        auto issue = [&](int64_t x_off, int head, int first, int count) {
             const T* src = static_cast<const T*>(a.ptr[kLrX]) + x_off + head + static_cast<int64_t>(first) * VE;
             for (int p = 0; p < count && ok; p += L::kChunkPacks, ++g) {
                 const int slot = static_cast<int>(g % NS);
@@ -408,9 +409,16 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             }
         };
         // The teacher's list of one row. Entries lane, lane + 32, ... of the first kAhead * 32 are fetched a row
-        // ahead into registers (z, at); longer lists are read in place.
-        double z[kAhead];
-        int64_t at[kAhead];
+        // ahead into registers, as they lie in memory, so that nothing waits for them; longer lists are read in
+        // place.
+        uint64_t raw_t[kAhead], raw_at[kAhead];
+        auto as_real = [&](uint64_t v) -> double {
+            switch (a.dtype[kLrTeacher]) {
+            case CTB_FLOAT32: return __uint_as_float(static_cast<uint32_t>(v));
+            case CTB_FLOAT64: return __longlong_as_double(static_cast<long long>(v));
+            default: return __uint_as_float(static_cast<uint32_t>(v) << 16);
+            }
+        };
         auto scaled = [&](int64_t t_off, int k) {
             return load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
         };
@@ -419,18 +427,22 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int k = lane + 32 * u;
-                z[u] = k < a.top ? scaled(t_off, k) : -INFINITY;
-                at[u] = k < a.top ? load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in) : -1;
+                if (k < a.top) {
+                    const int64_t o = t_off + k * a.t_in, io = ti_off + k * a.ti_in;
+                    if (a.dtype[kLrTeacher] == CTB_FLOAT32) raw_t[u] = static_cast<const uint32_t*>(a.ptr[kLrTeacher])[o];
+                    else if (a.dtype[kLrTeacher] == CTB_FLOAT64) raw_t[u] = static_cast<const uint64_t*>(a.ptr[kLrTeacher])[o];
+                    else raw_t[u] = static_cast<const uint16_t*>(a.ptr[kLrTeacher])[o];
+                    if (a.dtype[kLrTeacherIdx] == CTB_INT32) raw_at[u] = static_cast<const uint32_t*>(a.ptr[kLrTeacherIdx])[io];
+                    else raw_at[u] = static_cast<const uint64_t*>(a.ptr[kLrTeacherIdx])[io];
+                }
             }
         };
         // Joins the list of the row whose stages are g0 to g1 with the row's logits: sums for the row warp, and -inf
         // in place of the named logits, so that the consumers' sum is that of the others. `next`: the row to
         // fetch ahead, or -1.
-        auto read_list = [&](int64_t row, int64_t next, int64_t x_off, int head, int packs, uint32_t g0, uint32_t g1,
-                             float* edge) {
+        auto read_list = [&](int64_t row, int64_t next, int64_t x_off, int head, int packs, int first, int count, uint32_t g0,
+                             uint32_t g1, float* edge) {
             const int side = static_cast<int>(live & 1u);
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars.list_empty[side], ((live >> 1) & 1u) ^ 1u));
-            if (!ok) return;
             int* e_idx = reinterpret_cast<int*>(sm + L::kEntries + static_cast<size_t>(side) * 12 * a.top);
             float* e_x = reinterpret_cast<float*>(e_idx + a.top);
             float* e_q = e_x + a.top;
@@ -438,8 +450,26 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             const int64_t t_off = loss_offset(a, kLrTeacher, row), ti_off = loss_offset(a, kLrTeacherIdx, row);
             double zr[kAhead];
             int jr[kAhead];
-            float xr[kAhead];
+            T xraw[kAhead];
             int bad = 0;
+            // all loads of logits first
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                zr[u] = lane + 32 * u < a.top ? as_real(raw_t[u]) * a.inv_temp : -INFINITY;
+                const int64_t at = a.dtype[kLrTeacherIdx] == CTB_INT32 ? static_cast<int64_t>(static_cast<int32_t>(raw_at[u]))
+                                                                       : static_cast<int64_t>(raw_at[u]);
+                jr[u] = zr[u] == -INFINITY ? -1 : at >= 0 && at < a.cols ? static_cast<int>(at) : -2;
+                if (jr[u] >= 0) xraw[u] = x[jr[u]];
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (jr[u] == -2) {
+                    bad = 1;
+                    if (rank == 0)
+                        note_bad_index(a, a.dtype[kLrTeacherIdx] == CTB_INT32 ? static_cast<int64_t>(static_cast<int32_t>(raw_at[u]))
+                                                                              : static_cast<int64_t>(raw_at[u]));
+                    jr[u] = -1;
+                }
             // a valid entry's column, -1 for padding and for an index outside the row
             auto column = [&](double zk, int64_t k) -> int {
                 if (zk == -INFINITY) return -1;
@@ -448,48 +478,29 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 if (rank == 0) note_bad_index(a, k);
                 return -1;
             };
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                zr[u] = z[u];
-                jr[u] = column(zr[u], at[u]);
-                xr[u] = jr[u] >= 0 ? LossElem<T>::up(x[jr[u]]) : -INFINITY;
-            }
             if (next >= 0) fetch_list(next);
-            // which columns of this CTA's slice are named already
-            uint4* b16 = reinterpret_cast<uint4*>(bits);
-            for (int i = lane; i < kCons * RP / 16; i += 32) b16[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (lane == 0) lists[side].edge_named = 0u;
-            double mx = -INFINITY;
-            float x_max = -INFINITY;
+            // the teacher alone, while those are on their way: q = weight * exp(z - base), with weight 1 and the
+            // teacher's own log-sum-exp, or 1 / sum and the maximum
+            double base = -INFINITY, log_sum = 0.0, weight = 1.0;
             int entries = 0;
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                mx = fmax(mx, zr[u]);
-                x_max = fmaxf(x_max, xr[u]);
+                base = fmax(base, zr[u]);
                 entries += zr[u] != -INFINITY;
-                if (lane + 32 * u < a.top) {
-                    e_idx[lane + 32 * u] = jr[u];
-                    e_x[lane + 32 * u] = xr[u];
-                }
             }
             for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
                 const double zk = scaled(t_off, k);
-                const int j = column(zk, load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in));
-                const float xk = j >= 0 ? LossElem<T>::up(x[j]) : -INFINITY;
-                mx = fmax(mx, zk);
-                x_max = fmaxf(x_max, xk);
+                base = fmax(base, zk);
                 entries += zk != -INFINITY;
-                e_idx[k] = j;
-                e_x[k] = xk;
             }
-#pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            x_max = warp_max(x_max);
             entries = __reduce_add_sync(0xffffffffu, entries);
-            // q = weight * exp(z - base): weight 1 and the teacher's own log-sum-exp, or 1 / sum and the maximum
-            double base = mx, log_sum = 0.0, weight = 1.0;
+            if (a.tail) {
+                base = entries ? row_real(a, kLrTeacherLse, row) : 0.0;
+            } else {
+#pragma unroll
+                for (int d = 16; d >= 1; d >>= 1) base = fmax(base, __shfl_xor_sync(0xffffffffu, base, d));
+            }
             double er[kAhead];
-            if (a.tail && entries) base = row_real(a, kLrTeacherLse, row);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) er[u] = zr[u] == -INFINITY ? 0.0 : exp(zr[u] - base);
             if (!a.tail) {
@@ -501,6 +512,32 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 weight = 1.0 / sum;
                 log_sum = log(sum);
             }
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.list_empty[side], ((live >> 1) & 1u) ^ 1u));
+            if (!ok) return;
+            float xr[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) xr[u] = jr[u] >= 0 ? LossElem<T>::up(xraw[u]) : -INFINITY;
+            // which columns of this CTA's slice are named already
+            uint4* b16 = reinterpret_cast<uint4*>(bits);
+            for (int i = lane; i < kCons * RP / 16; i += 32) b16[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (lane == 0) lists[side].edge_named = 0u;
+            float x_max = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                x_max = fmaxf(x_max, xr[u]);
+                if (lane + 32 * u < a.top) {
+                    e_idx[lane + 32 * u] = jr[u];
+                    e_x[lane + 32 * u] = xr[u];
+                }
+            }
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
+                const int j = column(scaled(t_off, k), load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in));
+                const float xk = j >= 0 ? LossElem<T>::up(x[j]) : -INFINITY;
+                x_max = fmaxf(x_max, xk);
+                e_idx[k] = j;
+                e_x[k] = xk;
+            }
+            x_max = warp_max(x_max);
             const double ref = x_max == -INFINITY ? 0.0 : static_cast<double>(x_max);
             double sums[4] = {0.0, 0.0, 0.0, 0.0};  // mass, q log q, q (x - ref), exp((x - x_max) / T)
             auto add = [&](int k, double zk, double ek, int j, float xk) {
@@ -528,8 +565,6 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             for (uint32_t k = g0; k != g1; ++k) ok = mbar_wait(&bars.full[k % NS], (k / NS) & 1u) && ok;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
-            int first, count;
-            slice_of(packs, rank, size, first, count);
             for (int k = lane; k < a.top; k += 32) {
                 const int j = e_idx[k];
                 if (j < 0) continue;
@@ -579,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             int64_t x_off = 0;
             RowMeta r{};
             if (lane < n) {
-                r = read_meta<T, OP>(a, cluster + (b * kBatch + lane) * clusters, x_off);
+                r = read_meta<T, OP>(a, cluster + (b * kBatch + lane) * clusters, rank, size, x_off);
                 metas[side * kBatch + lane] = r;
             }
             if (rank == 0) {
@@ -607,23 +642,25 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 const uint32_t later = todo & (todo - 1);
                 const int i2 = later ? __ffs(later) - 1 : i;
                 const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
-                const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
+                const int head = __shfl_sync(0xffffffffu, r.head, i);
+                const int first = __shfl_sync(0xffffffffu, r.first, i), count = __shfl_sync(0xffffffffu, r.count, i);
                 uint32_t g0 = g_next, g1 = g;
                 if (!issued) {
                     g0 = g;
-                    issue(off, head, packs);
+                    issue(off, head, first, count);
                     g1 = g;
                 }
                 if (OP == kLossDistill && ok) {
                     const int64_t row = __shfl_sync(0xffffffffu, r.row, i), next = __shfl_sync(0xffffffffu, r.row, i2);
+                    const int packs = __shfl_sync(0xffffffffu, r.packs, i);
                     if (todo == counting) fetch_list(row);  // the batch's first: nobody fetched it ahead
                     issued = kTwo && later;
                     if (issued) {
                         g_next = g;
                         issue(__shfl_sync(0xffffffffu, x_off, i2), __shfl_sync(0xffffffffu, r.head, i2),
-                              __shfl_sync(0xffffffffu, r.packs, i2));
+                              __shfl_sync(0xffffffffu, r.first, i2), __shfl_sync(0xffffffffu, r.count, i2));
                     }
-                    if (ok) read_list(row, later ? next : -1, off, head, packs, g0, g1, edges + (side * kBatch + i) * 16);
+                    if (ok) read_list(row, later ? next : -1, off, head, packs, first, count, g0, g1, edges + (side * kBatch + i) * 16);
                 }
                 ++live;
             }
@@ -706,7 +743,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                         const double lift = exp((m - r.xt) * a.inv_temp);
                         const double s = mf == INFINITY ? quiet_nan() : static_cast<double>(warp_sum(part));
                         const double st = s * lift;
-                        double ratio = r.exp_old / st, ed = r.exp_ref * st - 1.0, rest = 1.0 - 1.0 / st, logp = 0.0;
+                        const double pt = 1.0 / st;
+                        double ratio = r.exp_old * pt, ed = r.exp_ref * st - 1.0, rest = 1.0 - pt, logp = 0.0;
                         const bool far = !(st < 1e300 && r.exp_old < 1e300 && r.exp_old > 1e-300 && r.exp_ref < 1e300) || r.target < 0;
                         if (far) {  // numbers outside these forms' range: through the logarithm
                             logp = r.target >= 0 ? (r.xt - m) * a.inv_temp - log(s) : quiet_nan();
@@ -752,8 +790,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                             ok = __all_sync(0xffffffffu, mbar_wait(&bars.done[par], phase));
                             if (!ok) break;
                             T* gr = G + r.g_off;
-                            int first, count;
-                            slice_of(r.packs, rank, size, first, count);
+                            const int first = r.first, count = r.count;
                             const int* e_idx = reinterpret_cast<const int*>(sm + L::kEntries + static_cast<size_t>(par) * 12 * a.top);
                             const float* e_x = reinterpret_cast<const float*>(e_idx + a.top);
                             const float* e_q = e_x + a.top;
@@ -791,8 +828,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
             if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.meta_full[side], (b >> 1) & 1));
             if (!ok) break;
             const RowMeta& r = metas[side * kBatch + i % kBatch];
-            int first, count;
-            slice_of(r.packs, rank, size, first, count);
+            const int first = r.first, count = r.count;
             T* gr = a.ptr[kLrGrad] ? static_cast<T*>(a.ptr[kLrGrad]) + r.g_off : nullptr;
             // Packs are stored whole where the gradient's rows are aligned like the logits', element by element
             // elsewhere (which costs eight times the store instructions, and takes any stride).
@@ -920,15 +956,15 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_rows_kernel(const __gri
                 float s0, s1;
                 un(add2(acc0, acc1), s0, s1);
                 float s = warp_sum(s0 + s1 + ee);
+                if (OP == kLossDistill && warp == 0 && lists[par].bad) s = NAN;
+                if (lane < size)
+                    send8(&mail[par * kMaxCluster * kConsWarps + rank * kConsWarps + warp], &bars.mail[par], lane,
+                          static_cast<uint64_t>(__float_as_uint(mw)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
                 // every lane's reads have arrived here: their values are in the sum
                 release_fence();
                 if (lane == 0)
                     for (uint32_t k = g - static_cast<uint32_t>((count + L::kChunkPacks - 1) / L::kChunkPacks); k != g; ++k)
                         mbar_arrive(&bars.empty[k % NS]);
-                if (OP == kLossDistill && warp == 0 && lists[par].bad) s = NAN;
-                if (lane < size)
-                    send8(&mail[par * kMaxCluster * kConsWarps + rank * kConsWarps + warp], &bars.mail[par], lane,
-                          static_cast<uint64_t>(__float_as_uint(mw)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
                 ok = __all_sync(0xffffffffu, mbar_wait(&bars.coef[par], phase));
                 if (!ok) break;
                 const Coef c = coefs[par];
