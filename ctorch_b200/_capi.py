@@ -88,7 +88,7 @@ def _load() -> ctypes.CDLL:
         "ctb_peer_trace": (i32, [vp, ctypes.POINTER(ctypes.c_uint64)]),
         "ctb_chain_rows_allsum": (i32, [i32, i32, P, P, P, P, i32, P, vp, vp, i32, i32, u64, P, vp, u64, vp]),
         # the losses take their views as packed bytes too (losses.py), so these arguments are untyped pointers
-        "ctb_loss_scratch_bytes": (sz, [V, i64]),
+        "ctb_loss_scratch_bytes": (sz, [V, i64, i64]),
         "ctb_token_logprobs": (i32, [V, V, V, f64, V, V, vp, vp]),
         "ctb_token_logprobs_backward": (i32, [V, V, V, V, V, V, f64, V, vp, vp]),
         "ctb_distill_loss": (i32, [V, V, V, V, V, f64, f64, V, V, V, vp, vp, sz, vp]),

@@ -338,6 +338,8 @@ size_t partial_bytes(int64_t rows) {
     return static_cast<size_t>(rows < kLossMaxCtas ? rows : kLossMaxCtas) * sizeof(double);
 }
 
+size_t distill_bytes(int64_t rows, int64_t top) { return partial_bytes(rows) + loss_lists_bytes(rows, top); }
+
 size_t preference_bytes(int64_t rows, int64_t pairs) {
     return static_cast<size_t>(3 * rows + pairs) * sizeof(double);
 }
@@ -355,12 +357,17 @@ int check_status(const int32_t* status) {
                                                    : CTB_OK;
 }
 
-int run_rows(const LossPlan& p, int* ctas, cudaStream_t st) {
-    if (loss_rows_fit(p.args, p.op != kLossToken)) return loss_rows_fast(p, ctas, st);
-    return loss_rows_general(p, ctas, st);
+int run_rows(const LossPlan& p, int* parts, cudaStream_t st) {
+    if (loss_stream_fit(p.args)) {
+        if (p.op == kLossToken) return loss_token_stream(p.args, st);
+        if (int rc = loss_held(p, parts, st)) return rc;
+        if (*parts >= 0) return CTB_OK;
+    }
+    return loss_rows_general(p, parts, st);
 }
+
 int run_backward(const LossArgs& a, cudaStream_t st) {
-    return loss_rows_fit(a, false) ? loss_backward_fast(a, st) : loss_backward_general(a, st);
+    return loss_stream_fit(a) ? loss_backward_stream(a, st) : loss_backward_general(a, st);
 }
 
 int run_total(const double* partials, int n, const ctb_view* out, cudaStream_t st) {
@@ -371,9 +378,11 @@ int run_total(const double* partials, int n, const ctb_view* out, cudaStream_t s
 
 // Rows with their weighted sum: the forward-and-gradient kernels.
 int run_loss(Builder& b, const ctb_view* loss, void* scratch, size_t scratch_bytes, cudaStream_t st) {
-    const size_t need = loss ? partial_bytes(b.a().rows) : 0;
+    const bool lists = b.plan.op == kLossDistill;
+    const size_t need = lists ? distill_bytes(b.a().rows, b.a().top) : loss ? partial_bytes(b.a().rows) : 0;
     if (int rc = check_scratch(scratch, scratch_bytes, need)) return rc;
     b.finish();
+    if (lists) b.a().lists = static_cast<unsigned char*>(scratch) + partial_bytes(b.a().rows);
     b.a().partials = loss ? static_cast<double*>(scratch) : nullptr;
     int ctas = 0;
     if (!b.plan.empty)
@@ -443,11 +452,11 @@ int ctb_token_logprobs_backward(const ctb_view* grad_logprobs, const ctb_view* l
     });
 }
 
-size_t ctb_loss_scratch_bytes(const ctb_view* logits, int64_t pairs) {
-    if (!logits || logits->ndim < 1 || logits->ndim > kMaxDims || pairs < 0) return 0;
+size_t ctb_loss_scratch_bytes(const ctb_view* logits, int64_t pairs, int64_t top) {
+    if (!logits || logits->ndim < 1 || logits->ndim > kMaxDims || pairs < 0 || top < 0 || top > kLossMaxTop) return 0;
     int64_t rows = 1;
     for (int d = 0; d < logits->ndim - 1; ++d) rows *= logits->shape[d];
-    return pairs ? preference_bytes(rows, pairs) : partial_bytes(rows);
+    return pairs ? preference_bytes(rows, pairs) : top ? distill_bytes(rows, top) : partial_bytes(rows);
 }
 
 int ctb_distill_loss(const ctb_view* logits, const ctb_view* teacher_logits, const ctb_view* teacher_indices,

@@ -55,6 +55,7 @@ struct LossArgs {
     int64_t x_in, g_in;   // strides along the vocabulary
     int64_t t_in, ti_in;  // strides along the teacher's entries
     int top;              // the teacher's entries a row
+    void* lists;          // distill: scratch for the teacher's prepared entries (losses_held.cu)
     int tail;             // distill: the mass outside the top entries is one more event
     double temp, inv_temp;
     float c2;             // log2(e) / T
@@ -324,9 +325,12 @@ constexpr int64_t kLossMaxDistillCols = int64_t(1) << 20;  // columns of a disti
 // the scratch query.
 constexpr int kLossMaxCtas = 148 * 16;
 
-bool loss_rows_fit(const LossArgs& a, bool held);                             // losses_rows.cu
-int loss_backward_fast(const LossArgs& a, cudaStream_t st);                   // losses_rows.cu
-int loss_rows_fast(const LossPlan& p, int* parts, cudaStream_t st);           // losses_rows.cu
+bool loss_stream_fit(const LossArgs& a);                                      // losses_stream.cu
+int loss_token_stream(const LossArgs& a, cudaStream_t st);                    // losses_stream.cu
+int loss_backward_stream(const LossArgs& a, cudaStream_t st);                 // losses_stream.cu
+// *parts: how many partial sums were written; negative when the rows are too long (nothing was launched).
+int loss_held(const LossPlan& p, int* parts, cudaStream_t st);                // losses_held.cu
+size_t loss_lists_bytes(int64_t rows, int64_t top);                           // losses_held.cu
 int loss_rows_general(const LossPlan& p, int* ctas, cudaStream_t st);      // losses_general.cu
 int loss_backward_general(const LossArgs& a, cudaStream_t st);              // losses_general.cu
 

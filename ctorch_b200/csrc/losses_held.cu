@@ -1,0 +1,889 @@
+// losses_held.cu — the policy and distillation losses over rows of unit stride (float32, bfloat16): each logit is
+// read from memory once, takes one exponential, and its gradient is written from the same pass.
+//
+// A row belongs to a thread-block cluster of C CTAs (C = 1 for rows that one CTA can hold), a CTA to a
+// contiguous slice of the row's 16-byte packs. Clusters are persistent: cluster c takes rows c, c + n,
+// c + 2n, ... In a CTA
+//   * the producer warp copies the slices of the coming rows into a ring of shared-memory stages, one stage a
+//     row (bulk asynchronous copies), and reads the rows' small operands, 32 rows at a time;
+//   * the consumer warps take a slice into registers, find the warp's maximum, turn the logits into
+//     e = exp((x - m_w) / T) and send (m_w, sum e) to every CTA of the cluster (st.async into its mailbox,
+//     completion counted on its mbarrier: no cluster-wide barrier);
+//   * the row warp joins the C * W partial sums and publishes the row's coefficient A;
+//   * the consumers put g = e * A exp((m_w - m) / T) over the slice in its stage, and the producer sends the
+//     stage to memory before it fills it again.
+// The consumers fold row r before they write row r - 1, so that the exchange of a row (0.2 us) and the row warp's
+// arithmetic (0.7 us) pass while they work. What a row's losses need is kept by the row warp and worked out for 32
+// rows at once, a lane a row.
+//
+// Rows longer than the registers of a cluster hold (KEEP = false) are folded straight from the stage and their
+// exponentials taken a second time.
+//
+// Distillation. The teacher's entries are prepared by a kernel of their own (loss_lists), a warp a row: q and the
+// sums that need no logit. The producer joins them with the row's slice when that has landed: it reads the
+// named logits, and puts -inf in their place in the stage, so that the consumers' sum is that of the others
+// (1 - sum p would lose it to cancellation) and their gradient there 0; the row warp then writes the named
+// elements' own gradient into the stage.
+#include <string>
+
+#include "losses_ring.cuh"
+
+namespace ctb {
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// the teacher's entries
+
+// Of one row's entries, by loss_lists.
+struct ListSums {
+    double q_logq, mass;  // sum q log q, sum q
+    int count, bad;       // entries that are not padding; an index outside the row
+};
+
+// Scratch of a distillation: [rows] ListSums, then q and columns [rows, top].
+__host__ __device__ inline size_t list_sums_bytes(int64_t rows) { return static_cast<size_t>(rows) * sizeof(ListSums); }
+
+// q_k = exp(z_k - base) * weight with z = teacher / T: renormalised over the entries (base their maximum, weight
+// 1 / sum), or with the teacher's own log-sum-exp. A warp a row; a few numbers a row, bound by latency.
+__global__ void __launch_bounds__(256) loss_lists(const __grid_constant__ LossArgs a) {
+    dependent_wait();
+    allow_dependents();
+    const int lane = threadIdx.x & 31;
+    ListSums* sums = static_cast<ListSums*>(a.lists);
+    float* qs = reinterpret_cast<float*>(static_cast<unsigned char*>(a.lists) + list_sums_bytes(a.rows));
+    int* columns = reinterpret_cast<int*>(qs + a.rows * a.top);
+    for (int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; row < a.rows;
+         row += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
+        ListSums out;
+        out.q_logq = out.mass = 0.0;
+        out.count = out.bad = 0;
+        if (row_weight(a, row) != 0.0) {
+            const int64_t t_off = loss_offset(a, kLrTeacher, row), ti_off = loss_offset(a, kLrTeacherIdx, row);
+            auto scaled = [&](int k) {
+                return load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
+            };
+            double base = -INFINITY;
+            int count = 0;
+            for (int k = lane; k < a.top; k += 32) {
+                const double z = scaled(k);
+                base = fmax(base, z);
+                count += z != -INFINITY;
+            }
+            out.count = __reduce_add_sync(0xffffffffu, count);
+            if (out.count) {
+                double log_sum = 0.0, weight = 1.0;
+                if (a.tail) {
+                    base = row_real(a, kLrTeacherLse, row);
+                } else {
+#pragma unroll
+                    for (int d = 16; d >= 1; d >>= 1) base = fmax(base, __shfl_xor_sync(0xffffffffu, base, d));
+                    double sum = 0.0;
+                    for (int k = lane; k < a.top; k += 32) sum += exp(scaled(k) - base);
+                    sum = warp_sum(sum);
+                    weight = 1.0 / sum;
+                    log_sum = log(sum);
+                }
+                int bad = 0;
+                for (int k = lane; k < a.top; k += 32) {
+                    const double z = scaled(k), q = z == -INFINITY ? 0.0 : weight * exp(z - base);
+                    int j = -1;
+                    if (z != -INFINITY) {
+                        const int64_t at = load_index(a.ptr[kLrTeacherIdx], a.dtype[kLrTeacherIdx], ti_off + k * a.ti_in);
+                        if (at >= 0 && at < a.cols) {
+                            j = static_cast<int>(at);
+                        } else {
+                            bad = 1;
+                            note_bad_index(a, at);
+                        }
+                    }
+                    if (q != 0.0) {  // NaN too
+                        out.mass += q;
+                        out.q_logq += q * (z - base - log_sum);
+                    }
+                    qs[row * a.top + k] = static_cast<float>(q);
+                    columns[row * a.top + k] = j;
+                }
+                out.mass = warp_sum(out.mass);
+                out.q_logq = warp_sum(out.q_logq);
+                out.bad = __any_sync(0xffffffffu, bad);
+            }
+        }
+        if (lane == 0) sums[row] = out;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// shared memory
+
+// A row's operands, read before its logits.
+struct RowMeta {
+    double w;                 // 0: the row does not count
+    double xt, adv;           // policy: the target's logit
+    double old, ref;
+    double exp_old, exp_ref;  // exp(-old), exp(ref)
+    ListSums list;            // distill
+    long long row;
+    const void* src;          // this CTA's slice of the logits
+    void* out;                // of the gradient, where its rows are aligned like the logits' (else null)
+    void* grad;               // the gradient's row, null without one
+    int count;                // packs of the slice
+    int body;                 // column of the slice's first element
+    int target;               // column of the target, -1: bad
+    uint32_t edges;           // which of the 16 elements around the whole packs there are (CTA 0 of the cluster)
+    int behind;               // column of the first element behind the whole packs
+    int pad_;
+};
+
+// What joining a list with the row's logits gives the row warp.
+struct ListInfo {
+    double q_x, ref;  // sum of q (x - ref)
+    double named;     // sum of exp((x - x_max) / T)
+    float x_max;
+    uint32_t edge_named;  // the producer's own
+};
+
+struct Coef {
+    float a, m, at_target, pad_;
+};
+
+constexpr int kSides = 4;   // rows whose sums and lists may be in use at once
+constexpr int kMaxRing = 8;
+constexpr int kAhead = 4;   // entries a lane of the producer fetches a row ahead
+
+// What lies behind the ring's stages.
+template <int W> struct Shared {
+    uint64_t mail[kSides][kMaxCluster * W];
+    RowMeta meta[2][kBatch];
+    float edge[2][kBatch][16];
+    ListInfo list[kSides];
+    Coef coef[2];
+    struct {
+        void* to;
+        uint32_t bytes, pad_;
+    } out[kMaxRing];  // where a stage goes when its row is done (the producer's own)
+    uint64_t full[kMaxRing], empty[kMaxRing], done[kMaxRing];
+    uint64_t meta_full[2], meta_empty[2];
+    uint64_t list_full[kSides], list_empty[kSides];
+    uint64_t mail_full[kSides], coef_full[2];
+};
+
+// Bytes behind the stages: Shared, then for distillation a bit a column of the slice (a byte a pack) and the
+// named logits of kSides rows.
+template <int W> __host__ __device__ constexpr size_t bits_at() { return (sizeof(Shared<W>) + 15) / 16 * 16; }
+template <int W> __host__ __device__ inline size_t behind_bytes(int op, int top, int slice_packs) {
+    return op == kLossDistill ? bits_at<W>() + (slice_packs + 15) / 16 * 16 + static_cast<size_t>(kSides) * top * 4 : sizeof(Shared<W>);
+}
+
+// A position in the ring, advanced a row at a time.
+struct Ring {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++slot == stages) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------
+
+// W consumer warps; E logits a consumer thread keeps (KEEP). `stages` stages of `stage_bytes`.
+template <class T, int OP, int W, int E, bool KEEP, int PER_SM>
+__global__ void __launch_bounds__(W * 32 + 64, PER_SM)
+    loss_held_kernel(const __grid_constant__ LossArgs a, int stages, int stage_bytes, int slice_packs) {
+    using P = PackOf<T>;
+    using S = Shared<W>;
+    constexpr int VE = P::VE, RP = KEEP ? E / VE : 1, kCons = W * 32;
+    extern __shared__ __align__(128) unsigned char sm[];
+    S& sh = *reinterpret_cast<S*>(sm + static_cast<size_t>(stages) * stage_bytes);
+    unsigned char* const behind = reinterpret_cast<unsigned char*>(&sh);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_rank()), size = static_cast<int>(cluster_size());
+    const uint32_t mail_bytes = static_cast<uint32_t>(size) * W * 8;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; ++i) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], OP == kLossDistill ? 1 : W);  // distill: the row warp's, after the named elements
+            mbar_init(&sh.done[i], W);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.meta_full[i], 1);
+            mbar_init(&sh.meta_empty[i], W + 1);
+            mbar_init(&sh.coef_full[i], 1);
+        }
+        for (int i = 0; i < kSides; ++i) {
+            mbar_init(&sh.list_full[i], 1);
+            mbar_init(&sh.list_empty[i], 1);
+            mbar_init(&sh.mail_full[i], 1);
+        }
+        mbar_fence_init();
+        for (int i = 0; i < kSides; ++i) mbar_arrive_expect_tx(&sh.mail_full[i], mail_bytes);
+    }
+    __syncthreads();
+    cluster_sync();
+    dependent_wait();  // the previous kernel in the stream has completed and its writes are visible
+
+    const int64_t cluster = blockIdx.x / size, clusters = gridDim.x / size;
+    const int rows = static_cast<int>(cluster < a.rows ? (a.rows - cluster + clusters - 1) / clusters : 0);
+    const float* list_q = nullptr;
+    const int* list_col = nullptr;
+    if (OP == kLossDistill) {
+        list_q = reinterpret_cast<const float*>(static_cast<const unsigned char*>(a.lists) + list_sums_bytes(a.rows));
+        list_col = reinterpret_cast<const int*>(list_q + a.rows * a.top);
+    }
+    bool ok = true;
+
+    if (warp == W) {
+        // ---- producer
+        int prepared = 0;    // batches whose operands have been read
+        uint32_t live = 0;   // rows that count, issued
+        Ring ring;
+        const T* X = static_cast<const T*>(a.ptr[kLrX]);
+        T* G = static_cast<T*>(a.ptr[kLrGrad]);
+        auto prepare = [&]() {
+            const int b = prepared++, side = b & 1, n = min(kBatch, rows - b * kBatch);
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_empty[side], ((b >> 1) & 1) ^ 1));
+            if (!ok) return;
+            RowMeta r{};
+            int64_t x_off = 0;
+            if (lane < n) {
+                r.row = cluster + static_cast<int64_t>(b * kBatch + lane) * clusters;
+                r.w = row_weight(a, r.row);
+                if (OP == kLossDistill) {
+                    r.list = static_cast<const ListSums*>(a.lists)[r.row];
+                    if (r.list.count == 0) r.w = 0.0;  // nothing but padding
+                }
+                x_off = loss_offset(a, kLrX, r.row);
+                const int64_t head64 = ((16 - (reinterpret_cast<uintptr_t>(X + x_off) & 15)) & 15) / sizeof(T);
+                const int head = static_cast<int>(head64 < a.cols ? head64 : a.cols);
+                const int packs = static_cast<int>((a.cols - head) / VE);
+                int first;
+                slice_of(packs, rank, size, first, r.count);
+                r.body = head + first * VE;
+                r.behind = head + packs * VE;
+                r.src = X + x_off + r.body;
+                if (G) {
+                    T* g = G + loss_offset(a, kLrGrad, r.row);
+                    r.grad = g;
+                    if (a.g_in == 1 && (reinterpret_cast<uintptr_t>(g + r.body) & 15) == 0) r.out = g + r.body;
+                }
+                if (rank == 0) r.edges = (1u << head) - 1 | ((1u << (static_cast<int>(a.cols) - r.behind)) - 1) << 8;
+                r.target = -1;
+                if (OP == kLossPolicy && r.w != 0.0) {
+                    const int64_t t = load_index(a.ptr[kLrTarget], a.dtype[kLrTarget], loss_offset(a, kLrTarget, r.row));
+                    r.old = row_real(a, kLrOld, r.row);
+                    r.adv = row_real(a, kLrAdv, r.row);
+                    if (a.ptr[kLrRef]) r.ref = row_real(a, kLrRef, r.row);
+                    if (t >= 0 && t < a.cols) {
+                        r.target = static_cast<int>(t);
+                        r.xt = LossElem<T>::up(X[x_off + t]);
+                    } else {
+                        note_bad_index(a, t);
+                    }
+                    r.exp_old = exp(-r.old);
+                    if (a.ptr[kLrRef]) r.exp_ref = exp(r.ref);
+                }
+                sh.meta[side][lane] = r;
+            }
+            for (int i = 0; i < n; ++i) {
+                const uint32_t there = __shfl_sync(0xffffffffu, r.w != 0.0 ? r.edges : 0u, i);
+                if (!there) continue;
+                const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
+                const int tail = __shfl_sync(0xffffffffu, r.behind, i);
+                if (lane < 16)
+                    sh.edge[side][i][lane] =
+                        there >> lane & 1u ? LossElem<T>::up(X[off + (lane < 8 ? lane : tail + lane - 8)]) : -INFINITY;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.meta_full[side]);
+        };
+        // Sends the stage's last row to memory and starts the copy of row i into it.
+        auto issue = [&](int i) {
+            const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
+            if (r.w == 0.0) return;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[ring.slot], ring.phase ^ 1u));
+            if (!ok) return;
+            if (lane == 0) {
+                unsigned char* st = sm + static_cast<size_t>(ring.slot) * stage_bytes;
+                auto& o = sh.out[ring.slot];
+                if (live >= static_cast<uint32_t>(stages) && o.bytes) {
+                    bulk_store(o.to, st, o.bytes);
+                    bulk_commit();
+                    bulk_wait_read();
+                }
+                const uint32_t bytes = static_cast<uint32_t>(r.count) * 16u;
+                mbar_arrive_expect_tx(&sh.full[ring.slot], bytes);
+                if (bytes) bulk_load(st, r.src, bytes, &sh.full[ring.slot]);
+                o.to = r.out;
+                o.bytes = r.out ? bytes : 0u;
+            }
+            __syncwarp();
+            ring.next(stages);
+            ++live;
+        };
+        // Distill: entries lane, lane + 32, ... of the first kAhead * 32 of a row, fetched a row ahead.
+        int col_ahead[kAhead];
+        float q_ahead[kAhead];
+        auto fetch_list = [&](int64_t row) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int k = lane + 32 * u;
+                col_ahead[u] = k < a.top ? list_col[row * a.top + k] : -1;
+                q_ahead[u] = k < a.top ? list_q[row * a.top + k] : 0.f;
+            }
+        };
+        uint32_t listed = 0;
+        Ring list_ring;
+        auto join_list = [&](int i, int64_t next) {
+            const int side = static_cast<int>(listed % kSides), ms = i / kBatch & 1, mi = i % kBatch;
+            const RowMeta& r = sh.meta[ms][mi];
+            const T* x = X + loss_offset(a, kLrX, r.row);
+            float* e_x = reinterpret_cast<float*>(behind + bits_at<W>() + (slice_packs + 15) / 16 * 16) + side * a.top;
+            unsigned char* bits = behind + bits_at<W>();
+            unsigned char* st = sm + static_cast<size_t>(list_ring.slot) * stage_bytes;
+            ListInfo& li = sh.list[side];
+            int col[kAhead];
+            float q[kAhead];
+            T raw[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                col[u] = col_ahead[u];
+                q[u] = q_ahead[u];
+                if (col[u] >= 0) raw[u] = x[col[u]];
+            }
+            if (next >= 0) fetch_list(next);
+            for (int k = lane; k < (slice_packs + 15) / 16; k += 32) reinterpret_cast<uint4*>(bits)[k] = make_uint4(0u, 0u, 0u, 0u);
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.list_empty[side], ((listed / kSides) & 1u) ^ 1u));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&sh.full[list_ring.slot], list_ring.phase));
+            if (!ok) return;
+            if (lane == 0) li.edge_named = 0u;
+            __syncwarp();
+            float x_max = -INFINITY;
+            float xs[kAhead];
+            T* twice_at = nullptr;
+            float* twice_edge = nullptr;
+            // notes a named logit and takes it out of this CTA's slice
+            auto take = [&](int k, int j, float xk) {
+                e_x[k] = xk;
+                x_max = fmaxf(x_max, xk);
+                if (j < 0) return;
+                const int at = j - r.body;
+                const bool inside = at >= 0 && at < r.count * VE;
+                const int l = j < 8 && (r.edges >> j & 1u) ? j : j >= r.behind ? 8 + j - r.behind : -1;
+                if (!inside && (rank != 0 || l < 0)) return;
+                uint32_t* word = inside ? reinterpret_cast<uint32_t*>(bits) + (at / VE >> 2) : &li.edge_named;
+                const uint32_t bit = inside ? 1u << ((at / VE & 3) * 8 + at % VE) : 1u << l;
+                const bool twice = atomicOr(word, bit) & bit;
+                if (twice) note_bad_index(a, j);
+                if (inside) {
+                    reinterpret_cast<T*>(st)[at] = LossElem<T>::down(-INFINITY);
+                    if (twice) twice_at = reinterpret_cast<T*>(st) + at;
+                } else {
+                    sh.edge[ms][mi][l] = -INFINITY;
+                    if (twice) twice_edge = &sh.edge[ms][mi][l];
+                }
+            };
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                xs[u] = col[u] >= 0 ? LossElem<T>::up(raw[u]) : -INFINITY;
+                if (lane + 32 * u < a.top) take(lane + 32 * u, col[u], xs[u]);
+            }
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
+                const int j = list_col[r.row * a.top + k];
+                take(k, j, j >= 0 ? LossElem<T>::up(x[j]) : -INFINITY);
+            }
+            __syncwarp();
+            // a column named twice makes the whole row NaN
+            if (twice_at) *twice_at = LossElem<T>::down(NAN);
+            if (twice_edge) *twice_edge = NAN;
+            x_max = warp_max(x_max);
+            const float ref = x_max == -INFINITY ? 0.f : x_max;
+            float named = 0.f;
+            double q_x = 0.0;
+            auto add = [&](float qk, int j, float xk) {
+                if (j >= 0) named += exp_one(a, xk, ref);
+                if (qk != 0.f) q_x += static_cast<double>(qk) * (static_cast<double>(xk) - ref);
+            };
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) add(q[u], col[u], xs[u]);
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32)
+                add(list_q[r.row * a.top + k], list_col[r.row * a.top + k], e_x[k]);
+            named = warp_sum(named);
+            q_x = warp_sum(q_x);
+            release_fence();
+            if (lane == 0) {
+                li.q_x = q_x;
+                li.ref = ref;
+                li.named = named;
+                li.x_max = x_max;
+                mbar_arrive(&sh.list_full[side]);
+            }
+            __syncwarp();
+            list_ring.next(stages);
+            ++listed;
+        };
+        if constexpr (OP == kLossPolicy) {
+            for (int i = 0; i < rows && ok; ++i) {
+                if (i % kBatch == 0) prepare();
+                if (ok) issue(i);
+            }
+        } else {
+            // A list is joined with its row once that has landed, so copies run `lead` rows ahead of the lists. The
+            // copy of row i + lead waits for row i + lead - stages, which must not itself wait for list i: the
+            // consumers finish row j after they have seen row j + 1.
+            const int lead = stages >= 6 ? stages - 4 : 1;
+            int issued = 0;
+            auto counts = [&](int i) { return sh.meta[i / kBatch & 1][i % kBatch].w != 0.0; };
+            int64_t ahead = -1;  // the row whose entries have been fetched
+            for (int i = 0; i < rows && ok; ++i) {
+                for (; issued <= i + lead && issued < rows && ok; ++issued) {
+                    if (issued % kBatch == 0) prepare();
+                    if (ok) issue(issued);
+                }
+                if (!ok || !counts(i)) continue;
+                const int64_t row = sh.meta[i / kBatch & 1][i % kBatch].row;
+                if (ahead != row) fetch_list(row);
+                int j = i + 1;
+                while (j < issued && !counts(j)) ++j;
+                ahead = j < issued ? sh.meta[j / kBatch & 1][j % kBatch].row : -1;
+                join_list(i, ahead);
+            }
+        }
+        // the last rows
+        const uint32_t left = live < static_cast<uint32_t>(stages) ? live : static_cast<uint32_t>(stages);
+        Ring last;
+        if (live > left) last = ring;  // the ring is full: the oldest row is the next slot's
+        if (live > left) last.phase ^= 1u;
+        for (uint32_t k = 0; k < left && ok; ++k) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[last.slot], last.phase));
+            if (ok && lane == 0 && sh.out[last.slot].bytes)
+                bulk_store(sh.out[last.slot].to, sm + static_cast<size_t>(last.slot) * stage_bytes, sh.out[last.slot].bytes);
+            last.next(stages);
+        }
+        if (lane == 0) {
+            bulk_commit();
+            bulk_wait();
+        }
+        __syncwarp();
+        if (!ok) {
+            if (lane == 0) note_timeout(a.timeouts);
+            // the copies in flight land before the CTA's memory goes away
+            for (int i = 0; i < stages; ++i)
+                if (static_cast<uint32_t>(i) < live) mbar_wait(&sh.full[i], i < ring.slot ? ring.phase : ring.phase ^ 1u, 100000000ull);
+        }
+    } else if (warp == W + 1) {
+        // ---- row warp: joins the sums, publishes the coefficient, and keeps what the losses are made of
+        uint32_t live = 0;
+        Ring ring;
+        double total = 0.0, kept_s = 0.0, kept_rest = 0.0, kept_x = 0.0, kept_ref = 0.0;  // kept_x: ratio, or sum q (x - ref)
+        float kept_m = 0.f;
+        for (int i = 0; i < rows && ok; ++i) {
+            const int ms = i / kBatch & 1, mi = i % kBatch;
+            if (mi == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[ms], (i / kBatch >> 1) & 1));
+            if (!ok) break;
+            const RowMeta& r = sh.meta[ms][mi];
+            if (r.w != 0.0) {
+                const int par = static_cast<int>(live & 1u), side = static_cast<int>(live % kSides);
+                const uint32_t phase = (live / kSides) & 1u;
+                ok = mbar_wait_cluster(&sh.mail_full[side], phase);
+                if (OP == kLossDistill) ok = ok && mbar_wait(&sh.list_full[side], phase);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int parts = size * W;
+                constexpr int kJoin = kMaxCluster * W / 32;
+                float pm[kJoin], ps[kJoin], mf = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k) {
+                    const uint64_t v = lane + 32 * k < parts ? sh.mail[side][lane + 32 * k] : 0xff800000ull;
+                    pm[k] = __uint_as_float(static_cast<uint32_t>(v));
+                    ps[k] = __uint_as_float(static_cast<uint32_t>(v >> 32));
+                    mf = fmaxf(mf, pm[k]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&sh.mail_full[side], mail_bytes);  // for the row kSides later
+                const ListInfo& li = sh.list[side];
+                mf = warp_max(mf);
+                if (OP == kLossDistill) mf = fmaxf(mf, li.x_max);
+                const double m = mf;
+                // Every consumer of the cluster waits for the coefficient, so only what it needs is computed first:
+                // no logarithm.
+                double lift = 1.0;
+                if (OP == kLossPolicy) lift = exp((m - r.xt) * a.inv_temp);
+                float part = 0.f;
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k)
+                    if (32 * k < parts) part += pm[k] == -INFINITY ? ps[k] : ps[k] * (pm[k] == mf ? 1.f : exp_one(a, pm[k], mf));
+                double s = warp_sum(part), s_rest = s;
+                if (mf == INFINITY) s = s_rest = quiet_nan();
+                Coef c;
+                c.m = mf;
+                c.at_target = c.pad_ = 0.f;
+                double ratio = 0.0, big_q = 1.0;
+                if (OP == kLossPolicy) {
+                    // s relative to the target's logit instead of the maximum: r = exp(-old) / s', p_t = 1 / s'
+                    const double st = s * lift, pt = 1.0 / st;
+                    ratio = r.exp_old * pt;
+                    double ed = r.exp_ref * st - 1.0, rest = 1.0 - pt;
+                    if (!(st < 1e300 && r.exp_old < 1e300 && r.exp_old > 1e-300 && r.exp_ref < 1e300) || r.target < 0) {
+                        // numbers outside these forms' range: through the logarithm
+                        const double logp = r.target >= 0 ? (r.xt - m) * a.inv_temp - log(s) : quiet_nan();
+                        ratio = exp(logp - r.old);
+                        ed = expm1(r.ref - logp);
+                        rest = -expm1(logp);
+                    }
+                    const double g = policy_terms(a, r.w, r.adv, ratio, 0.0, ed).g;
+                    c.a = -static_cast<float>(g) / static_cast<float>(s);
+                    c.at_target = static_cast<float>(g * rest);
+                } else {
+                    s = s_rest + li.named * (li.x_max == -INFINITY ? 0.f : exp_one(a, li.x_max, mf));
+                    if (r.list.bad || !(s > 0.0)) s = quiet_nan();
+                    c.a = static_cast<float>(distill_slope(a, r.w, s, s_rest, r.list.mass, r.list.count == a.cols, big_q));
+                    if (s != s) c.a = NAN;
+                }
+                if (lane == 0) {
+                    sh.coef[par] = c;
+                    mbar_arrive(&sh.coef_full[par]);
+                }
+                if (lane == mi) {
+                    kept_s = s;
+                    kept_rest = s_rest;
+                    kept_m = mf;
+                    kept_x = OP == kLossPolicy ? ratio : li.q_x;
+                    kept_ref = OP == kLossPolicy ? 0.0 : li.ref;
+                }
+                if constexpr (OP == kLossDistill) {
+                    // The named elements of this CTA's slice, over what the consumers leave there.
+                    constexpr int kSome = 8;
+                    int col[kSome];
+                    float q[kSome];
+                    auto entry = [&](int k0) {
+#pragma unroll
+                        for (int u = 0; u < kSome; ++u) {
+                            const int k = k0 + lane + 32 * u;
+                            col[u] = r.grad && k < a.top ? list_col[r.row * a.top + k] : -1;
+                            q[u] = r.grad && k < a.top ? list_q[r.row * a.top + k] : 0.f;
+                        }
+                    };
+                    entry(0);
+                    const float* e_x = reinterpret_cast<const float*>(behind + bits_at<W>() + (slice_packs + 15) / 16 * 16) + side * a.top;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.done[ring.slot], ring.phase));
+                    if (!ok) break;
+                    if (r.grad) {
+                        T* st = reinterpret_cast<T*>(sm + static_cast<size_t>(ring.slot) * stage_bytes);
+                        T* gr = static_cast<T*>(r.grad);
+                        const float scale = static_cast<float>(r.w * a.inv_temp), p_scale = static_cast<float>(big_q) / static_cast<float>(s);
+                        // a bad row is NaN throughout: its named columns too, whoever found it
+                        const float poison = c.a == c.a ? 0.f : c.a;
+                        for (int k0 = 0; k0 < a.top; k0 += 32 * kSome) {
+                            if (k0) entry(k0);
+#pragma unroll
+                            for (int u = 0; u < kSome; ++u) {
+                                const int j = col[u], at = j - r.body;
+                                const bool inside = at >= 0 && at < r.count * VE;
+                                const bool edge = (j < 8 && j >= 0 && (r.edges >> j & 1u)) || (rank == 0 && j >= r.behind);
+                                if (j < 0 || !(inside || edge)) continue;
+                                const T v = LossElem<T>::down(scale * (exp_one(a, e_x[k0 + lane + 32 * u], mf) * p_scale - q[u]) + poison);
+                                if (inside && r.out) st[at] = v;
+                                else gr[j * a.g_in] = v;
+                            }
+                        }
+                    }
+                    release_fence();
+                    if (lane == 0) {
+                        mbar_arrive(&sh.empty[ring.slot]);
+                        mbar_arrive(&sh.list_empty[side]);
+                    }
+                    ring.next(stages);
+                }
+                ++live;
+            }
+            __syncwarp();
+            if (mi == kBatch - 1 || i + 1 == rows) {
+                if (rank == 0 && lane <= mi) {
+                    const RowMeta& mine = sh.meta[ms][lane];
+                    const double m = kept_m;
+                    if (mine.w == 0.0) {
+                        put_empty_row(a, mine.row);
+                    } else if (OP == kLossDistill) {
+                        const double cross = mine.list.q_logq - a.inv_temp * (kept_x + (kept_ref - m) * mine.list.mass) +
+                                             mine.list.mass * log(kept_s);
+                        const double loss = distill_loss_of(a, kept_s, kept_rest, cross, mine.list.mass, mine.list.count == a.cols);
+                        put_row(a, kLrRowLoss, mine.row, loss);
+                        total += mine.w * loss;
+                    } else {
+                        const double logp = mine.target >= 0 ? (mine.xt - m) * a.inv_temp - log(kept_s) : quiet_nan();
+                        const double d = mine.ref - logp;
+                        const PolicyTerms t = policy_terms(a, mine.w, mine.adv, kept_x, d, a.ptr[kLrRef] ? expm1(d) : 0.0);
+                        put_row(a, kLrLogp, mine.row, logp);
+                        put_row(a, kLrKl, mine.row, t.kl);
+                        put_row(a, kLrRowLoss, mine.row, t.loss);
+                        total += mine.w * t.loss;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.meta_empty[ms]);
+            }
+        }
+        if (!ok && lane == 0) note_timeout(a.timeouts);
+        total = warp_sum(total);
+        if (a.partials && rank == 0 && lane == 0) a.partials[cluster] = total;
+    } else {
+        // ---- consumers
+        const int t = threadIdx.x;
+        const ExpConst kc = exp_const(a);
+        struct Slice {
+            F2 e[RP][VE / 2];
+            float m;
+        };
+        uint32_t live = 0;
+        Ring ring, held_ring;
+        int held = -1;  // the row that waits for its gradient
+        auto stage_of = [&](const Ring& g) { return reinterpret_cast<uint4*>(sm + static_cast<size_t>(g.slot) * stage_bytes); };
+        // Folds row i: its sum goes to the cluster.
+        auto fold = [&](int i, const RowMeta& r, Slice& in) {
+            const int side = static_cast<int>(live % kSides);
+            if (OP == kLossDistill) ok = mbar_wait(&sh.list_full[side], (live / kSides) & 1u);
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(&sh.full[ring.slot], ring.phase));
+            if (!ok) return;
+            const uint4* st = stage_of(ring) + t;
+            const float xe = t < 16 && (r.edges >> t & 1u) ? sh.edge[i / kBatch & 1][i % kBatch][t] : -INFINITY;
+            const int count = r.count - t;  // packs t, t + kCons, ... of the slice
+            float m, s0, s1;
+            if constexpr (KEEP) {
+                uint4 raw[RP];
+#pragma unroll
+                for (int p = 0; p < RP; ++p) raw[p] = p * kCons < count ? st[p * kCons] : P::lowest();
+                float mx = xe;
+#pragma unroll
+                for (int p = 0; p < RP; ++p) mx = fmaxf(mx, P::max(raw[p]));
+                m = warp_max(mx);
+                const float at = m == -INFINITY ? 0.f : m;
+                const F2 minus = f2(-at, -at);
+                F2 acc0 = f2(exp_one(a, xe, at), 0.f), acc1 = f2(0.f, 0.f);
+#pragma unroll
+                for (int p = 0; p < RP; ++p) {
+                    P::up(raw[p], in.e[p]);
+#pragma unroll
+                    for (int h = 0; h < VE / 2; ++h) {
+                        in.e[p][h] = exp_pair(in.e[p][h], minus, kc);
+                        if (h & 1) acc1 = add2(acc1, in.e[p][h]);
+                        else acc0 = add2(acc0, in.e[p][h]);
+                    }
+                }
+                in.m = m;
+                un(add2(acc0, acc1), s0, s1);
+            } else {
+                // a maximum a warp; the sum is brought down when it grows (a few times a row)
+                constexpr int CP = 4;
+                m = warp_max(xe);
+                F2 sum = f2(exp_one(a, xe, m == -INFINITY ? 0.f : m), 0.f);
+                for (int p0 = 0; p0 < r.count; p0 += CP * kCons) {
+                    uint4 raw[CP];
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < CP; ++u) {
+                        raw[u] = p0 + u * kCons < count ? st[p0 + u * kCons] : P::lowest();
+                        mx = fmaxf(mx, P::max(raw[u]));
+                    }
+                    mx = warp_max(mx);
+                    if (mx > m) {
+                        const float down = exp_one(a, m, mx);
+                        sum = mul2(sum, f2(down, down));
+                        m = mx;
+                    }
+                    const float at = m == -INFINITY ? 0.f : m;
+                    const F2 minus = f2(-at, -at);
+                    F2 acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
+#pragma unroll
+                    for (int u = 0; u < CP; ++u) {
+                        F2 e[VE / 2];
+                        P::up(raw[u], e);
+#pragma unroll
+                        for (int h = 0; h < VE / 2; h += 2) {
+                            acc0 = add2(acc0, exp_pair(e[h], minus, kc));
+                            acc1 = add2(acc1, exp_pair(e[h + 1], minus, kc));
+                        }
+                    }
+                    sum = add2(sum, add2(acc0, acc1));
+                }
+                un(sum, s0, s1);
+            }
+            const float s = warp_sum(s0 + s1);
+            // A side of the mailbox is written again four rows later: this warp has then waited for the coefficient of
+            // the row before the last one, which its own CTA published after it had read that row's side; and so
+            // had every CTA whose sums made up that coefficient read the side of two rows before.
+            if (lane < size)
+                send8(&sh.mail[side][rank * W + warp], &sh.mail_full[side], lane,
+                      static_cast<uint64_t>(__float_as_uint(m)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
+        };
+        // Writes the gradient of row i, the l-th that counts.
+        auto write = [&](int i, uint32_t l, const Slice& out) {
+            const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.coef_full[l & 1u], (l >> 1) & 1u));
+            if (!ok) return;
+            const Coef c = sh.coef[l & 1u];
+            uint4* st = stage_of(held_ring) + t;
+            const int count = r.count - t;
+            const float f = KEEP ? c.a * exp_one(a, out.m, c.m) : c.a;
+            const F2 ff = f2(f, f), minus = f2(-c.m, -c.m);
+            auto pack = [&](int p) {
+                F2 e[VE / 2];
+                if constexpr (KEEP) {
+#pragma unroll
+                    for (int h = 0; h < VE / 2; ++h) e[h] = mul2(out.e[p][h], ff);
+                } else {
+                    P::up(st[p * kCons], e);
+#pragma unroll
+                    for (int h = 0; h < VE / 2; ++h) e[h] = mul2(exp_pair(e[h], minus, kc), ff);
+                }
+                return P::down(e);
+            };
+            if (r.out) {
+                if constexpr (KEEP) {
+#pragma unroll
+                    for (int p = 0; p < RP; ++p)
+                        if (p * kCons < count) st[p * kCons] = pack(p);
+                } else {
+#pragma unroll 4
+                    for (int p = 0; p * kCons < count; ++p) st[p * kCons] = pack(p);
+                }
+                if (OP == kLossPolicy) {
+                    const int at = r.target - r.body;  // the target's own value, by the thread that wrote its pack
+                    if (r.target >= 0 && at >= 0 && at < r.count * VE && (at / VE) % kCons == t)
+                        reinterpret_cast<T*>(stage_of(held_ring))[at] = LossElem<T>::down(c.at_target);
+                }
+            } else if (r.grad) {
+                // where the gradient's rows are not aligned like the logits', or strided: element by element
+                T* gr = static_cast<T*>(r.grad);
+                auto scatter = [&](int p, const uint4& o) {
+                    const T* v = reinterpret_cast<const T*>(&o);
+                    const int j = r.body + (p * kCons + t) * VE;
+#pragma unroll
+                    for (int k = 0; k < VE; ++k)
+                        gr[(j + k) * a.g_in] = OP == kLossPolicy && j + k == r.target ? LossElem<T>::down(c.at_target) : v[k];
+                };
+                if constexpr (KEEP) {
+#pragma unroll
+                    for (int p = 0; p < RP; ++p)
+                        if (p * kCons < count) scatter(p, pack(p));
+                } else {
+                    for (int p = 0; p * kCons < count; ++p) scatter(p, pack(p));
+                }
+            }
+            if (r.grad && t < 16 && (r.edges >> t & 1u)) {
+                const int j = t < 8 ? t : r.behind + t - 8;
+                const float v = c.a * exp_one(a, sh.edge[i / kBatch & 1][i % kBatch][t], c.m);
+                static_cast<T*>(r.grad)[j * a.g_in] = LossElem<T>::down(OP == kLossPolicy && j == r.target ? c.at_target : v);
+            }
+            release_fence();  // the copy out of the stage, and the next one into it, come after this
+            if (lane == 0) mbar_arrive(OP == kLossDistill ? &sh.done[held_ring.slot] : &sh.empty[held_ring.slot]);
+        };
+        auto step = [&](int i, Slice& in, const Slice& out) {
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[i / kBatch & 1], (i / kBatch >> 1) & 1));
+            if (!ok) return;
+            const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
+            const bool counts = r.w != 0.0;
+            if (counts) fold(i, r, in);
+            if (ok && held >= 0) write(held, live - 1, out);
+            if (!ok) return;
+            held = -1;
+            if (counts) {
+                held = i;
+                held_ring = ring;
+                ring.next(stages);
+                ++live;
+            } else if (r.grad) {
+                T* gr = static_cast<T*>(r.grad);
+                if (r.out)
+                    for (int p = t; p < r.count; p += kCons) static_cast<uint4*>(r.out)[p] = make_uint4(0u, 0u, 0u, 0u);
+                else
+                    for (int k = t; k < r.count * VE; k += kCons) gr[(r.body + k) * a.g_in] = LossElem<T>::down(0.f);
+                if (t < 16 && (r.edges >> t & 1u)) gr[(t < 8 ? t : r.behind + t - 8) * a.g_in] = LossElem<T>::down(0.f);
+            }
+            __syncwarp();
+            // the batch before this one is done with: its last row has its gradient
+            if (i % kBatch == 0 && i > 0 && lane == 0) mbar_arrive(&sh.meta_empty[(i / kBatch - 1) & 1]);
+        };
+        Slice one, two;
+        int i = 0;
+        for (; i + 1 < rows && ok; i += 2) {
+            step(i, one, two);
+            if (ok) step(i + 1, two, one);
+        }
+        if (i < rows && ok) {
+            step(i, one, two);
+            if (ok && held >= 0) write(held, live - 1, one);
+        } else if (ok && held >= 0) {
+            write(held, live - 1, two);
+        }
+        if (!ok && lane == 0) note_timeout(a.timeouts);
+    }
+    allow_dependents();
+    leave_cluster(ok);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+
+// Launches with clusters of `cluster` CTAs; *parts < 0 when three stages do not fit.
+template <class T, int OP, int W, int E, bool KEEP, int PER_SM>
+int held_typed(const LossArgs& a, int64_t cluster, int most_stages, int* parts, cudaStream_t st) {
+    const int64_t packs = a.cols / PackOf<T>::VE;
+    int slice = static_cast<int>((packs + cluster - 1) / cluster);
+    int stage = (slice < 1 ? 1 : slice) * 16;
+    stage = (stage + 127) / 128 * 128;
+    const size_t rest = behind_bytes<W>(OP, a.top, slice);
+    // an equal share of an SM's shared memory (228 KiB, of which a CTA takes 1 KiB more than it asks for)
+    const size_t room = (PER_SM > 1 ? 228 * 1024 / PER_SM - 1024 : static_cast<size_t>(kMaxSmem));
+    int64_t stages = rest < room ? static_cast<int64_t>((room - rest) / stage) : 0;
+    if (stages < 3) stages = rest < kMaxSmem ? static_cast<int64_t>((kMaxSmem - rest) / stage) : 0;
+    if (stages > most_stages) stages = most_stages;
+    *parts = -1;
+    if (stages < 3) return CTB_OK;
+    const size_t smem = static_cast<size_t>(stages) * stage + rest;
+    auto fn = loss_held_kernel<T, OP, W, E, KEEP, PER_SM>;
+    const int threads = W * 32 + 64;
+    int n = 0;
+    if (int rc = resident_blocks(reinterpret_cast<const void*>(fn), threads, static_cast<int>(cluster), smem, &n)) return rc;
+    int64_t clusters = n < a.rows ? n : a.rows;
+    if (clusters > kLossMaxCtas) clusters = kLossMaxCtas;
+    *parts = static_cast<int>(clusters);
+    if (OP == kLossDistill) {
+        launch_dependent(loss_lists, grid_for((a.rows + 7) / 8, 8), 256, 0, st, a);
+        count_launch();
+        if (int rc = check_launch("loss lists")) return rc;
+    }
+    LossArgs args = a;
+    int ring = static_cast<int>(stages);
+    void* argv[4] = {&args, &ring, &stage, &slice};
+    return launch_cluster(reinterpret_cast<const void*>(fn), static_cast<unsigned>(clusters * cluster), threads,
+                          static_cast<int>(cluster), smem, st, argv);
+}
+
+template <class T, int OP> int held_sized(const LossArgs& a, int* parts, cudaStream_t st) {
+    const int64_t v = a.cols;
+    auto share = [&](int64_t most) { return (v + most - 1) / most; };
+    *parts = -1;
+    if (v <= 4096) return held_typed<T, OP, 8, 16, true, 3>(a, 1, 4, parts, st);
+    if (share(16 * 32 * 32) <= kMaxCluster) {
+        if (int rc = held_typed<T, OP, 16, 32, true, 1>(a, share(16 * 32 * 32), kMaxRing, parts, st)) return rc;
+        if (*parts >= 0) return CTB_OK;
+    }
+    return held_typed<T, OP, 16, 0, false, 1>(a, kMaxCluster, kMaxRing, parts, st);
+}
+
+}  // namespace
+
+size_t loss_lists_bytes(int64_t rows, int64_t top) { return list_sums_bytes(rows) + static_cast<size_t>(rows) * top * 8; }
+
+int loss_held(const LossPlan& p, int* parts, cudaStream_t st) {
+    const LossArgs& a = p.args;
+    const bool bf = a.dtype[kLrX] == CTB_BFLOAT16;
+    if (p.op == kLossPolicy)
+        return bf ? held_sized<__nv_bfloat16, kLossPolicy>(a, parts, st) : held_sized<float, kLossPolicy>(a, parts, st);
+    return bf ? held_sized<__nv_bfloat16, kLossDistill>(a, parts, st) : held_sized<float, kLossDistill>(a, parts, st);
+}
+
+}  // namespace ctb

@@ -185,7 +185,7 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weig
     n = prod(rows)
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
-    need = C.lib.ctb_loss_scratch_bytes(vx, 0)
+    need = C.lib.ctb_loss_scratch_bytes(vx, 0, teacher_logits.shape[-1] if teacher_logits.dim() else 0)
     scratch, (row_loss, loss) = _results(logits, dev, [n, 1], need)
     row_loss, loss = _shaped(row_loss, rows), loss.view(())
     _run(name, dev, C.lib.ctb_distill_loss, vx, _view(teacher_logits), _view(teacher_indices), _view(teacher_lse),
@@ -210,7 +210,7 @@ def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, we
     n = prod(rows)
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
-    need = C.lib.ctb_loss_scratch_bytes(vx, 0)
+    need = C.lib.ctb_loss_scratch_bytes(vx, 0, 0)
     scratch, (row_loss, logp, kl, loss) = _results(logits, dev, [n, n, n, 1], need)
     row_loss, logp, kl, loss = _shaped(row_loss, rows), _shaped(logp, rows), _shaped(kl, rows), loss.view(())
     _run(name, dev, C.lib.ctb_policy_loss, vx, _view(targets), _view(old_logprobs), _view(advantages),
@@ -241,7 +241,7 @@ def preference_loss(logits, targets, pairs: int, ref_logprobs=None, mask=None, o
     rows = logits.shape[:-1]
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
-    need = C.lib.ctb_loss_scratch_bytes(vx, pairs)
+    need = C.lib.ctb_loss_scratch_bytes(vx, pairs, 0)
     scratch, (logp, pair_loss, rewards, loss) = _results(logits, dev, [prod(rows), pairs, 2 * pairs, 1], need)
     logp, loss = _shaped(logp, rows), loss.view(())
     _run(name, dev, C.lib.ctb_preference_loss, vx, _view(targets), pairs, _view(offsets), _view(ref_logprobs),

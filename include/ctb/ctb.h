@@ -322,9 +322,9 @@ CTB_API int ctb_token_logprobs_backward(const ctb_view* grad_logprobs, const ctb
                                         const ctb_view* mask, double temperature, const ctb_view* grad,
                                         int32_t* d_status, ctb_stream stream);
 
-/* Scratch bytes of the losses below (8-byte aligned): pairs = 0 for ctb_distill_loss and
- * ctb_policy_loss (needed there only when `loss` is wanted). */
-CTB_API size_t ctb_loss_scratch_bytes(const ctb_view* logits, int64_t pairs);
+/* Scratch bytes of the losses below (8-byte aligned): pairs of ctb_preference_loss, else 0; top = the
+ * teacher's entries a row of ctb_distill_loss, else 0. ctb_policy_loss needs it only when `loss` is wanted. */
+CTB_API size_t ctb_loss_scratch_bytes(const ctb_view* logits, int64_t pairs, int64_t top);
 
 /* Distillation from a teacher's top entries: teacher_logits [..., K] (also bfloat16) and their
  * vocabulary indices [..., K], K up to 2048, V up to 2^20. An entry of -inf is padding: its index is

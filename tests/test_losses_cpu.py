@@ -189,11 +189,12 @@ def test_token_refusals():
 def test_scratch_bytes():
     C = _lib()
     need = C.lib.ctb_loss_scratch_bytes
-    assert need(P(view(C, [2, 3, 8])), 0) == 6 * 8
-    assert need(P(view(C, [10 ** 6, 8])), 0) <= 148 * 16 * 8
-    assert need(P(view(C, [6, 8])), 3) == (3 * 6 + 3) * 8
-    assert need(P(view(C, [0, 8])), 0) == 0
-    assert need(None, 0) == 0
+    assert need(P(view(C, [2, 3, 8])), 0, 0) == 6 * 8
+    assert need(P(view(C, [10 ** 6, 8])), 0, 0) <= 148 * 16 * 8
+    assert need(P(view(C, [6, 8])), 3, 0) == (3 * 6 + 3) * 8
+    assert need(P(view(C, [6, 8])), 0, 5) == 6 * 8 + 6 * (24 + 5 * 8)
+    assert need(P(view(C, [0, 8])), 0, 0) == 0
+    assert need(None, 0, 0) == 0
 
 
 def test_python_front_refuses_cpu_tensors_and_types():
