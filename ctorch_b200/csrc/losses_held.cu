@@ -16,14 +16,12 @@
 // arithmetic (0.7 us) pass while they work. What a row's losses need is kept by the row warp and worked out for 32
 // rows at once, a lane a row.
 //
-// Rows longer than the registers of a cluster hold (KEEP = false) are folded straight from the stage and their
-// exponentials taken a second time.
-//
 // Distillation. The teacher's entries are prepared by a kernel of their own (loss_lists), a warp a row: q and the
 // sums that need no logit. The producer joins them with the row's slice when that has landed: it reads the
 // named logits, and puts -inf in their place in the stage, so that the consumers' sum is that of the others
 // (1 - sum p would lose it to cancellation) and their gradient there 0; the row warp then writes the named
 // elements' own gradient into the stage.
+#include <cstdlib>
 #include <string>
 
 #include "losses_ring.cuh"
@@ -189,13 +187,13 @@ struct Ring {
 
 // ------------------------------------------------------------------------------------------------
 
-// W consumer warps; E logits a consumer thread keeps (KEEP). `stages` stages of `stage_bytes`.
-template <class T, int OP, int W, int E, bool KEEP, int PER_SM>
+// W consumer warps; `stages` stages of `stage_bytes`.
+template <class T, int OP, int W, int PER_SM>
 __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
     loss_held_kernel(const __grid_constant__ LossArgs a, int stages, int stage_bytes, int slice_packs) {
     using P = PackOf<T>;
     using S = Shared<W>;
-    constexpr int VE = P::VE, RP = KEEP ? E / VE : 1, kCons = W * 32;
+    constexpr int VE = P::VE, kCons = W * 32;
     extern __shared__ __align__(128) unsigned char sm[];
     S& sh = *reinterpret_cast<S*>(sm + static_cast<size_t>(stages) * stage_bytes);
     unsigned char* const behind = reinterpret_cast<unsigned char*>(&sh);
@@ -244,7 +242,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
         T* G = static_cast<T*>(a.ptr[kLrGrad]);
         auto prepare = [&]() {
             const int b = prepared++, side = b & 1, n = min(kBatch, rows - b * kBatch);
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_empty[side], ((b >> 1) & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_empty[side], ((b >> 1) & 1) ^ 1));
             if (!ok) return;
             RowMeta r{};
             int64_t x_off = 0;
@@ -303,7 +301,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
         auto issue = [&](int i) {
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
             if (r.w == 0.0) return;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[ring.slot], ring.phase ^ 1u));
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.empty[ring.slot], ring.phase ^ 1u));
             if (!ok) return;
             if (lane == 0) {
                 unsigned char* st = sm + static_cast<size_t>(ring.slot) * stage_bytes;
@@ -355,8 +353,8 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             }
             if (next >= 0) fetch_list(next);
             for (int k = lane; k < (slice_packs + 15) / 16; k += 32) reinterpret_cast<uint4*>(bits)[k] = make_uint4(0u, 0u, 0u, 0u);
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.list_empty[side], ((listed / kSides) & 1u) ^ 1u));
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(&sh.full[list_ring.slot], list_ring.phase));
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.list_empty[side], ((listed / kSides) & 1u) ^ 1u));
+            ok = __all_sync(0xffffffffu, ok && wait_phase(&sh.full[list_ring.slot], list_ring.phase));
             if (!ok) return;
             if (lane == 0) li.edge_named = 0u;
             __syncwarp();
@@ -457,7 +455,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
         if (live > left) last = ring;  // the ring is full: the oldest row is the next slot's
         if (live > left) last.phase ^= 1u;
         for (uint32_t k = 0; k < left && ok; ++k) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[last.slot], last.phase));
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.empty[last.slot], last.phase));
             if (ok && lane == 0 && sh.out[last.slot].bytes)
                 bulk_store(sh.out[last.slot].to, sm + static_cast<size_t>(last.slot) * stage_bytes, sh.out[last.slot].bytes);
             last.next(stages);
@@ -481,14 +479,14 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
         float kept_m = 0.f;
         for (int i = 0; i < rows && ok; ++i) {
             const int ms = i / kBatch & 1, mi = i % kBatch;
-            if (mi == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[ms], (i / kBatch >> 1) & 1));
+            if (mi == 0) ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_full[ms], (i / kBatch >> 1) & 1));
             if (!ok) break;
             const RowMeta& r = sh.meta[ms][mi];
             if (r.w != 0.0) {
                 const int par = static_cast<int>(live & 1u), side = static_cast<int>(live % kSides);
                 const uint32_t phase = (live / kSides) & 1u;
-                ok = mbar_wait_cluster(&sh.mail_full[side], phase);
-                if (OP == kLossDistill) ok = ok && mbar_wait(&sh.list_full[side], phase);
+                ok = wait_phase<true>(&sh.mail_full[side], phase);
+                if (OP == kLossDistill) ok = ok && wait_phase(&sh.list_full[side], phase);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const int parts = size * W;
@@ -568,7 +566,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                     };
                     entry(0);
                     const float* e_x = reinterpret_cast<const float*>(behind + bits_at<W>() + (slice_packs + 15) / 16 * 16) + side * a.top;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.done[ring.slot], ring.phase));
+                    ok = __all_sync(0xffffffffu, wait_phase(&sh.done[ring.slot], ring.phase));
                     if (!ok) break;
                     if (r.grad) {
                         T* st = reinterpret_cast<T*>(sm + static_cast<size_t>(ring.slot) * stage_bytes);
@@ -633,83 +631,54 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
         // ---- consumers
         const int t = threadIdx.x;
         const ExpConst kc = exp_const(a);
-        struct Slice {
-            F2 e[RP][VE / 2];
-            float m;
-        };
         uint32_t live = 0;
         Ring ring, held_ring;
         int held = -1;  // the row that waits for its gradient
         auto stage_of = [&](const Ring& g) { return reinterpret_cast<uint4*>(sm + static_cast<size_t>(g.slot) * stage_bytes); };
         // Folds row i: its sum goes to the cluster.
-        auto fold = [&](int i, const RowMeta& r, Slice& in) {
+        auto fold = [&](int i, const RowMeta& r) {
             const int side = static_cast<int>(live % kSides);
-            if (OP == kLossDistill) ok = mbar_wait(&sh.list_full[side], (live / kSides) & 1u);
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(&sh.full[ring.slot], ring.phase));
+            if (OP == kLossDistill) ok = wait_phase(&sh.list_full[side], (live / kSides) & 1u);
+            ok = __all_sync(0xffffffffu, ok && wait_phase(&sh.full[ring.slot], ring.phase));
             if (!ok) return;
             const uint4* st = stage_of(ring) + t;
             const float xe = t < 16 && (r.edges >> t & 1u) ? sh.edge[i / kBatch & 1][i % kBatch][t] : -INFINITY;
             const int count = r.count - t;  // packs t, t + kCons, ... of the slice
             float m, s0, s1;
-            if constexpr (KEEP) {
-                uint4 raw[RP];
+            // a maximum a warp; the sum is brought down when it grows (a few times a row)
+            constexpr int CP = 4;
+            m = warp_max(xe);
+            F2 sum = f2(exp_one(a, xe, m == -INFINITY ? 0.f : m), 0.f);
+            for (int p0 = 0; p0 < r.count; p0 += CP * kCons) {
+                uint4 raw[CP];
+                float mx = -INFINITY;
 #pragma unroll
-                for (int p = 0; p < RP; ++p) raw[p] = p * kCons < count ? st[p * kCons] : P::lowest();
-                float mx = xe;
-#pragma unroll
-                for (int p = 0; p < RP; ++p) mx = fmaxf(mx, P::max(raw[p]));
-                m = warp_max(mx);
+                for (int u = 0; u < CP; ++u) {
+                    raw[u] = p0 + u * kCons < count ? st[p0 + u * kCons] : P::lowest();
+                    mx = fmaxf(mx, P::max(raw[u]));
+                }
+                mx = warp_max(mx);
+                if (mx > m) {
+                    const float down = exp_one(a, m, mx);
+                    sum = mul2(sum, f2(down, down));
+                    m = mx;
+                }
                 const float at = m == -INFINITY ? 0.f : m;
                 const F2 minus = f2(-at, -at);
-                F2 acc0 = f2(exp_one(a, xe, at), 0.f), acc1 = f2(0.f, 0.f);
+                F2 acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
 #pragma unroll
-                for (int p = 0; p < RP; ++p) {
-                    P::up(raw[p], in.e[p]);
+                for (int u = 0; u < CP; ++u) {
+                    F2 e[VE / 2];
+                    P::up(raw[u], e);
 #pragma unroll
-                    for (int h = 0; h < VE / 2; ++h) {
-                        in.e[p][h] = exp_pair(in.e[p][h], minus, kc);
-                        if (h & 1) acc1 = add2(acc1, in.e[p][h]);
-                        else acc0 = add2(acc0, in.e[p][h]);
+                    for (int h = 0; h < VE / 2; h += 2) {
+                        acc0 = add2(acc0, exp_pair(e[h], minus, kc));
+                        acc1 = add2(acc1, exp_pair(e[h + 1], minus, kc));
                     }
                 }
-                in.m = m;
-                un(add2(acc0, acc1), s0, s1);
-            } else {
-                // a maximum a warp; the sum is brought down when it grows (a few times a row)
-                constexpr int CP = 4;
-                m = warp_max(xe);
-                F2 sum = f2(exp_one(a, xe, m == -INFINITY ? 0.f : m), 0.f);
-                for (int p0 = 0; p0 < r.count; p0 += CP * kCons) {
-                    uint4 raw[CP];
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int u = 0; u < CP; ++u) {
-                        raw[u] = p0 + u * kCons < count ? st[p0 + u * kCons] : P::lowest();
-                        mx = fmaxf(mx, P::max(raw[u]));
-                    }
-                    mx = warp_max(mx);
-                    if (mx > m) {
-                        const float down = exp_one(a, m, mx);
-                        sum = mul2(sum, f2(down, down));
-                        m = mx;
-                    }
-                    const float at = m == -INFINITY ? 0.f : m;
-                    const F2 minus = f2(-at, -at);
-                    F2 acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
-#pragma unroll
-                    for (int u = 0; u < CP; ++u) {
-                        F2 e[VE / 2];
-                        P::up(raw[u], e);
-#pragma unroll
-                        for (int h = 0; h < VE / 2; h += 2) {
-                            acc0 = add2(acc0, exp_pair(e[h], minus, kc));
-                            acc1 = add2(acc1, exp_pair(e[h + 1], minus, kc));
-                        }
-                    }
-                    sum = add2(sum, add2(acc0, acc1));
-                }
-                un(sum, s0, s1);
+                sum = add2(sum, add2(acc0, acc1));
             }
+            un(sum, s0, s1);
             const float s = warp_sum(s0 + s1);
             // A side of the mailbox is written again four rows later: this warp has then waited for the coefficient of
             // the row before the last one, which its own CTA published after it had read that row's side; and so
@@ -719,36 +688,24 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                       static_cast<uint64_t>(__float_as_uint(m)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
         };
         // Writes the gradient of row i, the l-th that counts.
-        auto write = [&](int i, uint32_t l, const Slice& out) {
+        auto write = [&](int i, uint32_t l) {
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.coef_full[l & 1u], (l >> 1) & 1u));
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.coef_full[l & 1u], (l >> 1) & 1u));
             if (!ok) return;
             const Coef c = sh.coef[l & 1u];
             uint4* st = stage_of(held_ring) + t;
             const int count = r.count - t;
-            const float f = KEEP ? c.a * exp_one(a, out.m, c.m) : c.a;
-            const F2 ff = f2(f, f), minus = f2(-c.m, -c.m);
+            const F2 ga = f2(c.a, c.a), minus = f2(-c.m, -c.m);
             auto pack = [&](int p) {
                 F2 e[VE / 2];
-                if constexpr (KEEP) {
+                P::up(st[p * kCons], e);
 #pragma unroll
-                    for (int h = 0; h < VE / 2; ++h) e[h] = mul2(out.e[p][h], ff);
-                } else {
-                    P::up(st[p * kCons], e);
-#pragma unroll
-                    for (int h = 0; h < VE / 2; ++h) e[h] = mul2(exp_pair(e[h], minus, kc), ff);
-                }
+                for (int h = 0; h < VE / 2; ++h) e[h] = mul2(exp_pair(e[h], minus, kc), ga);
                 return P::down(e);
             };
             if (r.out) {
-                if constexpr (KEEP) {
-#pragma unroll
-                    for (int p = 0; p < RP; ++p)
-                        if (p * kCons < count) st[p * kCons] = pack(p);
-                } else {
 #pragma unroll 4
-                    for (int p = 0; p * kCons < count; ++p) st[p * kCons] = pack(p);
-                }
+                for (int p = 0; p * kCons < count; ++p) st[p * kCons] = pack(p);
                 if (OP == kLossPolicy) {
                     const int at = r.target - r.body;  // the target's own value, by the thread that wrote its pack
                     if (r.target >= 0 && at >= 0 && at < r.count * VE && (at / VE) % kCons == t)
@@ -764,13 +721,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                     for (int k = 0; k < VE; ++k)
                         gr[(j + k) * a.g_in] = OP == kLossPolicy && j + k == r.target ? LossElem<T>::down(c.at_target) : v[k];
                 };
-                if constexpr (KEEP) {
-#pragma unroll
-                    for (int p = 0; p < RP; ++p)
-                        if (p * kCons < count) scatter(p, pack(p));
-                } else {
-                    for (int p = 0; p * kCons < count; ++p) scatter(p, pack(p));
-                }
+                for (int p = 0; p * kCons < count; ++p) scatter(p, pack(p));
             }
             if (r.grad && t < 16 && (r.edges >> t & 1u)) {
                 const int j = t < 8 ? t : r.behind + t - 8;
@@ -780,14 +731,14 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             release_fence();  // the copy out of the stage, and the next one into it, come after this
             if (lane == 0) mbar_arrive(OP == kLossDistill ? &sh.done[held_ring.slot] : &sh.empty[held_ring.slot]);
         };
-        auto step = [&](int i, Slice& in, const Slice& out) {
-            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[i / kBatch & 1], (i / kBatch >> 1) & 1));
-            if (!ok) return;
+        for (int i = 0; i < rows && ok; ++i) {
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_full[i / kBatch & 1], (i / kBatch >> 1) & 1));
+            if (!ok) break;
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
             const bool counts = r.w != 0.0;
-            if (counts) fold(i, r, in);
-            if (ok && held >= 0) write(held, live - 1, out);
-            if (!ok) return;
+            if (counts) fold(i, r);
+            if (ok && held >= 0) write(held, live - 1);
+            if (!ok) break;
             held = -1;
             if (counts) {
                 held = i;
@@ -805,19 +756,8 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             __syncwarp();
             // the batch before this one is done with: its last row has its gradient
             if (i % kBatch == 0 && i > 0 && lane == 0) mbar_arrive(&sh.meta_empty[(i / kBatch - 1) & 1]);
-        };
-        Slice one, two;
-        int i = 0;
-        for (; i + 1 < rows && ok; i += 2) {
-            step(i, one, two);
-            if (ok) step(i + 1, two, one);
         }
-        if (i < rows && ok) {
-            step(i, one, two);
-            if (ok && held >= 0) write(held, live - 1, one);
-        } else if (ok && held >= 0) {
-            write(held, live - 1, two);
-        }
+        if (ok && held >= 0) write(held, live - 1);
         if (!ok && lane == 0) note_timeout(a.timeouts);
     }
     allow_dependents();
@@ -828,7 +768,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
 // host side
 
 // Launches with clusters of `cluster` CTAs; *parts < 0 when three stages do not fit.
-template <class T, int OP, int W, int E, bool KEEP, int PER_SM>
+template <class T, int OP, int W, int PER_SM>
 int held_typed(const LossArgs& a, int64_t cluster, int most_stages, int* parts, cudaStream_t st) {
     const int64_t packs = a.cols / PackOf<T>::VE;
     int slice = static_cast<int>((packs + cluster - 1) / cluster);
@@ -843,10 +783,11 @@ int held_typed(const LossArgs& a, int64_t cluster, int most_stages, int* parts, 
     *parts = -1;
     if (stages < 3) return CTB_OK;
     const size_t smem = static_cast<size_t>(stages) * stage + rest;
-    auto fn = loss_held_kernel<T, OP, W, E, KEEP, PER_SM>;
+    auto fn = loss_held_kernel<T, OP, W, PER_SM>;
     const int threads = W * 32 + 64;
     int n = 0;
     if (int rc = resident_blocks(reinterpret_cast<const void*>(fn), threads, static_cast<int>(cluster), smem, &n)) return rc;
+    if (getenv("CTB_P")) printf("cluster %d stages %d resident %d\n", (int)cluster, (int)stages, n);
     int64_t clusters = n < a.rows ? n : a.rows;
     if (clusters > kLossMaxCtas) clusters = kLossMaxCtas;
     *parts = static_cast<int>(clusters);
@@ -866,12 +807,17 @@ template <class T, int OP> int held_sized(const LossArgs& a, int* parts, cudaStr
     const int64_t v = a.cols;
     auto share = [&](int64_t most) { return (v + most - 1) / most; };
     *parts = -1;
-    if (v <= 4096) return held_typed<T, OP, 8, 16, true, 3>(a, 1, 4, parts, st);
-    if (share(16 * 32 * 32) <= kMaxCluster) {
-        if (int rc = held_typed<T, OP, 16, 32, true, 1>(a, share(16 * 32 * 32), kMaxRing, parts, st)) return rc;
-        if (*parts >= 0) return CTB_OK;
-    }
-    return held_typed<T, OP, 16, 0, false, 1>(a, kMaxCluster, kMaxRing, parts, st);
+    static const int mode = getenv("CTB_MODE") ? atoi(getenv("CTB_MODE")) : 0;
+    const int64_t most = 65536 / sizeof(T);
+    if (mode == 1) return held_typed<T, OP, 8, 2>(a, share(most / 2), kMaxRing, parts, st);
+    if (mode == 2) return held_typed<T, OP, 8, 3>(a, share(most / 4), kMaxRing, parts, st);
+    if (mode == 3) return held_typed<T, OP, 4, 4>(a, share(most / 8), kMaxRing, parts, st);
+    if (mode == 4) return held_typed<T, OP, 4, 6>(a, share(most / 8), kMaxRing, parts, st);
+    if (mode == 5) return held_typed<T, OP, 14, 1>(a, share(most), kMaxRing, parts, st);
+    int64_t c = share(most);
+    if (getenv("CTB_C")) c = atoi(getenv("CTB_C"));
+    if (c > kMaxCluster) return CTB_OK;
+    return held_typed<T, OP, 16, 1>(a, c, kMaxRing, parts, st);
 }
 
 }  // namespace

@@ -204,26 +204,36 @@ __device__ __forceinline__ void leave_cluster(bool ok) {
     }
 }
 
-// Waits for a phase that threads of other CTAs of the cluster contribute to.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+// Waits as mbar_wait does, but asks the hardware to suspend the warp between looks: two helper warps and the
+// consumers that wait poll a quarter of a kernel's instructions away otherwise. CLUSTER: threads of other CTAs
+// of the cluster contribute to the phase.
+template <bool CLUSTER = false> __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
+    constexpr uint32_t kSuspendNs = 20000;
     uint64_t t0 = 0;
-    for (int i = 0;; ++i) {
+    for (;;) {
         uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(smem_addr(bar)), "r"(parity)
-            : "memory");
+        if (CLUSTER)
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(done)
+                : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendNs)
+                : "memory");
+        else
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(done)
+                : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendNs)
+                : "memory");
         if (done) return true;
-        if (i % 32 == 0) {
-            if (t0 == 0) t0 = global_ns();
-            else if (global_ns() - t0 > kWaitLimitNs) return false;
-        }
+        const uint64_t now = global_ns();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > kWaitLimitNs) return false;
     }
 }
-
 
 // Rank r's share of a row's packs.
 __device__ __forceinline__ void slice_of(int packs, int rank, int size, int& first, int& count) {

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
         for (int64_t b = 0; b * kBatch < my_rows && ok; ++b) {
             const int side = static_cast<int>(b & 1);
             const int n = static_cast<int>(min(static_cast<int64_t>(kBatch), my_rows - b * kBatch));
-            ok = __all_sync(0xffffffffu, mbar_wait(&meta_empty[side], ((b >> 1) & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, wait_phase(&meta_empty[side], ((b >> 1) & 1) ^ 1));
             if (!ok) break;
             int64_t x_off = 0;
             TokenMeta r{};
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
                 const T* src = X + off + head + static_cast<int64_t>(first) * VE;
                 for (int p = 0; p < count; p += L::kChunkPacks, ++g) {
                     const int slot = static_cast<int>(g % NS);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], ((g / NS) & 1u) ^ 1u));
+                    ok = __all_sync(0xffffffffu, wait_phase(&empty[slot], ((g / NS) & 1u) ^ 1u));
                     if (!ok) break;
                     const uint32_t bytes = static_cast<uint32_t>(min(L::kChunkPacks, count - p)) * 16u;
                     if (lane == 0) {
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
             if (lane == 0) note_timeout(a.timeouts);
             // the copies in flight land before the CTA's memory goes away
             for (uint32_t i = g > static_cast<uint32_t>(NS) ? g - NS : 0u; i < g; ++i)
-                mbar_wait(&full[i % NS], (i / NS) & 1u);
+                wait_phase(&full[i % NS], (i / NS) & 1u);
         }
     } else if (warp == kRowWarp) {
         // lane i keeps the i-th row of the batch
@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
         for (int64_t i = 0; i < my_rows && ok; ++i) {
             const int64_t b = i / kBatch;
             const int side = static_cast<int>(b & 1);
-            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&meta_full[side], (b >> 1) & 1));
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&meta_full[side], (b >> 1) & 1));
             if (!ok) break;
             if (metas[side * kBatch + i % kBatch].w != 0.0) {
                 const int ms = static_cast<int>(live % kSides);
-                ok = __all_sync(0xffffffffu, mbar_wait_cluster(&mail_full[ms], (live / kSides) & 1u));
+                ok = __all_sync(0xffffffffu, wait_phase<true>(&mail_full[ms], (live / kSides) & 1u));
                 if (!ok) break;
                 const int parts = size * kConsWarps;
                 constexpr int kJoin = kMaxCluster * kConsWarps / 32;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
         for (int64_t i = 0; i < my_rows && ok; ++i) {
             const int64_t b = i / kBatch;
             const int side = static_cast<int>(b & 1);
-            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&meta_full[side], (b >> 1) & 1));
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&meta_full[side], (b >> 1) & 1));
             if (!ok) break;
             const TokenMeta& r = metas[side * kBatch + i % kBatch];
             if (r.w != 0.0) {
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
                 F2 sum = f2(exp_one(a, xe, m == -INFINITY ? 0.f : m), 0.f);
                 for (int p0 = 0; p0 < count; p0 += L::kChunkPacks, ++g) {
                     const int slot = static_cast<int>(g % NS);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (g / NS) & 1u));
+                    ok = __all_sync(0xffffffffu, wait_phase(&full[slot], (g / NS) & 1u));
                     if (!ok) break;
                     const uint4* st = reinterpret_cast<const uint4*>(sm + static_cast<size_t>(slot) * L::kStage);
                     uint4 raw[CP];
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
                 // A side of the mailbox is written again four rows later: by then every CTA of the cluster has read it if
                 // each warp waits here for its own CTA to have joined the row before the last one.
                 if (ok && live >= 2)
-                    ok = __all_sync(0xffffffffu, mbar_wait(&joined[live & 1u], ((live - 2) >> 1) & 1u));
+                    ok = __all_sync(0xffffffffu, wait_phase(&joined[live & 1u], ((live - 2) >> 1) & 1u));
                 if (!ok) break;
                 if (lane < size)
                     send8(&mail[(live % kSides * kMaxCluster + rank) * kConsWarps + warp], &mail_full[live % kSides], lane,
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
         for (int64_t b = 0; b * kBatch < my_rows && ok; ++b) {
             const int side = static_cast<int>(b & 1);
             const int n = static_cast<int>(min(static_cast<int64_t>(kBatch), my_rows - b * kBatch));
-            ok = __all_sync(0xffffffffu, mbar_wait(&meta_empty[side], ((b >> 1) & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, wait_phase(&meta_empty[side], ((b >> 1) & 1) ^ 1));
             if (!ok) break;
             int64_t x_off = 0;
             PullMeta r{};
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
                 const T* src = X + off + head + static_cast<int64_t>(first) * VE;
                 for (int p = 0; p < count; p += L::kChunkPacks, ++g) {
                     const int slot = static_cast<int>(g % NS);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], ((g / NS) & 1u) ^ 1u));
+                    ok = __all_sync(0xffffffffu, wait_phase(&empty[slot], ((g / NS) & 1u) ^ 1u));
                     if (!ok) break;
                     const uint32_t bytes = static_cast<uint32_t>(min(L::kChunkPacks, count - p)) * 16u;
                     if (lane == 0) {
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
         if (!ok) {
             if (lane == 0) note_timeout(a.timeouts);
             for (uint32_t i = g > static_cast<uint32_t>(NS) ? g - NS : 0u; i < g; ++i)
-                mbar_wait(&full[i % NS], (i / NS) & 1u);
+                wait_phase(&full[i % NS], (i / NS) & 1u);
         }
         return;
     }
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
     for (int64_t i = 0; i < my_rows; ++i) {
         const int64_t b = i / kBatch;
         const int side = static_cast<int>(b & 1);
-        if (i % kBatch == 0) ok = __all_sync(0xffffffffu, mbar_wait(&meta_full[side], (b >> 1) & 1));
+        if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&meta_full[side], (b >> 1) & 1));
         if (!ok) break;
         const PullMeta r = metas[side * kBatch + i % kBatch];
         int first, count;
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
             const int tp = r.target >= 0 && tb >= 0 ? tb / VE - first : -1;
             for (int p0 = 0; p0 < count; p0 += L::kChunkPacks, ++g) {
                 const int slot = static_cast<int>(g % NS);
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (g / NS) & 1u));
+                ok = __all_sync(0xffffffffu, wait_phase(&full[slot], (g / NS) & 1u));
                 if (!ok) break;
                 const uint4* st = reinterpret_cast<const uint4*>(sm + static_cast<size_t>(slot) * L::kStage);
                 uint4 raw[CP];
