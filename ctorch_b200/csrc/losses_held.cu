@@ -6,22 +6,26 @@
 // c + 2n, ... In a CTA
 //   * the producer warp copies the slices of the coming rows into a ring of shared-memory stages, one stage a
 //     row (bulk asynchronous copies), and reads the rows' small operands, 32 rows at a time;
-//   * the consumer warps take a slice into registers, find the warp's maximum, turn the logits into
-//     e = exp((x - m_w) / T) and send (m_w, sum e) to every CTA of the cluster (st.async into its mailbox,
-//     completion counted on its mbarrier: no cluster-wide barrier);
+//   * the consumer warps fold a slice into each warp's (m_w, sum of exp((x - m_w) / T)) and send it to every CTA
+//     of the cluster (st.async into its mailbox, completion counted on its mbarrier: no cluster-wide barrier);
 //   * the row warp joins the C * W partial sums and publishes the row's coefficient A;
-//   * the consumers put g = e * A exp((m_w - m) / T) over the slice in its stage, and the producer sends the
-//     stage to memory before it fills it again.
-// The consumers fold row r before they write row r - 1, so that the exchange of a row (0.2 us) and the row warp's
-// arithmetic (0.7 us) pass while they work. What a row's losses need is kept by the row warp and worked out for 32
-// rows at once, a lane a row.
+//   * the consumers write g = A exp((x - m) / T) from the stage to memory and give the stage back.
+// The consumers fold up to three rows ahead of the row that they write, so that the exchange of a row (0.2 us) and the
+// row warp's arithmetic (0.7 us) pass while they work. What a row's losses need is kept by the row warp and worked
+// out for 32 rows at once, a lane a row.
+//
+// Each logit takes two exponentials, one for the sum and one for the gradient, both from the stage. Keeping the first
+// in registers instead halves the use of the exponential unit, but that code is unrolled through and through (the
+// warps wait for instructions) and slices are half as wide. Policy loss on [8192, 131072] bf16, B200: 962 us with
+// exponentials kept (two CTAs of eight warps an SM), 1018 us kept for two rows, 780 us this way. Writing the gradient
+// into the stage and from there by bulk copies took 790 us (distillation 715 us against 627 us: the stage is given
+// back later).
 //
 // Distillation. The teacher's entries are prepared by a kernel of their own (loss_lists), a warp a row: q and the
-// sums that need no logit. The producer joins them with the row's slice when that has landed: it reads the
-// named logits, and puts -inf in their place in the stage, so that the consumers' sum is that of the others
-// (1 - sum p would lose it to cancellation) and their gradient there 0; the row warp then writes the named
-// elements' own gradient into the stage.
-#include <cstdlib>
+// sums that need no logit. Two list warps, in turns, join them with the rows: read the named logits, and put -inf in
+// their place in the landed stage, so that the consumers' sum is that of the others (1 - sum p would lose it to
+// cancellation) and their gradient there 0; when the consumers have written the row, the list warp writes the named
+// elements' own gradient over that.
 #include <string>
 
 #include "losses_ring.cuh"
@@ -138,16 +142,20 @@ struct ListInfo {
     double q_x, ref;  // sum of q (x - ref)
     double named;     // sum of exp((x - x_max) / T)
     float x_max;
-    uint32_t edge_named;  // the producer's own
+    uint32_t edge_named;  // the list warp's own
 };
 
 struct Coef {
-    float a, m, at_target, pad_;
+    float a, m;
+    float at_target;  // policy
+    float p_scale;    // distill: Q / s
 };
 
-constexpr int kSides = 4;   // rows whose sums and lists may be in use at once
+constexpr int kMaxDepth = 3;               // rows folded before the oldest of them is written
+constexpr int kSides = 2 * kMaxDepth + 2;  // rows whose sums and lists may be in use at once
 constexpr int kMaxRing = 8;
-constexpr int kAhead = 4;   // entries a lane of the producer fetches a row ahead
+constexpr int kAhead = 4;      // entries a lane of a list warp fetches a row ahead
+constexpr int kListWarps = 2;  // they take turns
 
 // What lies behind the ring's stages.
 template <int W> struct Shared {
@@ -155,23 +163,22 @@ template <int W> struct Shared {
     RowMeta meta[2][kBatch];
     float edge[2][kBatch][16];
     ListInfo list[kSides];
-    Coef coef[2];
-    struct {
-        void* to;
-        uint32_t bytes, pad_;
-    } out[kMaxRing];  // where a stage goes when its row is done (the producer's own)
+    Coef coef[kMaxDepth + 1];
     uint64_t full[kMaxRing], empty[kMaxRing], done[kMaxRing];
     uint64_t meta_full[2], meta_empty[2];
-    uint64_t list_full[kSides], list_empty[kSides];
-    uint64_t mail_full[kSides], coef_full[2];
+    uint64_t list_full[kSides];
+    uint64_t mail_full[kSides], coef_full[kMaxDepth + 1];
 };
 
-// Bytes behind the stages: Shared, then for distillation a bit a column of the slice (a byte a pack) and the
-// named logits of kSides rows.
+// Bytes behind the stages: Shared, then for distillation, for each list warp, a bit a column of the slice (a byte a
+// pack) and the named logits of the rows in use.
 template <int W> __host__ __device__ constexpr size_t bits_at() { return (sizeof(Shared<W>) + 15) / 16 * 16; }
+__host__ __device__ inline size_t bits_bytes(int slice_packs) { return (slice_packs + 15) / 16 * 16; }
 template <int W> __host__ __device__ inline size_t behind_bytes(int op, int top, int slice_packs) {
-    return op == kLossDistill ? bits_at<W>() + (slice_packs + 15) / 16 * 16 + static_cast<size_t>(kSides) * top * 4 : sizeof(Shared<W>);
+    return op == kLossDistill ? bits_at<W>() + kListWarps * bits_bytes(slice_packs) + static_cast<size_t>(kSides) * top * 4
+                              : sizeof(Shared<W>);
 }
+template <int OP, int W> __host__ __device__ constexpr int held_threads() { return (W + 2 + (OP == kLossDistill ? kListWarps : 0)) * 32; }
 
 // A position in the ring, advanced a row at a time.
 struct Ring {
@@ -189,8 +196,8 @@ struct Ring {
 
 // W consumer warps; `stages` stages of `stage_bytes`.
 template <class T, int OP, int W, int PER_SM>
-__global__ void __launch_bounds__(W * 32 + 64, PER_SM)
-    loss_held_kernel(const __grid_constant__ LossArgs a, int stages, int stage_bytes, int slice_packs) {
+__global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
+    loss_held_kernel(const __grid_constant__ LossArgs a, int stages, int stage_bytes, int slice_packs, int depth) {
     using P = PackOf<T>;
     using S = Shared<W>;
     constexpr int VE = P::VE, kCons = W * 32;
@@ -203,17 +210,16 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) {
             mbar_init(&sh.full[i], 1);
-            mbar_init(&sh.empty[i], OP == kLossDistill ? 1 : W);  // distill: the row warp's, after the named elements
+            mbar_init(&sh.empty[i], W);
             mbar_init(&sh.done[i], W);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.meta_full[i], 1);
-            mbar_init(&sh.meta_empty[i], W + 1);
-            mbar_init(&sh.coef_full[i], 1);
+            mbar_init(&sh.meta_empty[i], W + 1 + (OP == kLossDistill ? kListWarps : 0));
         }
+        for (int i = 0; i <= kMaxDepth; ++i) mbar_init(&sh.coef_full[i], 1);
         for (int i = 0; i < kSides; ++i) {
             mbar_init(&sh.list_full[i], 1);
-            mbar_init(&sh.list_empty[i], 1);
             mbar_init(&sh.mail_full[i], 1);
         }
         mbar_fence_init();
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.meta_full[side]);
         };
-        // Sends the stage's last row to memory and starts the copy of row i into it.
+        // Starts the copy of row i into the next stage.
         auto issue = [&](int i) {
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
             if (r.w == 0.0) return;
@@ -305,166 +311,18 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             if (!ok) return;
             if (lane == 0) {
                 unsigned char* st = sm + static_cast<size_t>(ring.slot) * stage_bytes;
-                auto& o = sh.out[ring.slot];
-                if (live >= static_cast<uint32_t>(stages) && o.bytes) {
-                    bulk_store(o.to, st, o.bytes);
-                    bulk_commit();
-                    bulk_wait_read();
-                }
                 const uint32_t bytes = static_cast<uint32_t>(r.count) * 16u;
                 mbar_arrive_expect_tx(&sh.full[ring.slot], bytes);
                 if (bytes) bulk_load(st, r.src, bytes, &sh.full[ring.slot]);
-                o.to = r.out;
-                o.bytes = r.out ? bytes : 0u;
             }
             __syncwarp();
             ring.next(stages);
             ++live;
         };
-        // Distill: entries lane, lane + 32, ... of the first kAhead * 32 of a row, fetched a row ahead.
-        int col_ahead[kAhead];
-        float q_ahead[kAhead];
-        auto fetch_list = [&](int64_t row) {
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int k = lane + 32 * u;
-                col_ahead[u] = k < a.top ? list_col[row * a.top + k] : -1;
-                q_ahead[u] = k < a.top ? list_q[row * a.top + k] : 0.f;
-            }
-        };
-        uint32_t listed = 0;
-        Ring list_ring;
-        auto join_list = [&](int i, int64_t next) {
-            const int side = static_cast<int>(listed % kSides), ms = i / kBatch & 1, mi = i % kBatch;
-            const RowMeta& r = sh.meta[ms][mi];
-            const T* x = X + loss_offset(a, kLrX, r.row);
-            float* e_x = reinterpret_cast<float*>(behind + bits_at<W>() + (slice_packs + 15) / 16 * 16) + side * a.top;
-            unsigned char* bits = behind + bits_at<W>();
-            unsigned char* st = sm + static_cast<size_t>(list_ring.slot) * stage_bytes;
-            ListInfo& li = sh.list[side];
-            int col[kAhead];
-            float q[kAhead];
-            T raw[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                col[u] = col_ahead[u];
-                q[u] = q_ahead[u];
-                if (col[u] >= 0) raw[u] = x[col[u]];
-            }
-            if (next >= 0) fetch_list(next);
-            for (int k = lane; k < (slice_packs + 15) / 16; k += 32) reinterpret_cast<uint4*>(bits)[k] = make_uint4(0u, 0u, 0u, 0u);
-            ok = __all_sync(0xffffffffu, wait_phase(&sh.list_empty[side], ((listed / kSides) & 1u) ^ 1u));
-            ok = __all_sync(0xffffffffu, ok && wait_phase(&sh.full[list_ring.slot], list_ring.phase));
-            if (!ok) return;
-            if (lane == 0) li.edge_named = 0u;
-            __syncwarp();
-            float x_max = -INFINITY;
-            float xs[kAhead];
-            T* twice_at = nullptr;
-            float* twice_edge = nullptr;
-            // notes a named logit and takes it out of this CTA's slice
-            auto take = [&](int k, int j, float xk) {
-                e_x[k] = xk;
-                x_max = fmaxf(x_max, xk);
-                if (j < 0) return;
-                const int at = j - r.body;
-                const bool inside = at >= 0 && at < r.count * VE;
-                const int l = j < 8 && (r.edges >> j & 1u) ? j : j >= r.behind ? 8 + j - r.behind : -1;
-                if (!inside && (rank != 0 || l < 0)) return;
-                uint32_t* word = inside ? reinterpret_cast<uint32_t*>(bits) + (at / VE >> 2) : &li.edge_named;
-                const uint32_t bit = inside ? 1u << ((at / VE & 3) * 8 + at % VE) : 1u << l;
-                const bool twice = atomicOr(word, bit) & bit;
-                if (twice) note_bad_index(a, j);
-                if (inside) {
-                    reinterpret_cast<T*>(st)[at] = LossElem<T>::down(-INFINITY);
-                    if (twice) twice_at = reinterpret_cast<T*>(st) + at;
-                } else {
-                    sh.edge[ms][mi][l] = -INFINITY;
-                    if (twice) twice_edge = &sh.edge[ms][mi][l];
-                }
-            };
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                xs[u] = col[u] >= 0 ? LossElem<T>::up(raw[u]) : -INFINITY;
-                if (lane + 32 * u < a.top) take(lane + 32 * u, col[u], xs[u]);
-            }
-            for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
-                const int j = list_col[r.row * a.top + k];
-                take(k, j, j >= 0 ? LossElem<T>::up(x[j]) : -INFINITY);
-            }
-            __syncwarp();
-            // a column named twice makes the whole row NaN
-            if (twice_at) *twice_at = LossElem<T>::down(NAN);
-            if (twice_edge) *twice_edge = NAN;
-            x_max = warp_max(x_max);
-            const float ref = x_max == -INFINITY ? 0.f : x_max;
-            float named = 0.f;
-            double q_x = 0.0;
-            auto add = [&](float qk, int j, float xk) {
-                if (j >= 0) named += exp_one(a, xk, ref);
-                if (qk != 0.f) q_x += static_cast<double>(qk) * (static_cast<double>(xk) - ref);
-            };
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) add(q[u], col[u], xs[u]);
-            for (int k = lane + 32 * kAhead; k < a.top; k += 32)
-                add(list_q[r.row * a.top + k], list_col[r.row * a.top + k], e_x[k]);
-            named = warp_sum(named);
-            q_x = warp_sum(q_x);
-            release_fence();
-            if (lane == 0) {
-                li.q_x = q_x;
-                li.ref = ref;
-                li.named = named;
-                li.x_max = x_max;
-                mbar_arrive(&sh.list_full[side]);
-            }
-            __syncwarp();
-            list_ring.next(stages);
-            ++listed;
-        };
-        if constexpr (OP == kLossPolicy) {
-            for (int i = 0; i < rows && ok; ++i) {
-                if (i % kBatch == 0) prepare();
-                if (ok) issue(i);
-            }
-        } else {
-            // A list is joined with its row once that has landed, so copies run `lead` rows ahead of the lists. The
-            // copy of row i + lead waits for row i + lead - stages, which must not itself wait for list i: the
-            // consumers finish row j after they have seen row j + 1.
-            const int lead = stages >= 6 ? stages - 4 : 1;
-            int issued = 0;
-            auto counts = [&](int i) { return sh.meta[i / kBatch & 1][i % kBatch].w != 0.0; };
-            int64_t ahead = -1;  // the row whose entries have been fetched
-            for (int i = 0; i < rows && ok; ++i) {
-                for (; issued <= i + lead && issued < rows && ok; ++issued) {
-                    if (issued % kBatch == 0) prepare();
-                    if (ok) issue(issued);
-                }
-                if (!ok || !counts(i)) continue;
-                const int64_t row = sh.meta[i / kBatch & 1][i % kBatch].row;
-                if (ahead != row) fetch_list(row);
-                int j = i + 1;
-                while (j < issued && !counts(j)) ++j;
-                ahead = j < issued ? sh.meta[j / kBatch & 1][j % kBatch].row : -1;
-                join_list(i, ahead);
-            }
+        for (int i = 0; i < rows && ok; ++i) {
+            if (i % kBatch == 0) prepare();
+            if (ok) issue(i);
         }
-        // the last rows
-        const uint32_t left = live < static_cast<uint32_t>(stages) ? live : static_cast<uint32_t>(stages);
-        Ring last;
-        if (live > left) last = ring;  // the ring is full: the oldest row is the next slot's
-        if (live > left) last.phase ^= 1u;
-        for (uint32_t k = 0; k < left && ok; ++k) {
-            ok = __all_sync(0xffffffffu, wait_phase(&sh.empty[last.slot], last.phase));
-            if (ok && lane == 0 && sh.out[last.slot].bytes)
-                bulk_store(sh.out[last.slot].to, sm + static_cast<size_t>(last.slot) * stage_bytes, sh.out[last.slot].bytes);
-            last.next(stages);
-        }
-        if (lane == 0) {
-            bulk_commit();
-            bulk_wait();
-        }
-        __syncwarp();
         if (!ok) {
             if (lane == 0) note_timeout(a.timeouts);
             // the copies in flight land before the CTA's memory goes away
@@ -474,7 +332,6 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
     } else if (warp == W + 1) {
         // ---- row warp: joins the sums, publishes the coefficient, and keeps what the losses are made of
         uint32_t live = 0;
-        Ring ring;
         double total = 0.0, kept_s = 0.0, kept_rest = 0.0, kept_x = 0.0, kept_ref = 0.0;  // kept_x: ratio, or sum q (x - ref)
         float kept_m = 0.f;
         for (int i = 0; i < rows && ok; ++i) {
@@ -483,7 +340,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             if (!ok) break;
             const RowMeta& r = sh.meta[ms][mi];
             if (r.w != 0.0) {
-                const int par = static_cast<int>(live & 1u), side = static_cast<int>(live % kSides);
+                const int cs = static_cast<int>(live % (kMaxDepth + 1)), side = static_cast<int>(live % kSides);
                 const uint32_t phase = (live / kSides) & 1u;
                 ok = wait_phase<true>(&sh.mail_full[side], phase);
                 if (OP == kLossDistill) ok = ok && wait_phase(&sh.list_full[side], phase);
@@ -517,7 +374,7 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                 if (mf == INFINITY) s = s_rest = quiet_nan();
                 Coef c;
                 c.m = mf;
-                c.at_target = c.pad_ = 0.f;
+                c.at_target = c.p_scale = 0.f;
                 double ratio = 0.0, big_q = 1.0;
                 if (OP == kLossPolicy) {
                     // s relative to the target's logit instead of the maximum: r = exp(-old) / s', p_t = 1 / s'
@@ -539,10 +396,11 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                     if (r.list.bad || !(s > 0.0)) s = quiet_nan();
                     c.a = static_cast<float>(distill_slope(a, r.w, s, s_rest, r.list.mass, r.list.count == a.cols, big_q));
                     if (s != s) c.a = NAN;
+                    c.p_scale = static_cast<float>(big_q) / static_cast<float>(s);
                 }
                 if (lane == 0) {
-                    sh.coef[par] = c;
-                    mbar_arrive(&sh.coef_full[par]);
+                    sh.coef[cs] = c;
+                    mbar_arrive(&sh.coef_full[cs]);
                 }
                 if (lane == mi) {
                     kept_s = s;
@@ -550,50 +408,6 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                     kept_m = mf;
                     kept_x = OP == kLossPolicy ? ratio : li.q_x;
                     kept_ref = OP == kLossPolicy ? 0.0 : li.ref;
-                }
-                if constexpr (OP == kLossDistill) {
-                    // The named elements of this CTA's slice, over what the consumers leave there.
-                    constexpr int kSome = 8;
-                    int col[kSome];
-                    float q[kSome];
-                    auto entry = [&](int k0) {
-#pragma unroll
-                        for (int u = 0; u < kSome; ++u) {
-                            const int k = k0 + lane + 32 * u;
-                            col[u] = r.grad && k < a.top ? list_col[r.row * a.top + k] : -1;
-                            q[u] = r.grad && k < a.top ? list_q[r.row * a.top + k] : 0.f;
-                        }
-                    };
-                    entry(0);
-                    const float* e_x = reinterpret_cast<const float*>(behind + bits_at<W>() + (slice_packs + 15) / 16 * 16) + side * a.top;
-                    ok = __all_sync(0xffffffffu, wait_phase(&sh.done[ring.slot], ring.phase));
-                    if (!ok) break;
-                    if (r.grad) {
-                        T* st = reinterpret_cast<T*>(sm + static_cast<size_t>(ring.slot) * stage_bytes);
-                        T* gr = static_cast<T*>(r.grad);
-                        const float scale = static_cast<float>(r.w * a.inv_temp), p_scale = static_cast<float>(big_q) / static_cast<float>(s);
-                        // a bad row is NaN throughout: its named columns too, whoever found it
-                        const float poison = c.a == c.a ? 0.f : c.a;
-                        for (int k0 = 0; k0 < a.top; k0 += 32 * kSome) {
-                            if (k0) entry(k0);
-#pragma unroll
-                            for (int u = 0; u < kSome; ++u) {
-                                const int j = col[u], at = j - r.body;
-                                const bool inside = at >= 0 && at < r.count * VE;
-                                const bool edge = (j < 8 && j >= 0 && (r.edges >> j & 1u)) || (rank == 0 && j >= r.behind);
-                                if (j < 0 || !(inside || edge)) continue;
-                                const T v = LossElem<T>::down(scale * (exp_one(a, e_x[k0 + lane + 32 * u], mf) * p_scale - q[u]) + poison);
-                                if (inside && r.out) st[at] = v;
-                                else gr[j * a.g_in] = v;
-                            }
-                        }
-                    }
-                    release_fence();
-                    if (lane == 0) {
-                        mbar_arrive(&sh.empty[ring.slot]);
-                        mbar_arrive(&sh.list_empty[side]);
-                    }
-                    ring.next(stages);
                 }
                 ++live;
             }
@@ -627,13 +441,198 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
         if (!ok && lane == 0) note_timeout(a.timeouts);
         total = warp_sum(total);
         if (a.partials && rank == 0 && lane == 0) a.partials[cluster] = total;
+    } else if (OP == kLossDistill && warp > W + 1) {
+        // ---- list warps: every other row that counts
+        const uint32_t mine = static_cast<uint32_t>(warp - W - 2);
+        const T* X = static_cast<const T*>(a.ptr[kLrX]);
+        unsigned char* bits = behind + bits_at<W>() + mine * bits_bytes(slice_packs);
+        float* const e_xs = reinterpret_cast<float*>(behind + bits_at<W>() + kListWarps * bits_bytes(slice_packs));
+        int col_ahead[kAhead];
+        float q_ahead[kAhead];
+        // Entries lane, lane + 32, ... of the first kAhead * 32 of a row, fetched a row ahead.
+        auto fetch = [&](int64_t row) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int k = lane + 32 * u;
+                col_ahead[u] = k < a.top ? list_col[row * a.top + k] : -1;
+                q_ahead[u] = k < a.top ? list_q[row * a.top + k] : 0.f;
+            }
+        };
+        // Joins row i's entries with its logits, and takes those out of the slice.
+        auto take = [&](int i, uint32_t l, const Ring& ring) {
+            const int side = static_cast<int>(l % kSides), ms = i / kBatch & 1, mi = i % kBatch;
+            const RowMeta& r = sh.meta[ms][mi];
+            const T* x = X + loss_offset(a, kLrX, r.row);
+            float* e_x = e_xs + side * a.top;
+            T* st = reinterpret_cast<T*>(sm + static_cast<size_t>(ring.slot) * stage_bytes);
+            ListInfo& li = sh.list[side];
+            int col[kAhead];
+            float q[kAhead];
+            T raw[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                col[u] = col_ahead[u];
+                q[u] = q_ahead[u];
+                if (col[u] >= 0) raw[u] = x[col[u]];
+            }
+            for (int k = lane; k < (slice_packs + 15) / 16; k += 32) reinterpret_cast<uint4*>(bits)[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (lane == 0) li.edge_named = 0u;
+            float x_max = -INFINITY;
+            float xs[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                xs[u] = col[u] >= 0 ? LossElem<T>::up(raw[u]) : -INFINITY;
+                x_max = fmaxf(x_max, xs[u]);
+                if (lane + 32 * u < a.top) e_x[lane + 32 * u] = xs[u];
+            }
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32) {
+                const int j = list_col[r.row * a.top + k];
+                const float xk = j >= 0 ? LossElem<T>::up(x[j]) : -INFINITY;
+                x_max = fmaxf(x_max, xk);
+                e_x[k] = xk;
+            }
+            x_max = warp_max(x_max);
+            const float ref = x_max == -INFINITY ? 0.f : x_max;
+            float named = 0.f;
+            double q_x = 0.0;
+            auto add = [&](float qk, int j, float xk) {
+                if (j >= 0) named += exp_one(a, xk, ref);
+                if (qk != 0.f) q_x += static_cast<double>(qk) * (static_cast<double>(xk) - ref);
+            };
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) add(q[u], col[u], xs[u]);
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32)
+                add(list_q[r.row * a.top + k], list_col[r.row * a.top + k], e_x[k]);
+            named = warp_sum(named);
+            q_x = warp_sum(q_x);
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.full[ring.slot], ring.phase));
+            if (!ok) return;
+            // -inf in the place of each; a column named twice makes the whole row NaN
+            T* twice_at = nullptr;
+            float* twice_edge = nullptr;
+            const int body = r.body, inside_end = r.count * VE, tail = r.behind;
+            const uint32_t edges = r.edges;
+            auto remove = [&](int j) {
+                const int at = j - body;
+                if (j < 0) return;
+                if (at >= 0 && at < inside_end) {
+                    const uint32_t bit = 1u << ((at / VE & 3) * 8 + at % VE);
+                    const bool twice = atomicOr(reinterpret_cast<uint32_t*>(bits) + (at / VE >> 2), bit) & bit;
+                    st[at] = LossElem<T>::down(-INFINITY);
+                    if (twice) twice_at = st + at;
+                } else if (rank == 0) {
+                    const int l16 = j < 8 && (edges >> j & 1u) ? j : j >= tail ? 8 + j - tail : -1;
+                    if (l16 < 0) return;
+                    const bool twice = atomicOr(&li.edge_named, 1u << l16) >> l16 & 1u;
+                    sh.edge[ms][mi][l16] = -INFINITY;
+                    if (twice) twice_edge = &sh.edge[ms][mi][l16];
+                } else {
+                    return;
+                }
+                if (twice_at || twice_edge) note_bad_index(a, j);
+            };
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) remove(col[u]);
+            for (int k = lane + 32 * kAhead; k < a.top; k += 32) remove(list_col[r.row * a.top + k]);
+            __syncwarp();
+            if (twice_at) *twice_at = LossElem<T>::down(NAN);
+            if (twice_edge) *twice_edge = NAN;
+            release_fence();
+            if (lane == 0) {
+                li.q_x = q_x;
+                li.ref = ref;
+                li.named = named;
+                li.x_max = x_max;
+                mbar_arrive(&sh.list_full[side]);
+            }
+            __syncwarp();
+        };
+        // The named elements of this CTA's slice of row i, over what the consumers have left there.
+        auto put = [&](int i, uint32_t l, const Ring& ring) {
+            const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
+            const float* e_x = e_xs + static_cast<int>(l % kSides) * a.top;
+            int col[kAhead];
+            float q[kAhead];
+            auto entries = [&](int k0) {
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int k = k0 + lane + 32 * u;
+                    col[u] = r.grad && k < a.top ? list_col[r.row * a.top + k] : -1;
+                    q[u] = r.grad && k < a.top ? list_q[r.row * a.top + k] : 0.f;
+                }
+            };
+            entries(0);
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.done[ring.slot], ring.phase));
+            if (!ok) return;
+            if (r.grad) {
+                const Coef c = sh.coef[l % (kMaxDepth + 1)];
+                T* gr = static_cast<T*>(r.grad);
+                const float scale = static_cast<float>(r.w * a.inv_temp);
+                // a bad row is NaN throughout: its named columns too, whoever found it
+                const float poison = c.a == c.a ? 0.f : c.a;
+                const int body = r.body, inside_end = r.count * VE, tail = r.behind;
+                const uint32_t edges = r.edges;
+                for (int k0 = 0; k0 < a.top; k0 += 32 * kAhead) {
+                    if (k0) entries(k0);
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int j = col[u], at = j - body;
+                        if (j < 0) continue;
+                        const bool inside = at >= 0 && at < inside_end;
+                        if (!inside && !((j < 8 && (edges >> j & 1u)) || (rank == 0 && j >= tail))) continue;
+                        const T v = LossElem<T>::down(scale * (exp_one(a, e_x[k0 + lane + 32 * u], c.m) * c.p_scale - q[u]) + poison);
+                        gr[j * a.g_in] = v;
+                    }
+                }
+            }
+            __syncwarp();
+        };
+        uint32_t live = 0, held_l = 0;
+        int held = -1, freed = 0;  // the row that waits for its named elements; batches given back
+        int64_t fetched = -1;
+        Ring ring, held_ring;
+        for (int i = 0; i < rows && ok; ++i) {
+            if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_full[i / kBatch & 1], (i / kBatch >> 1) & 1));
+            if (!ok) break;
+            const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
+            if (r.w != 0.0) {
+                if (live % kListWarps == mine) {
+                    if (fetched != r.row) fetch(r.row);
+                    take(i, live, ring);
+                    // this warp's next row, as far as it is known
+                    const int end = min(rows, (i / kBatch + 1) * kBatch);
+                    int k = i + 1, others = 0;
+                    for (; k < end; ++k)
+                        if (sh.meta[k / kBatch & 1][k % kBatch].w != 0.0 && ++others == kListWarps) break;
+                    fetched = k < end ? sh.meta[k / kBatch & 1][k % kBatch].row : -1;
+                    if (ok && fetched >= 0) fetch(fetched);
+                    if (ok && held >= 0) put(held, held_l, held_ring);
+                    held = i;
+                    held_l = live;
+                    held_ring = ring;
+                }
+                ring.next(stages);
+                ++live;
+            }
+            // The operands of a batch are read again only when those of the one before the last are given back, so a
+            // row does not wait past the end of the next batch, however few rows of that count.
+            if (ok && i % kBatch == kBatch - 1 && held >= 0 && held < i / kBatch * kBatch) {
+                put(held, held_l, held_ring);
+                held = -1;
+            }
+            for (; ok && (freed + 1) * kBatch <= (held >= 0 ? held : i + 1); ++freed)
+                if (lane == 0) mbar_arrive(&sh.meta_empty[freed & 1]);
+        }
+        if (ok && held >= 0) put(held, held_l, held_ring);
+        if (!ok && lane == 0) note_timeout(a.timeouts);
     } else {
         // ---- consumers
         const int t = threadIdx.x;
         const ExpConst kc = exp_const(a);
-        uint32_t live = 0;
-        Ring ring, held_ring;
-        int held = -1;  // the row that waits for its gradient
+        uint32_t live = 0, written = 0;  // rows that count: folded, written
+        Ring ring, write_ring;
+        int held[kMaxDepth] = {};  // the rows between, the latest first
+        int freed = 0;             // batches given back
         auto stage_of = [&](const Ring& g) { return reinterpret_cast<uint4*>(sm + static_cast<size_t>(g.slot) * stage_bytes); };
         // Folds row i: its sum goes to the cluster.
         auto fold = [&](int i, const RowMeta& r) {
@@ -680,20 +679,21 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
             }
             un(sum, s0, s1);
             const float s = warp_sum(s0 + s1);
-            // A side of the mailbox is written again four rows later: this warp has then waited for the coefficient of
-            // the row before the last one, which its own CTA published after it had read that row's side; and so
-            // had every CTA whose sums made up that coefficient read the side of two rows before.
+            // A side of the mailbox is written again kSides = 2 depth + 2 rows later. This warp has by then waited for
+            // the coefficient of depth + 1 rows ago, to which every warp of the cluster sent its sum after it had
+            // itself waited for the one of depth + 1 rows before that, published when its CTA had read that side.
             if (lane < size)
                 send8(&sh.mail[side][rank * W + warp], &sh.mail_full[side], lane,
                       static_cast<uint64_t>(__float_as_uint(m)) | static_cast<uint64_t>(__float_as_uint(s)) << 32);
         };
-        // Writes the gradient of row i, the l-th that counts.
-        auto write = [&](int i, uint32_t l) {
+        // Writes the gradient of row i, the next one.
+        auto write = [&](int i) {
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
-            ok = __all_sync(0xffffffffu, wait_phase(&sh.coef_full[l & 1u], (l >> 1) & 1u));
+            const uint32_t cs = written % (kMaxDepth + 1);
+            ok = __all_sync(0xffffffffu, wait_phase(&sh.coef_full[cs], (written / (kMaxDepth + 1)) & 1u));
             if (!ok) return;
-            const Coef c = sh.coef[l & 1u];
-            uint4* st = stage_of(held_ring) + t;
+            const Coef c = sh.coef[cs];
+            const uint4* st = stage_of(write_ring) + t;
             const int count = r.count - t;
             const F2 ga = f2(c.a, c.a), minus = f2(-c.m, -c.m);
             auto pack = [&](int p) {
@@ -704,12 +704,13 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                 return P::down(e);
             };
             if (r.out) {
+                uint4* const to = static_cast<uint4*>(r.out) + t;
 #pragma unroll 4
-                for (int p = 0; p * kCons < count; ++p) st[p * kCons] = pack(p);
+                for (int p = 0; p * kCons < count; ++p) to[p * kCons] = pack(p);
                 if (OP == kLossPolicy) {
                     const int at = r.target - r.body;  // the target's own value, by the thread that wrote its pack
                     if (r.target >= 0 && at >= 0 && at < r.count * VE && (at / VE) % kCons == t)
-                        reinterpret_cast<T*>(stage_of(held_ring))[at] = LossElem<T>::down(c.at_target);
+                        static_cast<T*>(r.out)[at] = LossElem<T>::down(c.at_target);
                 }
             } else if (r.grad) {
                 // where the gradient's rows are not aligned like the logits', or strided: element by element
@@ -728,22 +729,27 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                 const float v = c.a * exp_one(a, sh.edge[i / kBatch & 1][i % kBatch][t], c.m);
                 static_cast<T*>(r.grad)[j * a.g_in] = LossElem<T>::down(OP == kLossPolicy && j == r.target ? c.at_target : v);
             }
-            release_fence();  // the copy out of the stage, and the next one into it, come after this
-            if (lane == 0) mbar_arrive(OP == kLossDistill ? &sh.done[held_ring.slot] : &sh.empty[held_ring.slot]);
+            release_fence();
+            if (lane == 0) {
+                mbar_arrive(&sh.empty[write_ring.slot]);
+                if (OP == kLossDistill) mbar_arrive(&sh.done[write_ring.slot]);
+            }
+            write_ring.next(stages);
+            ++written;
         };
         for (int i = 0; i < rows && ok; ++i) {
             if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_full[i / kBatch & 1], (i / kBatch >> 1) & 1));
             if (!ok) break;
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
-            const bool counts = r.w != 0.0;
-            if (counts) fold(i, r);
-            if (ok && held >= 0) write(held, live - 1);
-            if (!ok) break;
-            held = -1;
-            if (counts) {
-                held = i;
-                held_ring = ring;
+            if (r.w != 0.0) {
+                fold(i, r);
+                const int oldest = depth == 1 ? held[0] : depth == 2 ? held[1] : held[2];
                 ring.next(stages);
+                if (ok && live - written == static_cast<uint32_t>(depth)) write(oldest);
+                if (!ok) break;
+                held[2] = held[1];
+                held[1] = held[0];
+                held[0] = i;
                 ++live;
             } else if (r.grad) {
                 T* gr = static_cast<T*>(r.grad);
@@ -754,10 +760,18 @@ __global__ void __launch_bounds__(W * 32 + 64, PER_SM)
                 if (t < 16 && (r.edges >> t & 1u)) gr[(t < 8 ? t : r.behind + t - 8) * a.g_in] = LossElem<T>::down(0.f);
             }
             __syncwarp();
-            // the batch before this one is done with: its last row has its gradient
-            if (i % kBatch == 0 && i > 0 && lane == 0) mbar_arrive(&sh.meta_empty[(i / kBatch - 1) & 1]);
+            // The operands of a batch are read again only when those of the one before the last are given back, so a
+            // row does not wait past the end of the next batch, however few rows of that count.
+            auto first_waiting = [&]() {
+                const uint32_t n = live - written;
+                return n == 0 ? i + 1 : n == 1 ? held[0] : n == 2 ? held[1] : held[2];
+            };
+            if (i % kBatch == kBatch - 1)
+                while (ok && first_waiting() < i / kBatch * kBatch) write(first_waiting());
+            for (; ok && (freed + 1) * kBatch <= first_waiting(); ++freed)
+                if (lane == 0) mbar_arrive(&sh.meta_empty[freed & 1]);
         }
-        if (ok && held >= 0) write(held, live - 1);
+        while (ok && written < live) write(live - written == 1 ? held[0] : live - written == 2 ? held[1] : held[2]);
         if (!ok && lane == 0) note_timeout(a.timeouts);
     }
     allow_dependents();
@@ -784,10 +798,9 @@ int held_typed(const LossArgs& a, int64_t cluster, int most_stages, int* parts, 
     if (stages < 3) return CTB_OK;
     const size_t smem = static_cast<size_t>(stages) * stage + rest;
     auto fn = loss_held_kernel<T, OP, W, PER_SM>;
-    const int threads = W * 32 + 64;
+    constexpr int threads = held_threads<OP, W>();
     int n = 0;
     if (int rc = resident_blocks(reinterpret_cast<const void*>(fn), threads, static_cast<int>(cluster), smem, &n)) return rc;
-    if (getenv("CTB_P")) printf("cluster %d stages %d resident %d\n", (int)cluster, (int)stages, n);
     int64_t clusters = n < a.rows ? n : a.rows;
     if (clusters > kLossMaxCtas) clusters = kLossMaxCtas;
     *parts = static_cast<int>(clusters);
@@ -798,7 +811,9 @@ int held_typed(const LossArgs& a, int64_t cluster, int most_stages, int* parts, 
     }
     LossArgs args = a;
     int ring = static_cast<int>(stages);
-    void* argv[4] = {&args, &ring, &stage, &slice};
+    // one stage loads and one goes out besides the rows that wait and the one that is folded
+    int depth = stages >= 6 ? 3 : stages >= 5 ? 2 : 1;
+    void* argv[5] = {&args, &ring, &stage, &slice, &depth};
     return launch_cluster(reinterpret_cast<const void*>(fn), static_cast<unsigned>(clusters * cluster), threads,
                           static_cast<int>(cluster), smem, st, argv);
 }
@@ -807,16 +822,24 @@ template <class T, int OP> int held_sized(const LossArgs& a, int* parts, cudaStr
     const int64_t v = a.cols;
     auto share = [&](int64_t most) { return (v + most - 1) / most; };
     *parts = -1;
-    static const int mode = getenv("CTB_MODE") ? atoi(getenv("CTB_MODE")) : 0;
-    const int64_t most = 65536 / sizeof(T);
-    if (mode == 1) return held_typed<T, OP, 8, 2>(a, share(most / 2), kMaxRing, parts, st);
-    if (mode == 2) return held_typed<T, OP, 8, 3>(a, share(most / 4), kMaxRing, parts, st);
-    if (mode == 3) return held_typed<T, OP, 4, 4>(a, share(most / 8), kMaxRing, parts, st);
-    if (mode == 4) return held_typed<T, OP, 4, 6>(a, share(most / 8), kMaxRing, parts, st);
-    if (mode == 5) return held_typed<T, OP, 14, 1>(a, share(most), kMaxRing, parts, st);
+    const int64_t most = 65536 / sizeof(T);  // logits of a slice that leaves room for three stages
     int64_t c = share(most);
-    if (getenv("CTB_C")) c = atoi(getenv("CTB_C"));
     if (c > kMaxCluster) return CTB_OK;
+    // few rows: more CTAs a row, down to 8 KiB each
+    while (c * 2 <= kMaxCluster && a.rows * c * 2 <= sm_count() && v * static_cast<int64_t>(sizeof(T)) >= c * 2 * 8192) c *= 2;
+    // A row costs a CTA about 2 us whatever its length (the exchange, the row's arithmetic, the copies' latency), so
+    // short slices want several CTAs an SM. Policy loss on B200, us, by the slice's bytes (bf16 rows), CTAs an SM x
+    // consumer warps:
+    //     bytes     1 x 16   2 x 8   3 x 8   4 x 4
+    //      8 KiB       701     411     409     266
+    //     12 KiB       385     228     234     194
+    //     16 KiB       391     249     234     411
+    //     24 KiB       413     346     411     359
+    //     32 KiB       435     484     432     793
+    const int64_t bytes = (v + c - 1) / c * static_cast<int64_t>(sizeof(T));
+    if (bytes <= 12 * 1024) return held_typed<T, OP, 4, 4>(a, c, kMaxRing, parts, st);
+    if (bytes <= 18 * 1024) return held_typed<T, OP, 8, 3>(a, c, kMaxRing, parts, st);
+    if (bytes <= 28 * 1024) return held_typed<T, OP, 8, 2>(a, c, kMaxRing, parts, st);
     return held_typed<T, OP, 16, 1>(a, c, kMaxRing, parts, st);
 }
 

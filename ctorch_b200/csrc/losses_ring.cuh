@@ -140,17 +140,6 @@ __device__ __forceinline__ float exp_one(const LossArgs& a, float x, float m) {
     return exp2_fast(fmaf(d, a.c2_rest, d));
 }
 
-// Copies `bytes` (a multiple of 16, both addresses on 16 bytes) from this CTA's shared memory to global memory,
-// as one of the issuing thread's bulk groups.
-__device__ __forceinline__ void bulk_store(void* gdst, const void* smem_src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_addr(smem_src)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// Until the thread's groups have read their shared memory; until they are written.
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 // Gives a stage back after the warp's reads of it. The reads may still be in flight when the next copy is
 // allowed to start, and that copy belongs to another proxy: without the fence, a refill was seen to
 // overtake them (a few packs at the start of a stage, once in some ten thousand stages).

@@ -561,6 +561,30 @@ def test_every_element_of_many_rows(v, dtype):
         assert ((top[b].double() - p).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_few_rows_that_count(dtype):
+    """Long runs of rows that do not count between a few that do, more rows than the kernels' clusters times the rows
+    whose operands they read together."""
+    rows, v = 40000, 700
+    x = torch.randn(rows, v, device="cuda").to(dtype)
+    t = torch.randint(v, (rows,), device="cuda")
+    old, adv = torch.full((rows,), -6.0, device="cuda"), torch.ones(rows, device="cuda")
+    index = torch.randint(v // 4, (rows, 4), device="cuda") + torch.arange(4, device="cuda") * (v // 4)
+    teacher = torch.randn(rows, 4, device="cuda")
+    full = [cb().policy_loss(x, t, old, adv, weights=torch.ones(rows, device="cuda")),
+            cb().distill_loss(x, teacher, index, weights=torch.ones(rows, device="cuda"))]
+    for share in (0.0, 0.0005, 0.01, 0.3):
+        on = torch.rand(rows, device="cuda") < share
+        some = [cb().policy_loss(x, t, old, adv, weights=on), cb().distill_loss(x, teacher, index, weights=on)]
+        for f, s in zip(full, some):
+            assert torch.equal(s.grad, torch.where(on[:, None], f.grad, torch.zeros_like(f.grad)))
+            assert torch.equal(s.row_loss, torch.where(on, f.row_loss, torch.zeros_like(f.row_loss)))
+        assert torch.equal(cb().token_logprobs(x, t, on).logprobs,
+                           torch.where(on, cb().token_logprobs(x, t).logprobs, torch.zeros((), device="cuda")))
+    import ctorch_b200._capi as C
+    assert C.wait_timeouts() == 0
+
+
 def test_rows_far_apart():
     """Row offsets beyond 2^31 elements."""
     v, step = 1000, (1 << 31) // 2 + 8
