@@ -37,6 +37,8 @@ __global__ void __launch_bounds__(256) loss_total(const double* partials, int n,
     }
 }
 
+constexpr int kPairThreads = 512;
+
 struct PairArgs {
     const double* logp;  // [rows], by row number
     double* up;          // [rows] gradient of each log-probability, optional
@@ -61,17 +63,6 @@ __device__ __forceinline__ void put_real(void* p, int dt, int64_t off, double v)
     else static_cast<double*>(p)[off] = v;
 }
 
-__device__ __forceinline__ double block_sum(double v, double* sm) {
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < 8; ++w) t += sm[w];
-    return t;
-}
-
 // log(1 + e^x)
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
@@ -79,11 +70,11 @@ __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log
 // of logp - ref over the sequence's counted rows and h = R_p - R_{pairs + p},
 //     loss = (1 - e) softplus(-h) + e softplus(h)
 //     dloss/dR_p = e sigma(h) - (1 - e) sigma(-h) = -dloss/dR_{pairs + p}.
-// The last CTA clears the rows of no sequence. Reads a few numbers a row, so it is bound by its latency.
-__global__ void __launch_bounds__(256) loss_pairs(LossArgs a, PairArgs p) {
+// With offsets, one more CTA clears the rows of no sequence. Reads a few numbers a row, so it is bound by its latency.
+__global__ void __launch_bounds__(kPairThreads) loss_pairs(LossArgs a, PairArgs p) {
     dependent_wait();
     allow_dependents();
-    __shared__ double sm[8];
+    __shared__ double sm[kPairThreads / 32][4];
     __shared__ int bad;
     const int64_t n = 2 * p.pairs;
     if (threadIdx.x == 0) bad = 0;
@@ -93,7 +84,7 @@ __global__ void __launch_bounds__(256) loss_pairs(LossArgs a, PairArgs p) {
     };
     // offsets that fall, or point outside the rows, would give one row to two sequences: then no pair is valid
     if (p.offsets) {
-        for (int64_t s = threadIdx.x; s <= n; s += 256) {
+        for (int64_t s = threadIdx.x; s <= n; s += kPairThreads) {
             const int64_t o = offset(s);
             if (o < 0 || o > a.rows || (s > 0 && o < offset(s - 1))) {
                 bad = 1;
@@ -104,7 +95,7 @@ __global__ void __launch_bounds__(256) loss_pairs(LossArgs a, PairArgs p) {
     }
     if (static_cast<int64_t>(blockIdx.x) == p.pairs) {
         const int64_t first = bad ? a.rows : offset(0), last = bad ? a.rows : offset(n);
-        for (int64_t r = threadIdx.x; r < a.rows; r += 256)
+        for (int64_t r = threadIdx.x; r < a.rows; r += kPairThreads)
             if (r < first || r >= last) {
                 put_row(a, kLrLogp, r, bad ? quiet_nan() : 0.0);
                 if (p.up) p.up[r] = bad ? quiet_nan() : 0.0;
@@ -124,21 +115,38 @@ __global__ void __launch_bounds__(256) loss_pairs(LossArgs a, PairArgs p) {
         }
         return;
     }
+    // both sequences' sums and counts, joined together
+    double sums[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         const int64_t s = side * p.pairs + pair, first = offset(s), last = offset(s + 1);
-        double sum = 0.0, count = 0.0;
-        for (int64_t r = first + threadIdx.x; r < last; r += 256) {
+        for (int64_t r = first + threadIdx.x; r < last; r += kPairThreads) {
             const bool on = !a.ptr[kLrWeight] || row_real(a, kLrWeight, r) != 0.0;
             const double lp = on ? p.logp[r] : 0.0;
             put_row(a, kLrLogp, r, lp);
             if (on) {
-                sum += a.ptr[kLrRef] ? lp - row_real(a, kLrRef, r) : lp;
-                count += 1.0;
+                sums[2 * side] += a.ptr[kLrRef] ? lp - row_real(a, kLrRef, r) : lp;
+                sums[2 * side + 1] += 1.0;
             }
         }
-        sum = block_sum(sum, sm);
-        if (p.average) share[side] = 1.0 / fmax(block_sum(count, sm), 1.0);
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sums[v] += __shfl_xor_sync(0xffffffffu, sums[v], d);
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sm[threadIdx.x >> 5][v] = sums[v];
+    __syncthreads();
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        double sum = 0.0, count = 0.0;
+#pragma unroll
+        for (int w = 0; w < kPairThreads / 32; ++w) {
+            sum += sm[w][2 * side];
+            count += sm[w][2 * side + 1];
+        }
+        if (p.average) share[side] = 1.0 / fmax(count, 1.0);
         reward[side] = p.beta * sum * share[side];
     }
     const double h = reward[0] - reward[1], e = p.smoothing;
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(256) loss_pairs(LossArgs a, PairArgs p) {
     for (int side = 0; side < 2; ++side) {
         const int64_t s = side * p.pairs + pair, first = offset(s), last = offset(s + 1);
         const double g = w == 0.0 ? 0.0 : (side ? -dh : dh) * share[side];
-        for (int64_t r = first + threadIdx.x; r < last; r += 256)
+        for (int64_t r = first + threadIdx.x; r < last; r += kPairThreads)
             p.up[r] = !a.ptr[kLrWeight] || row_real(a, kLrWeight, r) != 0.0 ? g : 0.0;
     }
 }
@@ -626,7 +634,7 @@ int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets, int64_t
         p.beta = beta;
         p.smoothing = label_smoothing;
         p.average = average;
-        launch_dependent(loss_pairs, static_cast<unsigned>(pairs + 1), 256, 0, st, a, p);
+        launch_dependent(loss_pairs, static_cast<unsigned>(pairs + (offsets ? 1 : 0)), kPairThreads, 0, st, a, p);
         count_launch();
         CTB_TRY(check_launch("loss pairs"));
         // 3: the gradient

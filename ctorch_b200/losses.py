@@ -40,6 +40,9 @@ _SIZE = {torch.float32: 4, torch.float64: 8, torch.bfloat16: 2}
 _VIEW = [struct.Struct(f"<Qii{n}q{8 * (C.MAX_DIMS - n)}x{n}q{8 * (C.MAX_DIMS - n)}x") for n in range(C.MAX_DIMS + 1)]
 
 
+_VIEW1 = _VIEW[1].pack
+
+
 def _view(t):
     if t is None:
         return None
@@ -79,17 +82,24 @@ def _run(name, dev, fn, *args):
             _call(fn(*args, C.raw_stream(dev)), name)
 
 
-def _results(logits, dev, sizes, scratch=0):
-    """One allocation for scratch (bytes, first) and results of `sizes` elements in the type of a row's
-    results; returns the scratch's address and the results."""
-    dt = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    lead = -(-scratch // (8 if dt == torch.float64 else 4))
-    flat = torch.empty(lead + sum(sizes), dtype=dt, device=dev)
-    return flat.data_ptr(), flat.split_with_sizes([lead, *sizes])[1:]
-
-
-def _shaped(t, rows):
-    return t if len(rows) == 1 else t.view(rows)
+def _results(logits, dev, rows, per_row, others, scratch=0):
+    """One allocation for scratch (bytes, first), `per_row` results of the leading shape `rows` and vectors of
+    `others` elements, in the type of a row's results. Returns the scratch's address, the results and their
+    packed views."""
+    f64 = logits.dtype == torch.float64
+    size, code = (8, C.F64) if f64 else (4, C.F32)
+    sizes = [-(-scratch // size)] + [prod(rows)] * per_row + others
+    flat = torch.empty(sum(sizes), dtype=torch.float64 if f64 else torch.float32, device=dev)
+    base = at = flat.data_ptr()
+    out = flat.split_with_sizes(sizes)[1:]
+    views = []
+    for before, n in zip(sizes, sizes[1:]):
+        at += before * size
+        views.append(_VIEW1(at, code, 1, n, 1))
+    if len(rows) != 1:
+        out = [t.view(rows) for t in out[:per_row]] + list(out[per_row:])
+        views[:per_row] = [_view(t) for t in out[:per_row]]
+    return base, out, views
 
 
 def _grad_for(name, logits, out, dev):
@@ -143,12 +153,9 @@ def token_logprobs(logits, targets, mask=None, temperature: float = 1.0, status=
     token_logprobs_backward() pulls a gradient back through it."""
     name = "token_logprobs"
     dev = _check(name, logits, targets, mask)
-    rows = logits.shape[:-1]
-    n = prod(rows)
-    _, (logp, lse) = _results(logits, dev, [n, n])
-    logp, lse = _shaped(logp, rows), _shaped(lse, rows)
-    _run(name, dev, C.lib.ctb_token_logprobs, _view(logits), _view(targets), _view(mask), temperature, _view(logp),
-         _view(lse), _status(name, status, dev))
+    _, (logp, lse), (v_logp, v_lse) = _results(logits, dev, logits.shape[:-1], 2, [])
+    _run(name, dev, C.lib.ctb_token_logprobs, _view(logits), _view(targets), _view(mask), temperature, v_logp, v_lse,
+         _status(name, status, dev))
     return TokenLogprobs(logp, lse)
 
 
@@ -165,8 +172,8 @@ def token_logprobs_backward(grad_logprobs, logits, targets, logprobs, lse, mask=
     return grad
 
 
-def _scale(weights, n):
-    return 1.0 if weights is not None else 1.0 / max(n, 1)
+def _scale(weights, rows):
+    return 1.0 if weights is not None else 1.0 / max(prod(rows), 1)
 
 
 def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weights=None, temperature: float = 1.0,
@@ -182,16 +189,14 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weig
     name = "distill_loss"
     dev = _check(name, logits, teacher_logits, teacher_indices, teacher_lse, weights)
     rows = logits.shape[:-1]
-    n = prod(rows)
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
     need = C.lib.ctb_loss_scratch_bytes(vx, 0, teacher_logits.shape[-1] if teacher_logits.dim() else 0)
-    scratch, (row_loss, loss) = _results(logits, dev, [n, 1], need)
-    row_loss, loss = _shaped(row_loss, rows), loss.view(())
+    scratch, (row_loss, loss), (v_row, v_loss) = _results(logits, dev, rows, 1, [1], need)
     _run(name, dev, C.lib.ctb_distill_loss, vx, _view(teacher_logits), _view(teacher_indices), _view(teacher_lse),
-         _view(weights), _scale(weights, n), temperature, _view(loss), _view(row_loss), _view(g),
-         _status(name, status, dev), scratch, need)
-    return DistillLoss(loss, row_loss, g)
+         _view(weights), _scale(weights, rows), temperature, v_loss, v_row, _view(g), _status(name, status, dev),
+         scratch, need)
+    return DistillLoss(loss.squeeze_(0), row_loss, g)
 
 
 def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, weights=None, clip_low: float = 0.2,
@@ -207,16 +212,14 @@ def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, we
     name = "policy_loss"
     dev = _check(name, logits, targets, old_logprobs, advantages, ref_logprobs, weights)
     rows = logits.shape[:-1]
-    n = prod(rows)
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
     need = C.lib.ctb_loss_scratch_bytes(vx, 0, 0)
-    scratch, (row_loss, logp, kl, loss) = _results(logits, dev, [n, n, n, 1], need)
-    row_loss, logp, kl, loss = _shaped(row_loss, rows), _shaped(logp, rows), _shaped(kl, rows), loss.view(())
+    scratch, (row_loss, logp, kl, loss), (v_row, v_logp, v_kl, v_loss) = _results(logits, dev, rows, 3, [1], need)
     _run(name, dev, C.lib.ctb_policy_loss, vx, _view(targets), _view(old_logprobs), _view(advantages),
-         _view(ref_logprobs), _view(weights), _scale(weights, n), clip_low, clip_high, kl_coef, temperature,
-         _view(loss), _view(row_loss), _view(logp), _view(kl), _view(g), _status(name, status, dev), scratch, need)
-    return PolicyLoss(loss, row_loss, logp, kl, g)
+         _view(ref_logprobs), _view(weights), _scale(weights, rows), clip_low, clip_high, kl_coef, temperature,
+         v_loss, v_row, v_logp, v_kl, _view(g), _status(name, status, dev), scratch, need)
+    return PolicyLoss(loss.squeeze_(0), row_loss, logp, kl, g)
 
 
 def preference_loss(logits, targets, pairs: int, ref_logprobs=None, mask=None, offsets=None, weights=None,
@@ -238,13 +241,12 @@ def preference_loss(logits, targets, pairs: int, ref_logprobs=None, mask=None, o
     dev = _check(name, logits, targets, ref_logprobs, mask, offsets, weights)
     if pairs < 1:
         raise ValueError(f"ctorch::{name}: pairs must be at least 1")
-    rows = logits.shape[:-1]
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
     need = C.lib.ctb_loss_scratch_bytes(vx, pairs, 0)
-    scratch, (logp, pair_loss, rewards, loss) = _results(logits, dev, [prod(rows), pairs, 2 * pairs, 1], need)
-    logp, loss = _shaped(logp, rows), loss.view(())
+    scratch, (logp, pair_loss, rewards, loss), (v_logp, v_pair, v_rewards, v_loss) = _results(
+        logits, dev, logits.shape[:-1], 1, [pairs, 2 * pairs, 1], need)
     _run(name, dev, C.lib.ctb_preference_loss, vx, _view(targets), pairs, _view(offsets), _view(ref_logprobs),
-         _view(mask), _view(weights), _scale(weights, pairs), beta, label_smoothing, int(average), _view(loss),
-         _view(pair_loss), _view(rewards), _view(logp), _view(g), _status(name, status, dev), scratch, need)
-    return PreferenceLoss(loss, pair_loss, rewards, logp, g)
+         _view(mask), _view(weights), _scale(weights, (pairs,)), beta, label_smoothing, int(average), v_loss, v_pair,
+         v_rewards, v_logp, _view(g), _status(name, status, dev), scratch, need)
+    return PreferenceLoss(loss.squeeze_(0), pair_loss, rewards, logp, g)
