@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                     r.grad = g;
                     if (a.g_in == 1 && (reinterpret_cast<uintptr_t>(g + r.body) & 15) == 0) r.out = g + r.body;
                 }
-                if (rank == 0) r.edges = (1u << head) - 1 | ((1u << (static_cast<int>(a.cols) - r.behind)) - 1) << 8;
+                if (rank == 0) r.edges = edges_of(a, head, r.behind);
                 r.target = -1;
                 if (OP == kLossPolicy && r.w != 0.0) {
                     const int64_t t = load_index(a.ptr[kLrTarget], a.dtype[kLrTarget], loss_offset(a, kLrTarget, r.row));
@@ -291,15 +291,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 }
                 sh.meta[side][lane] = r;
             }
-            for (int i = 0; i < n; ++i) {
-                const uint32_t there = __shfl_sync(0xffffffffu, r.w != 0.0 ? r.edges : 0u, i);
-                if (!there) continue;
-                const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
-                const int tail = __shfl_sync(0xffffffffu, r.behind, i);
-                if (lane < 16)
-                    sh.edge[side][i][lane] =
-                        there >> lane & 1u ? LossElem<T>::up(X[off + (lane < 8 ? lane : tail + lane - 8)]) : -INFINITY;
-            }
+            if (rank == 0) read_edges(X, x_off, r.w != 0.0 ? r.edges : 0u, r.behind, n, lane, &sh.edge[side][0][0]);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.meta_full[side]);
         };
@@ -725,7 +717,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 for (int p = 0; p * kCons < count; ++p) scatter(p, pack(p));
             }
             if (r.grad && t < 16 && (r.edges >> t & 1u)) {
-                const int j = t < 8 ? t : r.behind + t - 8;
+                const int j = edge_column(t, r.behind);
                 const float v = c.a * exp_one(a, sh.edge[i / kBatch & 1][i % kBatch][t], c.m);
                 static_cast<T*>(r.grad)[j * a.g_in] = LossElem<T>::down(OP == kLossPolicy && j == r.target ? c.at_target : v);
             }
@@ -757,7 +749,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                     for (int p = t; p < r.count; p += kCons) static_cast<uint4*>(r.out)[p] = make_uint4(0u, 0u, 0u, 0u);
                 else
                     for (int k = t; k < r.count * VE; k += kCons) gr[(r.body + k) * a.g_in] = LossElem<T>::down(0.f);
-                if (t < 16 && (r.edges >> t & 1u)) gr[(t < 8 ? t : r.behind + t - 8) * a.g_in] = LossElem<T>::down(0.f);
+                if (t < 16 && (r.edges >> t & 1u)) gr[edge_column(t, r.behind) * a.g_in] = LossElem<T>::down(0.f);
             }
             __syncwarp();
             // The operands of a batch are read again only when those of the one before the last are given back, so a

@@ -115,15 +115,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) loss_token_kernel(const __gr
                 metas[side * kBatch + lane] = r;
             }
             if (rank == 0) {
-                for (int i = 0; i < n; ++i) {
-                    const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
-                    const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
-                    const bool counts = __shfl_sync(0xffffffffu, r.w != 0.0, i);
-                    if (lane < 16) {
-                        const int64_t at = edge_position(a, head, packs, VE, lane);
-                        edges[(side * kBatch + i) * 16 + lane] = at >= 0 && counts ? LossElem<T>::up(X[off + at]) : -INFINITY;
-                    }
-                }
+                const int behind = r.head + r.packs * VE;
+                read_edges(X, x_off, r.w != 0.0 ? edges_of(a, r.head, behind) : 0u, behind, n, lane, edges + side * kBatch * 16);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&meta_full[side]);
@@ -363,15 +356,8 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
                 metas[side * kBatch + lane] = r;
             }
             if (rank == 0) {
-                for (int i = 0; i < n; ++i) {
-                    const int64_t off = __shfl_sync(0xffffffffu, x_off, i);
-                    const int head = __shfl_sync(0xffffffffu, r.head, i), packs = __shfl_sync(0xffffffffu, r.packs, i);
-                    const bool zero = __shfl_sync(0xffffffffu, r.zero, i);
-                    if (lane < 16) {
-                        const int64_t at = edge_position(a, head, packs, VE, lane);
-                        if (at >= 0 && !zero) edges[(side * kBatch + i) * 16 + lane] = LossElem<T>::up(X[off + at]);
-                    }
-                }
+                const int behind = r.head + r.packs * VE;
+                read_edges(X, x_off, lane < n && !r.zero ? edges_of(a, r.head, behind) : 0u, behind, n, lane, edges + side * kBatch * 16);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&meta_full[side]);
@@ -425,7 +411,8 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
                 for (int k = 0; k < VE; ++k) dst[k * a.g_in] = ov[k];
             }
         };
-        const int64_t edge_at = rank == 0 && t < 16 ? edge_position(a, r.head, r.packs, VE, t) : -1;
+        const int behind = r.head + r.packs * VE;
+        const int edge_at = rank == 0 && t < 16 && (edges_of(a, r.head, behind) >> t & 1u) ? edge_column(t, behind) : -1;
         if (edge_at >= 0) {
             const float x = edges[(side * kBatch + i % kBatch) * 16 + t];
             const float v = r.zero ? 0.f : r.target == edge_at ? r.at_target : r.a * row_exp_shifted(a, x, r.at, r.shift);
