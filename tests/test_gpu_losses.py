@@ -93,6 +93,36 @@ def test_token_logprobs(rows, v, kind, how):
         check(grad, (want, tol), "grad")
 
 
+@pytest.mark.parametrize("kind,rows,v", [("bf16", 50, 65536), ("bf16", 2, 262144), ("bf16", 2, 262147), ("bf16", 1, 600001),
+                                         ("f32", 3, 131075), ("f32", 40, 100000), ("f32", 20, 50000)])
+def test_long_rows(kind, rows, v):
+    """Rows split over clusters of every size, up to the longest that a cluster holds, and beyond that."""
+    rng = np.random.default_rng(v)
+    x, hx = make(rng, rows, v, kind)
+    t = rng.integers(0, v, rows)
+    on = np.ones(rows, bool)
+    r = cb().token_logprobs(x, dev(t))
+    logp, lt, lse, st = O.token(hx, t, on, 1.0, kind)
+    check(r.logprobs, (logp, lt), "logprobs")
+    old, adv, w = (logp + 0.05).astype(np.float32), rng.normal(size=rows).astype(np.float32), np.full(rows, 0.5, np.float32)
+    f = lambda a: a.astype(np.float64)
+    want = O.policy(hx, t, f(old), f(adv), None, f(w), 0.2, 0.2, 0.0, 1.0, kind)
+    assert want["edge"].min() > 1e-5
+    got = cb().policy_loss(x, dev(t), dev(old), dev(adv), weights=dev(w))
+    for name in ("logprobs", "row_loss", "loss", "grad"):
+        check(getattr(got, name), want[name], name)
+    for top in (100, 2048):
+        index = np.stack([rng.permutation(v)[:top] for _ in range(rows)])
+        teacher = rng.normal(size=(rows, top)).astype(np.float32)
+        tl = (np.log(np.exp(f(teacher)).sum(1)) + 0.3).astype(np.float32)
+        want = O.distill(hx, f(teacher), index, f(tl), f(w), 1.0, kind)
+        got = cb().distill_loss(x, dev(teacher), dev(index), dev(tl), dev(w))
+        for name in ("row_loss", "loss", "grad"):
+            check(getattr(got, name), want[name], name)
+    import ctorch_b200._capi as C
+    assert C.wait_timeouts() == 0
+
+
 def test_leading_dims_and_broadcast_operands():
     rng = np.random.default_rng(5)
     b, l, v = 3, 5, 130
