@@ -366,6 +366,7 @@ int check_status(const int32_t* status) {
 }
 
 int run_rows(const LossPlan& p, int* parts, cudaStream_t st) {
+    if (loss_short_fit(p)) return loss_short(p, parts, st);
     if (loss_stream_fit(p.args)) {
         if (p.op == kLossToken) return loss_token_stream(p.args, st);
         if (int rc = loss_held(p, parts, st)) return rc;
@@ -375,6 +376,7 @@ int run_rows(const LossPlan& p, int* parts, cudaStream_t st) {
 }
 
 int run_backward(const LossArgs& a, cudaStream_t st) {
+    if (loss_backward_short_fit(a)) return loss_backward_short(a, st);
     return loss_stream_fit(a) ? loss_backward_stream(a, st) : loss_backward_general(a, st);
 }
 

@@ -265,13 +265,17 @@ template <class Acc> struct BackwardRow {
     int zero;        // nothing comes back to this row: its logits are not read
 };
 
+__device__ __forceinline__ double row_upstream(const LossArgs& a, int64_t row) {
+    return row_weight(a, row) != 0.0 ? row_real(a, kLrUp, row) : 0.0;
+}
+
 template <class T>
-__device__ __forceinline__ BackwardRow<typename LossElem<T>::Acc> backward_row(const LossArgs& a, int64_t row, const T* x) {
+__device__ __forceinline__ BackwardRow<typename LossElem<T>::Acc> backward_row(const LossArgs& a, int64_t row, const T* x,
+                                                                               double up) {
     using Acc = typename LossElem<T>::Acc;
     BackwardRow<Acc> b;
     b.at = b.shift = b.a = b.at_target = 0;
     b.target = -1;
-    const double up = row_weight(a, row) != 0.0 ? row_real(a, kLrUp, row) : 0.0;
     b.zero = up == 0.0;
     if (b.zero) return b;
     const double g = up * a.inv_temp;
@@ -328,6 +332,10 @@ constexpr int kLossMaxCtas = 148 * 16;
 bool loss_stream_fit(const LossArgs& a);                                      // losses_stream.cu
 int loss_token_stream(const LossArgs& a, cudaStream_t st);                    // losses_stream.cu
 int loss_backward_stream(const LossArgs& a, cudaStream_t st);                 // losses_stream.cu
+bool loss_short_fit(const LossPlan& p);                                       // losses_short.cu
+bool loss_backward_short_fit(const LossArgs& a);                              // losses_short.cu
+int loss_short(const LossPlan& p, int* parts, cudaStream_t st);               // losses_short.cu
+int loss_backward_short(const LossArgs& a, cudaStream_t st);                  // losses_short.cu
 // *parts: how many partial sums were written; negative when the rows are too long (nothing was launched).
 int loss_held(const LossPlan& p, int* parts, cudaStream_t st);                // losses_held.cu
 size_t loss_lists_bytes(int64_t rows, int64_t top);                           // losses_held.cu

@@ -236,7 +236,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) loss_backward_any
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* x = X + loss_offset(a, kLrX, row);
         T* g = G + loss_offset(a, kLrGrad, row);
-        if (threadIdx.x == 0) b = backward_row<T>(a, row, x);
+        if (threadIdx.x == 0) b = backward_row<T>(a, row, x, row_upstream(a, row));
         __syncthreads();
         const BackwardRow<Acc> c = b;
         for (int64_t j = threadIdx.x; j < a.cols; j += kThreads)

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kCons + 32, PER_SM) loss_pull_kernel(const __g
                 const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(X + x_off) & 15)) & 15) / sizeof(T);
                 r.head = static_cast<int>(head < a.cols ? head : a.cols);
                 r.packs = static_cast<int>((a.cols - r.head) / VE);
-                const BackwardRow<float> c = backward_row<T>(a, row, X + x_off);
+                const BackwardRow<float> c = backward_row<T>(a, row, X + x_off, row_upstream(a, row));
                 r.at = c.at;
                 r.shift = c.shift;
                 r.a = c.a;

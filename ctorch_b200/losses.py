@@ -103,9 +103,10 @@ def _results(logits, dev, rows, per_row, others, scratch=0):
 
 
 def _grad_for(name, logits, out, dev):
-    """The gradient's tensor: `out` (checked), or a new one whose rows lie like the logits' rows. Where
-    those all start on 16 bytes although V elements are not a multiple of it (a vocabulary padded in
-    memory), so do the new one's: rows of the two that are aligned alike move in 16-byte pieces."""
+    """The gradient's tensor: `out` (checked), or a new one. Rows of the two that are aligned alike modulo 16
+    bytes move in 16-byte pieces, so the new one's rows lie like the logits' rows: where those all start
+    on 16 bytes although V elements are not a multiple of it (a vocabulary padded in memory), so do the
+    new one's; where they start anywhere, it takes the logits' strides if that wastes little."""
     if out is not None:
         _cuda(name, logits, out)
         if out.dtype != logits.dtype:
@@ -115,13 +116,22 @@ def _grad_for(name, logits, out, dev):
         if may_overlap(out, logits) and not _same_view(out, logits):
             raise AliasError(f"ctorch::{name}: the gradient overlaps the logits without being the same view")
         return out
-    if logits.is_contiguous():
-        return torch.empty_like(logits)
-    shape, size, v = logits.shape, _SIZE[logits.dtype], logits.shape[-1]
-    if v * size % 16 and logits.dim() > 1 and logits.data_ptr() % 16 == 0 and \
-            all(st * size % 16 == 0 for s, st in zip(shape[:-1], logits.stride()) if s > 1):
-        pitch = -(-v * size // 128) * 128 // size
-        return torch.empty((*shape[:-1], pitch), dtype=logits.dtype, device=dev)[..., :v]
+    shape, strides, size = logits.shape, logits.stride(), _SIZE[logits.dtype]
+    lead, v = logits.data_ptr() % 16 // size, shape[-1]
+    if (logits.is_contiguous() and lead == 0) or logits.numel() == 0:
+        return torch.empty(shape, dtype=logits.dtype, device=dev)
+    if lead == 0 and all(st * size % 16 == 0 for s, st in zip(shape[:-1], strides) if s > 1):
+        if v * size % 16 and logits.dim() > 1:
+            pitch = -(-v * size // 128) * 128 // size
+            return torch.empty((*shape[:-1], pitch), dtype=logits.dtype, device=dev)[..., :v]
+    elif strides[-1] == 1:
+        span = 1  # elements from the first to the last, if the dims nest
+        for st, s in sorted((st, s) for s, st in zip(shape, strides) if s > 1):
+            span = span + (s - 1) * st if st >= span else 0
+            if not span:
+                break
+        if 0 < span <= logits.numel() * 5 // 4:
+            return torch.empty(lead + span, dtype=logits.dtype, device=dev).as_strided(shape, strides, lead)
     return torch.empty(shape, dtype=logits.dtype, device=dev)
 
 

@@ -93,6 +93,50 @@ def test_token_logprobs(rows, v, kind, how):
         check(grad, (want, tol), "grad")
 
 
+# 16-byte packs of a row around every number of them that a warp holds, and what is too long for a warp
+PACKS = [0, 1, 31, 32, 33, 64, 65, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 1700]
+
+
+@pytest.mark.parametrize("how", ["contiguous", "pitched", "offset"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("packs", PACKS)
+def test_rows_by_length(packs, kind, how):
+    size = 4 if kind == "f32" else 2
+    for more in (0, 16 // size - 1):
+        rows, v = 21, packs * 16 // size + more
+        if v == 0:
+            continue
+        rng = np.random.default_rng(v)
+        x, hx = make(rng, rows, v, kind)
+        t = rng.integers(0, v, rows)
+        t[:4] = [0, v - 1, v // 2, min(v - 1, 8)]
+        w = np.where(rng.random(rows) < 0.7, rng.random(rows), 0.0).astype(np.float32)
+        w[:4] = 0.5
+        on = w != 0
+        y = layouts(x, how)
+        r = cb().token_logprobs(y, dev(t), dev(w))
+        logp, lt, lse, st = O.token(hx, t, on, 1.0, kind)
+        check(r.logprobs, (logp, np.where(on, lt, 0)), "logprobs")
+        check(r.lse, (lse, np.where(on, st, 0)), "lse")
+        up = rng.normal(size=rows).astype(np.float32)
+        extra = np.minimum(lt, st) + 2 * O.EPS["f32"] * np.abs(logp)
+        want, tol = O.pull(hx, t, np.where(on, up, 0.0).astype(np.float64), 0.0, 1.0, kind, extra)
+        check(cb().token_logprobs_backward(dev(up), y, dev(t), r.logprobs, r.lse, dev(w)), (want, tol), "grad")
+        other = torch.full((rows, v + 1), 5.0, dtype=y.dtype, device="cuda")  # rows aligned unlike the logits'
+        cb().token_logprobs_backward(dev(up), y, dev(t), r.logprobs, r.lse, dev(w), out=other[:, 1:])
+        check(other[:, 1:], (want, tol), "grad into a view")
+        assert (other[:, 0] == 5.0).all()
+        old = (O.token(hx, t, np.ones(rows, bool), 1.0, "f64")[0] + 0.3 * rng.normal(size=rows)).astype(np.float32)
+        f = lambda a: a.astype(np.float64)
+        want = O.policy(hx, t, f(old), f(up), f(old), f(w), 0.1, 0.3, 0.1, 1.0, kind)
+        assert want["edge"].min() > 1e-6
+        got = cb().policy_loss(y, dev(t), dev(old), dev(up), dev(old), dev(w), 0.1, 0.3, 0.1)
+        for name in ("logprobs", "row_loss", "kl", "loss", "grad"):
+            check(getattr(got, name), want[name], name)
+        same = cb().policy_loss(y, dev(t), dev(old), dev(up), dev(old), dev(w), 0.1, 0.3, 0.1, out_grad=y)
+        assert same.grad is y and torch.equal(y, got.grad)
+
+
 @pytest.mark.parametrize("kind,rows,v", [("bf16", 50, 65536), ("bf16", 2, 262144), ("bf16", 2, 262147), ("bf16", 1, 600001),
                                          ("f32", 3, 131075), ("f32", 40, 100000), ("f32", 20, 50000)])
 def test_long_rows(kind, rows, v):
@@ -564,7 +608,16 @@ def test_every_element_of_many_rows(v, dtype):
     against float64, so that one pack read from the wrong copy shows. A pack of another row is off by a
     factor; the bound is 2^-15 of each element (64 roundings of float32 and more, see losses_oracle), and half a
     step of bfloat16."""
-    rows = 2000
+    every_element(2000, v, dtype)
+
+
+@pytest.mark.parametrize("rows,v,dtype", [(2100, 20001, torch.bfloat16), (2200, 9003, torch.float32), (20000, 1003, torch.float32),
+                                          (20000, 2048, torch.bfloat16), (50000, 130, torch.bfloat16), (6000, 8192, torch.bfloat16)])
+def test_every_element_of_rows_that_a_warp_takes_whole(rows, v, dtype):
+    every_element(rows, v, dtype)
+
+
+def every_element(rows, v, dtype):
     g = torch.Generator(device="cuda")
     g.manual_seed(v)
     x = (2 * torch.randn(rows, v, generator=g, device="cuda")).to(dtype)
@@ -581,7 +634,7 @@ def test_every_element_of_many_rows(v, dtype):
         b = slice(i, i + 200)
         p = torch.softmax(x[b].double(), -1)
         want = -p
-        want.scatter_add_(1, t[b, None], torch.ones(200, 1, dtype=torch.float64, device="cuda"))
+        want.scatter_add_(1, t[b, None], torch.ones(len(want), 1, dtype=torch.float64, device="cuda"))
         bound = (2.0 ** -15 + 2 * half) * want.abs() + 1e-30
         assert ((pull[b].double() - want).abs() <= bound).all()
         assert ((held[b].double() - want).abs() <= bound).all()
@@ -613,6 +666,38 @@ def test_few_rows_that_count(dtype):
                            torch.where(on, cb().token_logprobs(x, t).logprobs, torch.zeros((), device="cuda")))
     import ctorch_b200._capi as C
     assert C.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("v,dtype", [(5001, torch.float32), (9001, torch.bfloat16)])
+def test_few_long_rows_that_count(v, dtype):
+    """The same for the log-probabilities of rows that no warp takes whole (5000 of them leave its last wave empty)."""
+    rows = 5000
+    x = torch.randn(rows, v, device="cuda").to(dtype)
+    t, up = torch.randint(v, (rows,), device="cuda"), torch.randn(rows, device="cuda")
+    full = cb().token_logprobs(x, t)
+    grad = cb().token_logprobs_backward(up, x, t, full.logprobs, full.lse)
+    for share in (0.0, 0.0005, 0.01, 0.3):
+        on = torch.rand(rows, device="cuda") < share
+        r = cb().token_logprobs(x, t, on)
+        assert torch.equal(r.logprobs, torch.where(on, full.logprobs, torch.zeros((), device="cuda")))
+        g = cb().token_logprobs_backward(up, x, t, r.logprobs, r.lse, on)
+        assert torch.equal(g, torch.where(on[:, None], grad, torch.zeros_like(grad)))
+    import ctorch_b200._capi as C
+    assert C.wait_timeouts() == 0
+
+
+def test_new_gradients_lie_like_the_logits():
+    """A gradient that the call makes has the logits' rows' alignment where that wastes little."""
+    w = torch.randn(4, 9, 1001, device="cuda").bfloat16()
+    for k, x in enumerate((w[:, :-1], w[1:], w.flatten(0, 1)[1:], w[..., :1000], w[:, ::3], w[:1].expand(4, 9, 1001))):
+        t = torch.randint(1000, x.shape[:-1], device="cuda")
+        z = torch.zeros(t.shape, device="cuda")
+        g = cb().policy_loss(x, t, z, z + 1).grad
+        want = cb().policy_loss(x.contiguous(), t, z, z + 1).grad
+        # sums of float32 in another order (2^-14 and less apart) may round to neighbouring bfloat16: one step, 2^-7
+        assert g.shape == x.shape and ((g.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs()).all()
+        if k < 4:  # the others leave most of their memory unused, or broadcast
+            assert all((g[i].data_ptr() - x[i].data_ptr()) % 16 == 0 for i in range(len(x)))
 
 
 def test_rows_far_apart():
