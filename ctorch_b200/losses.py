@@ -91,7 +91,7 @@ def _results(logits, dev, rows, per_row, others, scratch=0):
     sizes = [-(-scratch // size)] + [prod(rows)] * per_row + others
     flat = torch.empty(sum(sizes), dtype=torch.float64 if f64 else torch.float32, device=dev)
     base = at = flat.data_ptr()
-    out = flat.split_with_sizes(sizes)[1:]
+    out = torch.unsafe_split_with_sizes(flat, sizes)[1:]  # nothing here is differentiated, so nothing needs tracking
     views = []
     for before, n in zip(sizes, sizes[1:]):
         at += before * size
@@ -116,9 +116,11 @@ def _grad_for(name, logits, out, dev):
         if may_overlap(out, logits) and not _same_view(out, logits):
             raise AliasError(f"ctorch::{name}: the gradient overlaps the logits without being the same view")
         return out
+    if logits.is_contiguous() and logits.data_ptr() % 16 == 0:
+        return torch.empty_like(logits)
     shape, strides, size = logits.shape, logits.stride(), _SIZE[logits.dtype]
     lead, v = logits.data_ptr() % 16 // size, shape[-1]
-    if (logits.is_contiguous() and lead == 0) or logits.numel() == 0:
+    if logits.numel() == 0:
         return torch.empty(shape, dtype=logits.dtype, device=dev)
     if lead == 0 and all(st * size % 16 == 0 for s, st in zip(shape[:-1], strides) if s > 1):
         if v * size % 16 and logits.dim() > 1:
