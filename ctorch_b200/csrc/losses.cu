@@ -63,14 +63,12 @@ __device__ __forceinline__ void put_real(void* p, int dt, int64_t off, double v)
     else static_cast<double*>(p)[off] = v;
 }
 
-// log(1 + e^x)
-__device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
-
 // CTA p: pair p, sequences p (chosen) and pairs + p (rejected). With R_s = beta times the sum (or mean)
 // of logp - ref over the sequence's counted rows and h = R_p - R_{pairs + p},
-//     loss = (1 - e) softplus(-h) + e softplus(h)
+//     loss = (1 - e) log(1 + exp(-h)) + e log(1 + exp(h))
 //     dloss/dR_p = e sigma(h) - (1 - e) sigma(-h) = -dloss/dR_{pairs + p}.
-// With offsets, one more CTA clears the rows of no sequence. Reads a few numbers a row, so it is bound by its latency.
+// With offsets, one more CTA clears the rows of no sequence. Reads a few numbers a row, so it is bound by its latency (B200,
+// 8 pairs of 2 x 255 rows: about 10 us with the kernel for the total, between the two passes over the logits).
 __global__ void __launch_bounds__(kPairThreads) loss_pairs(LossArgs a, PairArgs p) {
     dependent_wait();
     allow_dependents();
@@ -115,18 +113,23 @@ __global__ void __launch_bounds__(kPairThreads) loss_pairs(LossArgs a, PairArgs 
         }
         return;
     }
+    auto counts = [&](int64_t r) { return !a.ptr[kLrWeight] || row_real(a, kLrWeight, r) != 0.0; };
+    uint32_t seen[2] = {0u, 0u};  // which of this thread's first 32 rows of a side count
     // both sequences' sums and counts, joined together
     double sums[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         const int64_t s = side * p.pairs + pair, first = offset(s), last = offset(s + 1);
-        for (int64_t r = first + threadIdx.x; r < last; r += kPairThreads) {
-            const bool on = !a.ptr[kLrWeight] || row_real(a, kLrWeight, r) != 0.0;
-            const double lp = on ? p.logp[r] : 0.0;
-            put_row(a, kLrLogp, r, lp);
+        int i = 0;
+        for (int64_t r = first + threadIdx.x; r < last; r += kPairThreads, ++i) {
+            // all loads at once; what a row that does not count holds is not used
+            const double lp = p.logp[r], ref = a.ptr[kLrRef] ? row_real(a, kLrRef, r) : 0.0;
+            const bool on = counts(r);
+            put_row(a, kLrLogp, r, on ? lp : 0.0);
             if (on) {
-                sums[2 * side] += a.ptr[kLrRef] ? lp - row_real(a, kLrRef, r) : lp;
+                sums[2 * side] += lp - ref;
                 sums[2 * side + 1] += 1.0;
+                if (i < 32) seen[side] |= 1u << i;
             }
         }
     }
@@ -150,9 +153,11 @@ __global__ void __launch_bounds__(kPairThreads) loss_pairs(LossArgs a, PairArgs 
         reward[side] = p.beta * sum * share[side];
     }
     const double h = reward[0] - reward[1], e = p.smoothing;
-    const double loss = (1.0 - e) * softplus(-h) + e * softplus(h);
-    const double dh = w * p.beta * (e / (1.0 + exp(-h)) - (1.0 - e) / (1.0 + exp(h)));
+    // from t = exp(-|h|): sigma(|h|) = 1 / (1 + t), sigma(-|h|) = t / (1 + t), log(1 + e^h) = max(h, 0) + log(1 + t)
+    const double t = exp(-fabs(h)), high = 1.0 / (1.0 + t), low = t * high;
+    const double dh = w * p.beta * (h >= 0.0 ? e * high - (1.0 - e) * low : e * low - (1.0 - e) * high);
     if (threadIdx.x == 0) {
+        const double rest = log1p(t), loss = (1.0 - e) * (fmax(-h, 0.0) + rest) + e * (fmax(h, 0.0) + rest);
         p.weighted[pair] = w == 0.0 ? 0.0 : w * loss;
         put_real(p.pair_loss, p.out_dtype, pair * p.pair_loss_stride, loss);
         put_real(p.rewards, p.out_dtype, pair * p.rewards_stride, reward[0]);
@@ -163,8 +168,9 @@ __global__ void __launch_bounds__(kPairThreads) loss_pairs(LossArgs a, PairArgs 
     for (int side = 0; side < 2; ++side) {
         const int64_t s = side * p.pairs + pair, first = offset(s), last = offset(s + 1);
         const double g = w == 0.0 ? 0.0 : (side ? -dh : dh) * share[side];
-        for (int64_t r = first + threadIdx.x; r < last; r += kPairThreads)
-            p.up[r] = !a.ptr[kLrWeight] || row_real(a, kLrWeight, r) != 0.0 ? g : 0.0;
+        int i = 0;
+        for (int64_t r = first + threadIdx.x; r < last; r += kPairThreads, ++i)
+            p.up[r] = (i < 32 ? (seen[side] >> i & 1u) != 0u : counts(r)) ? g : 0.0;
     }
 }
 
