@@ -229,7 +229,7 @@ struct Builder {
         float down = static_cast<float>(c2);
         if (static_cast<double>(down) > c2) down = std::nextafterf(down, 0.0f);
         p.c2_down = down;
-        p.c2_rest = std::fmax(static_cast<float>((c2 - down) / down), 1e-30f);
+        p.c2_rest = std::fmax(static_cast<float>(c2 - down), 1.2e-38f);
         p.scale = 1.0;
         p.status = status;
         p.ptr[kLrX] = x->data;

@@ -59,7 +59,7 @@ struct LossArgs {
     int tail;             // distill: the mass outside the top entries is one more event
     double temp, inv_temp;
     float c2;             // log2(e) / T
-    float c2_down, c2_rest;  // the same rounded down, and what that leaves: c2_down (1 + c2_rest), at least 1e-30
+    float c2_down, c2_rest;  // the same rounded down, and what that leaves (positive)
     double scale;         // multiplies every weight
     double clip_lo, clip_hi, kl_coef;
     const void* offsets;  // preference, packed rows: rows before the first offset or from the last one on
