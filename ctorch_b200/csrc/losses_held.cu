@@ -168,9 +168,9 @@ template <int W> struct Shared {
     float edge[2][kBatch][16];
     ListInfo list[kSides];
     Coef coef[kMaxDepth + 1];
-    uint64_t full[kMaxRing], empty[kMaxRing], done[kMaxRing];
+    uint64_t full[kMaxRing], empty[kMaxRing];
     uint64_t meta_full[2], meta_empty[2];
-    uint64_t list_full[kSides];
+    uint64_t list_full[kSides], done[kSides];
     uint64_t mail_full[kSides], coef_full[kMaxDepth + 1];
 };
 
@@ -215,7 +215,6 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
         for (int i = 0; i < stages; ++i) {
             mbar_init(&sh.full[i], 1);
             mbar_init(&sh.empty[i], W);
-            mbar_init(&sh.done[i], W);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.meta_full[i], 1);
@@ -224,6 +223,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
         for (int i = 0; i <= kMaxDepth; ++i) mbar_init(&sh.coef_full[i], 1);
         for (int i = 0; i < kSides; ++i) {
             mbar_init(&sh.list_full[i], 1);
+            mbar_init(&sh.done[i], W);
             mbar_init(&sh.mail_full[i], 1);
         }
         mbar_fence_init();
@@ -454,6 +454,11 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 q_ahead[u] = k < a.top ? list_q[row * a.top + k] : 0.f;
             }
         };
+        // Waits until the consumers have written row l, the l-th that counts. The barrier is one of kSides, not the
+        // stage's: with three stages the next row of a stage is the other list warp's, and its phase could come and go
+        // before this warp looks. Row l + kSides is written only after this warp has given the list of row l + 4, which it
+        // does after its last look at row l; and before it takes row l it has put row l - 4, so no earlier phase is open.
+        auto written = [&](uint32_t l) { return wait_phase(&sh.done[l % kSides], (l / kSides) & 1u); };
         // Joins row i's entries with its logits, and takes those out of the slice.
         auto take = [&](int i, uint32_t l, const Ring& ring) {
             const int side = static_cast<int>(l % kSides), ms = i / kBatch & 1, mi = i % kBatch;
@@ -501,7 +506,11 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 add(list_q[r.row * a.top + k], list_col[r.row * a.top + k], e_x[k]);
             named = warp_sum(named);
             q_x = warp_sum(q_x);
-            ok = __all_sync(0xffffffffu, wait_phase(&sh.full[ring.slot], ring.phase));
+            // The row before in this stage may be the other list warp's: until that has landed, `full` still shows the
+            // phase before, whose parity is this row's.
+            ok = true;
+            if (l >= static_cast<uint32_t>(stages)) ok = written(l - stages);
+            ok = __all_sync(0xffffffffu, ok && wait_phase(&sh.full[ring.slot], ring.phase));
             if (!ok) return;
             // -inf in the place of each; a column named twice makes the whole row NaN
             T* twice_at = nullptr;
@@ -544,7 +553,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
             __syncwarp();
         };
         // The named elements of this CTA's slice of row i, over what the consumers have left there.
-        auto put = [&](int i, uint32_t l, const Ring& ring) {
+        auto put = [&](int i, uint32_t l) {
             const RowMeta& r = sh.meta[i / kBatch & 1][i % kBatch];
             const float* e_x = e_xs + static_cast<int>(l % kSides) * a.top;
             int col[kAhead];
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 }
             };
             entries(0);
-            ok = __all_sync(0xffffffffu, wait_phase(&sh.done[ring.slot], ring.phase));
+            ok = __all_sync(0xffffffffu, written(l));
             if (!ok) return;
             if (r.grad) {
                 const Coef c = sh.coef[l % (kMaxDepth + 1)];
@@ -586,7 +595,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
         uint32_t live = 0, held_l = 0;
         int held = -1, freed = 0;  // the row that waits for its named elements; batches given back
         int64_t fetched = -1;
-        Ring ring, held_ring;
+        Ring ring;
         for (int i = 0; i < rows && ok; ++i) {
             if (i % kBatch == 0) ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_full[i / kBatch & 1], (i / kBatch >> 1) & 1));
             if (!ok) break;
@@ -602,10 +611,9 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                         if (sh.meta[k / kBatch & 1][k % kBatch].w != 0.0 && ++others == kListWarps) break;
                     fetched = k < end ? sh.meta[k / kBatch & 1][k % kBatch].row : -1;
                     if (ok && fetched >= 0) fetch(fetched);
-                    if (ok && held >= 0) put(held, held_l, held_ring);
+                    if (ok && held >= 0) put(held, held_l);
                     held = i;
                     held_l = live;
-                    held_ring = ring;
                 }
                 ring.next(stages);
                 ++live;
@@ -613,13 +621,13 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
             // The operands of a batch are read again only when those of the one before the last are given back, so a
             // row does not wait past the end of the next batch, however few rows of that count.
             if (ok && i % kBatch == kBatch - 1 && held >= 0 && held < i / kBatch * kBatch) {
-                put(held, held_l, held_ring);
+                put(held, held_l);
                 held = -1;
             }
             for (; ok && (freed + 1) * kBatch <= (held >= 0 ? held : i + 1); ++freed)
                 if (lane == 0) mbar_arrive(&sh.meta_empty[freed & 1]);
         }
-        if (ok && held >= 0) put(held, held_l, held_ring);
+        if (ok && held >= 0) put(held, held_l);
         if (!ok && lane == 0) note_timeout(a.timeouts);
     } else {
         // ---- consumers
@@ -728,7 +736,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
             release_fence();
             if (lane == 0) {
                 mbar_arrive(&sh.empty[write_ring.slot]);
-                if (OP == kLossDistill) mbar_arrive(&sh.done[write_ring.slot]);
+                if (OP == kLossDistill) mbar_arrive(&sh.done[written % kSides]);
             }
             write_ring.next(stages);
             ++written;
