@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
             }
             for (int k = lane; k < (slice_packs + 15) / 16; k += 32) reinterpret_cast<uint4*>(bits)[k] = make_uint4(0u, 0u, 0u, 0u);
             if (lane == 0) li.edge_named = 0u;
+            __syncwarp();  // other lanes set bits there (votes and shuffles order no memory)
             float x_max = -INFINITY;
             float xs[kAhead];
 #pragma unroll
