@@ -227,29 +227,32 @@ __device__ __forceinline__ void put_empty_row(const LossArgs& a, int64_t row) {
 }
 
 // The loss and A of a distilled row, from sums over the teacher's entries: cross = sum q (log q - log p),
-// mass = sum q; s_rest is the part of s outside the entries. With q' = 1 - mass the rest's share under the
-// teacher, p' = s_rest / s under the student (tail only, else q' = 0) and Q = mass + q',
+// mass = sum q. The columns outside the entries keep a maximum m' and a sum s' of their own, because all of them
+// may lie so far below the entries that nothing of them is left in s (masked with a large finite value, or a low
+// temperature): lift = exp((m' - m) / T) may be 0 where s' is not. With q' = 1 - mass the rest's share under the
+// teacher, log p' = log s' + (m' - m) / T - log s under the student (tail only, else q' = 0) and Q = mass + q',
 //     loss    = cross + q' (log q' - log p')
-//     dl/dx_j = (Q p_j - q_j) / T on an entry, p_j (Q - q' / p') / T elsewhere;
-// renormalised entries have Q = 1.
+//     dl/dx_j = (Q p_j - q_j) / T on an entry, p_j (Q - q' / p') / T elsewhere,
+// the latter as A exp((x_j - m') / T) with A = (Q lift / s - q' / s') / T; renormalised entries have Q = 1.
 __device__ __forceinline__ double rest_of_teacher(const LossArgs& a, double mass, bool every_column) {
     if (!a.tail || every_column) return 0.0;
     return mass < 1.0 ? 1.0 - mass : mass == mass ? 0.0 : mass;
 }
 
-__device__ __forceinline__ double distill_slope(const LossArgs& a, double w, double s, double s_rest, double mass,
+__device__ __forceinline__ double distill_slope(const LossArgs& a, double w, double s, double s_rest, double lift, double mass,
                                                 bool every_column, double& big_q) {
     const double q_rest = rest_of_teacher(a, mass, every_column);
     big_q = a.tail ? mass + q_rest : 1.0;
-    if (!a.tail) return w * a.inv_temp / s;
+    if (!a.tail) return w * a.inv_temp * lift / s;
     // with no mass outside the entries every other p_j is 0 and so is its gradient
-    return s_rest > 0.0 ? w * a.inv_temp * (big_q / s - q_rest / s_rest) : s_rest == 0.0 ? 0.0 : s_rest;
+    return s_rest > 0.0 ? w * a.inv_temp * (big_q * lift / s - q_rest / s_rest) : s_rest == 0.0 ? 0.0 : s_rest;
 }
 
-__device__ __forceinline__ double distill_loss_of(const LossArgs& a, double s, double s_rest, double cross, double mass,
+// below = (m' - m) / T
+__device__ __forceinline__ double distill_loss_of(const LossArgs& a, double s, double s_rest, double below, double cross, double mass,
                                                   bool every_column) {
     const double q_rest = rest_of_teacher(a, mass, every_column);
-    return q_rest == 0.0 ? cross : cross + q_rest * (log(q_rest) - (log(s_rest) - log(s)));
+    return q_rest == 0.0 ? cross : cross + q_rest * (log(q_rest) - (log(s_rest) + below - log(s)));
 }
 
 // What the backward pass needs of a row: p_j = exp((x_j - at) / T) 2^shift, g_j = a p_j.

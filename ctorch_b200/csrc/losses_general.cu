@@ -133,12 +133,15 @@ template <class T, int OP> __global__ void __launch_bounds__(kThreads) loss_rows
             r.add(a, E::up(x[j * a.x_in]));
         }
         cta_join(a, r, sm_a);
-        double s_rest = 0.0;
+        double s_rest = 0.0, lift = 1.0, below = 0.0;
+        Acc at = r.m;  // what the gradient's exponentials are relative to
         if (OP == kLossDistill && a.tail) {
             cta_join(a, named, sm_a);
-            const RowSum<Acc> rest = r;
+            s_rest = r.s;
             r.join(a, named.m, named.s);
-            s_rest = rest.m == r.m ? rest.s : rest.s * row_exp(a, rest.m, r.m);
+            lift = at == r.m ? Acc(1) : row_exp(a, at, r.m);
+            below = (static_cast<double>(at) - r.m) * a.inv_temp;
+            if (at == static_cast<Acc>(-INFINITY)) at = 0;
         }
         r.finish();
         const double m = r.m, s = r.s;
@@ -180,8 +183,8 @@ template <class T, int OP> __global__ void __launch_bounds__(kThreads) loss_rows
             cross = cta_sum(cross, sm_d);
             mass = cta_sum(mass, sm_d);
             double big_q;
-            double slope = distill_slope(a, w, s, s_rest, mass, entries == a.cols, big_q);
-            double loss = distill_loss_of(a, s, s_rest, cross, mass, entries == a.cols);
+            double slope = distill_slope(a, w, s, s_rest, lift, mass, entries == a.cols, big_q);
+            double loss = distill_loss_of(a, s, s_rest, below, cross, mass, entries == a.cols);
             if (bad || !(s > 0.0)) slope = loss = quiet_nan();
             for (int k = threadIdx.x; k < a.top; k += kThreads) {
                 const double z = load_real(a.ptr[kLrTeacher], a.dtype[kLrTeacher], t_off + k * a.t_in) * a.inv_temp;
@@ -202,7 +205,7 @@ template <class T, int OP> __global__ void __launch_bounds__(kThreads) loss_rows
         __syncthreads();
         // pass 2: the gradient, then the named positions
         if (g) {
-            const Acc ga = static_cast<Acc>(sh[0]), at = r.m;
+            const Acc ga = static_cast<Acc>(sh[0]);
             for (int64_t j = threadIdx.x; j < a.cols; j += kThreads)
                 g[j * a.g_in] = E::down(ga * row_exp(a, E::up(x[j * a.x_in]), at));
             __syncthreads();

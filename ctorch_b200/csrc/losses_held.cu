@@ -150,8 +150,8 @@ struct ListInfo {
 };
 
 struct Coef {
-    float a, m;
-    float at_target;  // policy
+    float a, m;       // of every element but the named ones: a exp((x - m) / T)
+    float named;      // policy: the target's gradient; distill: the row's maximum, for the entries' own
     float p_scale;    // distill: Q / s
 };
 
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
         // ---- row warp: joins the sums, publishes the coefficient, and keeps what the losses are made of
         uint32_t live = 0;
         double total = 0.0, kept_s = 0.0, kept_rest = 0.0, kept_x = 0.0, kept_ref = 0.0;  // kept_x: ratio, or sum q (x - ref)
-        float kept_m = 0.f;
+        float kept_m = 0.f, kept_mr = 0.f;
         for (int i = 0; i < rows && ok; ++i) {
             const int ms = i / kBatch & 1, mi = i % kBatch;
             if (mi == 0) ok = __all_sync(0xffffffffu, wait_phase(&sh.meta_full[ms], (i / kBatch >> 1) & 1));
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&sh.mail_full[side], mail_bytes);  // for the row kSides later
                 const ListInfo& li = sh.list[side];
-                mf = warp_max(mf);
-                if (OP == kLossDistill) mf = fmaxf(mf, li.x_max);
+                const float mr = warp_max(mf);  // distill: of the columns that the teacher does not name
+                mf = OP == kLossDistill ? fmaxf(mr, li.x_max) : mr;
                 const double m = mf;
                 // Every consumer of the cluster waits for the coefficient, so only what it needs is computed first:
                 // no logarithm.
@@ -365,12 +365,12 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 float part = 0.f;
 #pragma unroll
                 for (int k = 0; k < kJoin; ++k)
-                    if (32 * k < parts) part += pm[k] == -INFINITY ? ps[k] : ps[k] * (pm[k] == mf ? 1.f : exp_one(a, pm[k], mf));
+                    if (32 * k < parts) part += pm[k] == -INFINITY ? ps[k] : ps[k] * (pm[k] == mr ? 1.f : exp_one(a, pm[k], mr));
                 double s = warp_sum(part), s_rest = s;
                 if (mf == INFINITY) s = s_rest = quiet_nan();
                 Coef c;
-                c.m = mf;
-                c.at_target = c.p_scale = 0.f;
+                c.m = mr == -INFINITY ? 0.f : mr;
+                c.named = c.p_scale = 0.f;
                 double ratio = 0.0, big_q = 1.0;
                 if (OP == kLossPolicy) {
                     // s relative to the target's logit instead of the maximum: r = exp(-old) / s', p_t = 1 / s'
@@ -386,13 +386,15 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                     }
                     const double g = policy_terms(a, r.w, r.adv, ratio, 0.0, ed).g;
                     c.a = -static_cast<float>(g) / static_cast<float>(s);
-                    c.at_target = static_cast<float>(g * rest);
+                    c.named = static_cast<float>(g * rest);
                 } else {
-                    s = s_rest + li.named * (li.x_max == -INFINITY ? 0.f : exp_one(a, li.x_max, mf));
+                    const float rise = mr == -INFINITY ? 0.f : exp_one(a, mr, mf);
+                    s = s_rest * rise + li.named * (li.x_max == -INFINITY ? 0.f : exp_one(a, li.x_max, mf));
                     if (r.list.bad || !(s > 0.0)) s = quiet_nan();
-                    c.a = static_cast<float>(distill_slope(a, r.w, s, s_rest, r.list.mass, r.list.count == a.cols, big_q));
+                    c.a = static_cast<float>(distill_slope(a, r.w, s, s_rest, rise, r.list.mass, r.list.count == a.cols, big_q));
                     if (s != s) c.a = NAN;
                     c.p_scale = static_cast<float>(big_q) / static_cast<float>(s);
+                    c.named = mf;
                 }
                 if (lane == 0) {
                     sh.coef[cs] = c;
@@ -402,6 +404,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                     kept_s = s;
                     kept_rest = s_rest;
                     kept_m = mf;
+                    kept_mr = mr;
                     kept_x = OP == kLossPolicy ? ratio : li.q_x;
                     kept_ref = OP == kLossPolicy ? 0.0 : li.ref;
                 }
@@ -417,7 +420,8 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                     } else if (OP == kLossDistill) {
                         const double cross = mine.list.q_logq - a.inv_temp * (kept_x + (kept_ref - m) * mine.list.mass) +
                                              mine.list.mass * log(kept_s);
-                        const double loss = distill_loss_of(a, kept_s, kept_rest, cross, mine.list.mass, mine.list.count == a.cols);
+                        const double loss = distill_loss_of(a, kept_s, kept_rest, (kept_mr - m) * a.inv_temp, cross, mine.list.mass,
+                                                            mine.list.count == a.cols);
                         put_row(a, kLrRowLoss, mine.row, loss);
                         total += mine.w * loss;
                     } else {
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                         if (j < 0) continue;
                         const bool inside = at >= 0 && at < inside_end;
                         if (!inside && !((j < 8 && (edges >> j & 1u)) || (rank == 0 && j >= tail))) continue;
-                        const T v = LossElem<T>::down(scale * (exp_one(a, e_x[k0 + lane + 32 * u], c.m) * c.p_scale - q[u]) + poison);
+                        const T v = LossElem<T>::down(scale * (exp_one(a, e_x[k0 + lane + 32 * u], c.named) * c.p_scale - q[u]) + poison);
                         gr[j * a.g_in] = v;
                     }
                 }
@@ -715,7 +719,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 if (OP == kLossPolicy) {
                     const int at = r.target - r.body;  // the target's own value, by the thread that wrote its pack
                     if (r.target >= 0 && at >= 0 && at < r.count * VE && (at / VE) % kCons == t)
-                        static_cast<T*>(r.out)[at] = LossElem<T>::down(c.at_target);
+                        static_cast<T*>(r.out)[at] = LossElem<T>::down(c.named);
                 }
             } else if (r.grad) {
                 // where the gradient's rows are not aligned like the logits', or strided: element by element
@@ -725,14 +729,14 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                     const int j = r.body + (p * kCons + t) * VE;
 #pragma unroll
                     for (int k = 0; k < VE; ++k)
-                        gr[(j + k) * a.g_in] = OP == kLossPolicy && j + k == r.target ? LossElem<T>::down(c.at_target) : v[k];
+                        gr[(j + k) * a.g_in] = OP == kLossPolicy && j + k == r.target ? LossElem<T>::down(c.named) : v[k];
                 };
                 for (int p = 0; p * kCons < count; ++p) scatter(p, pack(p));
             }
             if (r.grad && t < 16 && (r.edges >> t & 1u)) {
                 const int j = edge_column(t, r.behind);
                 const float v = c.a * exp_one(a, sh.edge[i / kBatch & 1][i % kBatch][t], c.m);
-                static_cast<T*>(r.grad)[j * a.g_in] = LossElem<T>::down(OP == kLossPolicy && j == r.target ? c.at_target : v);
+                static_cast<T*>(r.grad)[j * a.g_in] = LossElem<T>::down(OP == kLossPolicy && j == r.target ? c.named : v);
             }
             release_fence();
             if (lane == 0) {
