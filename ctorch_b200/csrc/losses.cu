@@ -651,6 +651,7 @@ int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets, int64_t
             by_row(back, kLrLogp, logp);
             by_row(back, kLrLse, lse);
             by_row(back, kLrUp, up);
+            back.up_final = true;
             CTB_TRY(run_backward(back, st));
         }
         return loss ? run_total(p.weighted, static_cast<int>(pairs), loss, st) : CTB_OK;

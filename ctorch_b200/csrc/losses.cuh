@@ -65,6 +65,7 @@ struct LossArgs {
     const void* offsets;  // preference, packed rows: rows before the first offset or from the last one on
     int32_t offsets_dtype;  // belong to no sequence and do not count
     int64_t offsets_end;    // element offset of the last one
+    bool up_final;        // preference: kLrUp is 0 in rows that do not count, and says by NaN that no row is valid
     double* partials;     // one weighted loss sum a CTA, optional
     int32_t* status;      // optional: int32 flag, int64 offending index at byte 8; written on error only
     unsigned long long* timeouts;  // device counter of timed-out waits (async_copy.cuh)
@@ -269,7 +270,7 @@ template <class Acc> struct BackwardRow {
 };
 
 __device__ __forceinline__ double row_upstream(const LossArgs& a, int64_t row) {
-    return row_weight(a, row) != 0.0 ? row_real(a, kLrUp, row) : 0.0;
+    return a.up_final || row_weight(a, row) != 0.0 ? row_real(a, kLrUp, row) : 0.0;
 }
 
 template <class T>

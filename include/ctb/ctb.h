@@ -359,7 +359,7 @@ CTB_API int ctb_policy_loss(const ctb_view* logits, const ctb_view* targets, con
  * (pair i is sequences i and pairs + i): equal shares of the leading dims' rows, or, for [rows, V]
  * logits, rows offsets[s] to offsets[s + 1] of sequence s (offsets [2 * pairs + 1], device; rows of no
  * sequence do not count; offsets that fall or point outside the rows are a bad index and make every
- * result NaN). Over a sequence's rows with mask, S = sum (logp - ref_logprobs) (ref NULL: 0),
+ * result NaN, in rows that the mask leaves out too). Over a sequence's rows with mask, S = sum (logp - ref_logprobs) (ref NULL: 0),
  * divided by their number when `average`; rewards = beta S, h = rewards of the chosen less the rejected:
  *     pair_loss = -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h)
  * loss = sum of weight_scale * weights * pair_loss (weights [pairs], NULL: 1), grad = its gradient.

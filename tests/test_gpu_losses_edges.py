@@ -65,3 +65,21 @@ def test_a_student_far_from_certain_of_the_rest(gap, temperature, v, top, kind, 
                             torch.ones(n, device="cuda"), temperature)
     check(got.row_loss, row_loss, "row_loss")
     check(got.grad, (grad[0] * scale, grad[1] * scale * (1 + 2.0 ** -20)), "grad")
+
+
+@pytest.mark.parametrize("how", LAYOUTS)
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("v", [5, 700, 20000])
+@pytest.mark.parametrize("offsets", [[0, 5, 3], [2, 4, 3, 6, 7], [0, 5, 10 ** 6], [-1, 5, 9], [8, 4, 0], [0, 0, -3]])
+def test_bad_offsets_make_every_result_nan(offsets, v, kind, how):
+    """Rows between, before and behind the sequences, masked or not: nothing in the results looks like a number."""
+    rows, pairs = 9, (len(offsets) - 1) // 2
+    rng = np.random.default_rng(v)
+    x = dev(rng.normal(size=(rows, v)), torch.float64).to(KIND[kind])
+    t = rng.integers(0, v, rows)
+    t[8] = -100
+    mask = rng.random(rows) < 0.6
+    for m in (None, mask):
+        got = cb().preference_loss(layouts(x, how), dev(t), pairs, mask=None if m is None else dev(m), offsets=dev(np.array(offsets)))
+        for name in ("loss", "pair_loss", "rewards", "logprobs", "grad"):
+            assert torch.isnan(getattr(got, name)).all(), name
