@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(held_threads<OP, W>(), PER_SM)
                 double s = warp_sum(part), s_rest = s;
                 if (mf == INFINITY) s = s_rest = quiet_nan();
                 Coef c;
-                c.m = mr == -INFINITY ? 0.f : mr;
+                c.m = OP == kLossDistill && mr == -INFINITY ? 0.f : mr;
                 c.named = c.p_scale = 0.f;
                 double ratio = 0.0, big_q = 1.0;
                 if (OP == kLossPolicy) {

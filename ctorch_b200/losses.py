@@ -34,22 +34,30 @@ PolicyLoss = namedtuple("PolicyLoss", ["loss", "row_loss", "logprobs", "kl", "gr
 PreferenceLoss = namedtuple("PreferenceLoss", ["loss", "pair_loss", "rewards", "logprobs", "grad"])
 
 _SIZE = {torch.float32: 4, torch.float64: 8, torch.bfloat16: 2}
+# of a row's results, by the logits' type: dtype, its code, bytes
+_RESULT = {torch.float32: (torch.float32, C.F32, 4), torch.bfloat16: (torch.float32, C.F32, 4),
+           torch.float64: (torch.float64, C.F64, 8)}
 
 # A loss of a few rows takes the GPU less time than it takes Python to describe its operands, so the views
-# are packed in one go (ctb_view as bytes) and the results of a call share one allocation.
+# are packed in one go (ctb_view as bytes) and the results a row share one allocation, with the scratch where
+# that is small. The scalar loss has storage of its own: a program may keep it for every step, for its log.
 _VIEW = [struct.Struct(f"<Qii{n}q{8 * (C.MAX_DIMS - n)}x{n}q{8 * (C.MAX_DIMS - n)}x") for n in range(C.MAX_DIMS + 1)]
 
 
-_VIEW1 = _VIEW[1].pack
+_VIEW0, _VIEW1 = _VIEW[0].pack, _VIEW[1].pack
+_PACK = [v.pack for v in _VIEW]
+_CODE = C.CODE_OF_TORCH
+_SMALL = 8192  # bytes of scratch that the results a row carry along; more only where it is less than they are
 
 
 def _view(t):
     if t is None:
         return None
-    n = t.dim()
+    shape = t.shape
+    n = len(shape)
     if n > C.MAX_DIMS:
         raise ShapeError(f"ctorch: tensor rank exceeds kMaxRank (got {n})")
-    return _VIEW[n].pack(t.data_ptr(), C.CODE_OF_TORCH[t.dtype], n, *t.shape, *t.stride())
+    return _PACK[n](t.data_ptr(), _CODE[t.dtype], n, *shape, *t.stride())
 
 
 def _check(name, logits, *others):
@@ -66,40 +74,57 @@ def _check(name, logits, *others):
             raise TypeError(f"ctorch::{name}: expected a tensor")
         if t.device != dev:
             _cuda(name, logits, t)  # raises
-        if t.dtype not in C.CODE_OF_TORCH:
+        if t.dtype not in _CODE:
             raise DTypeError(f"ctorch::{name}: {t.dtype} is not supported")
     if logits.dim() == 0:
         raise ShapeError(f"ctorch::{name}: logits must have at least one dim (the vocabulary, last)")
     return dev
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _run(name, dev, fn, *args):
     """fn(*args, stream) on the current stream of the operands' device."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         _call(fn(*args, C.raw_stream(dev)), name)
     else:
         with torch.cuda.device(dev):
             _call(fn(*args, C.raw_stream(dev)), name)
 
 
-def _results(logits, dev, rows, per_row, others, scratch=0):
-    """One allocation for scratch (bytes, first), `per_row` results of the leading shape `rows` and vectors of
-    `others` elements, in the type of a row's results. Returns the scratch's address, the results and their
-    packed views."""
-    f64 = logits.dtype == torch.float64
-    size, code = (8, C.F64) if f64 else (4, C.F32)
-    sizes = [-(-scratch // size)] + [prod(rows)] * per_row + others
-    flat = torch.empty(sum(sizes), dtype=torch.float64 if f64 else torch.float32, device=dev)
+def _results(logits, dev, rows, per_row, others=(), scratch=0, scalar=True):
+    """Tensors for `per_row` results of the leading shape `rows`, vectors of `others` elements, and the scalar loss.
+    Returns the address of the scratch (bytes) and what keeps it, the results and their packed views."""
+    dtype, code, size = _RESULT[logits.dtype]
+    n = prod(rows)
+    apart = scratch > _SMALL and scratch > per_row * n * size
+    sizes = [n] * per_row
+    sizes += others
+    lead = 0 if apart else -(-scratch // size)
+    if lead:
+        sizes.insert(0, lead)
+    keep = flat = torch.empty(sum(sizes), dtype=dtype, device=dev)
     base = at = flat.data_ptr()
-    out = torch.unsafe_split_with_sizes(flat, sizes)[1:]  # nothing here is differentiated, so nothing needs tracking
+    if apart:
+        keep = torch.empty(scratch, dtype=torch.uint8, device=dev)
+        base = keep.data_ptr()
+    out = list(torch.unsafe_split_with_sizes(flat, sizes))  # nothing here is differentiated, so nothing needs tracking
     views = []
-    for before, n in zip(sizes, sizes[1:]):
-        at += before * size
+    for n in sizes:
         views.append(_VIEW1(at, code, 1, n, 1))
+        at += n * size
+    if lead:
+        del out[0], views[0]
     if len(rows) != 1:
-        out = [t.view(rows) for t in out[:per_row]] + list(out[per_row:])
-        views[:per_row] = [_view(t) for t in out[:per_row]]
-    return base, out, views
+        for i in range(per_row):
+            out[i] = out[i].view(rows)
+            views[i] = _view(out[i])
+    if scalar:
+        loss = torch.empty_strided((), (), dtype=dtype, device=dev)
+        out.append(loss)
+        views.append(_VIEW0(loss.data_ptr(), code, 0))
+    return (base, keep), out, views
 
 
 def _grad_for(name, logits, out, dev):
@@ -165,7 +190,7 @@ def token_logprobs(logits, targets, mask=None, temperature: float = 1.0, status=
     token_logprobs_backward() pulls a gradient back through it."""
     name = "token_logprobs"
     dev = _check(name, logits, targets, mask)
-    _, (logp, lse), (v_logp, v_lse) = _results(logits, dev, logits.shape[:-1], 2, [])
+    _, (logp, lse), (v_logp, v_lse) = _results(logits, dev, logits.shape[:-1], 2, scalar=False)
     _run(name, dev, C.lib.ctb_token_logprobs, _view(logits), _view(targets), _view(mask), temperature, v_logp, v_lse,
          _status(name, status, dev))
     return TokenLogprobs(logp, lse)
@@ -204,11 +229,11 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weig
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
     need = C.lib.ctb_loss_scratch_bytes(vx, 0, teacher_logits.shape[-1] if teacher_logits.dim() else 0)
-    scratch, (row_loss, loss), (v_row, v_loss) = _results(logits, dev, rows, 1, [1], need)
+    (scratch, _keep), (row_loss, loss), (v_row, v_loss) = _results(logits, dev, rows, 1, scratch=need)
     _run(name, dev, C.lib.ctb_distill_loss, vx, _view(teacher_logits), _view(teacher_indices), _view(teacher_lse),
          _view(weights), _scale(weights, rows), temperature, v_loss, v_row, _view(g), _status(name, status, dev),
          scratch, need)
-    return DistillLoss(loss.squeeze_(0), row_loss, g)
+    return DistillLoss(loss, row_loss, g)
 
 
 def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, weights=None, clip_low: float = 0.2,
@@ -227,11 +252,11 @@ def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, we
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
     need = C.lib.ctb_loss_scratch_bytes(vx, 0, 0)
-    scratch, (row_loss, logp, kl, loss), (v_row, v_logp, v_kl, v_loss) = _results(logits, dev, rows, 3, [1], need)
+    (scratch, _keep), (row_loss, logp, kl, loss), (v_row, v_logp, v_kl, v_loss) = _results(logits, dev, rows, 3, scratch=need)
     _run(name, dev, C.lib.ctb_policy_loss, vx, _view(targets), _view(old_logprobs), _view(advantages),
          _view(ref_logprobs), _view(weights), _scale(weights, rows), clip_low, clip_high, kl_coef, temperature,
          v_loss, v_row, v_logp, v_kl, _view(g), _status(name, status, dev), scratch, need)
-    return PolicyLoss(loss.squeeze_(0), row_loss, logp, kl, g)
+    return PolicyLoss(loss, row_loss, logp, kl, g)
 
 
 def preference_loss(logits, targets, pairs: int, ref_logprobs=None, mask=None, offsets=None, weights=None,
@@ -256,9 +281,9 @@ def preference_loss(logits, targets, pairs: int, ref_logprobs=None, mask=None, o
     g = _grad_for(name, logits, out_grad, dev) if grad or out_grad is not None else None
     vx = _view(logits)
     need = C.lib.ctb_loss_scratch_bytes(vx, pairs, 0)
-    scratch, (logp, pair_loss, rewards, loss), (v_logp, v_pair, v_rewards, v_loss) = _results(
-        logits, dev, logits.shape[:-1], 1, [pairs, 2 * pairs, 1], need)
+    (scratch, _keep), (logp, pair_loss, rewards, loss), (v_logp, v_pair, v_rewards, v_loss) = _results(
+        logits, dev, logits.shape[:-1], 1, (pairs, 2 * pairs), need)
     _run(name, dev, C.lib.ctb_preference_loss, vx, _view(targets), pairs, _view(offsets), _view(ref_logprobs),
          _view(mask), _view(weights), _scale(weights, (pairs,)), beta, label_smoothing, int(average), v_loss, v_pair,
          v_rewards, v_logp, _view(g), _status(name, status, dev), scratch, need)
-    return PreferenceLoss(loss.squeeze_(0), pair_loss, rewards, logp, g)
+    return PreferenceLoss(loss, pair_loss, rewards, logp, g)

@@ -83,3 +83,27 @@ def test_bad_offsets_make_every_result_nan(offsets, v, kind, how):
         got = cb().preference_loss(layouts(x, how), dev(t), pairs, mask=None if m is None else dev(m), offsets=dev(np.array(offsets)))
         for name in ("loss", "pair_loss", "rewards", "logprobs", "grad"):
             assert torch.isnan(getattr(got, name)).all(), name
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+def test_results_keep_no_scratch_alive(kind):
+    """A program may keep the scalar of every step, or its row losses, and save them: their storage holds them and little
+    else (8 KiB of scratch at most, or as much as they take themselves), whatever the call needed."""
+    rows, v = 600, 300
+    x = torch.randn(rows, v, device="cuda").to(KIND[kind])
+    t = torch.randint(v, (rows,), device="cuda")
+    z = torch.zeros(rows, device="cuda")
+    index = torch.stack([torch.randperm(v, device="cuda")[:100] for _ in range(rows)])
+    calls = [lambda n: cb().policy_loss(x[:n], t[:n], z[:n], z[:n], weights=z[:n] + 1)]
+    for top in (1, 100):
+        calls.append(lambda n, top=top: cb().distill_loss(x[:n], index[:n, :top].float(), index[:n, :top], weights=z[:n] + 1))
+    calls.append(lambda n: cb().preference_loss(x[:n], t[:n], 2))
+    for call in calls:
+        for n in (4, 600):
+            r = call(n)
+            size = r.loss.element_size()
+            assert r.loss.shape == () and r.loss.untyped_storage().nbytes() == size
+            for name, a in zip(r._fields, r):
+                if name not in ("loss", "grad"):
+                    assert a.untyped_storage().nbytes() <= 8192 + 3 * n * size + 64, name
+            assert r.grad.untyped_storage().nbytes() <= 2 * r.grad.nbytes
