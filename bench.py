@@ -154,9 +154,21 @@ def calibrate_rows(budget_s, n_steps, threads, probe_rows=1024):
     return p
 
 
+def missing_reference():
+    """Why ctorch's CPU path cannot be timed, or None."""
+    from oracle.oracle import REF_SO, ref_available
+
+    if ref_available():
+        return None
+    return f"ctorch's CPU backend ({os.path.relpath(REF_SO, ROOT)}) is not built: its sources were not there"
+
+
 def run_reference(args):
     rank, world, _ = env_rank()
     if rank != 0:
+        return 0
+    if missing := missing_reference():
+        print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
         return 0
     threads = host_threads()
     rows = args.cpu_rows or calibrate_rows(150.0, args.steps + args.warmup, threads)
@@ -833,6 +845,9 @@ def main():
     args = ap.parse_args()
     if args.case:
         return run_case(args)
+    if args.impl != "reference" and not args.no_cpu_baseline and (missing := missing_reference()):
+        print(f"no CPU baseline: {missing}", file=sys.stderr)
+        args.no_cpu_baseline = True
     if args.suite:
         return run_suite(args)
     if args.warmup < 3:
