@@ -13,7 +13,8 @@
 // float64 ones); differences are taken before scaling, (x_j - m) * (log2(e) / T), so that a row of
 // the type's lowest values still gives a uniform p instead of an overflow, and a common offset of
 // the logits costs nothing. What happens once a row (logarithms, ratios, the loss) is float64: it
-// is a few hundred instructions a row, and the losses subtract numbers that nearly cancel.
+// is a few hundred instructions a row, and the losses subtract numbers that nearly cancel. (Float32 are:
+// the joining of a row's partial sums in losses_held.cu and losses_short.cu, and the teacher's probabilities in the former.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -310,6 +311,9 @@ __device__ __forceinline__ BackwardRow<typename LossElem<T>::Acc> backward_row(c
     return b;
 }
 
+// One multiply-add with log2(e)/T as a float32 and the hardware's 2^t as it is: a p_j of the backward pass is off by up to
+// 6e-8 |t| to one side, t the exponent, and 5e-8 more. The forward kernels correct for both (losses_ring.cuh) because
+// sequences add their results up; a gradient's elements are rounded one by one.
 __device__ __forceinline__ float row_exp_shifted(const LossArgs& a, float x, float at, float shift) {
     return exp2_fast(fmaf(x - at, a.c2, shift));
 }

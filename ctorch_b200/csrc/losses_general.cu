@@ -2,8 +2,11 @@
 // element through the strides, the row read twice (statistics, then gradient; the second read comes
 // from L2 unless the row is huge). Rows of unit stride in float32 or bfloat16 have kernels of their
 // own (losses_stream.cu, losses_held.cu); this one takes float64, rows that are strided along the
-// vocabulary, and losses over rows too long for those (more than 8 slices of 64 KiB, less where the
-// teacher's entries need the room). B200: policy loss on [8192, 131072] bf16 6.3 ms against 0.78 ms.
+// vocabulary, and losses over rows that those cannot hold: policy loss and distillation of more than 262144 bf16 or
+// 131072 float32 logits (8 slices of 64 KiB), distillation with more entries than fit beside three of the slices
+// (from 187 a row on, where slices are 64 KiB; losses_held.cu). It is 4 to 8 times slower. B200: policy loss on
+// [8192, 131072] bf16 6.3 ms against 0.78 ms; on [2048, 131072] float32 361 us by the other kernel, on [2048, 131080] 1508 us
+// by this one; float64 [1024, 131072] 1377 us, 24% of the copy rate.
 #include "losses.cuh"
 
 namespace ctb {

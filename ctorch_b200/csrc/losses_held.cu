@@ -1,5 +1,5 @@
 // losses_held.cu — the policy and distillation losses over rows of unit stride (float32, bfloat16): each logit is
-// read from memory once, takes one exponential, and its gradient is written from the same pass.
+// read from memory once, and its gradient is written from the same pass.
 //
 // A row belongs to a thread-block cluster of C CTAs (C = 1 for rows that one CTA can hold), a CTA to a
 // contiguous slice of the row's 16-byte packs. Clusters are persistent: cluster c takes rows c, c + n,
@@ -20,15 +20,19 @@
 // exponentials kept (two CTAs of eight warps an SM), 1018 us kept for two rows, 780 us this way. Writing the gradient
 // into the stage and from there by bulk copies took 790 us (distillation 715 us against 627 us: the stage is given
 // back later). Measured: policy loss [8192, 131072] bf16 780 us (90% of the rows count; 5.2 TB/s), [3001, 50021] bf16 with
-// rows padded to 50048 (85%) 136 us; distillation [4096, 131072] bf16 with 128 entries a row and a tail 530 us. Bound by
-// memory and instruction issue together on wide slices (80% of the copy rate), by what every row costs whatever its
-// length (about 2 us a cluster) on narrow ones.
+// rows padded to 50048 (85%) 136 us; distillation [4096, 131072] bf16 with 128 entries a row and a tail 530 us. On
+// wide slices nothing is used up (80% of the copy rate; the exponential pipe and instruction issue a little over half busy),
+// but of 64 KiB stages there are three: one is folded, one written, one loads. Narrow ones are bound by what every row
+// costs whatever its length (about 2 us a cluster).
 //
 // Distillation. The teacher's entries are prepared by a kernel of their own (loss_lists), a warp a row: q and the
 // sums that need no logit. Two list warps, in turns, join them with the rows: read the named logits, and put -inf in
 // their place in the landed stage, so that the consumers' sum is that of the others (1 - sum p would lose it to
 // cancellation) and their gradient there 0; when the consumers have written the row, the list warp writes the named
-// elements' own gradient over that.
+// elements' own gradient over that. With a 64 KiB slice three stages fit, and beside them the entries only up to 186 a
+// row: more go to losses_general.cu ([4096, 131072] bf16 with 186 entries 617 us, with 187 3.9 ms; [4096, 32768] 182 and
+// 790 us). On narrower slices many entries leave an SM one CTA of few warps ([8192, 6144] with 64 entries 104 us, with 256
+// 572 us; the sizes below were chosen for the policy loss).
 #include <string>
 
 #include "losses_ring.cuh"
@@ -50,7 +54,9 @@ struct ListSums {
 __host__ __device__ inline size_t list_sums_bytes(int64_t rows) { return static_cast<size_t>(rows) * sizeof(ListSums); }
 
 // q_k = exp(z_k - base) * weight with z = teacher / T: renormalised over the entries (base their maximum, weight
-// 1 / sum), or with the teacher's own log-sum-exp. A warp a row; a few numbers a row, bound by latency
+// 1 / sum), or with the teacher's own log-sum-exp. Sums are float64; q itself is kept in float32, half the bytes a list
+// warp fetches, and so sum q x and with it the loss carry up to 2^-24 sum q |x - max| / T (a KL of nearly 0 is not exact
+// below that; the row's float32 sum leaves it no better). A warp a row; a few numbers a row, bound by latency
 // (a few microseconds, the first of them beside the kernel before it).
 __global__ void __launch_bounds__(256) loss_lists(const __grid_constant__ LossArgs a) {
     dependent_wait();
@@ -158,6 +164,7 @@ struct Coef {
 constexpr int kMaxDepth = 3;               // rows folded before the oldest of them is written
 constexpr int kSides = 2 * kMaxDepth + 2;  // rows whose sums and lists may be in use at once
 constexpr int kMaxRing = 8;
+static_assert(kMaxRing <= kSides, "a row waits for the row before in its stage by its side");
 constexpr int kAhead = 4;      // entries a lane of a list warp fetches a row ahead
 constexpr int kListWarps = 2;  // they take turns
 

@@ -5,7 +5,8 @@
 // Accuracy of the sums. log2(e)/T as one float32 is off by up to 6e-8 relative, and so is every t = d log2(e)/T
 // and with it, one-sidedly, the sum; a sequence's log-probabilities add that up. So t is taken with log2(e)/T in two
 // parts, rounded once, and raised by the mean error of the hardware's 2^t (log-probabilities on B200, [4000, 32768]
-// at T = 0.8, 1, 2: mean error 8e-9, 5e-9, 9e-9 and less; 4e-8 to 8e-8 without either). Long sums are taken in two levels, a stage's share of a
+// at T = 0.8, 1, 2: mean error 8e-9, 5e-9, 9e-9 and less; 4e-8 to 8e-8 without either). The gradients of the losses use it
+// too; the backward pass of the log-probabilities does without (row_exp_shifted). Long sums are taken in two levels, a stage's share of a
 // thread and then the stages, so that small terms are not lost against a grown sum ([2048, 131072] logits of
 // standard deviation 4 in one level: 1.7e-7 low on average).
 #pragma once

@@ -268,8 +268,15 @@ template <int OP> int any_type(const LossArgs& a, int* parts, cudaStream_t st) {
 // Which rows a warp takes whole. Policy rows: those of which two fit the registers, 4 KiB (measured above).
 // Otherwise rows up to 16 KiB, and longer ones where the last wave of the resident warps is nearly full, since
 // each of them is as long as a row (B200, log-probabilities of 32768 bfloat16 against the ring: 4736 rows, two waves,
-// 57 us against 64; 8192 rows, 3.5 waves, 100 against 104; 3000 rows, 1.3 waves, 48 against 44). The backward pass of
-// long float32 rows is the ring's, which then has the fewer instructions a byte to issue and copies better
+// 57 us against 64; 8192 rows, 3.5 waves, 100 against 104; 3000 rows, 1.3 waves, 48 against 44). Near the limit of 85%
+// the two differ by a few per cent either way; time here over time there, by how full two and three waves are:
+//     rows of             78%                      85%                      92%                 100%
+//     16384 bfloat16   0.88-0.96, 0.94-0.97   0.88-0.92, 0.91        0.84-0.86, 0.88        0.80-0.82, 0.86-0.87
+//     32768            1.02-1.10, 0.99-1.02   0.99-1.05, 0.96-0.97   0.95-0.98, 0.93-0.96   0.92, 0.91-0.96
+//     65536            1.06-1.14, 1.01-1.03   1.05-1.07, 0.96-0.97   1.01, 0.92-0.95        0.91-0.95, 0.92-0.93
+//     16384 float32    0.99-1.03              0.95-1.00              0.96-0.97              0.92-0.97
+// (forward, backward; a single wave is like them forward, 0.93-1.02 backward from 85% on). The
+// backward pass of long float32 rows is the ring's (here 1.01-1.12 times as long at every share), which then has the fewer instructions a byte to issue and copies better
 // ([8192, 50021] 573 us against 557, [8192, 65536] bfloat16 378 against 384). So are several waves of long rows
 // of which some may not count: each wave takes as long as one that counts (the preference loss of 4080 rows of 32768
 // bfloat16 at 60%, 180 us against 163).

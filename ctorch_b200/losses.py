@@ -222,7 +222,8 @@ def distill_loss(logits, teacher_logits, teacher_indices, teacher_lse=None, weig
 
     row_loss = KL(teacher || student) of each row at `temperature` (not multiplied by its square);
     loss = sum(weights * row_loss), or the mean of the rows when weights is None; grad = the gradient of
-    loss, None when grad=False."""
+    loss, None when grad=False. Fastest with up to 186 entries, in rows of unit stride of up to 262144 logits
+    (float32: 131072)."""
     name = "distill_loss"
     dev = _check(name, logits, teacher_logits, teacher_indices, teacher_lse, weights)
     rows = logits.shape[:-1]
@@ -245,7 +246,8 @@ def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, we
         row_loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * kl,   kl = exp(d) - 1 - d
 
     loss = sum(weights * row_loss), or the mean of the rows when weights is None; logprobs = logp; kl is 0
-    without ref_logprobs; grad = the gradient of loss, None when grad=False."""
+    without ref_logprobs; grad = the gradient of loss, None when grad=False. Fastest in rows of unit stride of up
+    to 262144 logits (float32: 131072)."""
     name = "policy_loss"
     dev = _check(name, logits, targets, old_logprobs, advantages, ref_logprobs, weights)
     rows = logits.shape[:-1]

@@ -300,8 +300,8 @@ CTB_API int ctb_minmax_combine(int op, const ctb_view* values, const ctb_view* i
  * a fixed order and rounded once: equal calls give equal bits.
  * A row whose mask or weight is 0 does not count: its logits, targets and other operands are not looked
  * at (they may hold anything), its results are 0 and its gradient row is 0. Logits of -inf have
- * probability 0; a row with +inf or NaN, or of -inf alone, gives NaN in its own results. A row of the
- * type's lowest finite value is uniform.
+ * probability 0; a row with +inf or NaN, or of -inf alone, gives NaN in its own results (but the lse of
+ * -inf alone is -inf). A row of the type's lowest finite value is uniform.
  * grad has the logits' shape and dtype; it may be the logits' own view (the gradient then replaces the
  * logits) and must not overlap them otherwise. Rows of unit stride are read and written fastest where
  * logits and grad start their rows at the same offset from a 16-byte boundary.
@@ -316,7 +316,8 @@ CTB_API int ctb_token_logprobs(const ctb_view* logits, const ctb_view* targets, 
                                int32_t* d_status, ctb_stream stream);
 
 /* grad = the gradient of sum(grad_logprobs * logprobs): grad_logprobs / T * (1[target] - p). logprobs,
- * lse, mask and temperature are those of the forward call. Rows with a zero grad_logprobs are not read. */
+ * lse, mask and temperature are those of the forward call. Rows with a zero grad_logprobs are not read. p comes from
+ * whichever of logprobs and lse is the more exact; where logprobs is -inf that is lse, rounded to its type. */
 CTB_API int ctb_token_logprobs_backward(const ctb_view* grad_logprobs, const ctb_view* logits,
                                         const ctb_view* targets, const ctb_view* logprobs, const ctb_view* lse,
                                         const ctb_view* mask, double temperature, const ctb_view* grad,
@@ -333,7 +334,9 @@ CTB_API size_t ctb_loss_scratch_bytes(const ctb_view* logits, int64_t pairs, int
  *     row_loss = sum_k q_k (log q_k - log p[index_k])
  * With teacher_lse = the log-sum-exp of the teacher's whole row of logits / T, q_k = exp(teacher_k / T -
  * teacher_lse), and the mass outside the entries, q' = max(0, 1 - sum q) and p' = 1 - sum p[index_k],
- * is one more event: row_loss += q' (log q' - log p'). (With an entry for every logit there is none.)
+ * is one more event: row_loss += q' (log q' - log p'). (With an entry for every logit there is none; where
+ * the other logits are all -inf, p' = 0: the loss is infinite and the gradient there 0.)
+ * Fastest with up to 186 entries, and up to 262144 logits (float32: 131072), in rows of unit stride.
  * loss = sum of weight_scale * weights * row_loss (weights NULL: 1), grad = its gradient. loss,
  * row_loss and grad may each be NULL. */
 CTB_API int ctb_distill_loss(const ctb_view* logits, const ctb_view* teacher_logits,
@@ -347,7 +350,8 @@ CTB_API int ctb_distill_loss(const ctb_view* logits, const ctb_view* teacher_log
  *     row_loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - 1 - d)
  * (the gradient goes through r A where the two are equal). loss and grad as in ctb_distill_loss.
  * kl = exp(d) - 1 - d (0 without ref_logprobs). ref_logprobs may be NULL when kl_coef is 0; loss,
- * row_loss, logprobs, kl and grad may each be NULL. */
+ * row_loss, logprobs, kl and grad may each be NULL. Fastest in rows of unit stride of up to 262144 logits
+ * (float32: 131072). */
 CTB_API int ctb_policy_loss(const ctb_view* logits, const ctb_view* targets, const ctb_view* old_logprobs,
                             const ctb_view* advantages, const ctb_view* ref_logprobs, const ctb_view* weights,
                             double weight_scale, double clip_low, double clip_high, double kl_coef,

@@ -8,14 +8,16 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("rows,share", [(1, 1.0), (37, 1.0), (200, 1.0), (2600, 0.02), (2600, 0.2), (2600, 0.9)])
 @pytest.mark.parametrize("tail", [False, True])
-def test_rows_of_three_stages(tail, rows, share):
+@pytest.mark.parametrize("v,dtype", [(131072, torch.bfloat16), (16384, torch.float32), (15003, torch.float32)])
+def test_rows_of_three_stages(v, dtype, tail, rows, share):
     import ctorch_b200 as cb
     from ctorch_b200 import _capi as C
 
-    v, top = 131072, 100
+    rows *= 4 if dtype == torch.float32 else 1  # a CTA has a row where four share one of 131072
+    top = 100
     g = torch.Generator(device="cuda")
     g.manual_seed(rows)
-    x = torch.randn(rows, v, generator=g, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(rows, v, generator=g, device="cuda", dtype=dtype)
     index = torch.randint(v // top, (rows, top), generator=g, device="cuda") + torch.arange(top, device="cuda") * (v // top)
     teacher = torch.randn(rows, top, generator=g, device="cuda")
     lse = teacher.logsumexp(1) + 0.3 if tail else None
@@ -38,6 +40,6 @@ def test_rows_of_three_stages(tail, rows, share):
         want *= on[b, None]
         # 2^-15: 64 roundings of float32 and more (losses_oracle); on an element that the teacher names p - q may cancel,
         # and with a tail 1 - q'/p' does: their terms' own errors count. Half a step of bfloat16 is 2^-8 of the value.
-        bound = 2.0 ** -8 * want.abs() + 2.0 ** -15 * p * on[b, None] + 1e-30
+        bound = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -15 * p * on[b, None] + 1e-30
         bound.scatter_add_(1, index[b], 2.0 ** -20 * q)
         assert ((got.grad[b].double() - want).abs() <= bound).all()
