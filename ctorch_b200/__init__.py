@@ -5,7 +5,8 @@ of that ABI:
   * ctorch_plugin/cuda_backend.cpp — the C++ drop-in for ctorch itself: it defines ctorch's four
     CUDA registration hooks and fills every CUDA dispatch slot;
   * this package — the same ops for torch CUDA tensors (ops.py mirrors ctorch's public API and
-    error types), the losses over logits rows with their gradients (losses.py), plus the
+    error types), the losses over logits rows with their gradients (losses.py), what a
+    language model's step has around them (model.py: norm, projection with cross entropy, balance loss), plus the
     row-sharded multi-GPU workload (sharded.py).
 """
 from .errors import AliasError, CommTimeoutError, DeviceError, DTypeError, Error, ShapeError  # noqa: F401
@@ -21,6 +22,16 @@ from .losses import (  # noqa: F401
     preference_loss,
     token_logprobs,
     token_logprobs_backward,
+)
+from .model import (  # noqa: F401
+    BalanceLoss,
+    LinearCrossEntropy,
+    RmsNorm,
+    RmsNormGrad,
+    balance_loss,
+    linear_cross_entropy,
+    rms_norm,
+    rms_norm_backward,
 )
 from .ops import (  # noqa: F401
     ValuesIndices,

@@ -18,6 +18,7 @@ ABI_VERSION = 1
 
 # dtype codes (ctorch::dtype enumerator order)
 F32, F64, I32, I64, BOOL, BF16 = 0, 1, 2, 3, 4, 5
+F8E4M3 = 6  # an output of rms_norm only: not among CODE_OF_TORCH, so every other operator refuses it
 CODE_OF_TORCH = {
     torch.float32: F32,
     torch.float64: F64,
@@ -94,6 +95,13 @@ def _load() -> ctypes.CDLL:
         "ctb_distill_loss": (i32, [V, V, V, V, V, f64, f64, V, V, V, vp, vp, sz, vp]),
         "ctb_policy_loss": (i32, [V, V, V, V, V, V, f64, f64, f64, f64, f64, V, V, V, V, V, vp, vp, sz, vp]),
         "ctb_preference_loss": (i32, [V, V, i64, V, V, V, V, f64, f64, f64, i32, V, V, V, V, V, vp, vp, sz, vp]),
+        "ctb_rms_norm": (i32, [V, V, V, f64, i32, V, V, V, V, vp]),
+        "ctb_rms_norm_backward_scratch_bytes": (sz, [V]),
+        "ctb_rms_norm_backward": (i32, [V, V, V, V, V, V, V, vp, sz, vp]),
+        "ctb_linear_loss_scratch_bytes": (sz, [V, V, i32, i32]),
+        "ctb_linear_cross_entropy": (i32, [V, V, V, V, f64, f64, f64, V, V, V, V, V, vp, vp, sz, vp]),
+        "ctb_balance_loss_scratch_bytes": (sz, [V, i64]),
+        "ctb_balance_loss": (i32, [V, V, V, i64, f64, f64, V, V, V, V, vp, vp, sz, vp]),
         "ctb_fill_random": (i32, [P, i32, u64, u64, i64, ctypes.c_double, ctypes.c_double, vp]),
         "ctb_debug_plan_elementwise": (i32, [P, ctypes.POINTER(P), i32, i32, ctypes.c_char_p, i32,
                                              ctypes.POINTER(ctypes.c_int),

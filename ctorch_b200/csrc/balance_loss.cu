@@ -1,0 +1,362 @@
+// balance_loss.cu — the balance loss of routed experts, with the experts' counts and the router's gradient
+// (include/ctb/ctb.h).
+//
+// For a group of rows of which n count, with p = softmax(x) of a row, its k chosen experts and lse = log sum exp x:
+//     f_e = (times e was chosen) / (n k),  P_e = mean p_e,  loss = coef E sum_e f_e P_e + z_coef mean lse^2
+//     dloss/dx_j = p_j / n (a_j - sum_e a_e p_e + 2 z_coef lse),  a_e = coef E f_e
+// A row's gradient needs the whole group's counts, so the rows are read twice: balance_rows sums a run of rows of one
+// group per CTA, balance_join adds the runs in their order, balance_grad writes the gradient.
+#include <algorithm>
+#include <cmath>
+
+#include "rows.cuh"
+
+namespace ctb {
+
+namespace {
+
+enum BalanceRow : int { kBlX = 0, kBlExperts, kBlMask, kBlGrad, kBlViews };
+
+constexpr int kMaxExperts = 4096;
+constexpr int kMaxGroups = 1 << 20;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+
+struct BalanceRun {  // of one CTA's rows
+    double lse2;
+    int32_t rows, bad;
+};
+
+struct BalanceGroup {
+    double loss, rows;
+    int32_t bad, pad;
+};
+
+struct BalanceArgs {
+    RowViews<kBlViews> v;
+    int64_t chosen, groups, length;  // experts a row; rows a group
+    int64_t runs, run_rows;          // CTAs a group, rows of each
+    double coef, z_coef;
+    float* run_probs;    // [groups * runs][E]
+    int32_t* run_counts; // the same
+    BalanceRun* run;     // [groups * runs]
+    float* slope;        // [groups][E] a_e
+    BalanceGroup* group; // [groups]
+    float* loss;
+    int64_t* counts;
+    int64_t counts_stride[2];
+    float* probs;
+    int64_t probs_stride[2];
+    int32_t* status;
+};
+
+__device__ __forceinline__ float warp_max(float x) {
+    for (int d = 16; d >= 1; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+    for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+
+__device__ __forceinline__ bool row_counts(const BalanceArgs& a, int64_t r) {
+    return !a.v.ptr[kBlMask] || real_at(a.v.ptr[kBlMask], a.v.dtype[kBlMask], row_offset(a.v, kBlMask, r)) != 0.0;
+}
+
+struct RowStats {
+    float m, s;  // maximum, sum of exp(x - m); s is NaN where the row has no softmax
+};
+
+template <class T> __device__ __forceinline__ RowStats row_stats(const T* x, int64_t inner, int experts) {
+    RowStats o{-INFINITY, 0.0f};
+    for (int e = threadIdx.x & 31; e < experts; e += 32) o.m = fmaxf(o.m, to_float(x[e * inner]));
+    o.m = warp_max(o.m);
+    for (int e = threadIdx.x & 31; e < experts; e += 32) o.s += expf(to_float(x[e * inner]) - o.m);
+    o.s = warp_sum(o.s);
+    return o;
+}
+
+// A warp a row; every lane keeps its columns' sums of p in its warp's part of shared memory.
+template <class T> __global__ void __launch_bounds__(kThreads) balance_rows(BalanceArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    dependent_wait();
+    const int experts = static_cast<int>(a.v.cols), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int32_t* const counts = reinterpret_cast<int32_t*>(smem);
+    float* const sums = reinterpret_cast<float*>(counts + experts);  // [kWarps][experts]
+    __shared__ double lse2[kWarps];
+    __shared__ int32_t live[kWarps];
+    __shared__ int32_t bad;
+    for (int e = threadIdx.x; e < experts; e += kThreads) counts[e] = 0;
+    for (int e = threadIdx.x; e < experts * kWarps; e += kThreads) sums[e] = 0.0f;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    const int64_t group = blockIdx.x / a.runs, run = blockIdx.x % a.runs;
+    const int64_t lo = group * a.length + run * a.run_rows, hi = min(lo + a.run_rows, (group + 1) * a.length);
+    double l2 = 0.0;
+    int n = 0;
+    for (int64_t r = lo + warp; r < hi; r += kWarps) {
+        if (!row_counts(a, r)) continue;
+        ++n;
+        const T* const x = static_cast<const T*>(a.v.ptr[kBlX]) + row_offset(a.v, kBlX, r);
+        const RowStats o = row_stats(x, a.v.inner[kBlX], experts);
+        const float inv = 1.0f / o.s;
+        for (int e = lane; e < experts; e += 32) sums[warp * experts + e] += expf(to_float(x[e * a.v.inner[kBlX]]) - o.m) * inv;
+        const double lse = static_cast<double>(o.m) + log(static_cast<double>(o.s));
+        l2 += lse * lse;
+        const int64_t at = row_offset(a.v, kBlExperts, r);
+        for (int64_t k = lane; k < a.chosen; k += 32) {
+            const int64_t e = index_at(a.v.ptr[kBlExperts], a.v.dtype[kBlExperts], at + k * a.v.inner[kBlExperts]);
+            if (e >= 0 && e < experts) {
+                atomicAdd(counts + e, 1);  // integers: any order gives the same
+            } else {
+                bad = 1;
+                record_bad_index(a.status, e);
+            }
+        }
+    }
+    if (lane == 0) {
+        lse2[warp] = l2;
+        live[warp] = n;
+    }
+    __syncthreads();
+    float* const out = a.run_probs + blockIdx.x * a.v.cols;
+    int32_t* const out_counts = a.run_counts + blockIdx.x * a.v.cols;
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        float s = 0.0f;
+        for (int w = 0; w < kWarps; ++w) s += sums[w * experts + e];
+        out[e] = s;
+        out_counts[e] = counts[e];
+    }
+    if (threadIdx.x == 0) {
+        BalanceRun b{0.0, 0, bad};
+        for (int w = 0; w < kWarps; ++w) {
+            b.lse2 += lse2[w];
+            b.rows += live[w];
+        }
+        a.run[blockIdx.x] = b;
+    }
+    allow_dependents();
+}
+
+// A CTA a group: its runs added in their order, in float64.
+__global__ void __launch_bounds__(kThreads) balance_join(BalanceArgs a) {
+    dependent_wait();
+    allow_dependents();
+    __shared__ double part[kWarps], total_lse2, total_rows;
+    __shared__ int32_t any_bad;
+    const int64_t g = blockIdx.x, experts = a.v.cols;
+    if (threadIdx.x == 0) {
+        double l2 = 0.0, n = 0.0;
+        int32_t bad = 0;
+        for (int64_t i = 0; i < a.runs; ++i) {
+            const BalanceRun b = a.run[g * a.runs + i];
+            l2 += b.lse2;
+            n += b.rows;
+            bad |= b.bad;
+        }
+        total_lse2 = l2;
+        total_rows = n;
+        any_bad = bad;
+    }
+    __syncthreads();
+    const double n = fmax(total_rows, 1.0);
+    double inner = 0.0;
+    for (int64_t e = threadIdx.x; e < experts; e += kThreads) {
+        double p = 0.0;
+        int64_t c = 0;
+        for (int64_t i = 0; i < a.runs; ++i) {
+            p += a.run_probs[(g * a.runs + i) * experts + e];
+            c += a.run_counts[(g * a.runs + i) * experts + e];
+        }
+        p /= n;
+        const double slope = a.coef * static_cast<double>(experts) * static_cast<double>(c) / (n * static_cast<double>(a.chosen));
+        inner += slope * p;
+        a.slope[g * experts + e] = any_bad ? NAN : static_cast<float>(slope);
+        if (a.counts) a.counts[g * a.counts_stride[0] + e * a.counts_stride[1]] = c;
+        if (a.probs) a.probs[g * a.probs_stride[0] + e * a.probs_stride[1]] = static_cast<float>(p);
+    }
+    for (int d = 16; d >= 1; d >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, d);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = inner;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (int w = 0; w < kWarps; ++w) s += part[w];
+        BalanceGroup b;
+        b.loss = any_bad ? nan("") : s + (a.z_coef != 0.0 ? a.z_coef * total_lse2 / n : 0.0);
+        b.rows = n;
+        b.bad = any_bad;
+        b.pad = 0;
+        a.group[g] = b;
+    }
+}
+
+template <class T> __global__ void __launch_bounds__(kThreads) balance_grad(BalanceArgs a) {
+    dependent_wait();
+    const int experts = static_cast<int>(a.v.cols), lane = threadIdx.x & 31;
+    if (a.loss && blockIdx.x == 0 && threadIdx.x == 0) {
+        double s = 0.0;
+        for (int64_t g = 0; g < a.groups; ++g) s += a.group[g].loss;
+        *a.loss = static_cast<float>(s / static_cast<double>(a.groups));
+    }
+    if (!a.v.ptr[kBlGrad]) return;
+    for (int64_t r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < a.v.rows; r += gridDim.x * kWarps) {
+        T* const grad = static_cast<T*>(a.v.ptr[kBlGrad]) + row_offset(a.v, kBlGrad, r);
+        if (!row_counts(a, r)) {
+            for (int e = lane; e < experts; e += 32) grad[e * a.v.inner[kBlGrad]] = from_float<T>(0.0f);
+            continue;
+        }
+        const T* const x = static_cast<const T*>(a.v.ptr[kBlX]) + row_offset(a.v, kBlX, r);
+        const int64_t g = r / a.length;
+        const float* const slope = a.slope + g * experts;
+        const RowStats o = row_stats(x, a.v.inner[kBlX], experts);
+        const float inv = 1.0f / o.s;
+        float dot = 0.0f;
+        for (int e = lane; e < experts; e += 32) dot += slope[e] * expf(to_float(x[e * a.v.inner[kBlX]]) - o.m) * inv;
+        dot = warp_sum(dot);
+        const double lse = static_cast<double>(o.m) + log(static_cast<double>(o.s));
+        const float up = a.z_coef != 0.0 ? static_cast<float>(2.0 * a.z_coef * lse) : 0.0f;
+        const float f = static_cast<float>(1.0 / (a.group[g].rows * static_cast<double>(a.groups)));
+        for (int e = lane; e < experts; e += 32) {
+            const float p = expf(to_float(x[e * a.v.inner[kBlX]]) - o.m) * inv;
+            grad[e * a.v.inner[kBlGrad]] = from_float<T>(p * (slope[e] - dot + up) * f);
+        }
+    }
+    allow_dependents();
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+
+struct Layout {
+    int64_t runs, run_rows;
+    size_t probs, counts, run, slope, group, bytes;
+};
+
+// Runs: enough CTAs for the GPU, of at least 32 rows each.
+Layout lay_out(int64_t rows, int64_t experts, int64_t groups) {
+    Layout l;
+    const int64_t length = rows / groups;
+    const int64_t want = std::max<int64_t>(1, sm_count() * 2 / groups);
+    l.run_rows = std::max<int64_t>(32, (length + want - 1) / want);
+    l.runs = std::max<int64_t>(1, (length + l.run_rows - 1) / l.run_rows);
+    size_t at = 0;
+    auto add = [&](int64_t n, size_t size) {
+        const size_t here = at;
+        at += (static_cast<size_t>(n) * size + 15) / 16 * 16;
+        return here;
+    };
+    l.probs = add(groups * l.runs * experts, 4);
+    l.counts = add(groups * l.runs * experts, 4);
+    l.run = add(groups * l.runs, sizeof(BalanceRun));
+    l.slope = add(groups * experts, 4);
+    l.group = add(groups, sizeof(BalanceGroup));
+    l.bytes = at;
+    return l;
+}
+
+int check_groups(int64_t rows, int64_t groups) {
+    if (groups < 1 || groups > kMaxGroups)
+        return fail(CTB_ERR_ARGUMENT, "groups must be 1 to " + std::to_string(kMaxGroups));
+    if (rows % groups) return fail(CTB_ERR_SHAPE, "the rows do not divide into " + std::to_string(groups) + " groups");
+    return CTB_OK;
+}
+
+template <class T> int run(const BalanceArgs& a, cudaStream_t st) {
+    const size_t smem = static_cast<size_t>(a.v.cols) * 4 * (kWarps + 1);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(balance_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxExperts * 4 * (kWarps + 1));
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail(CTB_ERR_CUDA, std::string("balance loss: ") + cudaGetErrorString(e));
+        }
+    }
+    launch_dependent(balance_rows<T>, static_cast<unsigned>(a.groups * a.runs), kThreads, smem, st, a);
+    count_launch();
+    CTB_CHECK(check_launch("balance loss"));
+    launch_dependent(balance_join, static_cast<unsigned>(a.groups), kThreads, 0, st, a);
+    count_launch();
+    CTB_CHECK(check_launch("balance loss"));
+    launch_dependent(balance_grad<T>, a.v.ptr[kBlGrad] ? grid_for((a.v.rows + kWarps - 1) / kWarps, 8) : 1u, kThreads, 0, st, a);
+    count_launch();
+    return check_launch("balance loss");
+}
+
+}  // namespace
+}  // namespace ctb
+
+using namespace ctb;
+
+extern "C" {
+
+size_t ctb_balance_loss_scratch_bytes(const ctb_view* logits, int64_t groups) {
+    if (!logits || logits->ndim < 1 || logits->ndim > kMaxDims || groups < 1 || groups > kMaxGroups) return 0;
+    int64_t rows = 1;
+    for (int d = 0; d < logits->ndim - 1; ++d) rows *= logits->shape[d];
+    return lay_out(rows, logits->shape[logits->ndim - 1], groups).bytes;
+}
+
+int ctb_balance_loss(const ctb_view* logits, const ctb_view* experts, const ctb_view* mask, int64_t groups, double coef,
+                     double z_coef, const ctb_view* loss, const ctb_view* counts, const ctb_view* probs,
+                     const ctb_view* grad, int32_t* d_status, void* scratch, size_t scratch_bytes, ctb_stream stream) {
+    return c_entry([&]() -> int {
+        BalanceArgs a{};
+        RowBuilder<kBlViews> b;
+        CTB_CHECK(b.begin(kBlX, logits, kDtypeMatrix, "logits"));
+        if (b.v.cols > kMaxExperts) return fail(CTB_ERR_SHAPE, "more than " + std::to_string(kMaxExperts) + " experts are not supported");
+        CTB_CHECK(check_groups(b.v.rows, groups));
+        CTB_CHECK(check_row_view(experts, "experts"));
+        if (experts->ndim < 1) return fail(CTB_ERR_SHAPE, "experts must be [..., chosen]");
+        a.chosen = experts->shape[experts->ndim - 1];
+        if (a.chosen < 1) return fail(CTB_ERR_SHAPE, "experts must name at least one expert a row");
+        CTB_CHECK(b.matrix(kBlExperts, experts, kDtypeIndex, a.chosen, false, "experts"));
+        if (mask) CTB_CHECK(b.operand(kBlMask, mask, kDtypeWeight, "mask"));
+        if (!(std::fabs(coef) <= 1e30)) return fail(CTB_ERR_ARGUMENT, "coef must be finite");
+        if (!(std::fabs(z_coef) <= 1e30)) return fail(CTB_ERR_ARGUMENT, "z_coef must be finite");
+        if (loss) {
+            CTB_CHECK(check_row_view(loss, "loss"));
+            CTB_CHECK(check_row_dtype(loss, 1u << CTB_FLOAT32, "loss"));
+            for (int d = 0; d < loss->ndim; ++d)
+                if (loss->shape[d] != 1) return fail(CTB_ERR_SHAPE, "loss must hold one element");
+            a.loss = static_cast<float*>(loss->data);
+        }
+        auto table = [&](const ctb_view* t, int dtype, const char* what, int64_t (&strides)[2]) -> int {
+            CTB_CHECK(check_row_view(t, what));
+            CTB_CHECK(check_row_dtype(t, 1u << dtype, what));
+            if (t->ndim != 2 || t->shape[0] != groups || t->shape[1] != b.v.cols)
+                return fail(CTB_ERR_SHAPE, std::string(what) + " must be [groups, experts]");
+            strides[0] = t->strides[0];
+            strides[1] = t->strides[1];
+            return check_written(t, what);
+        };
+        if (counts) {
+            CTB_CHECK(table(counts, CTB_INT64, "counts", a.counts_stride));
+            a.counts = static_cast<int64_t*>(counts->data);
+        }
+        if (probs) {
+            CTB_CHECK(table(probs, CTB_FLOAT32, "probs", a.probs_stride));
+            a.probs = static_cast<float*>(probs->data);
+        }
+        if (grad) CTB_CHECK(b.matrix(kBlGrad, grad, 1u << logits->dtype, b.v.cols, true, "grad"));
+        CTB_CHECK(check_row_status(d_status));
+        const Layout l = lay_out(b.v.rows, b.v.cols, groups);
+        CTB_CHECK(check_row_scratch(scratch, scratch_bytes, l.bytes, 16));
+        b.finish();
+        a.v = b.v;
+        a.groups = groups;
+        a.length = b.v.rows / groups;
+        a.runs = l.runs;
+        a.run_rows = l.run_rows;
+        a.coef = coef;
+        a.z_coef = z_coef;
+        a.status = d_status;
+        unsigned char* const s = static_cast<unsigned char*>(scratch);
+        a.run_probs = reinterpret_cast<float*>(s + l.probs);
+        a.run_counts = reinterpret_cast<int32_t*>(s + l.counts);
+        a.run = reinterpret_cast<BalanceRun*>(s + l.run);
+        a.slope = reinterpret_cast<float*>(s + l.slope);
+        a.group = reinterpret_cast<BalanceGroup*>(s + l.group);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        return logits->dtype == CTB_FLOAT32 ? run<float>(a, st) : run<__nv_bfloat16>(a, st);
+    });
+}
+
+}  // extern "C"

@@ -116,6 +116,7 @@ size_t dtype_size(int dt) {
     case CTB_INT64: return 8;
     case CTB_BOOL: return 1;
     case CTB_BFLOAT16: return 2;
+    case CTB_FLOAT8_E4M3: return 1;
     }
     return 0;
 }
@@ -128,6 +129,7 @@ const char* dtype_name(int dt) {
     case CTB_INT64: return "int64";
     case CTB_BOOL: return "bool";
     case CTB_BFLOAT16: return "bfloat16";
+    case CTB_FLOAT8_E4M3: return "float8_e4m3";
     }
     return "unknown";
 }

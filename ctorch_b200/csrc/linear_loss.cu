@@ -1,0 +1,470 @@
+// linear_loss.cu — the projection to the vocabulary with its cross entropy (include/ctb/ctb.h): checks, the plan of a
+// call and its scratch, and the small kernels around the three products (linear_loss_tc.cu for bfloat16,
+// linear_loss_f32.cu for float32): the list of rows that count, packed copies, the rows' softmax, the join of split
+// sums, the scalar loss.
+#include <algorithm>
+#include <cmath>
+
+#include "linear_loss.cuh"
+
+namespace ctb {
+
+unsigned long long* wait_timeout_counter();  // async.cu
+
+namespace {
+
+constexpr int64_t kHeldBytes = int64_t(2) << 30;  // of a block's logits or exponentials: 8192 rows of 131072 in 16 bits
+constexpr int kOrderThreads = 1024;
+
+__device__ __forceinline__ double row_weight(const LinearArgs& a, int64_t row) {
+    return a.v.ptr[kLnWeight] ? real_at(a.v.ptr[kLnWeight], a.v.dtype[kLnWeight], row_offset(a.v, kLnWeight, row)) : 1.0;
+}
+
+__device__ __forceinline__ void put(const LinearArgs& a, int slot, int64_t row, double x) {
+    if (a.v.ptr[slot]) static_cast<float*>(a.v.ptr[slot])[row_offset(a.v, slot, row)] = static_cast<float>(x);
+}
+
+// One CTA: the rows that count, then the others, each in their order; results of the others. A thread takes a run of
+// rows, so one scan of the threads' counts places them. Bound by its latency (a few microseconds at 8192 rows).
+__global__ void __launch_bounds__(kOrderThreads) linear_order(LinearArgs a) {
+    dependent_wait();
+    allow_dependents();
+    __shared__ int64_t counts[kOrderThreads];
+    __shared__ float largest[kOrderThreads / 32];
+    const int64_t rows = a.v.rows, each = (rows + kOrderThreads - 1) / kOrderThreads;
+    const int64_t lo = min(rows, each * threadIdx.x), hi = min(rows, lo + each);
+    int64_t mine = 0;
+    float top = 0.0f;
+    for (int64_t r = lo; r < hi; ++r) {
+        const double w = row_weight(a, r);
+        if (w != 0.0) {
+            ++mine;
+            top = fmaxf(top, static_cast<float>(fabs(w)));
+        }
+    }
+    counts[threadIdx.x] = mine;
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int d = 1; d < kOrderThreads; d <<= 1) {
+        const int64_t before = threadIdx.x >= d ? counts[threadIdx.x - d] : 0;
+        __syncthreads();
+        counts[threadIdx.x] += before;
+        __syncthreads();
+    }
+    const int64_t n = counts[kOrderThreads - 1];
+    int64_t on = counts[threadIdx.x] - mine, off = n + lo - on;
+    for (int64_t r = lo; r < hi; ++r) {
+        if (row_weight(a, r) != 0.0) {
+            a.order[on++] = static_cast<int32_t>(r);
+        } else {
+            a.order[off++] = static_cast<int32_t>(r);
+            a.weighted[r] = 0.0;
+            put(a, kLnRowLoss, r, 0.0);
+            put(a, kLnLse, r, 0.0);
+        }
+    }
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kOrderThreads / 32; ++w) top = fmaxf(top, largest[w]);
+        a.facts->count = static_cast<int32_t>(n);
+        a.facts->wmax = top;
+    }
+}
+
+// Rows as the products want them: contiguous, 16-byte aligned, zero up to the pitch. ORDERED: hidden's rows that
+// count, and zeros up to a multiple of 64 rows (they are a product's inner dimension too).
+template <class From, class To, bool ORDERED>
+__global__ void __launch_bounds__(256) linear_pack(LinearArgs a, Matrix2 from, Matrix2 to, int64_t rows, int64_t cols) {
+    dependent_wait();
+    const int64_t n = ORDERED && a.order ? a.facts->count : rows;
+    const int64_t upto = ORDERED ? min(rows, (n + 63) / 64 * 64) : rows;
+    for (int64_t i = blockIdx.x; i < upto; i += gridDim.x) {
+        To* const out = static_cast<To*>(to.ptr) + i * to.row;
+        const int64_t r = ORDERED && a.order && i < n ? a.order[i] : i;
+        const From* const in = static_cast<const From*>(from.ptr) + (ORDERED ? row_offset(a.v, kLnHidden, r) : r * from.row);
+        for (int64_t j = threadIdx.x; j < to.row; j += 256)
+            out[j] = i < n && j < cols ? from_float<To>(to_float(in[j * from.col])) : from_float<To>(0.0f);
+    }
+    allow_dependents();
+}
+
+// ------------------------------------------------------------------------------------------------
+// the rows' softmax
+
+struct RowResult {
+    double lse, loss, w;  // w: weight over the block's factor
+    int64_t row, target;
+    bool bad;
+};
+
+__device__ __forceinline__ RowResult row_result(const LinearArgs& a, int64_t i, double m, double s, double zt) {
+    RowResult o;
+    o.row = a.order ? a.order[i] : i;
+    o.target = index_at(a.v.ptr[kLnTarget], a.v.dtype[kLnTarget], row_offset(a.v, kLnTarget, o.row));
+    o.bad = o.target < 0 || o.target >= a.vocab;
+    const double w = row_weight(a, o.row), rest = log(s);
+    o.lse = m * a.inv_temp + rest;
+    o.loss = o.bad ? nan("") : (m - zt) * a.inv_temp + rest + (a.z_coef != 0.0 ? a.z_coef * o.lse * o.lse : 0.0);
+    o.w = a.order ? w / static_cast<double>(a.facts->wmax) : 1.0;
+    return o;
+}
+
+__device__ __forceinline__ void put_row_result(const LinearArgs& a, const RowResult& o) {
+    if (o.bad) record_bad_index(a.status, o.target);
+    put(a, kLnRowLoss, o.row, o.loss);
+    put(a, kLnLse, o.row, o.bad ? nan("") : o.lse);
+    a.weighted[o.row] = a.scale * row_weight(a, o.row) * o.loss;
+}
+
+__device__ __forceinline__ float exp2_approx(float t) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+    return y;
+}
+
+// Joins (maximum, sum) pairs; s is relative to m.
+__device__ __forceinline__ void join_sums(float& m, float& s, float om, float os, float c2) {
+    const float top = fmaxf(m, om);
+    const float at = top == -INFINITY ? 0.0f : top;
+    s = s * exp2_approx((m - at) * c2) + os * exp2_approx((om - at) * c2);
+    m = om != om || m != m ? NAN : top;
+}
+
+template <int THREADS> __device__ __forceinline__ void join_block(float& m, float& s, float c2) {
+    __shared__ float sm[THREADS / 32], ss[THREADS / 32];
+    for (int d = 16; d >= 1; d >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, d), os = __shfl_xor_sync(0xffffffffu, s, d);
+        join_sums(m, s, om, os, c2);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+        sm[threadIdx.x >> 5] = m;
+        ss[threadIdx.x >> 5] = s;
+    }
+    __syncthreads();
+    m = sm[0];
+    s = ss[0];
+    for (int w = 1; w < THREADS / 32; ++w) join_sums(m, s, sm[w], ss[w], c2);
+    if (m == INFINITY) s = NAN;
+}
+
+// float32: a CTA a row of held logits; statistics, then G in their place. The row's second pass comes from L2.
+__global__ void __launch_bounds__(512) linear_rows_f32(LinearArgs a, int64_t first, int grad) {
+    dependent_wait();
+    const int64_t n = a.order ? linear_block_rows(a, first) : min(a.block, a.v.rows - first);
+    for (int64_t b = blockIdx.x; b < n; b += gridDim.x) {
+        float* const z = static_cast<float*>(a.held) + b * a.held_pitch;
+        float m = -INFINITY, s = 0.0f;
+        for (int64_t j = threadIdx.x; j < a.vocab; j += 512) m = z[j] != z[j] ? NAN : m != m ? m : fmaxf(m, z[j]);
+        const float at = m == -INFINITY ? 0.0f : m;
+        for (int64_t j = threadIdx.x; j < a.vocab; j += 512) s += exp2_approx((z[j] - at) * a.c2);
+        join_block<512>(m, s, a.c2);
+        const int64_t t0 = index_at(a.v.ptr[kLnTarget], a.v.dtype[kLnTarget],
+                                    row_offset(a.v, kLnTarget, a.order ? a.order[first + b] : first + b));
+        const bool inside = t0 >= 0 && t0 < a.vocab;
+        const float zt = inside ? z[t0] : 0.0f;
+        const RowResult o = row_result(a, first + b, m, s, zt);
+        __syncthreads();
+        if (threadIdx.x == 0) put_row_result(a, o);
+        if (!grad) continue;
+        const double up = 1.0 + 2.0 * a.z_coef * o.lse;
+        const float c = o.bad ? NAN : static_cast<float>(o.w * up / static_cast<double>(s));
+        for (int64_t j = threadIdx.x; j < a.held_pitch; j += 512) {
+            float g = 0.0f;
+            if (j < a.vocab) {
+                g = c * exp2_approx((z[j] - m) * a.c2);
+                if (j == t0) {
+                    const double logp = (static_cast<double>(zt) - m) * a.inv_temp - log(static_cast<double>(s));
+                    g = static_cast<float>(o.w * (expm1(logp) + 2.0 * a.z_coef * o.lse * exp(logp)));
+                }
+            }
+            z[j] = g;
+        }
+    }
+    allow_dependents();
+}
+
+// grad_hidden's rows of a block: the splits of dH = G W added in their order, times the factor; zeros where rows do
+// not count (with the last block).
+template <class T> __global__ void __launch_bounds__(256) linear_join(LinearArgs a, int64_t first, int64_t upto) {
+    dependent_wait();
+    const int64_t n = a.order ? a.facts->count : a.v.rows;
+    const double f = linear_factor(a);
+    T* const grad = static_cast<T*>(a.v.ptr[kLnGrad]);
+    const int64_t inner = a.v.inner[kLnGrad];
+    for (int64_t i = first + blockIdx.x; i < upto; i += gridDim.x) {
+        const int64_t r = a.order ? a.order[i] : i;
+        T* const out = grad + row_offset(a.v, kLnGrad, r);
+        const float* const p = a.partial + (i - first) * a.part_pitch;
+        for (int64_t j = threadIdx.x; j < a.v.cols; j += 256) {
+            float x = 0.0f;
+            if (i < n)
+                for (int s = 0; s < a.splits; ++s) x += p[s * a.block * a.part_pitch + j];
+            out[j * inner] = from_float<T>(static_cast<float>(f * static_cast<double>(x)));
+        }
+    }
+    allow_dependents();
+}
+
+// out = the sum of n numbers in a fixed order, rounded once.
+__global__ void __launch_bounds__(1024) linear_total(const double* x, int64_t n, float* out) {
+    dependent_wait();
+    allow_dependents();
+    __shared__ double sm[32];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += x[i];
+    for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int w = 0; w < 32; ++w) t += sm[w];
+        *out = static_cast<float>(t);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// Whether the products can read a matrix of unit inner stride in place (vector loads and tensor copies start on 16 bytes).
+bool in_place(const void* p, int64_t row, int64_t col, int64_t rows, int64_t cols, int dtype, int want) {
+    const int64_t size = static_cast<int64_t>(dtype_size(dtype));
+    return dtype == want && (col == 1 || cols == 1) && reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+           (rows == 1 || (row * size % 16 == 0 && row >= cols));
+}
+
+struct Layout {
+    size_t bytes = 0;
+    size_t add(int64_t n, int64_t size) {
+        const size_t at = bytes;
+        bytes += static_cast<size_t>(round_up(n * size, 256));
+        return at;
+    }
+};
+
+struct LinearPlan {
+    LinearArgs a{};
+    bool grad = false, weighted = false, pack_h = false, pack_w = false;
+    int64_t h_row = -1;      // hidden's row stride, where its leading dims are one
+    int work = CTB_FLOAT32;  // the products' operand type
+    int64_t blocks = 0;
+    size_t bytes = 0;
+    size_t facts, order, weights, target_z, stats, held, partial, acc, h, w;
+};
+
+// The sizes of a call's pieces. Everything here follows from shapes, strides and alignment alone.
+void lay_out(LinearPlan& p) {
+    LinearArgs& a = p.a;
+    const int64_t rows = a.v.rows, dim = a.v.cols, vocab = a.vocab;
+    p.work = CTB_FLOAT32;
+    const int64_t size = static_cast<int64_t>(dtype_size(p.work)), pack = 16 / size;
+    const int64_t pitch = round_up(dim, pack);
+    a.held_pitch = round_up(vocab, pack);
+    a.tiles = (vocab + 255) / 256;
+    a.block = std::max<int64_t>(256, kHeldBytes / (a.held_pitch * size) / 256 * 256);
+    a.block = std::min(a.block, rows);
+    p.blocks = (rows + a.block - 1) / a.block;
+    p.pack_h = p.weighted || p.h_row < 0 ||
+               !in_place(a.v.ptr[kLnHidden], p.h_row, a.v.inner[kLnHidden], rows, dim, a.v.dtype[kLnHidden], p.work);
+    p.pack_w = !in_place(a.weight.ptr, a.weight.row, a.weight.col, vocab, dim, a.weight.dtype, p.work);
+    // dH has few tiles of 128 x 128 and a long sum: it is split until the GPU is full
+    const int64_t tiles = ((a.block + 127) / 128) * ((dim + 127) / 128);
+    a.splits = static_cast<int>(std::min<int64_t>({16, std::max<int64_t>(1, 296 / tiles), (vocab + 511) / 512}));
+    a.part_pitch = pitch;
+    a.acc_pitch = pitch;
+    Layout l;
+    p.facts = l.add(1, sizeof(LinearFacts));
+    p.order = l.add(p.weighted ? rows : 0, 4);
+    p.weights = l.add(rows, 8);
+    p.target_z = l.add(a.block, 4);
+    p.stats = l.add(0, 8);
+    p.held = l.add(a.block * a.held_pitch, size);
+    p.partial = l.add(p.grad ? a.splits * a.block * a.part_pitch : 0, 4);
+    p.acc = l.add(p.grad && p.blocks > 1 ? vocab * a.acc_pitch : 0, 4);
+    p.h = l.add(p.pack_h ? rows * pitch : 0, size);
+    p.w = l.add(p.pack_w ? vocab * pitch : 0, size);
+    p.bytes = l.bytes;
+    a.h.row = p.pack_h ? pitch : p.h_row;
+    a.w.row = p.pack_w ? pitch : a.weight.row;
+    a.h.col = a.w.col = 1;
+    a.h.dtype = a.w.dtype = p.work;
+}
+
+void place(LinearPlan& p, void* scratch) {
+    LinearArgs& a = p.a;
+    unsigned char* const s = static_cast<unsigned char*>(scratch);
+    a.facts = reinterpret_cast<LinearFacts*>(s + p.facts);
+    a.order = p.weighted ? reinterpret_cast<int32_t*>(s + p.order) : nullptr;
+    a.weighted = reinterpret_cast<double*>(s + p.weights);
+    a.target_z = reinterpret_cast<float*>(s + p.target_z);
+    a.stats = reinterpret_cast<float2*>(s + p.stats);
+    a.held = s + p.held;
+    a.partial = reinterpret_cast<float*>(s + p.partial);
+    a.acc = p.blocks > 1 ? reinterpret_cast<float*>(s + p.acc) : nullptr;
+    a.h.ptr = p.pack_h ? static_cast<void*>(s + p.h) : a.v.ptr[kLnHidden];
+    a.w.ptr = p.pack_w ? static_cast<void*>(s + p.w) : a.weight.ptr;
+}
+
+template <class From, class To, bool ORDERED>
+void launch_pack(const LinearArgs& a, const Matrix2& from, const Matrix2& to, int64_t rows, int64_t cols, cudaStream_t st) {
+    launch_dependent(linear_pack<From, To, ORDERED>, grid_for(rows, 8), 256, 0, st, a, from, to, rows, cols);
+    count_launch();
+}
+
+template <bool ORDERED>
+int run_pack(const LinearPlan& p, const Matrix2& from, const Matrix2& to, int64_t rows, cudaStream_t st) {
+    const LinearArgs& a = p.a;
+    if (from.dtype == CTB_FLOAT32) launch_pack<float, float, ORDERED>(a, from, to, rows, a.v.cols, st);
+    else launch_pack<__nv_bfloat16, float, ORDERED>(a, from, to, rows, a.v.cols, st);
+    return check_launch("linear loss: packing");
+}
+
+int linear_run(const LinearPlan& p, const ctb_view* loss, cudaStream_t st) {
+    const LinearArgs& a = p.a;
+    const int64_t rows = a.v.rows;
+    if (rows && p.weighted) {
+        launch_dependent(linear_order, 1, kOrderThreads, 0, st, a);
+        count_launch();
+        CTB_CHECK(check_launch("linear loss: rows"));
+    }
+    if (p.pack_h) CTB_CHECK(run_pack<true>(p, Matrix2{a.v.ptr[kLnHidden], 0, a.v.inner[kLnHidden], a.v.dtype[kLnHidden]}, a.h, rows, st));
+    if (p.pack_w) CTB_CHECK(run_pack<false>(p, a.weight, a.w, a.vocab, st));
+    for (int64_t first = 0; first < rows; first += a.block) {
+        const int64_t n = std::min(a.block, rows - first);
+        CTB_CHECK(linear_logits_f32(a, first, n, st));
+        launch_dependent(linear_rows_f32, grid_for(n, 4), 512, 0, st, a, first, static_cast<int>(p.grad));
+        count_launch();
+        CTB_CHECK(check_launch("linear loss: rows"));
+        if (!p.grad) continue;
+        CTB_CHECK(linear_grad_hidden_f32(a, first, n, st));
+        auto join = a.v.dtype[kLnGrad] == CTB_FLOAT32 ? linear_join<float> : linear_join<__nv_bfloat16>;
+        launch_dependent(join, grid_for(n, 8), 256, 0, st, a, first, first + n);
+        count_launch();
+        CTB_CHECK(check_launch("linear loss: join"));
+        CTB_CHECK(linear_grad_weight_f32(a, first, n, first + n == rows, st));
+    }
+    if (rows == 0 && p.grad) CTB_CHECK(linear_grad_weight_f32(a, 0, 0, true, st));
+    if (loss) {
+        launch_dependent(linear_total, 1, 1024, 0, st, static_cast<const double*>(a.weighted), rows, static_cast<float*>(loss->data));
+        count_launch();
+        CTB_CHECK(check_launch("linear loss: total"));
+    }
+    return CTB_OK;
+}
+
+}  // namespace
+}  // namespace ctb
+
+using namespace ctb;
+
+namespace {
+
+int matrix_of(const ctb_view* v, const char* what, Matrix2& m) {
+    CTB_CHECK(check_row_view(v, what));
+    CTB_CHECK(check_row_dtype(v, kDtypeMatrix, what));
+    if (v->ndim != 2) return fail(CTB_ERR_SHAPE, std::string(what) + " must be [vocabulary, columns of hidden]");
+    m = Matrix2{v->data, v->strides[0], v->strides[1], v->dtype};
+    return CTB_OK;
+}
+
+// The checks that the scratch query shares with the call.
+int begin_plan(LinearPlan& p, RowBuilder<kLnViews>& b, const ctb_view* hidden, const ctb_view* weight) {
+    CTB_CHECK(b.begin(kLnHidden, hidden, kDtypeMatrix, "hidden"));
+    CTB_CHECK(matrix_of(weight, "weight", p.a.weight));
+    if (weight->dtype != hidden->dtype) return fail(CTB_ERR_DTYPE, "weight's dtype must equal hidden's");
+    if (weight->shape[1] != b.v.cols) return fail(CTB_ERR_SHAPE, "weight must be [vocabulary, columns of hidden]");
+    p.a.vocab = weight->shape[0];
+    // one stride from row to row, if there is one
+    p.h_row = 0;
+    int64_t extent = 1;
+    for (int d = b.lead - 1; d >= 0 && p.h_row >= 0; --d) {
+        if (hidden->shape[d] == 1) continue;
+        if (extent == 1) p.h_row = hidden->strides[d];
+        else if (hidden->strides[d] != p.h_row * extent) p.h_row = -1;
+        extent *= hidden->shape[d];
+    }
+    if (p.a.vocab < 1) return fail(CTB_ERR_SHAPE, "the vocabulary is empty (a softmax over no entries has no value)");
+    if (p.a.vocab >= (int64_t(1) << 31)) return fail(CTB_ERR_SHAPE, "vocabularies of 2^31 or more entries are not supported");
+    return CTB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad) {
+    size_t need = 0;
+    c_entry([&]() -> int {
+        LinearPlan p;
+        RowBuilder<kLnViews> b;
+        CTB_CHECK(begin_plan(p, b, hidden, weight));
+        b.finish();
+        p.a.v = b.v;
+        p.weighted = weighted != 0;
+        p.grad = grad != 0;
+        if (b.v.rows) lay_out(p);
+        need = p.bytes;
+        return CTB_OK;
+    });
+    return need;
+}
+
+int ctb_linear_cross_entropy(const ctb_view* hidden, const ctb_view* weight, const ctb_view* targets,
+                             const ctb_view* weights, double weight_scale, double temperature, double z_coef,
+                             const ctb_view* loss, const ctb_view* row_loss, const ctb_view* lse,
+                             const ctb_view* grad_hidden, const ctb_view* grad_weight, int32_t* d_status, void* scratch,
+                             size_t scratch_bytes, ctb_stream stream) {
+    return c_entry([&]() -> int {
+        LinearPlan p;
+        RowBuilder<kLnViews> b;
+        CTB_CHECK(begin_plan(p, b, hidden, weight));
+        LinearArgs& a = p.a;
+        CTB_CHECK(b.operand(kLnTarget, targets, kDtypeIndex, "targets"));
+        if (weights) CTB_CHECK(b.operand(kLnWeight, weights, kDtypeWeight, "weights"));
+        CTB_CHECK(b.result(kLnRowLoss, row_loss, 1u << CTB_FLOAT32, "row_loss"));
+        CTB_CHECK(b.result(kLnLse, lse, 1u << CTB_FLOAT32, "lse"));
+        if (!(temperature >= 1e-30 && temperature <= 1e30))
+            return fail(CTB_ERR_ARGUMENT, "temperature must be positive (1e-30 to 1e30)");
+        if (!(z_coef >= 0.0 && z_coef <= 1e30)) return fail(CTB_ERR_ARGUMENT, "z_coef must be finite and not negative");
+        if (!std::isfinite(weight_scale)) return fail(CTB_ERR_ARGUMENT, "weight_scale must be finite");
+        if (loss) {
+            CTB_CHECK(check_row_view(loss, "loss"));
+            CTB_CHECK(check_row_dtype(loss, 1u << CTB_FLOAT32, "loss"));
+            for (int d = 0; d < loss->ndim; ++d)
+                if (loss->shape[d] != 1) return fail(CTB_ERR_SHAPE, "loss must hold one element");
+        }
+        if (!grad_hidden != !grad_weight) return fail(CTB_ERR_ARGUMENT, "both gradients or none");
+        p.grad = grad_hidden != nullptr;
+        if (p.grad) {
+            CTB_CHECK(b.matrix(kLnGrad, grad_hidden, 1u << hidden->dtype, b.v.cols, true, "grad_hidden"));
+            CTB_CHECK(matrix_of(grad_weight, "grad_weight", a.grad_weight));
+            if (grad_weight->dtype != weight->dtype) return fail(CTB_ERR_DTYPE, "grad_weight's dtype must equal weight's");
+            if (grad_weight->shape[0] != weight->shape[0] || grad_weight->shape[1] != weight->shape[1])
+                return fail(CTB_ERR_SHAPE, "grad_weight's shape must equal weight's");
+            CTB_CHECK(check_written(grad_weight, "grad_weight"));
+        }
+        CTB_CHECK(check_row_status(d_status));
+        b.finish();
+        a.v = b.v;
+        a.scale = weight_scale;
+        a.inv_temp = 1.0 / temperature;
+        a.c2 = static_cast<float>(1.4426950408889634 * a.inv_temp);
+        a.z_coef = z_coef;
+        a.status = d_status;
+        a.timeouts = wait_timeout_counter();
+        p.weighted = weights != nullptr;
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (a.v.rows == 0) {  // no rows: a loss of 0 and a weight gradient of 0
+            a.block = 0;
+        } else {
+            lay_out(p);
+            CTB_CHECK(check_row_scratch(scratch, scratch_bytes, p.bytes, 256));
+            place(p, scratch);
+        }
+        return linear_run(p, loss, st);
+    });
+}
+
+}  // extern "C"

@@ -40,7 +40,7 @@ extern "C" {
 
 /* Element types; the codes are the enumerator values of ctorch::dtype (include/ctorch/dtype.h:24-31). */
 enum ctb_dtype { CTB_FLOAT32 = 0, CTB_FLOAT64 = 1, CTB_INT32 = 2, CTB_INT64 = 3, CTB_BOOL = 4,
-                 CTB_BFLOAT16 = 5 };
+                 CTB_BFLOAT16 = 5, CTB_FLOAT8_E4M3 = 6 /* an output of ctb_rms_norm only */ };
 
 /* Status codes. The ctorch shim maps them onto ctorch's exception tree (include/ctorch/errors.h). */
 enum ctb_status {
@@ -376,6 +376,75 @@ CTB_API int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets,
                                 const ctb_view* pair_loss, const ctb_view* rewards, const ctb_view* logprobs,
                                 const ctb_view* grad, int32_t* d_status, void* scratch, size_t scratch_bytes,
                                 ctb_stream stream);
+
+/* ---- around the losses: the norm, the projection with its cross entropy, the balance loss ---- */
+
+/* Common to the entry points of this section. Matrices are [..., columns]: any leading dims and strides, float32 or
+ * bfloat16; a "row" is one position of the leading dims of the first matrix, further matrices have the same leading
+ * shape, numbers a row broadcast (right-aligned) to it, results a row have exactly it and float32 elements.
+ * Statistics, sums and products are float32 or more, each result is rounded once, no sum's order changes: equal calls
+ * give equal bits. Nothing is kept between calls, so any of them may be captured into a graph and replayed; calls
+ * that may run at the same time need scratch of their own. d_status as in the losses. No ctorch counterpart. */
+
+/* The root-mean-square norm of rows, with the residual's addition:
+ *     s = x + residual (rounded to their type; x alone without a residual),  rstd = 1 / sqrt(mean(s^2) + eps),
+ *     y = s * rstd * weight
+ * summed = s (given exactly when residual is; it may be x's or residual's own view), out = y in x's type (it may be
+ * x's own view), or with quant 1 or 2 in 8 bits: out = y / scale as CTB_FLOAT8_E4M3 (rounded to nearest), one scale
+ * a row (1) or one for every 128 columns, [..., ceil(columns / 128)] (2); scale = the largest |y| / 448, and 1 where
+ * that is 0. weight is [columns], float32 or bfloat16. rstd may be NULL. Otherwise outputs must not overlap inputs. */
+CTB_API int ctb_rms_norm(const ctb_view* x, const ctb_view* weight, const ctb_view* residual, double eps, int quant,
+                         const ctb_view* out, const ctb_view* summed, const ctb_view* rstd, const ctb_view* scales,
+                         ctb_stream stream);
+
+/* Scratch bytes of ctb_rms_norm_backward where grad_weight is wanted (16-byte aligned). */
+CTB_API size_t ctb_rms_norm_backward_scratch_bytes(const ctb_view* summed);
+
+/* Its backward pass. With h = summed * rstd and g = grad_out * weight:
+ *     grad_x = rstd * (g - h * mean(g h)) + grad_summed,   grad_weight = sum over rows of grad_out * h
+ * summed and rstd are the forward call's (x itself without a residual); grad_summed is what comes back to `summed`
+ * from elsewhere (NULL: nothing). grad_x is the gradient of x and of the residual alike; it may be grad_out's,
+ * summed's or grad_summed's own view. grad_weight has weight's type and may be NULL. */
+CTB_API int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summed, const ctb_view* weight,
+                                  const ctb_view* rstd, const ctb_view* grad_summed, const ctb_view* grad_x,
+                                  const ctb_view* grad_weight, void* scratch, size_t scratch_bytes, ctb_stream stream);
+
+/* Scratch bytes of ctb_linear_cross_entropy (256-byte aligned); weighted: whether weights are given, grad: whether
+ * gradients are wanted. Up to 2 GiB for the pieces of the logits that are held at a time, beside copies of what
+ * cannot be read in place. Depends on the views' strides and alignment too. */
+CTB_API size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad);
+
+/* Cross entropy of the projection of hidden [..., D] to a vocabulary, weight [V, D] of the same type, without the
+ * logits z = hidden weight^T / temperature as a matrix: with lse = log sum exp z of a row,
+ *     row_loss = lse - z[target] + z_coef lse^2,    loss = sum of weight_scale * weights * row_loss (weights NULL: 1)
+ * and the gradients of loss, grad_hidden (hidden's shape) and grad_weight (weight's shape), both or neither.
+ * A row whose weight is 0 does not count: its hidden state and target are not looked at, its results and its row of
+ * grad_hidden are 0. A target outside [0, V) in a row that counts makes that row's results, its row of grad_hidden
+ * and all of grad_weight NaN. loss, row_loss and lse may each be NULL. Gradients must not overlap each other or the
+ * operands. Without rows loss and grad_weight are 0. In bfloat16 the gradient of a logit is rounded once to bfloat16
+ * (relative to its row's weight) before the products with weight and hidden, which sum in float32. */
+CTB_API int ctb_linear_cross_entropy(const ctb_view* hidden, const ctb_view* weight, const ctb_view* targets,
+                                     const ctb_view* weights, double weight_scale, double temperature, double z_coef,
+                                     const ctb_view* loss, const ctb_view* row_loss, const ctb_view* lse,
+                                     const ctb_view* grad_hidden, const ctb_view* grad_weight, int32_t* d_status,
+                                     void* scratch, size_t scratch_bytes, ctb_stream stream);
+
+/* Scratch bytes of ctb_balance_loss (16-byte aligned). */
+CTB_API size_t ctb_balance_loss_scratch_bytes(const ctb_view* logits, int64_t groups);
+
+/* The balance loss of routed experts. logits [..., E] are the router's (E up to 4096), experts [..., k] the experts
+ * chosen for each row (int32 or int64). The rows are `groups` equal shares in their order (sequences; 1: all as one).
+ * In a group of which n rows count (mask NULL: all), with p = softmax(logits) and lse = log sum exp of a row:
+ *     counts[e] = times e was chosen,  f = counts / (n k),  probs = mean of p,
+ *     group loss = coef E sum_e f_e probs_e + z_coef mean(lse^2),    loss = mean of the groups' losses
+ * grad = its gradient (counts are constants), in the logits' type; it may be the logits' own view. A row whose mask is 0
+ * does not count: nothing of it is looked at and its gradient is 0. A group of no rows gives 0. An expert outside
+ * [0, E) in a row that counts makes the loss and its group's gradients NaN (it is not counted). counts [groups, E]
+ * int64, probs [groups, E] float32; loss, counts, probs and grad may each be NULL. */
+CTB_API int ctb_balance_loss(const ctb_view* logits, const ctb_view* experts, const ctb_view* mask, int64_t groups,
+                             double coef, double z_coef, const ctb_view* loss, const ctb_view* counts,
+                             const ctb_view* probs, const ctb_view* grad, int32_t* d_status, void* scratch,
+                             size_t scratch_bytes, ctb_stream stream);
 
 /* ---- synthetic inputs ---- */
 
