@@ -5,6 +5,8 @@
 #include <algorithm>
 #include <cmath>
 
+#include <cuda_fp16.h>
+
 #include "linear_loss.cuh"
 
 namespace ctb {
@@ -73,17 +75,17 @@ __global__ void __launch_bounds__(kOrderThreads) linear_order(LinearArgs a) {
 
 // Rows as the products want them: contiguous, 16-byte aligned, zero up to the pitch. ORDERED: hidden's rows that
 // count, and zeros up to a multiple of 64 rows (they are a product's inner dimension too).
-template <class From, class To, bool ORDERED>
+template <class T, bool ORDERED>
 __global__ void __launch_bounds__(256) linear_pack(LinearArgs a, Matrix2 from, Matrix2 to, int64_t rows, int64_t cols) {
     dependent_wait();
     const int64_t n = ORDERED && a.order ? a.facts->count : rows;
     const int64_t upto = ORDERED ? min(rows, (n + 63) / 64 * 64) : rows;
     for (int64_t i = blockIdx.x; i < upto; i += gridDim.x) {
-        To* const out = static_cast<To*>(to.ptr) + i * to.row;
+        T* const out = static_cast<T*>(to.ptr) + i * to.row;
         const int64_t r = ORDERED && a.order && i < n ? a.order[i] : i;
-        const From* const in = static_cast<const From*>(from.ptr) + (ORDERED ? row_offset(a.v, kLnHidden, r) : r * from.row);
+        const T* const in = static_cast<const T*>(from.ptr) + (ORDERED ? row_offset(a.v, kLnHidden, r) : r * from.row);
         for (int64_t j = threadIdx.x; j < to.row; j += 256)
-            out[j] = i < n && j < cols ? from_float<To>(to_float(in[j * from.col])) : from_float<To>(0.0f);
+            out[j] = i < n && j < cols ? in[j * from.col] : from_float<T>(0.0f);
     }
     allow_dependents();
 }
@@ -184,6 +186,69 @@ __global__ void __launch_bounds__(512) linear_rows_f32(LinearArgs a, int64_t fir
     allow_dependents();
 }
 
+// bfloat16: a CTA a row. The pieces' maxima and sums give the row's; then 2^15 exp((z - m_piece) / T) of every element
+// becomes G = that times the row's and the piece's factors, rounded once to bfloat16 in its place. The target's entry is
+// worked out from its own logit. Rows behind the last one, up to a stage of the products, become zeros.
+// Bound by reading and writing 2 bytes an element.
+constexpr int kRowThreads = 512;
+__global__ void __launch_bounds__(kRowThreads) linear_rows_tc(LinearArgs a, int64_t first, int grad) {
+    dependent_wait();
+    const int64_t limit = min(a.block, a.v.rows - first);
+    const int64_t n = a.order ? linear_block_rows(a, first) : limit;
+    const int64_t upto = grad ? min(limit, (n + 63) / 64 * 64) : n;
+    const int64_t packs = a.held_pitch / 8;
+    for (int64_t b = blockIdx.x; b < upto; b += gridDim.x) {
+        uint4* const held = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + b * a.held_pitch);
+        if (b >= n) {
+            for (int64_t j = threadIdx.x; j < packs; j += kRowThreads) held[j] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
+        const float2* const stats = a.stats + b * a.tiles;
+        float m = -INFINITY, s = 0.0f;
+        for (int64_t j = threadIdx.x; j < a.tiles; j += kRowThreads) {
+            const float2 o = stats[j];
+            join_sums(m, s, o.x, o.y, a.c2);
+        }
+        join_block<kRowThreads>(m, s, a.c2);
+        const float zt = a.target_z[b];  // of a target outside: not looked at
+        const RowResult o = row_result(a, first + b, m, s, zt);
+        if (threadIdx.x == 0) put_row_result(a, o);
+        if (!grad) continue;
+        const double up = 1.0 + 2.0 * a.z_coef * o.lse;
+        // 2^-15 belongs to the held exponentials
+        const float c = o.bad ? NAN : static_cast<float>(o.w * up / static_cast<double>(s) * 0x1p-15);
+        const double logp = (static_cast<double>(zt) - m) * a.inv_temp - log(static_cast<double>(s));
+        const float at_target = static_cast<float>(o.w * (expm1(logp) + 2.0 * a.z_coef * o.lse * exp(logp)));
+        const int64_t t_pack = o.bad ? -1 : o.target / 8;
+#pragma unroll 4
+        for (int64_t j = threadIdx.x; j < packs; j += kRowThreads) {
+            uint4 h = held[j];
+            const float pm = stats[j / (kLinearPiece / 8)].x;
+            const float f = pm == -INFINITY ? 0.0f : c * exp2_approx((pm - m) * a.c2);
+            uint32_t* const u = reinterpret_cast<uint32_t*>(&h);
+            float g[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float2 e = __half22float2(*reinterpret_cast<const __half2*>(u + q));
+                g[2 * q] = e.x * f;
+                g[2 * q + 1] = e.y * f;
+            }
+            if (j == t_pack) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q == static_cast<int>(o.target & 7)) g[q] = at_target;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(g[2 * q], g[2 * q + 1]);
+                u[q] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+            held[j] = h;
+        }
+    }
+    allow_dependents();
+}
+
 // grad_hidden's rows of a block: the splits of dH = G W added in their order, times the factor; zeros where rows do
 // not count (with the last block).
 template <class T> __global__ void __launch_bounds__(256) linear_join(LinearArgs a, int64_t first, int64_t upto) {
@@ -248,30 +313,49 @@ struct LinearPlan {
     LinearArgs a{};
     bool grad = false, weighted = false, pack_h = false, pack_w = false;
     int64_t h_row = -1;      // hidden's row stride, where its leading dims are one
-    int work = CTB_FLOAT32;  // the products' operand type
+    int work = CTB_FLOAT32;  // the products' operand type, hidden's
     int64_t blocks = 0;
     size_t bytes = 0;
     size_t facts, order, weights, target_z, stats, held, partial, acc, h, w;
 };
 
+// dH has few tiles and a long sum over the vocabulary: it is split where that fills the GPU's last round of tiles
+// better than writing and reading the splits' float32 sums costs.
+int splits_of(bool tc, int64_t rows, int64_t dim, int64_t vocab) {
+    const int64_t tile = tc ? 256 : 128, units = tc ? sm_count() / 2 : sm_count() * 2;
+    const int64_t tiles = (rows + tile - 1) / tile * ((dim + tile - 1) / tile);
+    // seconds: a unit's rate, and 6 TB/s for the sums
+    const double whole = 2.0 * tile * tile * vocab / (tc ? 2 * 10e12 : 0.2e12);
+    const int64_t most = std::min<int64_t>(64, (vocab + 511) / 512);
+    int64_t best = 1;
+    double least = 1e300;
+    for (int64_t s = 1; s <= most; ++s) {
+        const double cost = static_cast<double>((tiles * s + units - 1) / units) * whole / s + 8.0 * s * rows * dim / 6e12;
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return static_cast<int>(best);
+}
+
 // The sizes of a call's pieces. Everything here follows from shapes, strides and alignment alone.
 void lay_out(LinearPlan& p) {
     LinearArgs& a = p.a;
     const int64_t rows = a.v.rows, dim = a.v.cols, vocab = a.vocab;
-    p.work = CTB_FLOAT32;
+    p.work = a.v.dtype[kLnHidden];
+    const bool tc = p.work == CTB_BFLOAT16;
     const int64_t size = static_cast<int64_t>(dtype_size(p.work)), pack = 16 / size;
     const int64_t pitch = round_up(dim, pack);
     a.held_pitch = round_up(vocab, pack);
-    a.tiles = (vocab + 255) / 256;
+    a.tiles = (vocab + kLinearPiece - 1) / kLinearPiece;
     a.block = std::max<int64_t>(256, kHeldBytes / (a.held_pitch * size) / 256 * 256);
     a.block = std::min(a.block, rows);
     p.blocks = (rows + a.block - 1) / a.block;
     p.pack_h = p.weighted || p.h_row < 0 ||
                !in_place(a.v.ptr[kLnHidden], p.h_row, a.v.inner[kLnHidden], rows, dim, a.v.dtype[kLnHidden], p.work);
     p.pack_w = !in_place(a.weight.ptr, a.weight.row, a.weight.col, vocab, dim, a.weight.dtype, p.work);
-    // dH has few tiles of 128 x 128 and a long sum: it is split until the GPU is full
-    const int64_t tiles = ((a.block + 127) / 128) * ((dim + 127) / 128);
-    a.splits = static_cast<int>(std::min<int64_t>({16, std::max<int64_t>(1, 296 / tiles), (vocab + 511) / 512}));
+    a.splits = splits_of(tc, a.block, dim, vocab);
     a.part_pitch = pitch;
     a.acc_pitch = pitch;
     Layout l;
@@ -279,15 +363,15 @@ void lay_out(LinearPlan& p) {
     p.order = l.add(p.weighted ? rows : 0, 4);
     p.weights = l.add(rows, 8);
     p.target_z = l.add(a.block, 4);
-    p.stats = l.add(0, 8);
+    p.stats = l.add(tc ? a.block * a.tiles : 0, 8);
     p.held = l.add(a.block * a.held_pitch, size);
     p.partial = l.add(p.grad ? a.splits * a.block * a.part_pitch : 0, 4);
     p.acc = l.add(p.grad && p.blocks > 1 ? vocab * a.acc_pitch : 0, 4);
     p.h = l.add(p.pack_h ? rows * pitch : 0, size);
     p.w = l.add(p.pack_w ? vocab * pitch : 0, size);
     p.bytes = l.bytes;
-    a.h.row = p.pack_h ? pitch : p.h_row;
-    a.w.row = p.pack_w ? pitch : a.weight.row;
+    a.h.row = p.pack_h || rows == 1 ? pitch : p.h_row;  // a single row's stride may be anything
+    a.w.row = p.pack_w || vocab == 1 ? pitch : a.weight.row;
     a.h.col = a.w.col = 1;
     a.h.dtype = a.w.dtype = p.work;
 }
@@ -307,23 +391,18 @@ void place(LinearPlan& p, void* scratch) {
     a.w.ptr = p.pack_w ? static_cast<void*>(s + p.w) : a.weight.ptr;
 }
 
-template <class From, class To, bool ORDERED>
-void launch_pack(const LinearArgs& a, const Matrix2& from, const Matrix2& to, int64_t rows, int64_t cols, cudaStream_t st) {
-    launch_dependent(linear_pack<From, To, ORDERED>, grid_for(rows, 8), 256, 0, st, a, from, to, rows, cols);
-    count_launch();
-}
-
 template <bool ORDERED>
 int run_pack(const LinearPlan& p, const Matrix2& from, const Matrix2& to, int64_t rows, cudaStream_t st) {
-    const LinearArgs& a = p.a;
-    if (from.dtype == CTB_FLOAT32) launch_pack<float, float, ORDERED>(a, from, to, rows, a.v.cols, st);
-    else launch_pack<__nv_bfloat16, float, ORDERED>(a, from, to, rows, a.v.cols, st);
+    auto kernel = p.work == CTB_FLOAT32 ? linear_pack<float, ORDERED> : linear_pack<__nv_bfloat16, ORDERED>;
+    launch_dependent(kernel, grid_for(rows, 8), 256, 0, st, p.a, from, to, rows, p.a.v.cols);
+    count_launch();
     return check_launch("linear loss: packing");
 }
 
 int linear_run(const LinearPlan& p, const ctb_view* loss, cudaStream_t st) {
     const LinearArgs& a = p.a;
     const int64_t rows = a.v.rows;
+    const bool tc = p.work == CTB_BFLOAT16;
     if (rows && p.weighted) {
         launch_dependent(linear_order, 1, kOrderThreads, 0, st, a);
         count_launch();
@@ -333,18 +412,19 @@ int linear_run(const LinearPlan& p, const ctb_view* loss, cudaStream_t st) {
     if (p.pack_w) CTB_CHECK(run_pack<false>(p, a.weight, a.w, a.vocab, st));
     for (int64_t first = 0; first < rows; first += a.block) {
         const int64_t n = std::min(a.block, rows - first);
-        CTB_CHECK(linear_logits_f32(a, first, n, st));
-        launch_dependent(linear_rows_f32, grid_for(n, 4), 512, 0, st, a, first, static_cast<int>(p.grad));
+        CTB_CHECK(tc ? linear_logits_tc(a, first, n, p.grad, st) : linear_logits_f32(a, first, n, st));
+        launch_dependent(tc ? linear_rows_tc : linear_rows_f32, grid_for(n, 4), kRowThreads, 0, st, a, first, static_cast<int>(p.grad));
         count_launch();
         CTB_CHECK(check_launch("linear loss: rows"));
         if (!p.grad) continue;
-        CTB_CHECK(linear_grad_hidden_f32(a, first, n, st));
+        CTB_CHECK((tc ? linear_grad_hidden_tc : linear_grad_hidden_f32)(a, first, n, st));
         auto join = a.v.dtype[kLnGrad] == CTB_FLOAT32 ? linear_join<float> : linear_join<__nv_bfloat16>;
         launch_dependent(join, grid_for(n, 8), 256, 0, st, a, first, first + n);
         count_launch();
         CTB_CHECK(check_launch("linear loss: join"));
-        CTB_CHECK(linear_grad_weight_f32(a, first, n, first + n == rows, st));
+        CTB_CHECK((tc ? linear_grad_weight_tc : linear_grad_weight_f32)(a, first, n, first + n == rows, st));
     }
+    // without rows the weight's gradient is 0: the float32 product over no rows writes that, whatever the type
     if (rows == 0 && p.grad) CTB_CHECK(linear_grad_weight_f32(a, 0, 0, true, st));
     if (loss) {
         launch_dependent(linear_total, 1, 1024, 0, st, static_cast<const double*>(a.weighted), rows, static_cast<float*>(loss->data));

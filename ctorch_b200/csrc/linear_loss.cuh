@@ -37,10 +37,10 @@ struct LinearArgs {
     int32_t* order;    // [rows] the rows that count in their order, then the others
     double* weighted;  // [rows] w_r row_loss_r, by row
     float* target_z;   // [block] z_rt
-    float2* stats;     // [block][tiles] (maximum, sum of exponentials) of a tile's columns
-    void* held;        // [block][held_pitch] logits or exponentials of a block, then G
+    float2* stats;     // [block][tiles] bfloat16: (maximum, sum of exponentials) of every 128 columns
+    void* held;        // [block][held_pitch] float32 logits or 16-bit exponentials of a block, then G
     int64_t held_pitch;
-    int64_t tiles;     // pieces of the vocabulary
+    int64_t tiles;     // pieces of 128 columns
     float* partial;    // [splits][block][part_pitch]
     int64_t part_pitch;
     float* acc;        // [V][acc_pitch] dW over the blocks so far, where there are several
@@ -69,5 +69,11 @@ __device__ __forceinline__ double linear_factor(const LinearArgs& a) {
 int linear_logits_f32(const LinearArgs& a, int64_t first, int64_t rows, cudaStream_t st);             // linear_loss_f32.cu
 int linear_grad_hidden_f32(const LinearArgs& a, int64_t first, int64_t rows, cudaStream_t st);        // linear_loss_f32.cu
 int linear_grad_weight_f32(const LinearArgs& a, int64_t first, int64_t rows, bool last, cudaStream_t st);  // linear_loss_f32.cu
+
+int linear_logits_tc(const LinearArgs& a, int64_t first, int64_t rows, bool hold, cudaStream_t st);      // linear_loss_tc.cu
+int linear_grad_hidden_tc(const LinearArgs& a, int64_t first, int64_t rows, cudaStream_t st);         // linear_loss_tc.cu
+int linear_grad_weight_tc(const LinearArgs& a, int64_t first, int64_t rows, bool last, cudaStream_t st);  // linear_loss_tc.cu
+
+constexpr int kLinearPiece = 128;  // columns of logits that share a maximum in bfloat16's held exponentials
 
 }  // namespace ctb

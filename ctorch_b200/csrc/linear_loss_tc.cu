@@ -1,0 +1,406 @@
+// linear_loss_tc.cu — the three products of the projection with its cross entropy in bfloat16, on the tensor cores.
+//
+// One kernel for all three: pairs of CTAs, one pair per two SMs, walk over 256 x 256 tiles. In each CTA one warp brings
+// stages of 64 of the inner dimension (32 KiB a CTA) into a ring of shared memory, one thread of the pair issues the
+// products, and eight warps take finished tiles out of tensor memory (two tiles' worth, so the next tile's products run
+// meanwhile), each 32 rows by 128 columns, and do what the product is for:
+//   z = H W^T      (maximum, sum of exponentials) of every 128 columns of a row, the target's z, and for the gradients
+//                  exp(z - maximum) in 16 bits
+//   dH = G W       float32 sums, split along the vocabulary where there are few tiles
+//   dW = G^T H     rounded once, or added up in float32 over the blocks of rows
+// H and G have the inner dimension of z = H W^T and dH = G W contiguous; the other operands their outer one, which the
+// tensor cores read as it lies.
+#include <cuda_fp16.h>
+
+#include "linear_loss.cuh"
+#include "tensor_core.cuh"
+
+namespace ctb {
+
+namespace {
+
+constexpr int kTile = 256, kHalf = 128, kK = 64, kStages = 6;
+constexpr int kStageBytes = 2 * kHalf * kK * 2;  // of one CTA: its halves of both operands
+constexpr int kEpilogueWarps = 8, kThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kGroup = 8;  // tiles of rows walked together, so that both operands are met again in L2
+
+enum Product : int { kLogits = 0, kLogitsOnly = 1, kGradHidden = 2, kGradWeight = 3 };
+
+struct ProductArgs {
+    int64_t m, n, k;  // of the block at most
+    int64_t first;    // the block's first row
+    int last;         // the last block
+};
+
+struct Bars {
+    uint64_t full[kStages], empty[kStages], done[2], free[2];
+    uint32_t tmem;
+};
+
+struct Work {
+    int64_t m, n;      // tile
+    int64_t kb0, kbs;  // stages of the inner dimension
+    int64_t split;
+};
+
+template <int P> struct Schedule {
+    int64_t tm, tn, kblocks, splits, total;
+    __device__ Schedule(const LinearArgs& a, const ProductArgs& p, int64_t rows) {
+        const int64_t m = P == kGradWeight ? p.m : rows, k = P == kGradWeight ? rows : p.k;
+        tm = (m + kTile - 1) / kTile;
+        tn = (p.n + kTile - 1) / kTile;
+        kblocks = (k + kK - 1) / kK;
+        splits = P == kGradHidden ? a.splits : 1;
+        total = tm * tn * splits;
+    }
+    // Groups of kGroup tiles of m, the columns of tiles after one another within a group, splits last.
+    __device__ Work at(int64_t w) const {
+        Work o;
+        o.split = w / (tm * tn);
+        w -= o.split * tm * tn;
+        const int64_t group = w / (kGroup * tn), m0 = group * kGroup, size = min(static_cast<int64_t>(kGroup), tm - m0);
+        w -= group * kGroup * tn;
+        o.n = w / size;
+        o.m = m0 + w % size;
+        const int64_t each = (kblocks + splits - 1) / splits;
+        o.kb0 = min(kblocks, o.split * each);
+        o.kbs = min(kblocks, o.kb0 + each) - o.kb0;
+        return o;
+    }
+};
+
+__device__ __forceinline__ float exp2_approx(float t) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+    return y;
+}
+
+// Two numbers in one word of 16-bit floats, the first one low.
+__device__ __forceinline__ uint32_t two_halves(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t two_bf16(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+
+// 128 columns of a row of logits: their maximum and the sum of exp((z - max) / T), the target's z, and with HOLD
+// 2^15 exp((z - max) / T) in 16 bits: 11 bits of precision down to 2^-29 of the largest, nothing below 2^-40.
+template <bool HOLD>
+__device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf], int64_t i, int64_t col, int64_t target, bool live) {
+    const int64_t left = a.vocab - col;
+    if (left < kHalf) {
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+            if (j >= left) z[j] = -INFINITY;
+    }
+    const int64_t t = target - col;
+    const bool here = live && t >= 0 && t < kHalf && t < left;
+    if (__any_sync(0xffffffffu, here)) {
+        float zt = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+            if (j == t) zt = z[j];
+        if (here) a.target_z[i] = zt;
+    }
+    float m = z[0];
+#pragma unroll
+    for (int j = 1; j < kHalf; ++j) m = fmaxf(m, z[j]);
+    const float at = m == -INFINITY ? 0.0f : m;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kHalf; ++j) {
+        z[j] = exp2_approx(fmaf(z[j] - at, a.c2, 15.0f));
+        s[j & 3] += z[j];
+    }
+    if (!live) return;
+    a.stats[i * a.tiles + col / kHalf] = make_float2(m, ((s[0] + s[1]) + (s[2] + s[3])) * 3.0517578125e-05f);
+    if (!HOLD) return;
+    uint4* const out = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + i * a.held_pitch + col);
+#pragma unroll
+    for (int q = 0; q < kHalf / 8; ++q)
+        if (q * 8 < left)  // the pitch is whole vectors
+            out[q] = make_uint4(two_halves(z[8 * q], z[8 * q + 1]), two_halves(z[8 * q + 2], z[8 * q + 3]),
+                                two_halves(z[8 * q + 4], z[8 * q + 5]), two_halves(z[8 * q + 6], z[8 * q + 7]));
+}
+
+constexpr int kChunk = 32;  // columns of a gradient that a thread has in hand at a time
+
+__device__ __forceinline__ void grad_hidden_row(const LinearArgs& a, const float (&x)[kChunk], int64_t i, int64_t col, int64_t cols,
+                                                int64_t split) {
+    float* const out = a.partial + (split * a.block + i) * a.part_pitch + col;
+#pragma unroll
+    for (int q = 0; q < kChunk / 4; ++q)
+        if (col + q * 4 < cols) *reinterpret_cast<float4*>(out + q * 4) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+}
+
+__device__ __forceinline__ void grad_weight_row(const LinearArgs& a, const ProductArgs& p, float (&x)[kChunk], int64_t v, int64_t col,
+                                                int64_t cols, float factor) {
+    if (a.acc) {
+        float* const acc = a.acc + v * a.acc_pitch + col;
+#pragma unroll
+        for (int q = 0; q < kChunk / 4; ++q) {
+            if (col + q * 4 >= cols) continue;
+            float4* const to = reinterpret_cast<float4*>(acc + q * 4);
+            if (p.first > 0) {
+                const float4 y = *to;
+                x[4 * q] += y.x;
+                x[4 * q + 1] += y.y;
+                x[4 * q + 2] += y.z;
+                x[4 * q + 3] += y.w;
+            }
+            if (!p.last) *to = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+        }
+        if (!p.last) return;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) x[j] *= factor;
+    __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(a.grad_weight.ptr) + v * a.grad_weight.row + col * a.grad_weight.col;
+    if (a.grad_weight.col == 1 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && col + kChunk <= cols) {
+#pragma unroll
+        for (int q = 0; q < kChunk / 8; ++q)
+            reinterpret_cast<uint4*>(out)[q] = make_uint4(two_bf16(x[8 * q], x[8 * q + 1]), two_bf16(x[8 * q + 2], x[8 * q + 3]),
+                                                          two_bf16(x[8 * q + 4], x[8 * q + 5]), two_bf16(x[8 * q + 6], x[8 * q + 7]));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j)
+        if (col + j < cols) out[j * a.grad_weight.col] = __float2bfloat16_rn(x[j]);
+}
+
+template <int P>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    linear_product_tc(const __grid_constant__ LinearArgs a, const __grid_constant__ ProductArgs p,
+                      const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+    extern __shared__ unsigned char raw[];
+    __shared__ Bars bars;
+    unsigned char* const smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    constexpr bool kAOuter = P == kGradWeight, kBOuter = P == kGradHidden || P == kGradWeight;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&bars.full[s], 1);
+            mbar_init(&bars.empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bars.done[s], 1);
+            mbar_init(&bars.free[s], 2 * kEpilogueWarps);
+        }
+        mbar_fence_init();
+    }
+    if (warp == kEpilogueWarps) tmem_alloc_pair(&bars.tmem, 2 * kTile);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = bars.tmem;
+    dependent_wait();
+
+    const int64_t rows = a.order ? linear_block_rows(a, p.first) : (P == kGradWeight ? p.k : p.m);
+    const Schedule<P> plan(a, p, rows);
+    const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    bool ok = true;
+
+    if (warp == kEpilogueWarps) {
+        // brings this CTA's halves: 128 of the tile's rows of the left operand, 128 of its columns of the right one
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            for (int64_t w = pair; ok && w < plan.total; w += pairs) {
+                const Work o = plan.at(w);
+                const int64_t i0 = o.m * kTile + rank * kHalf, j0 = o.n * kTile + rank * kHalf;
+                for (int64_t kb = 0; kb < o.kbs; ++kb) {
+                    if (!mbar_wait(&bars.empty[stage], phase ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(&bars.full[stage], 2 * kStageBytes);
+                    const uint32_t bar = in_first_cta(&bars.full[stage]);
+                    const uint32_t sa = smem_addr(smem + stage * kStageBytes), sb = sa + kStageBytes / 2;
+                    const int k0 = static_cast<int>((o.kb0 + kb) * kK);
+                    if (kAOuter) {
+                        tensor_load_pair(sa, &map_a, static_cast<int>(i0), k0, bar);
+                        tensor_load_pair(sa + 8192, &map_a, static_cast<int>(i0) + 64, k0, bar);
+                    } else {
+                        const int64_t base = P == kLogits || P == kLogitsOnly ? p.first : 0;
+                        tensor_load_pair(sa, &map_a, k0, static_cast<int>(base + i0), bar);
+                    }
+                    if (kBOuter) {
+                        const int kb_row = k0 + static_cast<int>(P == kGradWeight ? p.first : 0);
+                        tensor_load_pair(sb, &map_b, static_cast<int>(j0), kb_row, bar);
+                        tensor_load_pair(sb + 8192, &map_b, static_cast<int>(j0) + 64, kb_row, bar);
+                    } else {
+                        tensor_load_pair(sb, &map_b, k0, static_cast<int>(j0), bar);
+                    }
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // no copy or arrival is on its way to this CTA once its last stages are given back (unused ones count as such)
+            for (int s = 0; ok && s < kStages; ++s) {
+                if (!mbar_wait(&bars.empty[stage], phase ^ 1u)) ok = false;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == kEpilogueWarps + 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t kInstruction = instruction_bf16(kTile, kTile, kAOuter, kBOuter);
+            constexpr uint32_t kAStep = kAOuter ? 2048 : 32, kBStep = kBOuter ? 2048 : 32;  // bytes of 16 of the inner dimension
+            uint32_t stage = 0, phase = 0;
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            for (int64_t w = pair; ok && w < plan.total; w += pairs) {
+                const Work o = plan.at(w);
+                if (o.kbs == 0) continue;
+                if (!mbar_wait(&bars.free[acc], acc_phase ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem + acc * kTile;
+                for (int64_t kb = 0; kb < o.kbs; ++kb) {
+                    if (!mbar_wait(&bars.full[stage], phase)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_addr(smem + stage * kStageBytes), sb = sa + kStageBytes / 2;
+#pragma unroll
+                    for (int k = 0; k < kK / 16; ++k)
+                        mma_pair(d, matrix_descriptor(sa + k * kAStep, 8192, 1024), matrix_descriptor(sb + k * kBStep, 8192, 1024),
+                                 kInstruction, kb > 0 || k > 0);
+                    mma_commit_pair(&bars.empty[stage]);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                mma_commit_pair(&bars.done[acc]);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+        }
+    } else {
+        const int quarter = warp & 3, half = warp >> 2;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        const float factor = P == kGradWeight ? static_cast<float>(linear_factor(a)) : 0.0f;
+        const int64_t m = P == kGradWeight ? p.m : rows;
+        for (int64_t w = pair; ok && w < plan.total; w += pairs) {
+            const Work o = plan.at(w);
+            const int64_t i = o.m * kTile + rank * kHalf + quarter * 32 + lane, col = o.n * kTile + half * kHalf;
+            int64_t target = -1;
+            if ((P == kLogits || P == kLogitsOnly) && i < m) {
+                const int64_t r = a.order ? a.order[p.first + i] : p.first + i;
+                target = index_at(a.v.ptr[kLnTarget], a.v.dtype[kLnTarget], row_offset(a.v, kLnTarget, r));
+            }
+            if (o.kbs != 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.done[acc], acc_phase));
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const uint32_t from = tmem + acc * kTile + half * kHalf + (static_cast<uint32_t>(quarter * 32) << 16);
+            // gives the sums back to the products once they are in registers
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(in_first_cta(&bars.free[acc]));
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            };
+            if constexpr (P == kLogits || P == kLogitsOnly) {
+                float z[kHalf];
+#pragma unroll
+                for (int c = 0; c < kHalf / 32; ++c) tmem_load32(z + c * 32, from + c * 32);
+                tmem_load_wait();
+                release();
+                if (col < p.n) logits_row<P == kLogits>(a, z, i, col, target, i < m);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < kHalf / kChunk; ++c) {
+                    float x[kChunk];
+                    if (o.kbs == 0) {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) x[j] = 0.0f;
+                    } else {
+                        tmem_load32(x, from + c * kChunk);
+                        tmem_load_wait();
+                    }
+                    if (c == kHalf / kChunk - 1 && o.kbs != 0) release();
+                    if (i >= m || col + c * kChunk >= p.n) continue;
+                    if (P == kGradHidden) grad_hidden_row(a, x, i, col + c * kChunk, p.n, o.split);
+                    else grad_weight_row(a, p, x, i, col + c * kChunk, p.n, factor);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (!ok) {
+        // a wait ran out: count it, and leave the copies and products in flight time to land before the memory goes
+        note_timeout(a.timeouts);
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    __syncwarp();
+    allow_dependents();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == kEpilogueWarps) {
+        tc_fence_after();
+        tmem_free_pair(tmem, 2 * kTile);
+    }
+}
+
+template <int P>
+int launch(const LinearArgs& a, const ProductArgs& p, const CUtensorMap& map_a, const CUtensorMap& map_b, cudaStream_t st) {
+    auto kernel = linear_product_tc<P>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(CTB_ERR_CUDA, std::string("linear loss: ") + cudaGetErrorString(e));
+    }
+    launch_dependent(kernel, static_cast<unsigned>(sm_count() / 2 * 2), kThreads, kSmem, st, a, p, map_a, map_b);
+    count_launch();
+    return check_launch("linear loss: product");
+}
+
+int no_map() { return fail(CTB_ERR_CUDA, "linear loss: the driver refused a tensor map"); }
+
+}  // namespace
+
+int linear_logits_tc(const LinearArgs& a, int64_t first, int64_t rows, bool hold, cudaStream_t st) {
+    CUtensorMap h, w;
+    if (!encode_matrix_map(&h, a.h.ptr, a.v.rows, a.v.cols, a.h.row, kHalf) ||
+        !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kHalf))
+        return no_map();
+    const ProductArgs p{rows, a.vocab, a.v.cols, first, 0};
+    return hold ? launch<kLogits>(a, p, h, w, st) : launch<kLogitsOnly>(a, p, h, w, st);
+}
+
+int linear_grad_hidden_tc(const LinearArgs& a, int64_t first, int64_t rows, cudaStream_t st) {
+    CUtensorMap g, w;
+    if (!encode_matrix_map(&g, a.held, rows, a.vocab, a.held_pitch, kHalf) ||
+        !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kK))
+        return no_map();
+    return launch<kGradHidden>(a, ProductArgs{rows, a.v.cols, a.vocab, first, 0}, g, w, st);
+}
+
+int linear_grad_weight_tc(const LinearArgs& a, int64_t first, int64_t rows, bool last, cudaStream_t st) {
+    CUtensorMap g, h;
+    if (!encode_matrix_map(&g, a.held, rows, a.vocab, a.held_pitch, kK) ||
+        !encode_matrix_map(&h, a.h.ptr, a.v.rows, a.v.cols, a.h.row, kK))
+        return no_map();
+    return launch<kGradWeight>(a, ProductArgs{a.vocab, a.v.cols, rows, first, last ? 1 : 0}, g, h, st);
+}
+
+}  // namespace ctb

@@ -63,8 +63,9 @@ def norm_grad(up, s, weight, eps, passed):
 # ------------------------------------------------------------------------------------- head
 
 
-def head(hidden, weight, targets, weights, z_coef=0.0, temperature=1.0, grad=True):
-    """A dict of name: (value, bound). Rows whose weight is 0 may hold anything."""
+def head(hidden, weight, targets, weights, z_coef=0.0, temperature=1.0, grad=True, alike=1):
+    """A dict of name: (value, bound). Rows whose weight is 0 may hold anything. alike: how many rows are the same hidden
+    state; their logits' gradients round alike, so in grad_weight their errors add up as such, not as independent ones."""
     dim, vocab = hidden.shape[-1], weight.shape[0]
     rows = targets.numel()
     h, w, t = d(hidden).reshape(rows, dim), d(weight), targets.reshape(rows)
@@ -104,13 +105,14 @@ def head(hidden, weight, targets, weights, z_coef=0.0, temperature=1.0, grad=Tru
             least * w.abs().sum(0)
         gw = g.T @ h
         sums = (rows / 16 + 1) * 4 * U if half_g else (rows + 1) * U
-        bw = half(hidden.dtype) * gw.abs() + spread * torch.sqrt((g * g).T @ (h * h)) + \
+        bw = half(hidden.dtype) * gw.abs() + math.sqrt(alike) * spread * torch.sqrt((g * g).T @ (h * h)) + \
             ((rel[:, None] * mag).T @ h.abs() + sums * (mag.T @ h.abs()) + (least * h.abs()).sum(0))
         out["grad_hidden"] = (gh.view(hidden.shape), bh.view(hidden.shape))
         out["grad_weight"] = (gw, bw)
         # the norm of both if every logit's gradient were its row's weight at the target
         out["unit_grad_hidden"] = float(((hot @ w) * torch.where(on, share, 0.0)[:, None]).norm()) / temperature
         out["unit_grad_weight"] = float((h * torch.where(on, share, 0.0)[:, None]).norm()) / temperature
+    out["alike"] = alike
     for k in ("row_loss", "lse"):
         out[k] = tuple(v.view(targets.shape) for v in out[k])
     return out
