@@ -75,17 +75,28 @@ __global__ void __launch_bounds__(kOrderThreads) linear_order(LinearArgs a) {
 
 // Rows as the products want them: contiguous, 16-byte aligned, zero up to the pitch. ORDERED: hidden's rows that
 // count, and zeros up to a multiple of 64 rows (they are a product's inner dimension too).
+constexpr int kPackThreads = 128;
 template <class T, bool ORDERED>
-__global__ void __launch_bounds__(256) linear_pack(LinearArgs a, Matrix2 from, Matrix2 to, int64_t rows, int64_t cols) {
+__global__ void __launch_bounds__(kPackThreads) linear_pack(LinearArgs a, Matrix2 from, Matrix2 to, int64_t rows, int64_t cols) {
     dependent_wait();
     const int64_t n = ORDERED && a.order ? a.facts->count : rows;
     const int64_t upto = ORDERED ? min(rows, (n + 63) / 64 * 64) : rows;
+    constexpr int kPack = 16 / sizeof(T);
     for (int64_t i = blockIdx.x; i < upto; i += gridDim.x) {
         T* const out = static_cast<T*>(to.ptr) + i * to.row;
         const int64_t r = ORDERED && a.order && i < n ? a.order[i] : i;
         const T* const in = static_cast<const T*>(from.ptr) + (ORDERED ? row_offset(a.v, kLnHidden, r) : r * from.row);
-        for (int64_t j = threadIdx.x; j < to.row; j += 256)
-            out[j] = i < n && j < cols ? in[j * from.col] : from_float<T>(0.0f);
+        const bool whole = i < n && from.col == 1 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
+        for (int64_t j = static_cast<int64_t>(threadIdx.x) * kPack; j < to.row; j += kPackThreads * kPack) {
+            if (whole && j + kPack <= cols) {
+                *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(in + j);
+                continue;
+            }
+            Pack<T, kPack> v;
+#pragma unroll
+            for (int q = 0; q < kPack; ++q) v.v[q] = i < n && j + q < cols ? in[(j + q) * from.col] : from_float<T>(0.0f);
+            store_pack<T, kPack>(out + j, v);
+        }
     }
     allow_dependents();
 }
@@ -186,86 +197,139 @@ __global__ void __launch_bounds__(512) linear_rows_f32(LinearArgs a, int64_t fir
     allow_dependents();
 }
 
-// bfloat16: a CTA a row. The pieces' maxima and sums give the row's; then 2^15 exp((z - m_piece) / T) of every element
-// becomes G = that times the row's and the piece's factors, rounded once to bfloat16 in its place. The target's entry is
-// worked out from its own logit. Rows behind the last one, up to a stage of the products, become zeros.
-// Bound by reading and writing 2 bytes an element.
-constexpr int kRowThreads = 512;
-__global__ void __launch_bounds__(kRowThreads) linear_rows_tc(LinearArgs a, int64_t first, int grad) {
+// bfloat16: a warp a row joins the pieces' maxima and sums and works out the row's results and what its G needs:
+//     G_rv = c 2^((m_piece - m) log2(e) / T) held_rv,      at the target: worked out from its own logit
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) linear_rows_tc(LinearArgs a, int64_t first) {
     dependent_wait();
-    const int64_t limit = min(a.block, a.v.rows - first);
-    const int64_t n = a.order ? linear_block_rows(a, first) : limit;
-    const int64_t upto = grad ? min(limit, (n + 63) / 64 * 64) : n;
-    const int64_t packs = a.held_pitch / 8;
-    for (int64_t b = blockIdx.x; b < upto; b += gridDim.x) {
-        uint4* const held = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + b * a.held_pitch);
-        if (b >= n) {
-            for (int64_t j = threadIdx.x; j < packs; j += kRowThreads) held[j] = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-        }
+    allow_dependents();
+    const int64_t n = a.order ? linear_block_rows(a, first) : min(a.block, a.v.rows - first);
+    const int lane = threadIdx.x & 31;
+    for (int64_t b = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); b < n; b += gridDim.x * (kJoinThreads / 32)) {
         const float2* const stats = a.stats + b * a.tiles;
         float m = -INFINITY, s = 0.0f;
-        for (int64_t j = threadIdx.x; j < a.tiles; j += kRowThreads) {
+        for (int64_t j = lane; j < a.tiles; j += 32) {
             const float2 o = stats[j];
             join_sums(m, s, o.x, o.y, a.c2);
         }
-        join_block<kRowThreads>(m, s, a.c2);
+        for (int d = 16; d >= 1; d >>= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m, d), os = __shfl_xor_sync(0xffffffffu, s, d);
+            join_sums(m, s, om, os, a.c2);
+        }
+        if (lane != 0) continue;
+        if (m == INFINITY) s = NAN;
         const float zt = a.target_z[b];  // of a target outside: not looked at
         const RowResult o = row_result(a, first + b, m, s, zt);
-        if (threadIdx.x == 0) put_row_result(a, o);
-        if (!grad) continue;
-        const double up = 1.0 + 2.0 * a.z_coef * o.lse;
-        // 2^-15 belongs to the held exponentials
-        const float c = o.bad ? NAN : static_cast<float>(o.w * up / static_cast<double>(s) * 0x1p-15);
+        put_row_result(a, o);
         const double logp = (static_cast<double>(zt) - m) * a.inv_temp - log(static_cast<double>(s));
-        const float at_target = static_cast<float>(o.w * (expm1(logp) + 2.0 * a.z_coef * o.lse * exp(logp)));
-        const int64_t t_pack = o.bad ? -1 : o.target / 8;
-#pragma unroll 4
-        for (int64_t j = threadIdx.x; j < packs; j += kRowThreads) {
-            uint4 h = held[j];
-            const float pm = stats[j / (kLinearPiece / 8)].x;
-            const float f = pm == -INFINITY ? 0.0f : c * exp2_approx((pm - m) * a.c2);
-            uint32_t* const u = reinterpret_cast<uint32_t*>(&h);
+        LinearRowFactor f;
+        f.m = m;
+        // 2^-15 belongs to the held exponentials
+        f.c = o.bad ? NAN : static_cast<float>(o.w * (1.0 + 2.0 * a.z_coef * o.lse) / static_cast<double>(s) * 0x1p-15);
+        f.at_target = static_cast<float>(o.w * (expm1(logp) + 2.0 * a.z_coef * o.lse * exp(logp)));
+        f.target = o.bad ? -1 : static_cast<int32_t>(o.target);
+        a.factors[b] = f;
+    }
+}
+
+// Turns the held exponentials into G, rounded once to bfloat16, in their place; rows behind the last one, up to a stage of
+// the products, become zeros. A CTA takes spans of 8 KiB of a row, four vectors a thread on their way at a time. Bound by
+// reading and writing 2 bytes an element (B200, 3686 rows of 32768: see the table of cases).
+constexpr int kScaleThreads = 128, kScaleSpan = kScaleThreads * 4;  // vectors of 8
+__global__ void __launch_bounds__(kScaleThreads) linear_scale_tc(LinearArgs a, int64_t first) {
+    dependent_wait();
+    const int64_t limit = min(a.block, a.v.rows - first);
+    const int64_t n = a.order ? linear_block_rows(a, first) : limit;
+    const int64_t upto = min(limit, (n + 63) / 64 * 64);
+    const int64_t packs = a.held_pitch / 8, spans = (packs + kScaleSpan - 1) / kScaleSpan;
+    for (int64_t i = blockIdx.x; i < upto * spans; i += gridDim.x) {
+        const int64_t b = i / spans, p0 = (i - b * spans) * kScaleSpan + threadIdx.x;
+        uint4* const held = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + b * a.held_pitch);
+        const float2* const stats = a.stats + b * a.tiles;
+        uint4 h[4];
+        float pm[4];
+        const bool live = b < n;
+        LinearRowFactor f = {0.0f, 0.0f, 0.0f, -1};
+        if (live) {
+            f = a.factors[b];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t j = p0 + q * kScaleThreads;
+                if (j >= packs) continue;
+                h[q] = held[j];
+                pm[q] = j / (kLinearPiece / 8) < a.tiles ? stats[j / (kLinearPiece / 8)].x : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t j = p0 + q * kScaleThreads;
+            if (j >= packs) continue;
+            if (!live) {
+                held[j] = make_uint4(0u, 0u, 0u, 0u);
+                continue;
+            }
+            const float c = pm[q] == -INFINITY ? f.c * 0.0f : f.c * exp2_approx((pm[q] - f.m) * a.c2);
+            uint32_t* const u = reinterpret_cast<uint32_t*>(&h[q]);
             float g[8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float2 e = __half22float2(*reinterpret_cast<const __half2*>(u + q));
-                g[2 * q] = e.x * f;
-                g[2 * q + 1] = e.y * f;
+            for (int k = 0; k < 4; ++k) {
+                const float2 e = __half22float2(*reinterpret_cast<const __half2*>(u + k));
+                g[2 * k] = e.x * c;
+                g[2 * k + 1] = e.y * c;
             }
-            if (j == t_pack) {
+            if (f.target >= 0 && j == f.target / 8) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (q == static_cast<int>(o.target & 7)) g[q] = at_target;
+                for (int k = 0; k < 8; ++k)
+                    if (k == (f.target & 7)) g[k] = f.at_target;
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const __nv_bfloat162 y = __floats2bfloat162_rn(g[2 * q], g[2 * q + 1]);
-                u[q] = *reinterpret_cast<const uint32_t*>(&y);
+            for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(g[2 * k], g[2 * k + 1]);
+                u[k] = *reinterpret_cast<const uint32_t*>(&y);
             }
-            held[j] = h;
+            held[j] = h[q];
         }
     }
     allow_dependents();
 }
 
 // grad_hidden's rows of a block: the splits of dH = G W added in their order, times the factor; zeros where rows do
-// not count (with the last block).
-template <class T> __global__ void __launch_bounds__(256) linear_join(LinearArgs a, int64_t first, int64_t upto) {
+// not count (with the last block). A CTA takes 512 columns of a row, four a thread.
+constexpr int kSumThreads = 128;
+template <class T> __global__ void __launch_bounds__(kSumThreads) linear_join(LinearArgs a, int64_t first, int64_t upto) {
     dependent_wait();
     const int64_t n = a.order ? a.facts->count : a.v.rows;
     const double f = linear_factor(a);
-    T* const grad = static_cast<T*>(a.v.ptr[kLnGrad]);
-    const int64_t inner = a.v.inner[kLnGrad];
-    for (int64_t i = first + blockIdx.x; i < upto; i += gridDim.x) {
+    const int64_t inner = a.v.inner[kLnGrad], spans = (a.v.cols + kSumThreads * 4 - 1) / (kSumThreads * 4);
+    for (int64_t k = blockIdx.x; k < (upto - first) * spans; k += gridDim.x) {
+        const int64_t i = first + k / spans, j = (k % spans) * kSumThreads * 4 + threadIdx.x * 4;
+        if (j >= a.v.cols) continue;
         const int64_t r = a.order ? a.order[i] : i;
-        T* const out = grad + row_offset(a.v, kLnGrad, r);
-        const float* const p = a.partial + (i - first) * a.part_pitch;
-        for (int64_t j = threadIdx.x; j < a.v.cols; j += 256) {
-            float x = 0.0f;
-            if (i < n)
-                for (int s = 0; s < a.splits; ++s) x += p[s * a.block * a.part_pitch + j];
-            out[j * inner] = from_float<T>(static_cast<float>(f * static_cast<double>(x)));
+        T* const out = static_cast<T*>(a.v.ptr[kLnGrad]) + row_offset(a.v, kLnGrad, r) + j * inner;
+        const float* const p = a.partial + (i - first) * a.part_pitch + j;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (i < n) {
+#pragma unroll 4
+            for (int s = 0; s < a.splits; ++s) {
+                const float4 y = *reinterpret_cast<const float4*>(p + s * a.part_rows * a.part_pitch);
+                x[0] += y.x;
+                x[1] += y.y;
+                x[2] += y.z;
+                x[3] += y.w;
+            }
+        }
+        T y[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q] = from_float<T>(static_cast<float>(f * static_cast<double>(x[q])));
+        if (inner == 1 && j + 4 <= a.v.cols && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0) {
+            Pack<T, 4> v;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v.v[q] = y[q];
+            store_pack<T, 4>(out, v);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (j + q < a.v.cols) out[q * inner] = y[q];
         }
     }
     allow_dependents();
@@ -316,7 +380,7 @@ struct LinearPlan {
     int work = CTB_FLOAT32;  // the products' operand type, hidden's
     int64_t blocks = 0;
     size_t bytes = 0;
-    size_t facts, order, weights, target_z, stats, held, partial, acc, h, w;
+    size_t facts, order, weights, target_z, factors, stats, held, partial, acc, h, w;
 };
 
 // dH has few tiles and a long sum over the vocabulary: it is split where that fills the GPU's last round of tiles
@@ -347,7 +411,7 @@ void lay_out(LinearPlan& p) {
     const bool tc = p.work == CTB_BFLOAT16;
     const int64_t size = static_cast<int64_t>(dtype_size(p.work)), pack = 16 / size;
     const int64_t pitch = round_up(dim, pack);
-    a.held_pitch = round_up(vocab, pack);
+    a.held_pitch = round_up(vocab, 64);
     a.tiles = (vocab + kLinearPiece - 1) / kLinearPiece;
     a.block = std::max<int64_t>(256, kHeldBytes / (a.held_pitch * size) / 256 * 256);
     a.block = std::min(a.block, rows);
@@ -356,16 +420,18 @@ void lay_out(LinearPlan& p) {
                !in_place(a.v.ptr[kLnHidden], p.h_row, a.v.inner[kLnHidden], rows, dim, a.v.dtype[kLnHidden], p.work);
     p.pack_w = !in_place(a.weight.ptr, a.weight.row, a.weight.col, vocab, dim, a.weight.dtype, p.work);
     a.splits = splits_of(tc, a.block, dim, vocab);
-    a.part_pitch = pitch;
+    a.part_pitch = round_up(dim, 32);
+    a.part_rows = round_up(a.block, 256);
     a.acc_pitch = pitch;
     Layout l;
     p.facts = l.add(1, sizeof(LinearFacts));
     p.order = l.add(p.weighted ? rows : 0, 4);
     p.weights = l.add(rows, 8);
     p.target_z = l.add(a.block, 4);
+    p.factors = l.add(tc ? a.block : 0, sizeof(LinearRowFactor));
     p.stats = l.add(tc ? a.block * a.tiles : 0, 8);
     p.held = l.add(a.block * a.held_pitch, size);
-    p.partial = l.add(p.grad ? a.splits * a.block * a.part_pitch : 0, 4);
+    p.partial = l.add(p.grad ? a.splits * a.part_rows * a.part_pitch : 0, 4);
     p.acc = l.add(p.grad && p.blocks > 1 ? vocab * a.acc_pitch : 0, 4);
     p.h = l.add(p.pack_h ? rows * pitch : 0, size);
     p.w = l.add(p.pack_w ? vocab * pitch : 0, size);
@@ -384,6 +450,7 @@ void place(LinearPlan& p, void* scratch) {
     a.weighted = reinterpret_cast<double*>(s + p.weights);
     a.target_z = reinterpret_cast<float*>(s + p.target_z);
     a.stats = reinterpret_cast<float2*>(s + p.stats);
+    a.factors = reinterpret_cast<LinearRowFactor*>(s + p.factors);
     a.held = s + p.held;
     a.partial = reinterpret_cast<float*>(s + p.partial);
     a.acc = p.blocks > 1 ? reinterpret_cast<float*>(s + p.acc) : nullptr;
@@ -394,7 +461,7 @@ void place(LinearPlan& p, void* scratch) {
 template <bool ORDERED>
 int run_pack(const LinearPlan& p, const Matrix2& from, const Matrix2& to, int64_t rows, cudaStream_t st) {
     auto kernel = p.work == CTB_FLOAT32 ? linear_pack<float, ORDERED> : linear_pack<__nv_bfloat16, ORDERED>;
-    launch_dependent(kernel, grid_for(rows, 8), 256, 0, st, p.a, from, to, rows, p.a.v.cols);
+    launch_dependent(kernel, grid_for(rows, 16), kPackThreads, 0, st, p.a, from, to, rows, p.a.v.cols);
     count_launch();
     return check_launch("linear loss: packing");
 }
@@ -413,13 +480,19 @@ int linear_run(const LinearPlan& p, const ctb_view* loss, cudaStream_t st) {
     for (int64_t first = 0; first < rows; first += a.block) {
         const int64_t n = std::min(a.block, rows - first);
         CTB_CHECK(tc ? linear_logits_tc(a, first, n, p.grad, st) : linear_logits_f32(a, first, n, st));
-        launch_dependent(tc ? linear_rows_tc : linear_rows_f32, grid_for(n, 4), kRowThreads, 0, st, a, first, static_cast<int>(p.grad));
+        if (tc) launch_dependent(linear_rows_tc, grid_for((n + 7) / 8, 8), kJoinThreads, 0, st, a, first);
+        else launch_dependent(linear_rows_f32, grid_for(n, 4), 512, 0, st, a, first, static_cast<int>(p.grad));
         count_launch();
         CTB_CHECK(check_launch("linear loss: rows"));
         if (!p.grad) continue;
+        if (tc) {
+            launch_dependent(linear_scale_tc, grid_for(n * ((a.held_pitch / 8 + kScaleSpan - 1) / kScaleSpan), 16), kScaleThreads, 0, st, a, first);
+            count_launch();
+            CTB_CHECK(check_launch("linear loss: rows"));
+        }
         CTB_CHECK((tc ? linear_grad_hidden_tc : linear_grad_hidden_f32)(a, first, n, st));
         auto join = a.v.dtype[kLnGrad] == CTB_FLOAT32 ? linear_join<float> : linear_join<__nv_bfloat16>;
-        launch_dependent(join, grid_for(n, 8), 256, 0, st, a, first, first + n);
+        launch_dependent(join, grid_for(n * ((a.v.cols + 4 * kSumThreads - 1) / (4 * kSumThreads)), 16), kSumThreads, 0, st, a, first, first + n);
         count_launch();
         CTB_CHECK(check_launch("linear loss: join"));
         CTB_CHECK((tc ? linear_grad_weight_tc : linear_grad_weight_f32)(a, first, n, first + n == rows, st));

@@ -20,6 +20,11 @@ struct LinearFacts {
     float wmax;      // the largest |weight| among them; 1 without weights
 };
 
+struct LinearRowFactor {  // what turns a row's held exponentials into its G (bfloat16)
+    float m, c, at_target;
+    int32_t target;
+};
+
 struct Matrix2 {  // a matrix of a call's own, or an operand: element (i, j) at ptr[i * row + j * col]
     void* ptr;
     int64_t row, col;
@@ -41,8 +46,9 @@ struct LinearArgs {
     void* held;        // [block][held_pitch] float32 logits or 16-bit exponentials of a block, then G
     int64_t held_pitch;
     int64_t tiles;     // pieces of 128 columns
-    float* partial;    // [splits][block][part_pitch]
-    int64_t part_pitch;
+    LinearRowFactor* factors;  // [block]
+    float* partial;    // [splits][part_rows][part_pitch]
+    int64_t part_rows, part_pitch;
     float* acc;        // [V][acc_pitch] dW over the blocks so far, where there are several
     int64_t acc_pitch;
     Matrix2 h, w;      // what the products read: the operands, or packed copies

@@ -146,7 +146,7 @@ template <int P> __global__ void __launch_bounds__(kThreads, 2) linear_product_f
                 if (P == kLogits) {
                     static_cast<float*>(a.held)[row * a.held_pitch + col + h] = x;
                 } else if (P == kGradHidden) {
-                    a.partial[(split * a.block + row) * a.part_pitch + col + h] = x;
+                    a.partial[(split * a.part_rows + row) * a.part_pitch + col + h] = x;
                 } else {
                     if (a.acc && p.first > 0) x += a.acc[row * a.acc_pitch + col + h];
                     if (!p.last) {

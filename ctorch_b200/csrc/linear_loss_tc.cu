@@ -22,7 +22,8 @@ namespace {
 constexpr int kTile = 256, kHalf = 128, kK = 64, kStages = 6;
 constexpr int kStageBytes = 2 * kHalf * kK * 2;  // of one CTA: its halves of both operands
 constexpr int kEpilogueWarps = 8, kThreads = 32 * (kEpilogueWarps + 2);
-constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kBoxBytes = 32 * 128;  // of results on their way out, one a warp
+constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;
 constexpr int kGroup = 8;  // tiles of rows walked together, so that both operands are met again in L2
 
 enum Product : int { kLogits = 0, kLogitsOnly = 1, kGradHidden = 2, kGradWeight = 3 };
@@ -31,6 +32,7 @@ struct ProductArgs {
     int64_t m, n, k;  // of the block at most
     int64_t first;    // the block's first row
     int last;         // the last block
+    int boxes;        // dW leaves as boxes
 };
 
 struct Bars {
@@ -88,10 +90,36 @@ __device__ __forceinline__ uint32_t two_bf16(float x, float y) {
     return r;
 }
 
+// The tensor cores truncate a float32 sum at every step of 16 products, so what comes out is short by a share of itself that
+// grows with the steps. Measured on B200 for logits of 64 to 4096 columns, random and leaning ones: 1.5e-8 to 1.7e-8 a
+// step (a sum that grows evenly loses 2^-24 of 0.7 of half of itself a step at most). Given back on average: the
+// log-sum-exp of 4096 columns was 1.3e-6 off one way.
+constexpr double kTruncated = 1.6e-8;
+
+__device__ __forceinline__ float given_back(int64_t kblocks) { return static_cast<float>(1.0 + kTruncated * (kK / 16) * static_cast<double>(kblocks)); }
+
 // 128 columns of a row of logits: their maximum and the sum of exp((z - max) / T), the target's z, and with HOLD
 // 2^15 exp((z - max) / T) in 16 bits: 11 bits of precision down to 2^-29 of the largest, nothing below 2^-40.
+struct Out {  // where a warp's results leave through
+    const CUtensorMap* map;
+    uint32_t box;
+    int row;  // of its 32 rows, the first
+};
+
+// Gives the warp's box to the copy engine (every lane has written its row of it).
+__device__ __forceinline__ void send_box(const Out& o, int64_t col) {
+    proxy_fence();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tensor_store(o.map, static_cast<int>(col), o.row, o.box);
+}
+__device__ __forceinline__ void box_free() {
+    if ((threadIdx.x & 31) == 0) tensor_stores_read();
+    __syncwarp();
+}
+
 template <bool HOLD>
-__device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf], int64_t i, int64_t col, int64_t target, bool live) {
+__device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf], int64_t i, int64_t col, int64_t target, bool live, float back,
+                                           const Out& out) {
     const int64_t left = a.vocab - col;
     if (left < kHalf) {
 #pragma unroll
@@ -105,39 +133,59 @@ __device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf
 #pragma unroll
         for (int j = 0; j < kHalf; ++j)
             if (j == t) zt = z[j];
-        if (here) a.target_z[i] = zt;
+        if (here) a.target_z[i] = zt * back;
     }
     float m = z[0];
 #pragma unroll
     for (int j = 1; j < kHalf; ++j) m = fmaxf(m, z[j]);
-    const float at = m == -INFINITY ? 0.0f : m;
+    const float at = m == -INFINITY ? 0.0f : m, c2 = a.c2 * back;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < kHalf; ++j) {
-        z[j] = exp2_approx(fmaf(z[j] - at, a.c2, 15.0f));
+        z[j] = exp2_approx(fmaf(z[j] - at, c2, 15.0f));
         s[j & 3] += z[j];
     }
-    if (!live) return;
-    a.stats[i * a.tiles + col / kHalf] = make_float2(m, ((s[0] + s[1]) + (s[2] + s[3])) * 3.0517578125e-05f);
+    if (live) a.stats[i * a.tiles + col / kHalf] = make_float2(m * back, ((s[0] + s[1]) + (s[2] + s[3])) * 3.0517578125e-05f);
     if (!HOLD) return;
-    uint4* const out = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + i * a.held_pitch + col);
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int q = 0; q < kHalf / 8; ++q)
-        if (q * 8 < left)  // the pitch is whole vectors
-            out[q] = make_uint4(two_halves(z[8 * q], z[8 * q + 1]), two_halves(z[8 * q + 2], z[8 * q + 3]),
-                                two_halves(z[8 * q + 4], z[8 * q + 5]), two_halves(z[8 * q + 6], z[8 * q + 7]));
+    for (int h = 0; h < 2; ++h) {
+        if (h * 64 >= left) break;
+        box_free();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float* const e = z + h * 64 + q * 8;
+            store_shared16(swizzled_piece(out.box, lane, q), two_halves(e[0], e[1]), two_halves(e[2], e[3]), two_halves(e[4], e[5]),
+                           two_halves(e[6], e[7]));
+        }
+        send_box(out, col + h * 64);
+    }
 }
 
 constexpr int kChunk = 32;  // columns of a gradient that a thread has in hand at a time
 
-__device__ __forceinline__ void grad_hidden_row(const LinearArgs& a, const float (&x)[kChunk], int64_t i, int64_t col, int64_t cols,
-                                                int64_t split) {
-    float* const out = a.partial + (split * a.block + i) * a.part_pitch + col;
+__device__ __forceinline__ void grad_hidden_rows(const float (&x)[kChunk], int64_t col, const Out& out) {
+    box_free();
 #pragma unroll
-    for (int q = 0; q < kChunk / 4; ++q)
-        if (col + q * 4 < cols) *reinterpret_cast<float4*>(out + q * 4) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+    for (int q = 0; q < 8; ++q)
+        store_shared16(swizzled_piece(out.box, threadIdx.x & 31, q), __float_as_uint(x[4 * q]), __float_as_uint(x[4 * q + 1]),
+                       __float_as_uint(x[4 * q + 2]), __float_as_uint(x[4 * q + 3]));
+    send_box(out, col);
 }
 
+// 32 columns of dW into half of the warp's box, which leaves with every second piece.
+__device__ __forceinline__ void grad_weight_rows(const float (&x)[kChunk], int64_t col, float factor, int piece, const Out& out) {
+    if ((piece & 1) == 0) box_free();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float* const y = x + 8 * q;
+        store_shared16(swizzled_piece(out.box, threadIdx.x & 31, (piece & 1) * 4 + q), two_bf16(y[0] * factor, y[1] * factor),
+                       two_bf16(y[2] * factor, y[3] * factor), two_bf16(y[4] * factor, y[5] * factor), two_bf16(y[6] * factor, y[7] * factor));
+    }
+    if ((piece & 1) == 1) send_box(out, col - kChunk);
+}
+
+// The same for any layout of dW, and where the blocks before are added.
 __device__ __forceinline__ void grad_weight_row(const LinearArgs& a, const ProductArgs& p, float (&x)[kChunk], int64_t v, int64_t col,
                                                 int64_t cols, float factor) {
     if (a.acc) {
@@ -157,25 +205,17 @@ __device__ __forceinline__ void grad_weight_row(const LinearArgs& a, const Produ
         }
         if (!p.last) return;
     }
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) x[j] *= factor;
     __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(a.grad_weight.ptr) + v * a.grad_weight.row + col * a.grad_weight.col;
-    if (a.grad_weight.col == 1 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && col + kChunk <= cols) {
-#pragma unroll
-        for (int q = 0; q < kChunk / 8; ++q)
-            reinterpret_cast<uint4*>(out)[q] = make_uint4(two_bf16(x[8 * q], x[8 * q + 1]), two_bf16(x[8 * q + 2], x[8 * q + 3]),
-                                                          two_bf16(x[8 * q + 4], x[8 * q + 5]), two_bf16(x[8 * q + 6], x[8 * q + 7]));
-        return;
-    }
 #pragma unroll
     for (int j = 0; j < kChunk; ++j)
-        if (col + j < cols) out[j * a.grad_weight.col] = __float2bfloat16_rn(x[j]);
+        if (col + j < cols) out[j * a.grad_weight.col] = __float2bfloat16_rn(x[j] * factor);
 }
 
 template <int P>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     linear_product_tc(const __grid_constant__ LinearArgs a, const __grid_constant__ ProductArgs p,
-                      const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+                      const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                      const __grid_constant__ CUtensorMap map_out) {
     extern __shared__ unsigned char raw[];
     __shared__ Bars bars;
     unsigned char* const smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
@@ -293,11 +333,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int quarter = warp & 3, half = warp >> 2;
         int acc = 0;
         uint32_t acc_phase = 0;
-        const float factor = P == kGradWeight ? static_cast<float>(linear_factor(a)) : 0.0f;
+        const float factor = P == kGradWeight ? static_cast<float>(linear_factor(a)) : 1.0f;
         const int64_t m = P == kGradWeight ? p.m : rows;
+        Out out = {&map_out, smem_addr(smem + kStages * kStageBytes + warp * kBoxBytes), 0};
         for (int64_t w = pair; ok && w < plan.total; w += pairs) {
             const Work o = plan.at(w);
-            const int64_t i = o.m * kTile + rank * kHalf + quarter * 32 + lane, col = o.n * kTile + half * kHalf;
+            const int64_t i0 = o.m * kTile + rank * kHalf + quarter * 32, i = i0 + lane, col = o.n * kTile + half * kHalf;
+            out.row = static_cast<int>(i0 + (P == kGradHidden ? o.split * a.part_rows : 0));
             int64_t target = -1;
             if ((P == kLogits || P == kLogitsOnly) && i < m) {
                 const int64_t r = a.order ? a.order[p.first + i] : p.first + i;
@@ -323,7 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < kHalf / 32; ++c) tmem_load32(z + c * 32, from + c * 32);
                 tmem_load_wait();
                 release();
-                if (col < p.n) logits_row<P == kLogits>(a, z, i, col, target, i < m);
+                if (col < p.n && i0 < m) logits_row<P == kLogits>(a, z, i, col, target, i < m, given_back(o.kbs), out);
             } else {
 #pragma unroll 1
                 for (int c = 0; c < kHalf / kChunk; ++c) {
@@ -336,12 +378,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         tmem_load_wait();
                     }
                     if (c == kHalf / kChunk - 1 && o.kbs != 0) release();
-                    if (i >= m || col + c * kChunk >= p.n) continue;
-                    if (P == kGradHidden) grad_hidden_row(a, x, i, col + c * kChunk, p.n, o.split);
-                    else grad_weight_row(a, p, x, i, col + c * kChunk, p.n, factor);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) x[j] *= given_back(o.kbs);
+                    const int64_t at = col + c * kChunk;
+                    if (P == kGradHidden) {
+                        if (i0 < m && at < p.n) grad_hidden_rows(x, at, out);
+                    } else if (p.boxes) {
+                        if (i0 < m && col + (c & ~1) * kChunk < p.n) grad_weight_rows(x, at, factor, c, out);
+                    } else if (i < m && at < p.n) {
+                        grad_weight_row(a, p, x, i, at, p.n, factor);
+                    }
                 }
             }
         }
+        if (lane == 0) tensor_stores_done();
     }
     __syncwarp();
     if (!ok) {
@@ -362,14 +412,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 template <int P>
-int launch(const LinearArgs& a, const ProductArgs& p, const CUtensorMap& map_a, const CUtensorMap& map_b, cudaStream_t st) {
+int launch(const LinearArgs& a, const ProductArgs& p, const CUtensorMap& map_a, const CUtensorMap& map_b,
+           const CUtensorMap& map_out, cudaStream_t st) {
     auto kernel = linear_product_tc<P>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(CTB_ERR_CUDA, std::string("linear loss: ") + cudaGetErrorString(e));
     }
-    launch_dependent(kernel, static_cast<unsigned>(sm_count() / 2 * 2), kThreads, kSmem, st, a, p, map_a, map_b);
+    launch_dependent(kernel, static_cast<unsigned>(sm_count() / 2 * 2), kThreads, kSmem, st, a, p, map_a, map_b, map_out);
     count_launch();
     return check_launch("linear loss: product");
 }
@@ -379,28 +430,34 @@ int no_map() { return fail(CTB_ERR_CUDA, "linear loss: the driver refused a tens
 }  // namespace
 
 int linear_logits_tc(const LinearArgs& a, int64_t first, int64_t rows, bool hold, cudaStream_t st) {
-    CUtensorMap h, w;
+    CUtensorMap h, w, e;
     if (!encode_matrix_map(&h, a.h.ptr, a.v.rows, a.v.cols, a.h.row, kHalf) ||
-        !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kHalf))
+        !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kHalf) ||
+        !encode_matrix_map(&e, hold ? a.held : a.h.ptr, rows, hold ? a.vocab : 1, hold ? a.held_pitch : a.h.row, 32))
         return no_map();
-    const ProductArgs p{rows, a.vocab, a.v.cols, first, 0};
-    return hold ? launch<kLogits>(a, p, h, w, st) : launch<kLogitsOnly>(a, p, h, w, st);
+    const ProductArgs p{rows, a.vocab, a.v.cols, first, 0, 0};
+    return hold ? launch<kLogits>(a, p, h, w, e, st) : launch<kLogitsOnly>(a, p, h, w, e, st);
 }
 
 int linear_grad_hidden_tc(const LinearArgs& a, int64_t first, int64_t rows, cudaStream_t st) {
-    CUtensorMap g, w;
+    CUtensorMap g, w, out;
     if (!encode_matrix_map(&g, a.held, rows, a.vocab, a.held_pitch, kHalf) ||
-        !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kK))
+        !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kK) ||
+        !encode_matrix_map(&out, a.partial, a.splits * a.part_rows, a.v.cols, a.part_pitch, 32, 4))
         return no_map();
-    return launch<kGradHidden>(a, ProductArgs{rows, a.v.cols, a.vocab, first, 0}, g, w, st);
+    return launch<kGradHidden>(a, ProductArgs{rows, a.v.cols, a.vocab, first, 0, 0}, g, w, out, st);
 }
 
 int linear_grad_weight_tc(const LinearArgs& a, int64_t first, int64_t rows, bool last, cudaStream_t st) {
-    CUtensorMap g, h;
+    CUtensorMap g, h, out;
+    // a dW that a tensor map can describe, whole at once, leaves as boxes
+    const Matrix2& d = a.grad_weight;
+    const bool boxes = !a.acc && d.col == 1 && reinterpret_cast<uintptr_t>(d.ptr) % 16 == 0 && d.row % 8 == 0 && d.row >= a.v.cols;
     if (!encode_matrix_map(&g, a.held, rows, a.vocab, a.held_pitch, kK) ||
-        !encode_matrix_map(&h, a.h.ptr, a.v.rows, a.v.cols, a.h.row, kK))
+        !encode_matrix_map(&h, a.h.ptr, a.v.rows, a.v.cols, a.h.row, kK) ||
+        !(boxes ? encode_matrix_map(&out, d.ptr, a.vocab, a.v.cols, d.row, 32) : encode_matrix_map(&out, a.held, rows, a.vocab, a.held_pitch, 32)))
         return no_map();
-    return launch<kGradWeight>(a, ProductArgs{a.vocab, a.v.cols, rows, first, last ? 1 : 0}, g, h, st);
+    return launch<kGradWeight>(a, ProductArgs{a.vocab, a.v.cols, rows, first, last ? 1 : 0, boxes ? 1 : 0}, g, h, out, st);
 }
 
 }  // namespace ctb

@@ -100,8 +100,30 @@ __device__ __forceinline__ void tmem_load32(float* r, uint32_t address) {
 
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// A 2-D map of a row-major bfloat16 matrix [rows, cols] with `pitch` elements from row to row, for boxes of 64 columns
-// (one 128-byte swizzled row each) by box_rows rows; false where the driver refuses it.
-bool encode_matrix_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows);  // async.cu
+// A box out of shared memory (swizzled as the map says) into a matrix; what lies outside the matrix is left out. One thread
+// issues it, after proxy_fence() by the threads that wrote the box and a barrier among them.
+__device__ __forceinline__ void tensor_store(const CUtensorMap* map, int x, int y, uint32_t smem_src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(smem_src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Until the boxes stored so far have been read, or have been written.
+__device__ __forceinline__ void tensor_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tensor_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// 16 bytes of a row of 128 in a box of 32 rows, swizzled: the rows' same pieces lie in different banks.
+__device__ __forceinline__ uint32_t swizzled_piece(uint32_t box, int row, int piece) {
+    return box + static_cast<uint32_t>(row * 128 + ((piece ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void store_shared16(uint32_t to, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// A 2-D map of a row-major matrix [rows, cols] of 2- or 4-byte elements with `pitch` elements from row to row, for boxes of
+// 128 bytes (one swizzled row each) by box_rows rows; false where the driver refuses it.
+bool encode_matrix_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows,
+                       int size = 2);  // async.cu
 
 }  // namespace ctb
