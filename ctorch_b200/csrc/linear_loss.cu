@@ -233,43 +233,67 @@ __global__ void __launch_bounds__(kJoinThreads) linear_rows_tc(LinearArgs a, int
 }
 
 // Turns the held exponentials into G, rounded once to bfloat16, in their place; rows behind the last one, up to a stage of
-// the products, become zeros. A CTA takes spans of 8 KiB of a row, four vectors a thread on their way at a time. Bound by
-// reading and writing 2 bytes an element (B200, 3686 rows of 32768: see the table of cases).
-constexpr int kScaleThreads = 128, kScaleSpan = kScaleThreads * 4;  // vectors of 8
+// the products, become zeros. Bound by reading and writing 2 bytes an element, which run at the copy rate only if
+// reads stay on their way while results are written: a CTA walks its share of spans of a row (16 KiB each) in order and
+// has the next span's vectors under way before it writes this one's. B200, 8192 x 131072 (4.3 GB): 781 us with 16 CTAs
+// an SM, four times what is resident (853 with 8, 1119 with 4: the SMs do not all stream alike); without the next span
+// under way 802.
+constexpr int kScaleThreads = 256, kScaleVecs = 4, kScaleSpan = kScaleThreads * kScaleVecs;  // vectors of 8
+
+struct ScaleSpan {
+    uint4 h[kScaleVecs];
+    float pm[kScaleVecs];
+    LinearRowFactor f;
+};
+
 __global__ void __launch_bounds__(kScaleThreads) linear_scale_tc(LinearArgs a, int64_t first) {
     dependent_wait();
     const int64_t limit = min(a.block, a.v.rows - first);
     const int64_t n = a.order ? linear_block_rows(a, first) : limit;
     const int64_t upto = min(limit, (n + 63) / 64 * 64);
-    const int64_t packs = a.held_pitch / 8, spans = (packs + kScaleSpan - 1) / kScaleSpan;
-    for (int64_t i = blockIdx.x; i < upto * spans; i += gridDim.x) {
-        const int64_t b = i / spans, p0 = (i - b * spans) * kScaleSpan + threadIdx.x;
-        uint4* const held = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + b * a.held_pitch);
-        const float2* const stats = a.stats + b * a.tiles;
-        uint4 h[4];
-        float pm[4];
-        const bool live = b < n;
-        LinearRowFactor f = {0.0f, 0.0f, 0.0f, -1};
-        if (live) {
-            f = a.factors[b];
+    const int packs = static_cast<int>(a.held_pitch / 8), spans = (packs + kScaleSpan - 1) / kScaleSpan;
+    const int64_t total = upto * spans, lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+    if (lo >= hi) return;
+    const int tiles = static_cast<int>(a.tiles);
+    auto fetch = [&](ScaleSpan& s, int64_t b, int span) {
+        if (b >= n) return;
+        const uint4* const held = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.held) + b * a.held_pitch);
+        const float2* const stats = a.stats + b * tiles;
+        s.f = a.factors[b];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t j = p0 + q * kScaleThreads;
-                if (j >= packs) continue;
-                h[q] = held[j];
-                pm[q] = j / (kLinearPiece / 8) < a.tiles ? stats[j / (kLinearPiece / 8)].x : -INFINITY;
+        for (int q = 0; q < kScaleVecs; ++q) {
+            const int j = span * kScaleSpan + q * kScaleThreads + static_cast<int>(threadIdx.x);
+            if (j < packs) {
+                s.h[q] = held[j];
+                s.pm[q] = stats[min(j / (kLinearPiece / 8), tiles - 1)].x;
             }
         }
+    };
+    int64_t b = lo / spans;
+    int span = static_cast<int>(lo - b * spans);
+    ScaleSpan next;
+    fetch(next, b, span);
+    for (int64_t i = lo; i < hi; ++i) {
+        ScaleSpan s = next;
+        const int64_t row = b;
+        const int at = span;
+        if (++span == spans) {
+            span = 0;
+            ++b;
+        }
+        if (i + 1 < hi) fetch(next, b, span);
+        uint4* const held = reinterpret_cast<uint4*>(static_cast<__half*>(a.held) + row * a.held_pitch);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int64_t j = p0 + q * kScaleThreads;
+        for (int q = 0; q < kScaleVecs; ++q) {
+            const int j = at * kScaleSpan + q * kScaleThreads + static_cast<int>(threadIdx.x);
             if (j >= packs) continue;
-            if (!live) {
+            if (row >= n) {
                 held[j] = make_uint4(0u, 0u, 0u, 0u);
                 continue;
             }
-            const float c = pm[q] == -INFINITY ? f.c * 0.0f : f.c * exp2_approx((pm[q] - f.m) * a.c2);
-            uint32_t* const u = reinterpret_cast<uint32_t*>(&h[q]);
+            // a piece without a maximum has no mass
+            const float c = s.pm[q] == -INFINITY ? s.f.c * 0.0f : s.f.c * exp2_approx((s.pm[q] - s.f.m) * a.c2);
+            uint32_t* const u = reinterpret_cast<uint32_t*>(&s.h[q]);
             float g[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -277,17 +301,15 @@ __global__ void __launch_bounds__(kScaleThreads) linear_scale_tc(LinearArgs a, i
                 g[2 * k] = e.x * c;
                 g[2 * k + 1] = e.y * c;
             }
-            if (f.target >= 0 && j == f.target / 8) {
+            const int hit = s.f.target - j * 8;  // selects, not an index: those would put g into local memory
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k == (f.target & 7)) g[k] = f.at_target;
-            }
+            for (int k = 0; k < 8; ++k) g[k] = hit == k ? s.f.at_target : g[k];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const __nv_bfloat162 y = __floats2bfloat162_rn(g[2 * k], g[2 * k + 1]);
                 u[k] = *reinterpret_cast<const uint32_t*>(&y);
             }
-            held[j] = h[q];
+            held[j] = s.h[q];
         }
     }
     allow_dependents();

@@ -4,6 +4,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <type_traits>
 
 #include "rows.cuh"
 
@@ -22,6 +24,7 @@ struct NormArgs {
     const void* weight;
     int32_t weight_dtype;
     int64_t weight_stride;
+    bool weight_whole;  // contiguous, on 16 bytes
     float eps;
     int quant;  // 0: none, 1: a scale a row, 2: a scale for every 128 columns
 };
@@ -31,6 +34,7 @@ struct NormGradArgs {
     const void* weight;
     int32_t weight_dtype;
     int64_t weight_stride;
+    bool weight_whole;
     void* grad_weight;
     int64_t grad_weight_stride;
     float* partial;  // [CTAs][cols] sums of grad_weight
@@ -164,17 +168,270 @@ template <class T> __global__ void __launch_bounds__(kAnyThreads) norm_grad_any(
     allow_dependents();
 }
 
-// grad_weight: the CTAs' sums added in their order, in float64.
-__global__ void __launch_bounds__(256) norm_grad_weight(NormGradArgs a) {
+// grad_weight: the CTAs' sums added in float64, in an order that their number alone gives: 32 warps of a CTA take every
+// 32nd sum of 32 columns each.
+__global__ void __launch_bounds__(1024) norm_grad_weight(NormGradArgs a) {
     dependent_wait();
     allow_dependents();
-    for (int64_t j = blockIdx.x * 256 + threadIdx.x; j < a.v.cols; j += gridDim.x * 256) {
-        double s = 0.0;
-        for (int c = 0; c < a.ctas; ++c) s += a.partial[c * a.v.cols + j];
-        const float y = static_cast<float>(s);
-        if (a.weight_dtype == CTB_FLOAT32) static_cast<float*>(a.grad_weight)[j * a.grad_weight_stride] = y;
-        else static_cast<__nv_bfloat16*>(a.grad_weight)[j * a.grad_weight_stride] = __float2bfloat16_rn(y);
+    __shared__ double sm[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    double s = 0.0;
+    if (j < a.v.cols) {
+#pragma unroll 4
+        for (int c = warp; c < a.ctas; c += 32) s += a.partial[c * a.v.cols + j];
     }
+    sm[warp][lane] = s;
+    __syncthreads();
+    if (warp != 0 || j >= a.v.cols) return;
+    s = 0.0;
+    for (int w = 0; w < 32; ++w) s += sm[w][lane];
+    const float y = static_cast<float>(s);
+    if (a.weight_dtype == CTB_FLOAT32) static_cast<float*>(a.grad_weight)[j * a.grad_weight_stride] = y;
+    else static_cast<__nv_bfloat16*>(a.grad_weight)[j * a.grad_weight_stride] = __float2bfloat16_rn(y);
+}
+
+// ------------------------------------------------------------------------------------------------
+// rows held in registers
+
+// A group of G threads has a row, NP packs of VEC elements a thread: pack q of thread t is columns (q G + t) VEC and
+// on. Groups of a warp share a CTA of 128 threads, larger ones are a CTA. A row is read once and written once; what
+// keeps reads on their way while other rows are reduced is the number of groups an SM holds.
+template <int G> constexpr int group_threads() { return G < 128 ? 128 : G; }
+
+// The sum (or maximum) over the group; `turn` alternates between calls, so one barrier a call is enough.
+template <int G, bool MAX> __device__ __forceinline__ float group_join(float x, float (&sm)[2][32], int& turn) {
+    for (int d = 16; d >= 1; d >>= 1) {
+        const float o = __shfl_xor_sync(0xffffffffu, x, d);
+        x = MAX ? max_nan(x, o) : x + o;
+    }
+    if constexpr (G > 32) {
+        if ((threadIdx.x & 31) == 0) sm[turn][threadIdx.x >> 5] = x;
+        __syncthreads();
+        x = sm[turn][0];
+#pragma unroll
+        for (int w = 1; w < G / 32; ++w) x = MAX ? max_nan(x, sm[turn][w]) : x + sm[turn][w];
+        turn ^= 1;
+    }
+    return x;
+}
+
+template <class T, int VEC> __device__ __forceinline__ Pack<T, VEC> read_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+
+// VEC weights from column j on, as they lie (float32 or the rows' type) when they are contiguous.
+template <class T, int VEC>
+__device__ __forceinline__ void read_weights(float (&w)[VEC], const void* p, int dt, int64_t stride, bool whole, int64_t j) {
+    if (whole && dt == CTB_FLOAT32) {
+        constexpr int kPart = VEC < 4 ? VEC : 4;
+#pragma unroll
+        for (int h = 0; h < VEC; h += kPart) {
+            const Pack<float, kPart> v = read_pack<float, kPart>(static_cast<const float*>(p) + j + h);
+#pragma unroll
+            for (int q = 0; q < kPart; ++q) w[h + q] = v.v[q];
+        }
+    } else if (whole) {
+        const Pack<__nv_bfloat16, VEC> v = read_pack<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(p) + j);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) w[q] = __bfloat162float(v.v[q]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) w[q] = weight_at(p, dt, (j + q) * stride);
+    }
+}
+
+template <class T, int VEC, int G, int NP, bool RES, int QUANT>
+__global__ void __launch_bounds__(group_threads<G>()) norm_rows_held(NormArgs a) {
+    dependent_wait();
+    __shared__ float sm[2][32];
+    int turn = 0;
+    const RowViews<kNmViews>& v = a.v;
+    constexpr int kGroups = group_threads<G>() / G;
+    const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G; r < v.rows; r += static_cast<int64_t>(gridDim.x) * kGroups) {
+        const T* const x = static_cast<const T*>(v.ptr[kNmX]) + row_offset(v, kNmX, r);
+        Pack<T, VEC> s[NP], res[RES ? NP : 1];
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+            if ((q * G + t) * VEC < cols) s[q] = read_pack<T, VEC>(x + (q * G + t) * VEC);
+        if (RES) {
+            const T* const from = static_cast<const T*>(v.ptr[kNmResidual]) + row_offset(v, kNmResidual, r);
+            T* const kept = static_cast<T*>(v.ptr[kNmSummed]) + row_offset(v, kNmSummed, r);
+#pragma unroll
+            for (int q = 0; q < NP; ++q)
+                if ((q * G + t) * VEC < cols) res[q] = read_pack<T, VEC>(from + (q * G + t) * VEC);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                if ((q * G + t) * VEC >= cols) continue;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[q].v[e] = from_float<T>(to_float(s[q].v[e]) + to_float(res[q].v[e]));
+                store_pack_split<T, VEC>(kept + (q * G + t) * VEC, s[q]);
+            }
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if ((q * G + t) * VEC >= cols) continue;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) ss = fmaf(to_float(s[q].v[e]), to_float(s[q].v[e]), ss);
+        }
+        ss = group_join<G, false>(ss, sm, turn);
+        const float rstd = 1.0f / sqrtf(ss / static_cast<float>(cols) + a.eps);
+        if (t == 0 && v.ptr[kNmRstd]) static_cast<float*>(v.ptr[kNmRstd])[row_offset(v, kNmRstd, r)] = rstd;
+        if constexpr (QUANT == 0) {
+            T* const out = static_cast<T*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const int j = (q * G + t) * VEC;
+                if (j >= cols) continue;
+                float w[VEC];
+                read_weights<T, VEC>(w, a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, j);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[q].v[e] = from_float<T>(to_float(s[q].v[e]) * rstd * w[e]);
+                store_pack_split<T, VEC>(out + j, s[q]);
+            }
+        } else {
+            uint8_t* const out = static_cast<uint8_t*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r);
+            float* const scales = static_cast<float*>(v.ptr[kNmScales]) + row_offset(v, kNmScales, r);
+            float y[NP][VEC], top = 0.0f;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const int j = (q * G + t) * VEC;
+                if (j < cols) read_weights<T, VEC>(y[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, j);
+                float mine = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    y[q][e] = j < cols ? to_float(s[q].v[e]) * rstd * y[q][e] : 0.0f;
+                    mine = max_nan(mine, fabsf(y[q][e]));
+                }
+                if (QUANT == 1) {
+                    top = max_nan(top, mine);
+                    continue;
+                }
+                // the threads that have 128 columns are neighbours in a warp
+                constexpr int kShare = kScaleBlock / VEC;
+#pragma unroll
+                for (int d = kShare / 2; d >= 1; d >>= 1) mine = max_nan(mine, __shfl_xor_sync(0xffffffffu, mine, d));
+                const float scale = scale_of(mine), inv = 1.0f / scale;
+                if (j < cols && t % kShare == 0) scales[(j / kScaleBlock) * v.inner[kNmScales]] = scale;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) y[q][e] *= inv;
+            }
+            if (QUANT == 1) {
+                const float scale = scale_of(group_join<G, true>(top, sm, turn)), inv = 1.0f / scale;
+                if (t == 0) *scales = scale;
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) y[q][e] *= inv;
+            }
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const int j = (q * G + t) * VEC;
+                if (j >= cols) continue;
+                Pack<uint8_t, VEC> b;
+                if constexpr (VEC >= 2) {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) {
+                        const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(y[q][e], y[q][e + 1]), __NV_SATFINITE, __NV_E4M3);
+                        b.v[e] = static_cast<uint8_t>(two);
+                        b.v[e + 1] = static_cast<uint8_t>(two >> 8);
+                    }
+                } else {
+                    b.v[0] = to_e4m3(y[q][0]);
+                }
+                *reinterpret_cast<Pack<uint8_t, VEC>*>(out + j) = b;
+            }
+        }
+    }
+    allow_dependents();
+}
+
+// A thread keeps its columns' sums of grad_weight in registers over all rows of its group; the groups of a CTA are joined
+// in their order at the end.
+template <class T, int VEC, int G, int NP, bool PASSED>
+__global__ void __launch_bounds__(group_threads<G>()) norm_grad_held(NormGradArgs a) {
+    dependent_wait();
+    __shared__ float sm[2][32];
+    int turn = 0;
+    const RowViews<kNgViews>& v = a.v;
+    constexpr int kGroups = group_threads<G>() / G;
+    const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
+    float sums[NP][VEC];
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sums[q][e] = 0.0f;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G; r < v.rows; r += static_cast<int64_t>(gridDim.x) * kGroups) {
+        const T* const up = static_cast<const T*>(v.ptr[kNgUp]) + row_offset(v, kNgUp, r);
+        const T* const x = static_cast<const T*>(v.ptr[kNgSummed]) + row_offset(v, kNgSummed, r);
+        Pack<T, VEC> g[NP], s[NP], p[PASSED ? NP : 1];
+        float rstd = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            const int j = (q * G + t) * VEC;
+            if (j >= cols) continue;
+            g[q] = read_pack<T, VEC>(up + j);
+            s[q] = read_pack<T, VEC>(x + j);
+        }
+        if (PASSED) {
+            const T* const from = static_cast<const T*>(v.ptr[kNgPassed]) + row_offset(v, kNgPassed, r);
+#pragma unroll
+            for (int q = 0; q < NP; ++q)
+                if ((q * G + t) * VEC < cols) p[q] = read_pack<T, VEC>(from + (q * G + t) * VEC);
+        }
+        rstd = static_cast<const float*>(v.ptr[kNgRstd])[row_offset(v, kNgRstd, r)];
+        float dot = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            const int j = (q * G + t) * VEC;
+            if (j >= cols) continue;
+            float w[VEC];
+            read_weights<T, VEC>(w, a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, j);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float up_e = to_float(g[q].v[e]), hat = to_float(s[q].v[e]) * rstd;
+                sums[q][e] = fmaf(up_e, hat, sums[q][e]);
+                dot = fmaf(up_e * w[e], hat, dot);
+            }
+        }
+        dot = group_join<G, false>(dot, sm, turn) / static_cast<float>(cols);
+        T* const grad = static_cast<T*>(v.ptr[kNgGradX]) + row_offset(v, kNgGradX, r);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            const int j = (q * G + t) * VEC;
+            if (j >= cols) continue;
+            float w[VEC];
+            read_weights<T, VEC>(w, a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, j);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float hat = to_float(s[q].v[e]) * rstd;
+                float y = rstd * (to_float(g[q].v[e]) * w[e] - hat * dot);
+                if (PASSED) y += to_float(p[q].v[e]);
+                s[q].v[e] = from_float<T>(y);
+            }
+            store_pack_split<T, VEC>(grad + j, s[q]);
+        }
+    }
+    if (a.grad_weight) {
+        float* const part = a.partial + static_cast<int64_t>(blockIdx.x) * cols;
+        // groups of a warp: one after the other, through the CTA's row of partial sums
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+            if (k > 0) __syncthreads();
+            if (static_cast<int>(threadIdx.x) / G == k) {
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int j = (q * G + t) * VEC + e;
+                        if (j < cols) part[j] = k > 0 ? part[j] + sums[q][e] : sums[q][e];
+                    }
+            }
+        }
+    }
+    allow_dependents();
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -185,6 +442,77 @@ int weight_of(const ctb_view* w, int64_t cols, const char* what) {
     CTB_CHECK(check_row_dtype(w, kDtypeMatrix, what));
     if (w->ndim != 1 || w->shape[0] != cols) return fail(CTB_ERR_SHAPE, std::string(what) + " must be [" + std::to_string(cols) + "]");
     return CTB_OK;
+}
+
+bool weight_whole(const ctb_view* w) { return (w->strides[0] == 1 || w->shape[0] == 1) && aligned16(w->data); }
+
+// Elements a pack: 16 bytes where every row of every given matrix starts on that and is whole packs, else 1; 0 where the
+// columns of one are not contiguous.
+template <int N> int pack_of(const RowViews<N>& v, std::initializer_list<int> slots) {
+    int vec = 16 / static_cast<int>(dtype_size(v.dtype[0]));
+    if (v.cols % vec) vec = 1;
+    for (int s : slots) {
+        if (!v.ptr[s]) continue;
+        if (v.inner[s] != 1 && v.cols > 1) return 0;
+        const int64_t size = static_cast<int64_t>(dtype_size(v.dtype[s])), align = size == 1 ? 16 / static_cast<int64_t>(dtype_size(v.dtype[0])) : 16;
+        if (reinterpret_cast<uintptr_t>(v.ptr[s]) % align) vec = 1;
+        for (int d = 0; d < v.rank; ++d)
+            if (v.stride[s][d] * size % align) vec = 1;
+    }
+    return vec;
+}
+
+// Calls f(group, packs a thread) for the smallest group that holds `packs`, as compile-time numbers; false where none does
+// (eight 16-byte packs a thread do not fit the 64 registers that 1024 threads have).
+template <int VEC, class F> bool with_group(int64_t packs, F&& f) {
+    if (packs <= 32) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+    else if (packs <= 64) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
+    else if (packs <= 128) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+    else if (packs <= 256) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
+    else if (packs <= 512) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+    else if (packs <= 1024) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    else if (packs <= 2048) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
+    else if (packs <= 4096) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+    else if (packs > 8192 || VEC > 1) return false;
+    else if constexpr (VEC == 1) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
+    return true;
+}
+
+template <class T, int VEC> bool run_norm_held(const NormArgs& a, cudaStream_t st) {
+    return with_group<VEC>((a.v.cols + VEC - 1) / VEC, [&](auto g, auto np) {
+        constexpr int G = decltype(g)::value, NP = decltype(np)::value, threads = group_threads<G>(), groups = threads / G;
+        const bool res = a.v.ptr[kNmResidual] != nullptr;
+        auto launch = [&](auto kernel) {
+            launch_dependent(kernel, grid_for((a.v.rows + groups - 1) / groups, 64), threads, 0, st, a);
+        };
+        if (a.quant == 0) res ? launch(norm_rows_held<T, VEC, G, NP, true, 0>) : launch(norm_rows_held<T, VEC, G, NP, false, 0>);
+        else if (a.quant == 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 1>) : launch(norm_rows_held<T, VEC, G, NP, false, 1>);
+        else if constexpr (VEC > 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 2>) : launch(norm_rows_held<T, VEC, G, NP, false, 2>);
+    });
+}
+
+template <class T> void run_norm(const NormArgs& a, cudaStream_t st) {
+    constexpr int kVec = 16 / sizeof(T);
+    const int vec = pack_of(a.v, {kNmX, kNmResidual, kNmSummed, kNmOut});
+    const bool held = vec == kVec ? run_norm_held<T, kVec>(a, st) : vec == 1 && a.quant != 2 && run_norm_held<T, 1>(a, st);
+    if (!held) launch_dependent(norm_rows_any<T>, grid_for(a.v.rows, 8), kAnyThreads, 0, st, a);
+    count_launch();
+}
+
+template <class T, int VEC> bool run_grad_held(const NormGradArgs& a, cudaStream_t st) {
+    return with_group<VEC>((a.v.cols + VEC - 1) / VEC, [&](auto g, auto np) {
+        constexpr int G = decltype(g)::value, NP = decltype(np)::value;
+        auto kernel = a.v.ptr[kNgPassed] ? norm_grad_held<T, VEC, G, NP, true> : norm_grad_held<T, VEC, G, NP, false>;
+        launch_dependent(kernel, static_cast<unsigned>(a.ctas), group_threads<G>(), 0, st, a);
+    });
+}
+
+template <class T> void run_grad(const NormGradArgs& a, cudaStream_t st) {
+    constexpr int kVec = 16 / sizeof(T);
+    const int vec = pack_of(a.v, {kNgUp, kNgSummed, kNgPassed, kNgGradX});
+    const bool held = vec == kVec ? run_grad_held<T, kVec>(a, st) : vec == 1 && run_grad_held<T, 1>(a, st);
+    if (!held) launch_dependent(norm_grad_any<T>, static_cast<unsigned>(a.ctas), kAnyThreads, 0, st, a);
+    count_launch();
 }
 
 int grad_ctas(int64_t rows) { return static_cast<int>(std::min<int64_t>(rows, sm_count() * 4)); }
@@ -222,9 +550,10 @@ int ctb_rms_norm(const ctb_view* x, const ctb_view* weight, const ctb_view* resi
         a.eps = static_cast<float>(eps);
         a.quant = quant;
         if (a.v.rows == 0) return CTB_OK;
-        auto kernel = x->dtype == CTB_FLOAT32 ? norm_rows_any<float> : norm_rows_any<__nv_bfloat16>;
-        launch_dependent(kernel, grid_for(a.v.rows, 8), kAnyThreads, 0, static_cast<cudaStream_t>(stream), a);
-        count_launch();
+        a.weight_whole = weight_whole(weight);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (x->dtype == CTB_FLOAT32) run_norm<float>(a, st);
+        else run_norm<__nv_bfloat16>(a, st);
         return check_launch("rms norm");
     });
 }
@@ -269,13 +598,13 @@ int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summed, cons
         a.partial = static_cast<float*>(scratch);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (a.ctas) {
-            auto kernel = grad_out->dtype == CTB_FLOAT32 ? norm_grad_any<float> : norm_grad_any<__nv_bfloat16>;
-            launch_dependent(kernel, static_cast<unsigned>(a.ctas), kAnyThreads, 0, st, a);
-            count_launch();
+            a.weight_whole = weight_whole(weight);
+            if (grad_out->dtype == CTB_FLOAT32) run_grad<float>(a, st);
+            else run_grad<__nv_bfloat16>(a, st);
             CTB_CHECK(check_launch("rms norm backward"));
         }
         if (grad_weight) {
-            launch_dependent(norm_grad_weight, grid_for((cols + 255) / 256, 4), 256, 0, st, a);
+            launch_dependent(norm_grad_weight, static_cast<unsigned>((cols + 31) / 32), 1024, 0, st, a);
             count_launch();
             CTB_CHECK(check_launch("rms norm backward"));
         }
