@@ -195,9 +195,11 @@ __global__ void __launch_bounds__(1024) norm_grad_weight(NormGradArgs a) {
 // rows held in registers
 
 // A group of G threads has a row, NP packs of VEC elements a thread: pack q of thread t is columns (q G + t) VEC and
-// on. Groups of a warp share a CTA of 128 threads, larger ones are a CTA. A row is read once and written once; what
+// on. Groups of one warp share a CTA of 128 threads, larger ones are a CTA. A row is read once and written once; what
 // keeps reads on their way while other rows are reduced is the number of groups an SM holds.
-template <int G> constexpr int group_threads() { return G < 128 ? 128 : G; }
+template <int G> constexpr int group_threads() { return G == 32 ? 128 : G; }
+// CTAs an SM that the registers have to leave room for: 1024 threads (64 registers each), 768 backward (80).
+template <int G> constexpr int group_ctas(int threads) { return threads / group_threads<G>() > 1 ? threads / group_threads<G>() : 1; }
 
 // The sum (or maximum) over the group; `turn` alternates between calls, so one barrier a call is enough.
 template <int G, bool MAX> __device__ __forceinline__ float group_join(float x, float (&sm)[2][32], int& turn) {
@@ -242,7 +244,7 @@ __device__ __forceinline__ void read_weights(float (&w)[VEC], const void* p, int
 }
 
 template <class T, int VEC, int G, int NP, bool RES, int QUANT>
-__global__ void __launch_bounds__(group_threads<G>()) norm_rows_held(NormArgs a) {
+__global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(1024)) norm_rows_held(NormArgs a) {
     dependent_wait();
     __shared__ float sm[2][32];
     int turn = 0;
@@ -348,10 +350,165 @@ __global__ void __launch_bounds__(group_threads<G>()) norm_rows_held(NormArgs a)
     allow_dependents();
 }
 
+// The same for 16-byte packs, the rows on their way through shared memory: a thread copies its own packs of the next
+// kRing - 1 rows ahead (cp.async) and is the only one to read them, so nothing but the row's sum waits for other threads,
+// and the bytes on their way do not take registers. B200, 16384 x 4096 bfloat16 with a residual: 106 us with the rows in
+// registers, see the table of cases for this.
+// Stages of the ring for `arrays` matrices: three, or two where they would not fit (16384 columns backward).
+template <int G, int NP> constexpr int ring_stages(int arrays) { return 3 * arrays * NP * 16 * group_threads<G>() <= 200 * 1024 ? 3 : 2; }
+template <int G, int NP> constexpr int ring_bytes(int arrays) { return ring_stages<G, NP>(arrays) * arrays * NP * 16 * group_threads<G>(); }
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int STAGES> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
+
+template <class T, int VEC> __device__ __forceinline__ Pack<T, VEC> ring_pack(uint32_t at) {
+    Pack<T, VEC> v;
+    uint32_t* const u = reinterpret_cast<uint32_t*>(&v);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(at));
+    return v;
+}
+
+template <class T, int VEC, int G, int NP, bool RES, int QUANT>
+__global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_rows_ring(NormArgs a) {
+    extern __shared__ __align__(16) unsigned char ring[];
+    dependent_wait();
+    __shared__ float sm[2][32];
+    int turn = 0;
+    const RowViews<kNmViews>& v = a.v;
+    constexpr int kGroups = group_threads<G>() / G, kArrays = RES ? 2 : 1, kRing = ring_stages<G, NP>(kArrays);
+    const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, group = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
+    const int64_t lo = v.rows * group / groups, hi = v.rows * (group + 1) / groups;
+    const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
+    constexpr uint32_t kStep = group_threads<G>() * 16;  // from one pack of a thread to its next
+    auto fetch = [&](int64_t r, int stage) {
+        if (r < hi) {
+            const T* const x = static_cast<const T*>(v.ptr[kNmX]) + row_offset(v, kNmX, r) + t * VEC;
+            const T* const res = RES ? static_cast<const T*>(v.ptr[kNmResidual]) + row_offset(v, kNmResidual, r) + t * VEC : nullptr;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                if ((q * G + t) * VEC >= cols) continue;
+                copy16(mine + (stage * kArrays * NP + q) * kStep, x + q * G * VEC);
+                if (RES) copy16(mine + (stage * kArrays * NP + NP + q) * kStep, res + q * G * VEC);
+            }
+        }
+        copies_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kRing - 1; ++s) fetch(lo + s, s);
+    float w[NP][VEC];
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+        if ((q * G + t) * VEC < cols) read_weights<T, VEC>(w[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, (q * G + t) * VEC);
+    int stage = 0, ahead = kRing - 1;
+    for (int64_t r = lo; r < hi; ++r) {
+        copies_wait<kRing>();
+        Pack<T, VEC> s[NP];
+        T* const kept = RES ? static_cast<T*>(v.ptr[kNmSummed]) + row_offset(v, kNmSummed, r) + t * VEC : nullptr;
+        float ss = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if ((q * G + t) * VEC >= cols) continue;
+            s[q] = ring_pack<T, VEC>(mine + (stage * kArrays * NP + q) * kStep);
+            if (RES) {
+                const Pack<T, VEC> o = ring_pack<T, VEC>(mine + (stage * kArrays * NP + NP + q) * kStep);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[q].v[e] = from_float<T>(to_float(s[q].v[e]) + to_float(o.v[e]));
+                store_pack_split<T, VEC>(kept + q * G * VEC, s[q]);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) ss = fmaf(to_float(s[q].v[e]), to_float(s[q].v[e]), ss);
+        }
+        fetch(r + kRing - 1, ahead);
+        stage = stage + 1 == kRing ? 0 : stage + 1;
+        ahead = ahead + 1 == kRing ? 0 : ahead + 1;
+        ss = group_join<G, false>(ss, sm, turn);
+        const float rstd = 1.0f / sqrtf(ss / static_cast<float>(cols) + a.eps);
+        if (t == 0 && v.ptr[kNmRstd]) static_cast<float*>(v.ptr[kNmRstd])[row_offset(v, kNmRstd, r)] = rstd;
+        if constexpr (QUANT == 0) {
+            T* const out = static_cast<T*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r) + t * VEC;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                if ((q * G + t) * VEC >= cols) continue;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[q].v[e] = from_float<T>(to_float(s[q].v[e]) * rstd * w[q][e]);
+                store_pack_split<T, VEC>(out + q * G * VEC, s[q]);
+            }
+        } else {
+            uint8_t* const out = static_cast<uint8_t*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r);
+            float* const scales = static_cast<float*>(v.ptr[kNmScales]) + row_offset(v, kNmScales, r);
+            float inv = 0.0f;
+            if (QUANT == 1) {
+                float top = 0.0f;
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+                    if ((q * G + t) * VEC < cols)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) top = max_nan(top, fabsf(to_float(s[q].v[e]) * rstd * w[q][e]));
+                const float scale = scale_of(group_join<G, true>(top, sm, turn));
+                inv = 1.0f / scale;
+                if (t == 0) *scales = scale;
+            }
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const int j = (q * G + t) * VEC;
+                const bool live = j < cols;
+                float y[VEC], top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    y[e] = live ? to_float(s[q].v[e]) * rstd * w[q][e] : 0.0f;
+                    top = max_nan(top, fabsf(y[e]));
+                }
+                if (QUANT == 2) {
+                    // the threads that have 128 columns are neighbours in a warp
+                    constexpr int kShare = kScaleBlock / VEC;
+#pragma unroll
+                    for (int d = kShare / 2; d >= 1; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float scale = scale_of(top);
+                    inv = 1.0f / scale;
+                    if (live && t % kShare == 0) scales[(j / kScaleBlock) * v.inner[kNmScales]] = scale;
+                }
+                if (!live) continue;
+                Pack<uint8_t, VEC> b;
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(y[e] * inv, y[e + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                    b.v[e] = static_cast<uint8_t>(two);
+                    b.v[e + 1] = static_cast<uint8_t>(two >> 8);
+                }
+                *reinterpret_cast<Pack<uint8_t, VEC>*>(out + j) = b;
+            }
+        }
+    }
+    allow_dependents();
+}
+
+// The groups' sums of a CTA's rows, joined in their order, as the CTA's row of partial sums.
+template <int VEC, int G, int NP>
+__device__ __forceinline__ void put_partial(const NormGradArgs& a, const float (&sums)[NP][VEC], int t, int cols) {
+    float* const part = a.partial + static_cast<int64_t>(blockIdx.x) * cols;
+    constexpr int kGroups = group_threads<G>() / G;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        if (k > 0) __syncthreads();
+        if (static_cast<int>(threadIdx.x) / G != k) continue;
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int j = (q * G + t) * VEC + e;
+                if (j < cols) part[j] = k > 0 ? part[j] + sums[q][e] : sums[q][e];
+            }
+    }
+}
+
 // A thread keeps its columns' sums of grad_weight in registers over all rows of its group; the groups of a CTA are joined
 // in their order at the end.
 template <class T, int VEC, int G, int NP, bool PASSED>
-__global__ void __launch_bounds__(group_threads<G>()) norm_grad_held(NormGradArgs a) {
+__global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_grad_held(NormGradArgs a) {
     dependent_wait();
     __shared__ float sm[2][32];
     int turn = 0;
@@ -414,23 +571,90 @@ __global__ void __launch_bounds__(group_threads<G>()) norm_grad_held(NormGradArg
             store_pack_split<T, VEC>(grad + j, s[q]);
         }
     }
-    if (a.grad_weight) {
-        float* const part = a.partial + static_cast<int64_t>(blockIdx.x) * cols;
-        // groups of a warp: one after the other, through the CTA's row of partial sums
+    if (a.grad_weight) put_partial<VEC, G, NP>(a, sums, t, cols);
+    allow_dependents();
+}
+
+// The same with 16-byte packs on their way through shared memory, as norm_rows_ring.
+template <class T, int VEC, int G, int NP, bool PASSED>
+__global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_grad_ring(NormGradArgs a) {
+    extern __shared__ __align__(16) unsigned char ring[];
+    dependent_wait();
+    __shared__ float sm[2][32];
+    int turn = 0;
+    const RowViews<kNgViews>& v = a.v;
+    constexpr int kGroups = group_threads<G>() / G, kArrays = PASSED ? 3 : 2, kRing = ring_stages<G, NP>(kArrays);
+    const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, group = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
+    const int64_t lo = v.rows * group / groups, hi = v.rows * (group + 1) / groups;
+    const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
+    constexpr uint32_t kStep = group_threads<G>() * 16;
+    auto fetch = [&](int64_t r, int stage) {
+        if (r < hi) {
+            const T* const up = static_cast<const T*>(v.ptr[kNgUp]) + row_offset(v, kNgUp, r) + t * VEC;
+            const T* const x = static_cast<const T*>(v.ptr[kNgSummed]) + row_offset(v, kNgSummed, r) + t * VEC;
+            const T* const p = PASSED ? static_cast<const T*>(v.ptr[kNgPassed]) + row_offset(v, kNgPassed, r) + t * VEC : nullptr;
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-            if (k > 0) __syncthreads();
-            if (static_cast<int>(threadIdx.x) / G == k) {
-#pragma unroll
-                for (int q = 0; q < NP; ++q)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int j = (q * G + t) * VEC + e;
-                        if (j < cols) part[j] = k > 0 ? part[j] + sums[q][e] : sums[q][e];
-                    }
+            for (int q = 0; q < NP; ++q) {
+                if ((q * G + t) * VEC >= cols) continue;
+                copy16(mine + (stage * kArrays * NP + q) * kStep, up + q * G * VEC);
+                copy16(mine + (stage * kArrays * NP + NP + q) * kStep, x + q * G * VEC);
+                if (PASSED) copy16(mine + (stage * kArrays * NP + 2 * NP + q) * kStep, p + q * G * VEC);
             }
         }
+        copies_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kRing - 1; ++s) fetch(lo + s, s);
+    float w[NP][VEC], sums[NP][VEC];
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+        if ((q * G + t) * VEC < cols) read_weights<T, VEC>(w[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, (q * G + t) * VEC);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sums[q][e] = 0.0f;
     }
+    const float* const rstds = static_cast<const float*>(v.ptr[kNgRstd]);
+    float rstd = lo < hi ? rstds[row_offset(v, kNgRstd, lo)] : 0.0f;
+    int stage = 0, ahead = kRing - 1;
+    for (int64_t r = lo; r < hi; ++r) {
+        copies_wait<kRing>();
+        Pack<T, VEC> g[NP], s[NP];
+        float dot = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if ((q * G + t) * VEC >= cols) continue;
+            g[q] = ring_pack<T, VEC>(mine + (stage * kArrays * NP + q) * kStep);
+            s[q] = ring_pack<T, VEC>(mine + (stage * kArrays * NP + NP + q) * kStep);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float up = to_float(g[q].v[e]), hat = to_float(s[q].v[e]) * rstd;
+                sums[q][e] = fmaf(up, hat, sums[q][e]);
+                dot = fmaf(up * w[q][e], hat, dot);
+            }
+        }
+        const float next = r + 1 < hi ? rstds[row_offset(v, kNgRstd, r + 1)] : 0.0f;
+        fetch(r + kRing - 1, ahead);
+        ahead = ahead + 1 == kRing ? 0 : ahead + 1;
+        dot = group_join<G, false>(dot, sm, turn) / static_cast<float>(cols);
+        T* const grad = static_cast<T*>(v.ptr[kNgGradX]) + row_offset(v, kNgGradX, r) + t * VEC;
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if ((q * G + t) * VEC >= cols) continue;
+            Pack<T, VEC> p;
+            if (PASSED) p = ring_pack<T, VEC>(mine + (stage * kArrays * NP + 2 * NP + q) * kStep);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float hat = to_float(s[q].v[e]) * rstd;
+                float y = rstd * (to_float(g[q].v[e]) * w[q][e] - hat * dot);
+                if (PASSED) y += to_float(p.v[e]);
+                s[q].v[e] = from_float<T>(y);
+            }
+            store_pack_split<T, VEC>(grad + q * G * VEC, s[q]);
+        }
+        stage = stage + 1 == kRing ? 0 : stage + 1;
+        rstd = next;
+    }
+    if (a.grad_weight) put_partial<VEC, G, NP>(a, sums, t, cols);
     allow_dependents();
 }
 
@@ -467,27 +691,45 @@ template <int N> int pack_of(const RowViews<N>& v, std::initializer_list<int> sl
 template <int VEC, class F> bool with_group(int64_t packs, F&& f) {
     if (packs <= 32) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
     else if (packs <= 64) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 128) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+    else if (packs <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
     else if (packs <= 256) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 512) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
-    else if (packs <= 1024) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-    else if (packs <= 2048) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
+    else if (packs <= 512) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if (packs <= 1024) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
+    else if (packs <= 2048) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
     else if (packs <= 4096) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
     else if (packs > 8192 || VEC > 1) return false;
     else if constexpr (VEC == 1) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
     return true;
 }
 
+constexpr int kRingPacks = 2048;  // of a row that passes through shared memory: longer ones do not fit it
+
+// CTAs an SM in a grid: what is resident (768 threads, so 80 registers a thread), or eight times that in one-type norms,
+// where the SMs do not all stream alike (B200, 16384 x 4096 with a residual: 89 us, 96 without; to 8 bits with a
+// scale for every 128 columns, 8192 x 8192, the other way round: 123 against 109).
+int norm_ctas(int threads, int quant) { return std::max(1, 768 / threads) * (quant ? 1 : 8); }
+
+// Starts a kernel whose rows pass through shared memory, `per_sm` CTAs an SM at most.
+template <class A, class K> void launch_ring(K kernel, const A& a, unsigned grid, int threads, int bytes, cudaStream_t st) {
+    if (bytes > 47 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    launch_dependent(kernel, grid, threads, bytes, st, a);
+}
+
 template <class T, int VEC> bool run_norm_held(const NormArgs& a, cudaStream_t st) {
     return with_group<VEC>((a.v.cols + VEC - 1) / VEC, [&](auto g, auto np) {
         constexpr int G = decltype(g)::value, NP = decltype(np)::value, threads = group_threads<G>(), groups = threads / G;
         const bool res = a.v.ptr[kNmResidual] != nullptr;
-        auto launch = [&](auto kernel) {
-            launch_dependent(kernel, grid_for((a.v.rows + groups - 1) / groups, 64), threads, 0, st, a);
-        };
-        if (a.quant == 0) res ? launch(norm_rows_held<T, VEC, G, NP, true, 0>) : launch(norm_rows_held<T, VEC, G, NP, false, 0>);
-        else if (a.quant == 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 1>) : launch(norm_rows_held<T, VEC, G, NP, false, 1>);
-        else if constexpr (VEC > 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 2>) : launch(norm_rows_held<T, VEC, G, NP, false, 2>);
+        const unsigned grid = grid_for((a.v.rows + groups - 1) / groups, VEC > 1 && G * NP <= kRingPacks ? norm_ctas(threads, a.quant) : 64);
+        auto launch = [&](auto kernel, int arrays) { launch_ring(kernel, a, grid, threads, ring_bytes<G, NP>(arrays), st); };
+        if constexpr (VEC > 1 && G * NP <= kRingPacks) {
+            if (a.quant == 0) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 0>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 0>, 1);
+            else if (a.quant == 1) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 1>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 1>, 1);
+            else res ? launch(norm_rows_ring<T, VEC, G, NP, true, 2>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 2>, 1);
+        } else {
+            if (a.quant == 0) res ? launch(norm_rows_held<T, VEC, G, NP, true, 0>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 0>, 0);
+            else if (a.quant == 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 1>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 1>, 0);
+            else if constexpr (VEC > 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 2>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 2>, 0);
+        }
     });
 }
 
@@ -499,23 +741,32 @@ template <class T> void run_norm(const NormArgs& a, cudaStream_t st) {
     count_launch();
 }
 
-template <class T, int VEC> bool run_grad_held(const NormGradArgs& a, cudaStream_t st) {
+// CTAs of the backward pass at most, each with a row of partial sums: as many as are resident, fewer on longer rows.
+int64_t grad_ctas(int64_t rows, int64_t row_bytes) {
+    return std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * (row_bytes <= 4096 ? 6 : row_bytes <= 8192 ? 3 : 2));
+}
+
+template <class T, int VEC> bool run_grad_held(NormGradArgs& a, cudaStream_t st) {
     return with_group<VEC>((a.v.cols + VEC - 1) / VEC, [&](auto g, auto np) {
         constexpr int G = decltype(g)::value, NP = decltype(np)::value;
-        auto kernel = a.v.ptr[kNgPassed] ? norm_grad_held<T, VEC, G, NP, true> : norm_grad_held<T, VEC, G, NP, false>;
-        launch_dependent(kernel, static_cast<unsigned>(a.ctas), group_threads<G>(), 0, st, a);
+        const bool passed = a.v.ptr[kNgPassed] != nullptr;
+        constexpr int groups = group_threads<G>() / G, per_sm = 768 / group_threads<G>() > 1 ? 768 / group_threads<G>() : 1;
+        a.ctas = static_cast<int>(std::min<int64_t>({a.ctas, (a.v.rows + groups - 1) / groups, static_cast<int64_t>(sm_count()) * per_sm}));
+        auto launch = [&](auto kernel, int arrays) {
+            launch_ring(kernel, a, static_cast<unsigned>(a.ctas), group_threads<G>(), ring_bytes<G, NP>(arrays), st);
+        };
+        if constexpr (VEC > 1 && G * NP <= kRingPacks) passed ? launch(norm_grad_ring<T, VEC, G, NP, true>, 3) : launch(norm_grad_ring<T, VEC, G, NP, false>, 2);
+        else passed ? launch(norm_grad_held<T, VEC, G, NP, true>, 0) : launch(norm_grad_held<T, VEC, G, NP, false>, 0);
     });
 }
 
-template <class T> void run_grad(const NormGradArgs& a, cudaStream_t st) {
+template <class T> void run_grad(NormGradArgs& a, cudaStream_t st) {
     constexpr int kVec = 16 / sizeof(T);
     const int vec = pack_of(a.v, {kNgUp, kNgSummed, kNgPassed, kNgGradX});
     const bool held = vec == kVec ? run_grad_held<T, kVec>(a, st) : vec == 1 && run_grad_held<T, 1>(a, st);
     if (!held) launch_dependent(norm_grad_any<T>, static_cast<unsigned>(a.ctas), kAnyThreads, 0, st, a);
     count_launch();
 }
-
-int grad_ctas(int64_t rows) { return static_cast<int>(std::min<int64_t>(rows, sm_count() * 4)); }
 
 }  // namespace
 }  // namespace ctb
@@ -562,7 +813,8 @@ size_t ctb_rms_norm_backward_scratch_bytes(const ctb_view* summed) {
     if (!summed || summed->ndim < 1 || summed->ndim > kMaxDims) return 0;
     int64_t rows = 1;
     for (int d = 0; d < summed->ndim - 1; ++d) rows *= summed->shape[d];
-    return static_cast<size_t>(grad_ctas(rows)) * static_cast<size_t>(summed->shape[summed->ndim - 1]) * sizeof(float);
+    const int64_t cols = summed->shape[summed->ndim - 1];
+    return static_cast<size_t>(grad_ctas(rows, cols * static_cast<int64_t>(dtype_size(summed->dtype))) * cols) * sizeof(float);
 }
 
 int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summed, const ctb_view* weight, const ctb_view* rstd,
@@ -587,7 +839,7 @@ int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summed, cons
             a.grad_weight = grad_weight->data;
             a.grad_weight_stride = grad_weight->strides[0];
         }
-        a.ctas = grad_ctas(b.v.rows);
+        a.ctas = static_cast<int>(grad_ctas(b.v.rows, cols * static_cast<int64_t>(dtype_size(grad_out->dtype))));
         if (grad_weight)
             CTB_CHECK(check_row_scratch(scratch, scratch_bytes, static_cast<size_t>(a.ctas) * static_cast<size_t>(cols) * sizeof(float), 16));
         b.finish();
