@@ -27,7 +27,7 @@ struct BalanceRun {  // of one CTA's rows
 };
 
 struct BalanceGroup {
-    double loss, rows;
+    double lse2, rows;  // mean of lse^2; rows that count, 1 at least
     int32_t bad, pad;
 };
 
@@ -41,6 +41,9 @@ struct BalanceArgs {
     BalanceRun* run;     // [groups * runs]
     float* slope;        // [groups][E] a_e
     BalanceGroup* group; // [groups]
+    double* inner;       // [groups][chunks] sums of a_e P_e over 32 experts each
+    float2* row_stats;   // [rows] (maximum, sum of exponentials)
+    int64_t chunks;
     float* loss;
     int64_t* counts;
     int64_t counts_stride[2];
@@ -75,7 +78,29 @@ template <class T> __device__ __forceinline__ RowStats row_stats(const T* x, int
     return o;
 }
 
-// A warp a row; every lane keeps its columns' sums of p in its warp's part of shared memory.
+// A run's results out of shared memory: the warps' sums in their order.
+__device__ __forceinline__ void put_run(const BalanceArgs& a, const int32_t* counts, const float* sums, const double* lse2,
+                                        const int32_t* live, int32_t bad) {
+    const int experts = static_cast<int>(a.v.cols);
+    float* const out = a.run_probs + blockIdx.x * a.v.cols;
+    int32_t* const out_counts = a.run_counts + blockIdx.x * a.v.cols;
+    for (int e = threadIdx.x; e < experts; e += kThreads) {
+        float s = 0.0f;
+        for (int w = 0; w < kWarps; ++w) s += sums[w * experts + e];
+        out[e] = s;
+        out_counts[e] = counts[e];
+    }
+    if (threadIdx.x == 0) {
+        BalanceRun b{0.0, 0, bad};
+        for (int w = 0; w < kWarps; ++w) {
+            b.lse2 += lse2[w];
+            b.rows += live[w];
+        }
+        a.run[blockIdx.x] = b;
+    }
+}
+
+// Any layout and number of experts: a warp a row; every lane keeps its columns' sums of p in its warp's part of shared memory.
 template <class T> __global__ void __launch_bounds__(kThreads) balance_rows(BalanceArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     dependent_wait();
@@ -118,85 +143,289 @@ template <class T> __global__ void __launch_bounds__(kThreads) balance_rows(Bala
         live[warp] = n;
     }
     __syncthreads();
-    float* const out = a.run_probs + blockIdx.x * a.v.cols;
-    int32_t* const out_counts = a.run_counts + blockIdx.x * a.v.cols;
-    for (int e = threadIdx.x; e < experts; e += kThreads) {
-        float s = 0.0f;
-        for (int w = 0; w < kWarps; ++w) s += sums[w * experts + e];
-        out[e] = s;
-        out_counts[e] = counts[e];
-    }
-    if (threadIdx.x == 0) {
-        BalanceRun b{0.0, 0, bad};
-        for (int w = 0; w < kWarps; ++w) {
-            b.lse2 += lse2[w];
-            b.rows += live[w];
-        }
-        a.run[blockIdx.x] = b;
-    }
+    put_run(a, counts, sums, lse2, live, bad);
     allow_dependents();
 }
 
-// A CTA a group: its runs added in their order, in float64.
-__global__ void __launch_bounds__(kThreads) balance_join(BalanceArgs a) {
+// 32 experts of a group: its runs added in float64, in an order that their number alone gives (32 warps take every 32nd).
+constexpr int kJoinThreads = 1024;
+__global__ void __launch_bounds__(kJoinThreads) balance_join(BalanceArgs a) {
     dependent_wait();
     allow_dependents();
-    __shared__ double part[kWarps], total_lse2, total_rows;
-    __shared__ int32_t any_bad;
-    const int64_t g = blockIdx.x, experts = a.v.cols;
-    if (threadIdx.x == 0) {
-        double l2 = 0.0, n = 0.0;
-        int32_t bad = 0;
-        for (int64_t i = 0; i < a.runs; ++i) {
-            const BalanceRun b = a.run[g * a.runs + i];
-            l2 += b.lse2;
-            n += b.rows;
-            bad |= b.bad;
-        }
-        total_lse2 = l2;
-        total_rows = n;
-        any_bad = bad;
-    }
-    __syncthreads();
-    const double n = fmax(total_rows, 1.0);
-    double inner = 0.0;
-    for (int64_t e = threadIdx.x; e < experts; e += kThreads) {
-        double p = 0.0;
-        int64_t c = 0;
-        for (int64_t i = 0; i < a.runs; ++i) {
+    __shared__ double sums[32][33], lse2[32], rows[32];
+    __shared__ int64_t counts[32][33];
+    __shared__ int32_t bads[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t g = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, e = chunk * 32 + lane, experts = a.v.cols;
+    double p = 0.0;
+    int64_t c = 0;
+    if (e < experts) {
+#pragma unroll 4
+        for (int64_t i = warp; i < a.runs; i += 32) {
             p += a.run_probs[(g * a.runs + i) * experts + e];
             c += a.run_counts[(g * a.runs + i) * experts + e];
         }
+    }
+    sums[warp][lane] = p;
+    counts[warp][lane] = c;
+    double l2 = 0.0, n = 0.0;
+    int32_t bad = 0;
+    for (int64_t i = threadIdx.x; i < a.runs; i += kJoinThreads) {
+        const BalanceRun b = a.run[g * a.runs + i];
+        l2 += b.lse2;
+        n += b.rows;
+        bad |= b.bad;
+    }
+    for (int d = 16; d >= 1; d >>= 1) {
+        l2 += __shfl_xor_sync(0xffffffffu, l2, d);
+        n += __shfl_xor_sync(0xffffffffu, n, d);
+        bad |= __shfl_xor_sync(0xffffffffu, bad, d);
+    }
+    if (lane == 0) {
+        lse2[warp] = l2;
+        rows[warp] = n;
+        bads[warp] = bad;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    l2 = n = 0.0;
+    bad = 0;
+    p = 0.0;
+    c = 0;
+    for (int w = 0; w < 32; ++w) {
+        l2 += lse2[w];
+        n += rows[w];
+        bad |= bads[w];
+        p += sums[w][lane];
+        c += counts[w][lane];
+    }
+    n = fmax(n, 1.0);
+    double inner = 0.0;
+    if (e < experts) {
         p /= n;
         const double slope = a.coef * static_cast<double>(experts) * static_cast<double>(c) / (n * static_cast<double>(a.chosen));
-        inner += slope * p;
-        a.slope[g * experts + e] = any_bad ? NAN : static_cast<float>(slope);
+        inner = slope * p;
+        a.slope[g * experts + e] = bad ? NAN : static_cast<float>(slope);
         if (a.counts) a.counts[g * a.counts_stride[0] + e * a.counts_stride[1]] = c;
         if (a.probs) a.probs[g * a.probs_stride[0] + e * a.probs_stride[1]] = static_cast<float>(p);
     }
     for (int d = 16; d >= 1; d >>= 1) inner += __shfl_xor_sync(0xffffffffu, inner, d);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = inner;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double s = 0.0;
-        for (int w = 0; w < kWarps; ++w) s += part[w];
-        BalanceGroup b;
-        b.loss = any_bad ? nan("") : s + (a.z_coef != 0.0 ? a.z_coef * total_lse2 / n : 0.0);
-        b.rows = n;
-        b.bad = any_bad;
-        b.pad = 0;
-        a.group[g] = b;
+    if (lane == 0) {
+        a.inner[g * a.chunks + chunk] = bad ? nan("") : inner;
+        if (chunk == 0) a.group[g] = BalanceGroup{l2 / n, n, bad, 0};
     }
+}
+
+// The scalar, by one warp of the last kernel: the groups' losses in their order.
+__device__ __forceinline__ void put_loss(const BalanceArgs& a) {
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < a.groups * a.chunks; i += 32) s += a.inner[i];
+    if (a.z_coef != 0.0)
+        for (int64_t g = threadIdx.x; g < a.groups; g += 32) s += a.z_coef * a.group[g].lse2;
+    for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (threadIdx.x == 0) *a.loss = static_cast<float>(s / static_cast<double>(a.groups));
+}
+
+// ------------------------------------------------------------------------------------------------
+// rows held in registers: L lanes of a warp have a row, NP packs of VEC experts each; a warp has kRows rows of its run
+// under way at a time for each of its 32 / L groups of lanes. VEC is 4 where every row starts on 4 elements.
+
+__device__ __forceinline__ float exp_approx(float x) {  // of x <= 0: 2^-22 and its argument's rounding
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+    return y;
+}
+
+template <int L> __device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+    for (int d = L / 2; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+template <int L> __device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+    for (int d = L / 2; d >= 1; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+}
+
+template <class T, int VEC, int L, int NP> struct HeldRow {
+    static constexpr int kOf = VEC * NP;
+    float x[kOf];
+    // Experts that there are none of are -inf.
+    __device__ __forceinline__ void load(const T* p, int lane, int experts) {
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            const int e = (q * L + lane) * VEC;
+            if (e < experts) {
+                const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(p + e);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) x[q * VEC + k] = to_float(v.v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) x[q * VEC + k] = -INFINITY;
+            }
+        }
+    }
+};
+
+template <class T, int VEC, int L, int NP, int ROWS>
+__global__ void __launch_bounds__(kThreads) balance_rows_held(BalanceArgs a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    dependent_wait();
+    constexpr int kOf = VEC * NP, kSub = 32 / L;  // experts a lane; rows of a warp side by side
+    const int experts = static_cast<int>(a.v.cols), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in = lane % L, sub = lane / L;
+    int32_t* const counts = reinterpret_cast<int32_t*>(smem);
+    float* const sums = reinterpret_cast<float*>(counts + experts);  // [kWarps][experts]
+    __shared__ double lse2[kWarps];
+    __shared__ int32_t live[kWarps];
+    __shared__ int32_t bad;
+    for (int e = threadIdx.x; e < experts; e += kThreads) counts[e] = 0;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    const int64_t group = blockIdx.x / a.runs, run = blockIdx.x % a.runs;
+    const int64_t lo = group * a.length + run * a.run_rows, hi = min(lo + a.run_rows, (group + 1) * a.length);
+    const T* const logits = static_cast<const T*>(a.v.ptr[kBlX]);
+    float acc[kOf];
+#pragma unroll
+    for (int k = 0; k < kOf; ++k) acc[k] = 0.0f;
+    double l2 = 0.0;
+    int n = 0;
+    for (int64_t first = lo + warp * (kSub * ROWS); first < hi; first += kWarps * kSub * ROWS) {
+        HeldRow<T, VEC, L, NP> h[ROWS];
+        bool on[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t r = first + i * kSub + sub;
+            on[i] = r < hi && row_counts(a, r);
+            h[i].load(logits + (on[i] ? row_offset(a.v, kBlX, r) : 0), in, on[i] ? experts : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t r = first + i * kSub + sub;
+            float m = h[i].x[0];
+#pragma unroll
+            for (int k = 1; k < kOf; ++k) m = fmaxf(m, h[i].x[k]);
+            m = lanes_max<L>(m);
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kOf; ++k) {
+                // an expert that there is none of must stay out of a row without a softmax too
+                const bool there = ((k / VEC) * L + in) * VEC + k % VEC < experts;
+                h[i].x[k] = there ? exp_approx(h[i].x[k] - m) : 0.0f;
+                s += h[i].x[k];
+            }
+            s = lanes_sum<L>(s);
+            if (!on[i]) continue;
+            const float inv = 1.0f / s;
+#pragma unroll
+            for (int k = 0; k < kOf; ++k) acc[k] = fmaf(h[i].x[k], inv, acc[k]);
+            if (in == 0) {
+                a.row_stats[r] = make_float2(m, s);
+                const double lse = static_cast<double>(m + logf(s));
+                l2 += lse * lse;
+                ++n;
+            }
+            const int64_t at = row_offset(a.v, kBlExperts, r);
+            for (int64_t k = in; k < a.chosen; k += L) {
+                const int64_t e = index_at(a.v.ptr[kBlExperts], a.v.dtype[kBlExperts], at + k * a.v.inner[kBlExperts]);
+                if (e >= 0 && e < experts) {
+                    atomicAdd(counts + e, 1);  // integers: any order gives the same
+                } else {
+                    bad = 1;
+                    record_bad_index(a.status, e);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    // the warp's groups of lanes, then its warps
+#pragma unroll
+    for (int k = 0; k < kOf; ++k)
+#pragma unroll
+        for (int d = L; d < 32; d <<= 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], d);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+        l2 += __shfl_xor_sync(0xffffffffu, l2, d);
+        n += __shfl_xor_sync(0xffffffffu, n, d);
+    }
+    if (sub == 0) {
+#pragma unroll
+        for (int k = 0; k < kOf; ++k) {
+            const int e = ((k / VEC) * L + in) * VEC + k % VEC;
+            if (e < experts) sums[warp * experts + e] = acc[k];
+        }
+    }
+    if (lane == 0) {
+        lse2[warp] = l2;
+        live[warp] = n;
+    }
+    __syncthreads();
+    put_run(a, counts, sums, lse2, live, bad);
+    allow_dependents();
+}
+
+template <class T, int VEC, int L, int NP, int ROWS>
+__global__ void __launch_bounds__(kThreads) balance_grad_held(BalanceArgs a) {
+    dependent_wait();
+    if (a.loss && blockIdx.x == 0 && threadIdx.x < 32) put_loss(a);
+    constexpr int kOf = VEC * NP, kSub = 32 / L;
+    const int experts = static_cast<int>(a.v.cols), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in = lane % L, sub = lane / L;
+    const int64_t group = blockIdx.x / a.runs, run = blockIdx.x % a.runs;
+    const int64_t lo = group * a.length + run * a.run_rows, hi = min(lo + a.run_rows, (group + 1) * a.length);
+    const T* const logits = static_cast<const T*>(a.v.ptr[kBlX]);
+    T* const grads = static_cast<T*>(a.v.ptr[kBlGrad]);
+    float slope[kOf];
+#pragma unroll
+    for (int k = 0; k < kOf; ++k) {
+        const int e = ((k / VEC) * L + in) * VEC + k % VEC;
+        slope[k] = e < experts ? a.slope[group * experts + e] : 0.0f;
+    }
+    const float f = static_cast<float>(1.0 / (a.group[group].rows * static_cast<double>(a.groups)));
+    const float z2 = static_cast<float>(2.0 * a.z_coef);
+    for (int64_t first = lo + warp * (kSub * ROWS); first < hi; first += kWarps * kSub * ROWS) {
+        HeldRow<T, VEC, L, NP> h[ROWS];
+        float2 stats[ROWS];
+        bool on[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t r = first + i * kSub + sub;
+            on[i] = r < hi && row_counts(a, r);
+            h[i].load(logits + (on[i] ? row_offset(a.v, kBlX, r) : 0), in, on[i] ? experts : 0);
+            stats[i] = on[i] ? a.row_stats[r] : make_float2(0.0f, 1.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t r = first + i * kSub + sub;
+            const float inv = 1.0f / stats[i].y;
+            float dot = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kOf; ++k) {
+                h[i].x[k] = exp_approx(h[i].x[k] - stats[i].x) * inv;
+                const bool there = ((k / VEC) * L + in) * VEC + k % VEC < experts;
+                dot = there ? fmaf(slope[k], h[i].x[k], dot) : dot;
+            }
+            dot = lanes_sum<L>(dot);
+            if (r >= hi) continue;
+            const float up = z2 != 0.0f ? z2 * (stats[i].x + logf(stats[i].y)) : 0.0f;
+            T* const out = grads + row_offset(a.v, kBlGrad, r);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const int e = (q * L + in) * VEC;
+                if (e >= experts) continue;
+                Pack<T, VEC> v;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    v.v[k] = from_float<T>(on[i] ? h[i].x[q * VEC + k] * (slope[q * VEC + k] - dot + up) * f : 0.0f);
+                *reinterpret_cast<Pack<T, VEC>*>(out + e) = v;
+            }
+        }
+    }
+    allow_dependents();
 }
 
 template <class T> __global__ void __launch_bounds__(kThreads) balance_grad(BalanceArgs a) {
     dependent_wait();
     const int experts = static_cast<int>(a.v.cols), lane = threadIdx.x & 31;
-    if (a.loss && blockIdx.x == 0 && threadIdx.x == 0) {
-        double s = 0.0;
-        for (int64_t g = 0; g < a.groups; ++g) s += a.group[g].loss;
-        *a.loss = static_cast<float>(s / static_cast<double>(a.groups));
-    }
+    if (a.loss && blockIdx.x == 0 && threadIdx.x < 32) put_loss(a);
     if (!a.v.ptr[kBlGrad]) return;
     for (int64_t r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < a.v.rows; r += gridDim.x * kWarps) {
         T* const grad = static_cast<T*>(a.v.ptr[kBlGrad]) + row_offset(a.v, kBlGrad, r);
@@ -228,14 +457,14 @@ template <class T> __global__ void __launch_bounds__(kThreads) balance_grad(Bala
 
 struct Layout {
     int64_t runs, run_rows;
-    size_t probs, counts, run, slope, group, bytes;
+    size_t probs, counts, run, slope, group, inner, stats, bytes;
 };
 
 // Runs: enough CTAs for the GPU, of at least 32 rows each.
 Layout lay_out(int64_t rows, int64_t experts, int64_t groups) {
     Layout l;
     const int64_t length = rows / groups;
-    const int64_t want = std::max<int64_t>(1, sm_count() * 2 / groups);
+    const int64_t want = std::max<int64_t>(1, sm_count() * 4 / groups);
     l.run_rows = std::max<int64_t>(32, (length + want - 1) / want);
     l.runs = std::max<int64_t>(1, (length + l.run_rows - 1) / l.run_rows);
     size_t at = 0;
@@ -249,6 +478,8 @@ Layout lay_out(int64_t rows, int64_t experts, int64_t groups) {
     l.run = add(groups * l.runs, sizeof(BalanceRun));
     l.slope = add(groups * experts, 4);
     l.group = add(groups, sizeof(BalanceGroup));
+    l.inner = add(groups * ((experts + 31) / 32), 8);
+    l.stats = add(rows, 8);
     l.bytes = at;
     return l;
 }
@@ -260,24 +491,68 @@ int check_groups(int64_t rows, int64_t groups) {
     return CTB_OK;
 }
 
-template <class T> int run(const BalanceArgs& a, cudaStream_t st) {
-    const size_t smem = static_cast<size_t>(a.v.cols) * 4 * (kWarps + 1);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(balance_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxExperts * 4 * (kWarps + 1));
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return fail(CTB_ERR_CUDA, std::string("balance loss: ") + cudaGetErrorString(e));
-        }
+// 4 where rows of logits and gradient start on 4 elements and are whole packs, 1 where their experts are contiguous, else 0.
+int pack_of(const BalanceArgs& a) {
+    int vec = a.v.cols % 4 ? 1 : 4;
+    for (int s : {static_cast<int>(kBlX), static_cast<int>(kBlGrad)}) {
+        if (!a.v.ptr[s]) continue;
+        if (a.v.inner[s] != 1 && a.v.cols > 1) return 0;
+        const uintptr_t bytes = 4 * dtype_size(a.v.dtype[s]);
+        if (reinterpret_cast<uintptr_t>(a.v.ptr[s]) % bytes) vec = 1;
+        for (int d = 0; d < a.v.rank; ++d)
+            if (a.v.stride[s][d] % 4) vec = 1;
     }
-    launch_dependent(balance_rows<T>, static_cast<unsigned>(a.groups * a.runs), kThreads, smem, st, a);
+    return vec;
+}
+
+int wide_shared(const void* kernel, size_t bytes) {
+    if (bytes <= 47 * 1024) return CTB_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxExperts * 4 * (kWarps + 1));
+    if (e == cudaSuccess) return CTB_OK;
+    cudaGetLastError();
+    return fail(CTB_ERR_CUDA, std::string("balance loss: ") + cudaGetErrorString(e));
+}
+
+template <class T, class R, class G> int run(const BalanceArgs& a, R rows, G grad, unsigned grad_grid, cudaStream_t st) {
+    const size_t smem = static_cast<size_t>(a.v.cols) * 4 * (kWarps + 1);
+    CTB_CHECK(wide_shared(reinterpret_cast<const void*>(rows), smem));
+    launch_dependent(rows, static_cast<unsigned>(a.groups * a.runs), kThreads, smem, st, a);
     count_launch();
     CTB_CHECK(check_launch("balance loss"));
-    launch_dependent(balance_join, static_cast<unsigned>(a.groups), kThreads, 0, st, a);
+    launch_dependent(balance_join, static_cast<unsigned>(a.groups * a.chunks), kJoinThreads, 0, st, a);
     count_launch();
     CTB_CHECK(check_launch("balance loss"));
-    launch_dependent(balance_grad<T>, a.v.ptr[kBlGrad] ? grid_for((a.v.rows + kWarps - 1) / kWarps, 8) : 1u, kThreads, 0, st, a);
+    launch_dependent(grad, grad_grid, kThreads, 0, st, a);
     count_launch();
     return check_launch("balance loss");
+}
+
+template <class T, int VEC, int L, int NP> int run_held(const BalanceArgs& a, cudaStream_t st) {
+    constexpr int kRows = VEC * NP >= 16 ? 1 : VEC * NP >= 8 ? 2 : 4;  // 16 experts a lane at a time or more
+    auto grad = balance_grad_held<T, VEC, L, NP, kRows>;
+    // without a gradient the kernel is there for the scalar alone
+    if (!a.v.ptr[kBlGrad]) return run<T>(a, balance_rows_held<T, VEC, L, NP, kRows>, balance_grad<T>, 1u, st);
+    return run<T>(a, balance_rows_held<T, VEC, L, NP, kRows>, grad, static_cast<unsigned>(a.groups * a.runs), st);
+}
+
+template <class T, int VEC> int run_packs(const BalanceArgs& a, cudaStream_t st) {
+    const int64_t packs = (a.v.cols + VEC - 1) / VEC;
+    if (packs <= 2) return run_held<T, VEC, 2, 1>(a, st);
+    if (packs <= 4) return run_held<T, VEC, 4, 1>(a, st);
+    if (packs <= 8) return run_held<T, VEC, 8, 1>(a, st);
+    if (packs <= 16) return run_held<T, VEC, 16, 1>(a, st);
+    if (packs <= 32) return run_held<T, VEC, 32, 1>(a, st);
+    if (packs <= 64) return run_held<T, VEC, 32, 2>(a, st);
+    if (packs <= 128) return run_held<T, VEC, 32, 4>(a, st);
+    if (packs <= 256) return run_held<T, VEC, 32, 8>(a, st);
+    return run<T>(a, balance_rows<T>, balance_grad<T>, a.v.ptr[kBlGrad] ? grid_for((a.v.rows + kWarps - 1) / kWarps, 8) : 1u, st);
+}
+
+template <class T> int run_any(const BalanceArgs& a, cudaStream_t st) {
+    const int vec = pack_of(a);
+    if (vec == 4) return run_packs<T, 4>(a, st);
+    if (vec == 1) return run_packs<T, 1>(a, st);
+    return run<T>(a, balance_rows<T>, balance_grad<T>, a.v.ptr[kBlGrad] ? grid_for((a.v.rows + kWarps - 1) / kWarps, 8) : 1u, st);
 }
 
 }  // namespace
@@ -354,8 +629,11 @@ int ctb_balance_loss(const ctb_view* logits, const ctb_view* experts, const ctb_
         a.run = reinterpret_cast<BalanceRun*>(s + l.run);
         a.slope = reinterpret_cast<float*>(s + l.slope);
         a.group = reinterpret_cast<BalanceGroup*>(s + l.group);
+        a.inner = reinterpret_cast<double*>(s + l.inner);
+        a.row_stats = reinterpret_cast<float2*>(s + l.stats);
+        a.chunks = (a.v.cols + 31) / 32;
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return logits->dtype == CTB_FLOAT32 ? run<float>(a, st) : run<__nv_bfloat16>(a, st);
+        return logits->dtype == CTB_FLOAT32 ? run_any<float>(a, st) : run_any<__nv_bfloat16>(a, st);
     });
 }
 
