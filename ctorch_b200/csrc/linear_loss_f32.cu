@@ -28,47 +28,81 @@ __device__ __forceinline__ void fma2(float2& d, float2 x, float2 y) {
         : "l"(reinterpret_cast<const unsigned long long&>(x)), "l"(reinterpret_cast<const unsigned long long&>(y)));
 }
 
-// This thread's share of a tile of an operand, 2 vectors of 4. INNER: the product's inner dimension is contiguous
-// (rows of the matrix are rows of the tile), otherwise the outer one is. Elements outside are 0.
-template <bool INNER> __device__ __forceinline__ void fetch(float4 (&r)[2], const float* p, int64_t ld, int64_t outer0, int64_t outers,
-                                                            int64_t k0, int64_t k1) {
+constexpr int kLd = kBM + 4;  // of a tile in shared memory, [kBK][kLd]
+
+__device__ __forceinline__ void copy16(float* to, const float* from, int elements) {  // the rest becomes 0
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from),
+                 "r"(elements * 4)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// This thread's share of the tiles of an operand: two vectors of 4, whose addresses move on by a step at a time. Where the
+// product's outer dimension is contiguous they go to shared memory as they lie, asynchronously; where the inner one is
+// (INNER: rows of the matrix are rows of the tile) they pass through registers to be laid out the other way. Elements
+// outside are 0.
+template <bool INNER> struct Share {
+    const float* at;   // of the first vector; the second one is `apart` behind
+    int64_t apart, step;
+    int left[2];       // elements of a vector that exist along the contiguous dimension; INNER: whether its row exists
+    int rest;          // inner indexes left
+    float4 r[INNER ? 2 : 1];
+
+    __device__ __forceinline__ Share(const float* p, int64_t ld, int64_t outer0, int64_t outers, int64_t k0, int64_t k1) {
+        rest = static_cast<int>(k1 - k0);
+        if (INNER) {
+            const int64_t row = outer0 + (threadIdx.x >> 2);
+            apart = 64 * ld;
+            step = kBK;
+            left[0] = row < outers;
+            left[1] = row + 64 < outers;
+            at = p + row * ld + k0 + (threadIdx.x & 3) * 4;
+        } else {
+            const int64_t col = outer0 + (threadIdx.x & 31) * 4;
+            apart = 8 * ld;
+            step = kBK * ld;
+            left[0] = left[1] = static_cast<int>(col + 4 <= outers ? 4 : col < outers ? outers - col : 0);
+            at = p + (k0 + (threadIdx.x >> 5)) * ld + col;
+        }
+    }
+
+    // Sets the next tile's vectors on their way: into `sm`, or into registers until put().
+    __device__ __forceinline__ void fetch(float* sm) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int id = threadIdx.x + i * kThreads;  // 512 vectors
-        const int64_t row = INNER ? outer0 + (id >> 2) : k0 + (id >> 5);
-        const int64_t col = INNER ? k0 + (id & 3) * 4 : outer0 + (id & 31) * 4;
-        const int64_t rows = INNER ? outers : k1, cols = INNER ? k1 : outers;
-        r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (row < rows) {
-            const float* const q = p + row * ld + col;
-            if (col + 4 <= cols) {
-                r[i] = *reinterpret_cast<const float4*>(q);
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (INNER) {
+                const int n = left[i] ? rest - static_cast<int>(threadIdx.x & 3) * 4 : 0;
+                const float* const q = at + i * apart;
+                r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (n >= 4) {
+                    r[i] = *reinterpret_cast<const float4*>(q);
+                } else if (n > 0) {
+                    r[i].x = q[0];
+                    if (n > 1) r[i].y = q[1];
+                    if (n > 2) r[i].z = q[2];
+                }
             } else {
-                if (col < cols) r[i].x = q[0];
-                if (col + 1 < cols) r[i].y = q[1];
-                if (col + 2 < cols) r[i].z = q[2];
+                const int k = static_cast<int>(threadIdx.x >> 5) + 8 * i, n = k < rest ? left[i] : 0;
+                copy16(sm + k * kLd + (threadIdx.x & 31) * 4, n ? at + i * apart : at - (threadIdx.x & 31) * 4, n);
+            }
+        }
+        at += step;
+        rest -= kBK;
+    }
+
+    __device__ __forceinline__ void put(float* sm) {
+        if constexpr (INNER) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = static_cast<int>(threadIdx.x >> 2) + 64 * i, k = (threadIdx.x & 3) * 4;
+                sm[(k + 0) * kLd + row] = r[i].x;
+                sm[(k + 1) * kLd + row] = r[i].y;
+                sm[(k + 2) * kLd + row] = r[i].z;
+                sm[(k + 3) * kLd + row] = r[i].w;
             }
         }
     }
-}
-
-constexpr int kLd = kBM + 4;  // of a tile in shared memory, [kBK][kLd]
-
-template <bool INNER> __device__ __forceinline__ void put_tile(float* sm, const float4 (&r)[2]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int id = threadIdx.x + i * kThreads;
-        if (INNER) {
-            const int row = id >> 2, k = (id & 3) * 4;
-            sm[(k + 0) * kLd + row] = r[i].x;
-            sm[(k + 1) * kLd + row] = r[i].y;
-            sm[(k + 2) * kLd + row] = r[i].z;
-            sm[(k + 3) * kLd + row] = r[i].w;
-        } else {
-            *reinterpret_cast<float4*>(sm + (id >> 5) * kLd + (id & 31) * 4) = r[i];
-        }
-    }
-}
+};
 
 template <int P> __global__ void __launch_bounds__(kThreads, 2) linear_product_f32(LinearArgs a, ProductF32 p) {
     dependent_wait();
@@ -95,22 +129,24 @@ template <int P> __global__ void __launch_bounds__(kThreads, 2) linear_product_f
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float4 rx[2], ry[2];
+    Share<kXInner> share_x(p.x, p.ldx, i0, m, k0, k1);
+    Share<kYInner> share_y(p.y, p.ldy, j0, p.n, k0, k1);
     if (k0 < k1) {
-        fetch<kXInner>(rx, p.x, p.ldx, i0, m, k0, k1);
-        fetch<kYInner>(ry, p.y, p.ldy, j0, p.n, k0, k1);
-        put_tile<kXInner>(sx[0], rx);
-        put_tile<kYInner>(sy[0], ry);
+        share_x.fetch(sx[0]);
+        share_y.fetch(sy[0]);
+        share_x.put(sx[0]);
+        share_y.put(sy[0]);
+        copies_done();
     }
     __syncthreads();
     int at = 0;
-    for (int64_t kk = k0; kk < k1; kk += kBK) {
-        const bool more = kk + kBK < k1;
+    for (int steps = static_cast<int>((k1 - k0 + kBK - 1) / kBK); steps > 0; --steps) {
+        const bool more = steps > 1;
         if (more) {
-            fetch<kXInner>(rx, p.x, p.ldx, i0, m, kk + kBK, k1);
-            fetch<kYInner>(ry, p.y, p.ldy, j0, p.n, kk + kBK, k1);
+            share_x.fetch(sx[at ^ 1]);
+            share_y.fetch(sy[at ^ 1]);
         }
-#pragma unroll
+#pragma unroll 2
         for (int q = 0; q < kBK; ++q) {
             const float* const xs = sx[at] + q * kLd;
             const float* const ys = sy[at] + q * kLd;
@@ -124,8 +160,9 @@ template <int P> __global__ void __launch_bounds__(kThreads, 2) linear_product_f
                 for (int j = 0; j < 4; ++j) fma2(acc[i][j], make_float2(xv[i], xv[i]), yv[j]);
         }
         if (more) {
-            put_tile<kXInner>(sx[at ^ 1], rx);
-            put_tile<kYInner>(sy[at ^ 1], ry);
+            share_x.put(sx[at ^ 1]);
+            share_y.put(sy[at ^ 1]);
+            copies_done();
         }
         __syncthreads();
         at ^= 1;
