@@ -197,9 +197,14 @@ __global__ void __launch_bounds__(1024) norm_grad_weight(NormGradArgs a) {
 // A group of G threads has a row, NP packs of VEC elements a thread: pack q of thread t is columns (q G + t) VEC and
 // on. Groups of one warp share a CTA of 128 threads, larger ones are a CTA. A row is read once and written once; what
 // keeps reads on their way while other rows are reduced is the number of groups an SM holds.
+constexpr int kRingPacks = 2048;  // of a row that passes through shared memory: longer ones do not fit it
+
 template <int G> constexpr int group_threads() { return G == 32 ? 128 : G; }
-// CTAs an SM that the registers have to leave room for: 1024 threads (64 registers each), 768 backward (80).
+// CTAs an SM that the registers have to leave room for: 768 threads (80 registers each), 1024 in two groups of 512; 512
+// (128) in backward passes whose rows start anywhere.
 template <int G> constexpr int group_ctas(int threads) { return threads / group_threads<G>() > 1 ? threads / group_threads<G>() : 1; }
+template <int G> constexpr int forward_ctas() { return G == 512 ? 2 : group_ctas<G>(768); }
+template <int G, bool ODD> constexpr int backward_ctas() { return group_ctas<G>(ODD ? 512 : 768); }
 
 // The sum (or maximum) over the group; `turn` alternates between calls, so one barrier a call is enough.
 template <int G, bool MAX> __device__ __forceinline__ float group_join(float x, float (&sm)[2][32], int& turn) {
@@ -354,9 +359,14 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(1024)) norm_
 // kRing - 1 rows ahead (cp.async) and is the only one to read them, so nothing but the row's sum waits for other threads,
 // and the bytes on their way do not take registers. B200, 16384 x 4096 bfloat16 with a residual: 106 us with the rows in
 // registers, see the table of cases for this.
-// Stages of the ring for `arrays` matrices: three, or two where they would not fit (16384 columns backward).
-template <int G, int NP> constexpr int ring_stages(int arrays) { return 3 * arrays * NP * 16 * group_threads<G>() <= 200 * 1024 ? 3 : 2; }
-template <int G, int NP> constexpr int ring_bytes(int arrays) { return ring_stages<G, NP>(arrays) * arrays * NP * 16 * group_threads<G>(); }
+// Stages of the ring for `arrays` matrices: what the CTAs that an SM holds have room for, two at least and eight at most.
+// What is on its way has to cover the memory's latency whatever the group (B200, 16384 x 4095 bfloat16, one
+// CTA an SM: 279 us with three stages).
+template <int G, int NP> constexpr int ring_stages(int arrays, int ctas) {
+    const int fit = 222 * 1024 / ctas / (arrays * NP * 16 * group_threads<G>());
+    return fit < 2 ? 2 : fit > 8 ? 8 : fit;
+}
+template <int G, int NP> constexpr int ring_bytes(int arrays, int ctas) { return ring_stages<G, NP>(arrays, ctas) * arrays * NP * 16 * group_threads<G>(); }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
@@ -371,81 +381,222 @@ template <class T, int VEC> __device__ __forceinline__ Pack<T, VEC> ring_pack(ui
     return v;
 }
 
-template <class T, int VEC, int G, int NP, bool RES, int QUANT>
-__global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_rows_ring(NormArgs a) {
+// The rows and columns of a group of threads. ODD: rows start anywhere, all matrices' alike; packs are those of memory, so
+// the first and the last one of a row may be in part its neighbours': they are read whole, but for the first row's first
+// and the last row's last one, which might reach out of the matrix, and written element by element. How far a row
+// starts behind a pack repeats every `period` rows (a power of two), and a group takes rows of one kind: its columns,
+// and with them its weights and sums of grad_weight, stay the same.
+template <int VEC, int G, bool ODD> struct Share {
+    int64_t lo, hi, first, period;  // rows first + period * [lo, hi)
+    int behind;                     // elements from a pack's start to the row's
+
+    __device__ __forceinline__ Share(int64_t rows, int64_t group, int64_t groups, int base, int64_t stride) {
+        first = 0;
+        period = 1;
+        behind = 0;
+        if (ODD) {
+            const int off = static_cast<int>(stride & (VEC - 1));
+            while ((off * static_cast<int>(period)) & (VEC - 1)) period *= 2;
+            first = group & (period - 1);
+            group /= period;
+            groups /= period;
+            rows = (rows - first + period - 1) / period;  // at most period - 1 groups may have none
+            if (rows < 0) rows = 0;
+            behind = (base + off * static_cast<int>(first)) & (VEC - 1);
+        }
+        lo = rows * group / groups;
+        hi = rows * (group + 1) / groups;
+    }
+    __device__ __forceinline__ int64_t row(int64_t i) const { return ODD ? first + period * i : i; }
+    __device__ __forceinline__ int column(int pack) const { return pack * VEC - behind; }
+    // 2: all of the pack is the row's, 1: a part, 0: nothing
+    __device__ __forceinline__ int kind(int j, int cols) const {
+        if (!ODD) return j < cols ? 2 : 0;
+        return j >= 0 && j + VEC <= cols ? 2 : j + VEC > 0 && j < cols ? 1 : 0;
+    }
+};
+
+// A thread's pack of a row on its way into its place in the ring. What may reach out of the matrix (before its first row,
+// behind its last one) is read element by element at once.
+template <class T, int VEC, bool ODD>
+__device__ __forceinline__ void fetch_pack(uint32_t to, const T* row, int kind, int j, int cols, int64_t r, int64_t rows) {
+    if (!kind) return;
+    if (!ODD || kind == 2 || ((j >= 0 || r > 0) && (j + VEC <= cols || r + 1 < rows))) {
+        copy16(to, row + j);
+        return;
+    }
+#pragma unroll 1
+    for (int e = 0; e < VEC; ++e)
+        if (j + e >= 0 && j + e < cols) {
+            if constexpr (sizeof(T) == 4) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + e * 4), "f"(row[j + e]) : "memory");
+            else asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + e * 2), "h"(*reinterpret_cast<const uint16_t*>(row + j + e)) : "memory");
+        }
+}
+
+// The pack; what is not the row's is 0.
+template <class T, int VEC, bool ODD> __device__ __forceinline__ Pack<T, VEC> take_pack(uint32_t at, int kind, int j, int cols) {
+    Pack<T, VEC> v = ring_pack<T, VEC>(at);
+    if (ODD && kind == 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v.v[e] = j + e >= 0 && j + e < cols ? v.v[e] : from_float<T>(0.0f);
+    }
+    return v;
+}
+
+// Writes a pack; one that is in part the row's element by element, by way of the thread's place `at` in the ring (a loop, not
+// VEC copies of it: rows pass faster when their code fits the instruction cache).
+template <class T, int VEC, bool ODD>
+__device__ __forceinline__ void put_pack(int kind, T* row, int j, int cols, const Pack<T, VEC>& v, uint32_t at) {
+    if (!ODD || kind == 2) {
+        if constexpr (sizeof(T) * VEC >= 16) store_pack_split<T, VEC>(row + j, v);
+        else *reinterpret_cast<Pack<T, VEC>*>(row + j) = v;
+        return;
+    }
+    const uint32_t* const u = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(sizeof(v)) / 4; ++k) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + k * 4), "r"(u[k]) : "memory");
+#pragma unroll 1
+    for (int e = max(0, -j); e < min(VEC, cols - j); ++e) {
+        uint32_t x;
+        if constexpr (sizeof(T) == 4) {
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at + e * 4) : "memory");
+            *reinterpret_cast<uint32_t*>(row + j + e) = x;
+        } else if constexpr (sizeof(T) == 2) {
+            uint16_t y;
+            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(y) : "r"(at + e * 2) : "memory");
+            *reinterpret_cast<uint16_t*>(row + j + e) = y;
+        } else {
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(at + e) : "memory");
+            *reinterpret_cast<uint8_t*>(row + j + e) = static_cast<uint8_t>(x);
+        }
+    }
+}
+template <class T, int VEC, bool ODD>
+__device__ __forceinline__ void weights_of_pack(float (&w)[VEC], const void* p, int dt, int64_t stride, bool whole, int j, int cols) {
+    if constexpr (ODD) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] = j + e >= 0 && j + e < cols ? weight_at(p, dt, (j + e) * stride) : 0.0f;
+    } else {
+        read_weights<T, VEC>(w, p, dt, stride, whole, j);
+    }
+}
+template <class T, int VEC> __device__ __forceinline__ int elements_behind(const void* p) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(T) & (VEC - 1));
+}
+
+template <class T, int VEC, int G, int NP, bool RES, int QUANT, bool ODD>
+__global__ void __launch_bounds__(group_threads<G>(), forward_ctas<G>()) norm_rows_ring(NormArgs a) {
     extern __shared__ __align__(16) unsigned char ring[];
     dependent_wait();
     __shared__ float sm[2][32];
     int turn = 0;
     const RowViews<kNmViews>& v = a.v;
-    constexpr int kGroups = group_threads<G>() / G, kArrays = RES ? 2 : 1, kRing = ring_stages<G, NP>(kArrays);
+    __shared__ uint32_t block_tops[2][group_threads<G>() / G][ODD && QUANT == 2 ? kRingPacks * VEC / kScaleBlock + 1 : 1];
+    int turns = 0;
+    if (ODD && QUANT == 2) {
+        for (int k = threadIdx.x % G; k <= v.cols / kScaleBlock; k += G) block_tops[0][threadIdx.x / G][k] = 0u;
+    }
+    constexpr int kGroups = group_threads<G>() / G, kArrays = RES ? 2 : 1, kRing = ring_stages<G, NP>(kArrays, forward_ctas<G>());
     const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
     const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, group = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
-    const int64_t lo = v.rows * group / groups, hi = v.rows * (group + 1) / groups;
+    const Share<VEC, G, ODD> share(v.rows, group, groups, elements_behind<T, VEC>(v.ptr[kNmX]), v.stride[kNmX][0]);
     const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
     constexpr uint32_t kStep = group_threads<G>() * 16;  // from one pack of a thread to its next
-    auto fetch = [&](int64_t r, int stage) {
-        if (r < hi) {
-            const T* const x = static_cast<const T*>(v.ptr[kNmX]) + row_offset(v, kNmX, r) + t * VEC;
-            const T* const res = RES ? static_cast<const T*>(v.ptr[kNmResidual]) + row_offset(v, kNmResidual, r) + t * VEC : nullptr;
+    auto fetch = [&](int64_t i, int stage) {
+        if (i < share.hi) {
+            const int64_t r = share.row(i);
+            const T* const x = static_cast<const T*>(v.ptr[kNmX]) + row_offset(v, kNmX, r);
+            const T* const res = RES ? static_cast<const T*>(v.ptr[kNmResidual]) + row_offset(v, kNmResidual, r) : nullptr;
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
-                if ((q * G + t) * VEC >= cols) continue;
-                copy16(mine + (stage * kArrays * NP + q) * kStep, x + q * G * VEC);
-                if (RES) copy16(mine + (stage * kArrays * NP + NP + q) * kStep, res + q * G * VEC);
+                const int j = share.column(q * G + t), kind = share.kind(j, cols);
+                fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + q) * kStep, x, kind, j, cols, r, v.rows);
+                if (RES) fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + NP + q) * kStep, res, kind, j, cols, r, v.rows);
             }
         }
         copies_commit();
     };
-#pragma unroll
-    for (int s = 0; s < kRing - 1; ++s) fetch(lo + s, s);
+#pragma unroll 1
+    for (int s = 0; s < kRing - 1; ++s) fetch(share.lo + s, s);
     float w[NP][VEC];
 #pragma unroll
     for (int q = 0; q < NP; ++q)
-        if ((q * G + t) * VEC < cols) read_weights<T, VEC>(w[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, (q * G + t) * VEC);
+        if (share.kind(share.column(q * G + t), cols))
+            weights_of_pack<T, VEC, ODD>(w[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, share.column(q * G + t), cols);
     int stage = 0, ahead = kRing - 1;
-    for (int64_t r = lo; r < hi; ++r) {
+    for (int64_t i = share.lo; i < share.hi; ++i) {
+        const int64_t r = share.row(i);
         copies_wait<kRing>();
         Pack<T, VEC> s[NP];
-        T* const kept = RES ? static_cast<T*>(v.ptr[kNmSummed]) + row_offset(v, kNmSummed, r) + t * VEC : nullptr;
+        T* const kept = RES ? static_cast<T*>(v.ptr[kNmSummed]) + row_offset(v, kNmSummed, r) : nullptr;
         float ss = 0.0f;
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
-            if ((q * G + t) * VEC >= cols) continue;
-            s[q] = ring_pack<T, VEC>(mine + (stage * kArrays * NP + q) * kStep);
+            const int j = share.column(q * G + t), kind = share.kind(j, cols);
+            if (!kind) continue;
+            s[q] = take_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + q) * kStep, kind, j, cols);
             if (RES) {
-                const Pack<T, VEC> o = ring_pack<T, VEC>(mine + (stage * kArrays * NP + NP + q) * kStep);
+                const Pack<T, VEC> o = take_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + NP + q) * kStep, kind, j, cols);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) s[q].v[e] = from_float<T>(to_float(s[q].v[e]) + to_float(o.v[e]));
-                store_pack_split<T, VEC>(kept + q * G * VEC, s[q]);
+                put_pack<T, VEC, ODD>(kind, kept, j, cols, s[q], mine + (stage * kArrays * NP + q) * kStep);
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) ss = fmaf(to_float(s[q].v[e]), to_float(s[q].v[e]), ss);
         }
-        fetch(r + kRing - 1, ahead);
+        fetch(i + kRing - 1, ahead);
+        const int taken = stage;
         stage = stage + 1 == kRing ? 0 : stage + 1;
         ahead = ahead + 1 == kRing ? 0 : ahead + 1;
         ss = group_join<G, false>(ss, sm, turn);
         const float rstd = 1.0f / sqrtf(ss / static_cast<float>(cols) + a.eps);
         if (t == 0 && v.ptr[kNmRstd]) static_cast<float*>(v.ptr[kNmRstd])[row_offset(v, kNmRstd, r)] = rstd;
         if constexpr (QUANT == 0) {
-            T* const out = static_cast<T*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r) + t * VEC;
+            T* const out = static_cast<T*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r);
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
-                if ((q * G + t) * VEC >= cols) continue;
+                const int j = share.column(q * G + t), kind = share.kind(j, cols);
+                if (!kind) continue;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) s[q].v[e] = from_float<T>(to_float(s[q].v[e]) * rstd * w[q][e]);
-                store_pack_split<T, VEC>(out + q * G * VEC, s[q]);
+                put_pack<T, VEC, ODD>(kind, out, j, cols, s[q], mine + (taken * kArrays * NP + q) * kStep);
             }
         } else {
             uint8_t* const out = static_cast<uint8_t*>(v.ptr[kNmOut]) + row_offset(v, kNmOut, r);
             float* const scales = static_cast<float*>(v.ptr[kNmScales]) + row_offset(v, kNmScales, r);
             float inv = 0.0f;
+            // packs that reach over 128 columns' borders: the blocks' maxima meet in shared memory (as the bits of numbers that
+            // are not negative, which order like them, NaN above all)
+            constexpr bool kMeet = ODD && QUANT == 2;
+            uint32_t* const tops = kMeet ? block_tops[turns][threadIdx.x / G] : nullptr;
+            if constexpr (kMeet) {
+                for (int k = t; k <= cols / kScaleBlock; k += G) block_tops[turns ^ 1][threadIdx.x / G][k] = 0u;
+                turns ^= 1;
+#pragma unroll
+                for (int q = 0; q < NP; ++q) {
+                    const int j = share.column(q * G + t);
+                    if (!share.kind(j, cols)) continue;
+                    const int left = max(j, 0) / kScaleBlock, border = (left + 1) * kScaleBlock - j;
+                    uint32_t low = 0u, high = 0u;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const uint32_t bits = __float_as_uint(fabsf(to_float(s[q].v[e]) * rstd * w[q][e]));
+                        if (j + e < 0 || j + e >= cols) continue;
+                        if (e < border) low = max(low, bits);
+                        else high = max(high, bits);
+                    }
+                    atomicMax(tops + left, low);
+                    if (border < VEC && j + border < cols) atomicMax(tops + left + 1, high);
+                }
+                if (G > 32) __syncthreads();
+                else __syncwarp();
+                for (int k = t; k * kScaleBlock < cols; k += G) scales[k * v.inner[kNmScales]] = scale_of(__uint_as_float(tops[k]));
+            }
             if (QUANT == 1) {
                 float top = 0.0f;
 #pragma unroll
                 for (int q = 0; q < NP; ++q)
-                    if ((q * G + t) * VEC < cols)
+                    if (share.kind(share.column(q * G + t), cols))
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) top = max_nan(top, fabsf(to_float(s[q].v[e]) * rstd * w[q][e]));
                 const float scale = scale_of(group_join<G, true>(top, sm, turn));
@@ -454,15 +605,24 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_r
             }
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
-                const int j = (q * G + t) * VEC;
-                const bool live = j < cols;
+                const int j = share.column(q * G + t), kind = share.kind(j, cols);
+                const bool live = kind != 0;
                 float y[VEC], top = 0.0f;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     y[e] = live ? to_float(s[q].v[e]) * rstd * w[q][e] : 0.0f;
                     top = max_nan(top, fabsf(y[e]));
                 }
-                if (QUANT == 2) {
+                float inv_high = inv;
+                int border = VEC;
+                if (kMeet) {
+                    if (live) {
+                        const int left = max(j, 0) / kScaleBlock;
+                        border = (left + 1) * kScaleBlock - j;
+                        inv = 1.0f / scale_of(__uint_as_float(tops[left]));
+                        inv_high = border < VEC && j + border < cols ? 1.0f / scale_of(__uint_as_float(tops[left + 1])) : inv;
+                    }
+                } else if (QUANT == 2) {
                     // the threads that have 128 columns are neighbours in a warp
                     constexpr int kShare = kScaleBlock / VEC;
 #pragma unroll
@@ -475,11 +635,12 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_r
                 Pack<uint8_t, VEC> b;
 #pragma unroll
                 for (int e = 0; e < VEC; e += 2) {
-                    const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(y[e] * inv, y[e + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                    const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(y[e] * (kMeet && e >= border ? inv_high : inv), y[e + 1] * (kMeet && e + 1 >= border ? inv_high : inv)),
+                                                                               __NV_SATFINITE, __NV_E4M3);
                     b.v[e] = static_cast<uint8_t>(two);
                     b.v[e + 1] = static_cast<uint8_t>(two >> 8);
                 }
-                *reinterpret_cast<Pack<uint8_t, VEC>*>(out + j) = b;
+                put_pack<uint8_t, VEC, ODD>(kind, out, j, cols, b, mine + (taken * kArrays * NP + q) * kStep);
             }
         }
     }
@@ -488,7 +649,7 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_r
 
 // The groups' sums of a CTA's rows, joined in their order, as the CTA's row of partial sums.
 template <int VEC, int G, int NP>
-__device__ __forceinline__ void put_partial(const NormGradArgs& a, const float (&sums)[NP][VEC], int t, int cols) {
+__device__ __forceinline__ void put_partial(const NormGradArgs& a, const float (&sums)[NP][VEC], int t, int cols, int behind) {
     float* const part = a.partial + static_cast<int64_t>(blockIdx.x) * cols;
     constexpr int kGroups = group_threads<G>() / G;
 #pragma unroll
@@ -499,8 +660,8 @@ __device__ __forceinline__ void put_partial(const NormGradArgs& a, const float (
         for (int q = 0; q < NP; ++q)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int j = (q * G + t) * VEC + e;
-                if (j < cols) part[j] = k > 0 ? part[j] + sums[q][e] : sums[q][e];
+                const int j = (q * G + t) * VEC + e - behind;
+                if (j >= 0 && j < cols) part[j] = k > 0 ? part[j] + sums[q][e] : sums[q][e];
             }
     }
 }
@@ -571,60 +732,65 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_g
             store_pack_split<T, VEC>(grad + j, s[q]);
         }
     }
-    if (a.grad_weight) put_partial<VEC, G, NP>(a, sums, t, cols);
+    if (a.grad_weight) put_partial<VEC, G, NP>(a, sums, t, cols, 0);
     allow_dependents();
 }
 
 // The same with 16-byte packs on their way through shared memory, as norm_rows_ring.
-template <class T, int VEC, int G, int NP, bool PASSED>
-__global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_grad_ring(NormGradArgs a) {
+template <class T, int VEC, int G, int NP, bool PASSED, bool ODD>
+__global__ void __launch_bounds__(group_threads<G>(), backward_ctas<G, ODD>()) norm_grad_ring(NormGradArgs a) {
     extern __shared__ __align__(16) unsigned char ring[];
     dependent_wait();
     __shared__ float sm[2][32];
     int turn = 0;
     const RowViews<kNgViews>& v = a.v;
-    constexpr int kGroups = group_threads<G>() / G, kArrays = PASSED ? 3 : 2, kRing = ring_stages<G, NP>(kArrays);
+    constexpr int kGroups = group_threads<G>() / G, kArrays = PASSED ? 3 : 2, kRing = ring_stages<G, NP>(kArrays, backward_ctas<G, ODD>());
     const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
     const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, group = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
-    const int64_t lo = v.rows * group / groups, hi = v.rows * (group + 1) / groups;
+    const Share<VEC, G, ODD> share(v.rows, group, groups, elements_behind<T, VEC>(v.ptr[kNgUp]), v.stride[kNgUp][0]);
     const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
     constexpr uint32_t kStep = group_threads<G>() * 16;
-    auto fetch = [&](int64_t r, int stage) {
-        if (r < hi) {
-            const T* const up = static_cast<const T*>(v.ptr[kNgUp]) + row_offset(v, kNgUp, r) + t * VEC;
-            const T* const x = static_cast<const T*>(v.ptr[kNgSummed]) + row_offset(v, kNgSummed, r) + t * VEC;
-            const T* const p = PASSED ? static_cast<const T*>(v.ptr[kNgPassed]) + row_offset(v, kNgPassed, r) + t * VEC : nullptr;
+    auto row_of = [&](int slot, int64_t r) { return static_cast<const T*>(v.ptr[slot]) + row_offset(v, slot, r); };
+    auto fetch = [&](int64_t i, int stage) {
+        if (i < share.hi) {
+            const int64_t r = share.row(i);
+            const T* const up = row_of(kNgUp, r);
+            const T* const x = row_of(kNgSummed, r);
+            const T* const p = PASSED ? row_of(kNgPassed, r) : nullptr;
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
-                if ((q * G + t) * VEC >= cols) continue;
-                copy16(mine + (stage * kArrays * NP + q) * kStep, up + q * G * VEC);
-                copy16(mine + (stage * kArrays * NP + NP + q) * kStep, x + q * G * VEC);
-                if (PASSED) copy16(mine + (stage * kArrays * NP + 2 * NP + q) * kStep, p + q * G * VEC);
+                const int j = share.column(q * G + t), kind = share.kind(j, cols);
+                fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + q) * kStep, up, kind, j, cols, r, v.rows);
+                fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + NP + q) * kStep, x, kind, j, cols, r, v.rows);
+                if (PASSED) fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + 2 * NP + q) * kStep, p, kind, j, cols, r, v.rows);
             }
         }
         copies_commit();
     };
-#pragma unroll
-    for (int s = 0; s < kRing - 1; ++s) fetch(lo + s, s);
+#pragma unroll 1
+    for (int s = 0; s < kRing - 1; ++s) fetch(share.lo + s, s);
     float w[NP][VEC], sums[NP][VEC];
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
-        if ((q * G + t) * VEC < cols) read_weights<T, VEC>(w[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, (q * G + t) * VEC);
+        if (share.kind(share.column(q * G + t), cols))
+            weights_of_pack<T, VEC, ODD>(w[q], a.weight, a.weight_dtype, a.weight_stride, a.weight_whole, share.column(q * G + t), cols);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sums[q][e] = 0.0f;
     }
     const float* const rstds = static_cast<const float*>(v.ptr[kNgRstd]);
-    float rstd = lo < hi ? rstds[row_offset(v, kNgRstd, lo)] : 0.0f;
+    float rstd = share.lo < share.hi ? rstds[row_offset(v, kNgRstd, share.row(share.lo))] : 0.0f;
     int stage = 0, ahead = kRing - 1;
-    for (int64_t r = lo; r < hi; ++r) {
+    for (int64_t i = share.lo; i < share.hi; ++i) {
+        const int64_t r = share.row(i);
         copies_wait<kRing>();
         Pack<T, VEC> g[NP], s[NP];
         float dot = 0.0f;
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
-            if ((q * G + t) * VEC >= cols) continue;
-            g[q] = ring_pack<T, VEC>(mine + (stage * kArrays * NP + q) * kStep);
-            s[q] = ring_pack<T, VEC>(mine + (stage * kArrays * NP + NP + q) * kStep);
+            const int j = share.column(q * G + t), kind = share.kind(j, cols);
+            if (!kind) continue;
+            g[q] = take_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + q) * kStep, kind, j, cols);
+            s[q] = take_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + NP + q) * kStep, kind, j, cols);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float up = to_float(g[q].v[e]), hat = to_float(s[q].v[e]) * rstd;
@@ -632,16 +798,18 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_g
                 dot = fmaf(up * w[q][e], hat, dot);
             }
         }
-        const float next = r + 1 < hi ? rstds[row_offset(v, kNgRstd, r + 1)] : 0.0f;
-        fetch(r + kRing - 1, ahead);
+        const float next = i + 1 < share.hi ? rstds[row_offset(v, kNgRstd, share.row(i + 1))] : 0.0f;
+        fetch(i + kRing - 1, ahead);
         ahead = ahead + 1 == kRing ? 0 : ahead + 1;
         dot = group_join<G, false>(dot, sm, turn) / static_cast<float>(cols);
-        T* const grad = static_cast<T*>(v.ptr[kNgGradX]) + row_offset(v, kNgGradX, r) + t * VEC;
+        T* const grad = static_cast<T*>(v.ptr[kNgGradX]) + row_offset(v, kNgGradX, r);
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
-            if ((q * G + t) * VEC >= cols) continue;
+            const int j = share.column(q * G + t), kind = share.kind(j, cols);
+            if (!kind) continue;
             Pack<T, VEC> p;
-            if (PASSED) p = ring_pack<T, VEC>(mine + (stage * kArrays * NP + 2 * NP + q) * kStep);
+            if (PASSED)
+                p = take_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + 2 * NP + q) * kStep, kind, j, cols);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float hat = to_float(s[q].v[e]) * rstd;
@@ -649,12 +817,12 @@ __global__ void __launch_bounds__(group_threads<G>(), group_ctas<G>(768)) norm_g
                 if (PASSED) y += to_float(p.v[e]);
                 s[q].v[e] = from_float<T>(y);
             }
-            store_pack_split<T, VEC>(grad + q * G * VEC, s[q]);
+            put_pack<T, VEC, ODD>(kind, grad, j, cols, s[q], mine + (stage * kArrays * NP + q) * kStep);
         }
         stage = stage + 1 == kRing ? 0 : stage + 1;
         rstd = next;
     }
-    if (a.grad_weight) put_partial<VEC, G, NP>(a, sums, t, cols);
+    if (a.grad_weight) put_partial<VEC, G, NP>(a, sums, t, cols, share.behind);
     allow_dependents();
 }
 
@@ -686,28 +854,51 @@ template <int N> int pack_of(const RowViews<N>& v, std::initializer_list<int> sl
     return vec;
 }
 
-// Calls f(group, packs a thread) for the smallest group that holds `packs`, as compile-time numbers; false where none does
-// (eight 16-byte packs a thread do not fit the 64 registers that 1024 threads have).
-template <int VEC, class F> bool with_group(int64_t packs, F&& f) {
-    if (packs <= 32) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
-    else if (packs <= 64) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 128) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 256) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 512) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 1024) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 2048) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
-    else if (packs <= 4096) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
-    else if (packs > 8192 || VEC > 1) return false;
-    else if constexpr (VEC == 1) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
+// Whether all rows of the given matrices start equally far behind a pack (16 bytes of the rows' type), with unit strides along
+// and one stride across: packs of memory then serve all of them.
+template <int N> bool alike(const RowViews<N>& v, std::initializer_list<int> slots) {
+    if (v.rank != 1) return false;
+    const int64_t size = static_cast<int64_t>(dtype_size(v.dtype[0])), vec = 16 / size;
+    const int64_t base = reinterpret_cast<uintptr_t>(v.ptr[0]) / size % vec;
+    for (int s : slots) {
+        if (!v.ptr[s]) continue;
+        const int64_t own = static_cast<int64_t>(dtype_size(v.dtype[s]));
+        if (reinterpret_cast<uintptr_t>(v.ptr[s]) % own || static_cast<int64_t>(reinterpret_cast<uintptr_t>(v.ptr[s]) / own % vec) != base ||
+            ((v.stride[s][0] - v.stride[0][0]) & (vec - 1)) || (v.rows > 1 && v.stride[s][0] < v.cols))
+            return false;
+    }
     return true;
 }
 
-constexpr int kRingPacks = 2048;  // of a row that passes through shared memory: longer ones do not fit it
+// Calls f(group, packs a thread) for the smallest group that holds `packs`, as compile-time numbers; false where none does. A
+// thread has 16 elements at most, so that a backward pass has room for their weights and sums; longer rows are held by 1024
+// threads of up to 8 packs.
+template <int VEC, class F> bool with_group(int64_t packs, F&& f) {
+    auto take = [&](auto g, auto np) {
+        if (packs > static_cast<int64_t>(g) * np) return false;
+        f(g, np);
+        return true;
+    };
+#define CTB_TAKE(G, NP) take(std::integral_constant<int, G>{}, std::integral_constant<int, NP>{})
+    if constexpr (VEC == 4) {
+        return CTB_TAKE(32, 1) || CTB_TAKE(32, 2) || CTB_TAKE(32, 4) || CTB_TAKE(64, 4) || CTB_TAKE(128, 3) || CTB_TAKE(128, 4) ||
+               CTB_TAKE(256, 3) || CTB_TAKE(256, 4) || CTB_TAKE(512, 3) || CTB_TAKE(512, 4) || CTB_TAKE(1024, 4);
+    } else if constexpr (VEC == 8) {
+        return CTB_TAKE(32, 1) || CTB_TAKE(32, 2) || CTB_TAKE(64, 2) || CTB_TAKE(128, 2) || CTB_TAKE(256, 2) || CTB_TAKE(512, 2) ||
+               CTB_TAKE(1024, 2) || CTB_TAKE(1024, 4);
+    } else {
+        return CTB_TAKE(32, 2) || CTB_TAKE(128, 2) || CTB_TAKE(256, 2) || CTB_TAKE(512, 2) || CTB_TAKE(1024, 2) || CTB_TAKE(1024, 4) ||
+               CTB_TAKE(1024, 8);
+    }
+#undef CTB_TAKE
+}
 
-// CTAs an SM in a grid: what is resident (768 threads, so 80 registers a thread), or eight times that in one-type norms,
-// where the SMs do not all stream alike (B200, 16384 x 4096 with a residual: 89 us, 96 without; to 8 bits with a
+// CTAs an SM in a grid: what is resident, or eight times that where several groups share an SM and no row waits for a
+// second sum and there are enough of them: the SMs do not all stream alike (B200, 16384 x 4096 with a residual: 89 us, 96 without; to 8 bits with a
 // scale for every 128 columns, 8192 x 8192, the other way round: 123 against 109).
-int norm_ctas(int threads, int quant) { return std::max(1, 768 / threads) * (quant ? 1 : 8); }
+int norm_grid(int resident, int quant, int64_t rows) {
+    return resident > 2 && !quant && rows >= static_cast<int64_t>(sm_count()) * resident * 16 ? 8 * resident : resident;
+}
 
 // Starts a kernel whose rows pass through shared memory, `per_sm` CTAs an SM at most.
 template <class A, class K> void launch_ring(K kernel, const A& a, unsigned grid, int threads, int bytes, cudaStream_t st) {
@@ -715,17 +906,20 @@ template <class A, class K> void launch_ring(K kernel, const A& a, unsigned grid
     launch_dependent(kernel, grid, threads, bytes, st, a);
 }
 
-template <class T, int VEC> bool run_norm_held(const NormArgs& a, cudaStream_t st) {
-    return with_group<VEC>((a.v.cols + VEC - 1) / VEC, [&](auto g, auto np) {
+template <class T, int VEC, bool ODD> bool run_norm_held(const NormArgs& a, cudaStream_t st) {
+    const int64_t packs = ODD ? (a.v.cols + 2 * VEC - 2) / VEC : (a.v.cols + VEC - 1) / VEC;
+    if (ODD && packs > kRingPacks) return false;
+    return with_group<VEC>(packs, [&](auto g, auto np) {
         constexpr int G = decltype(g)::value, NP = decltype(np)::value, threads = group_threads<G>(), groups = threads / G;
         const bool res = a.v.ptr[kNmResidual] != nullptr;
-        const unsigned grid = grid_for((a.v.rows + groups - 1) / groups, VEC > 1 && G * NP <= kRingPacks ? norm_ctas(threads, a.quant) : 64);
-        auto launch = [&](auto kernel, int arrays) { launch_ring(kernel, a, grid, threads, ring_bytes<G, NP>(arrays), st); };
+        unsigned grid = grid_for((a.v.rows + groups - 1) / groups, VEC > 1 && G * NP <= kRingPacks ? norm_grid(forward_ctas<G>(), a.quant, a.v.rows) : 64);
+        if (ODD) grid = grid < VEC ? VEC : grid / VEC * VEC;  // whole periods of kinds of rows
+        auto launch = [&](auto kernel, int arrays) { launch_ring(kernel, a, grid, threads, ring_bytes<G, NP>(arrays, forward_ctas<G>()), st); };
         if constexpr (VEC > 1 && G * NP <= kRingPacks) {
-            if (a.quant == 0) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 0>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 0>, 1);
-            else if (a.quant == 1) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 1>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 1>, 1);
-            else res ? launch(norm_rows_ring<T, VEC, G, NP, true, 2>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 2>, 1);
-        } else {
+            if (a.quant == 0) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 0, ODD>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 0, ODD>, 1);
+            else if (a.quant == 1) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 1, ODD>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 1, ODD>, 1);
+            else res ? launch(norm_rows_ring<T, VEC, G, NP, true, 2, ODD>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 2, ODD>, 1);
+        } else if constexpr (!ODD) {
             if (a.quant == 0) res ? launch(norm_rows_held<T, VEC, G, NP, true, 0>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 0>, 0);
             else if (a.quant == 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 1>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 1>, 0);
             else if constexpr (VEC > 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 2>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 2>, 0);
@@ -736,7 +930,9 @@ template <class T, int VEC> bool run_norm_held(const NormArgs& a, cudaStream_t s
 template <class T> void run_norm(const NormArgs& a, cudaStream_t st) {
     constexpr int kVec = 16 / sizeof(T);
     const int vec = pack_of(a.v, {kNmX, kNmResidual, kNmSummed, kNmOut});
-    const bool held = vec == kVec ? run_norm_held<T, kVec>(a, st) : vec == 1 && a.quant != 2 && run_norm_held<T, 1>(a, st);
+    const bool held = vec == kVec ? run_norm_held<T, kVec, false>(a, st)
+                                  : vec == 1 && ((alike(a.v, {kNmX, kNmResidual, kNmSummed, kNmOut}) && run_norm_held<T, kVec, true>(a, st)) ||
+                                                 (a.quant != 2 && run_norm_held<T, 1, false>(a, st)));
     if (!held) launch_dependent(norm_rows_any<T>, grid_for(a.v.rows, 8), kAnyThreads, 0, st, a);
     count_launch();
 }
@@ -746,24 +942,29 @@ int64_t grad_ctas(int64_t rows, int64_t row_bytes) {
     return std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * (row_bytes <= 4096 ? 6 : row_bytes <= 8192 ? 3 : 2));
 }
 
-template <class T, int VEC> bool run_grad_held(NormGradArgs& a, cudaStream_t st) {
-    return with_group<VEC>((a.v.cols + VEC - 1) / VEC, [&](auto g, auto np) {
+template <class T, int VEC, bool ODD> bool run_grad_held(NormGradArgs& a, cudaStream_t st) {
+    const int64_t packs = ODD ? (a.v.cols + 2 * VEC - 2) / VEC : (a.v.cols + VEC - 1) / VEC;
+    if (ODD && (packs > kRingPacks || a.ctas < VEC)) return false;
+    return with_group<VEC>(packs, [&](auto g, auto np) {
         constexpr int G = decltype(g)::value, NP = decltype(np)::value;
         const bool passed = a.v.ptr[kNgPassed] != nullptr;
-        constexpr int groups = group_threads<G>() / G, per_sm = 768 / group_threads<G>() > 1 ? 768 / group_threads<G>() : 1;
+        constexpr int groups = group_threads<G>() / G, per_sm = backward_ctas<G, ODD>();
         a.ctas = static_cast<int>(std::min<int64_t>({a.ctas, (a.v.rows + groups - 1) / groups, static_cast<int64_t>(sm_count()) * per_sm}));
+        if (ODD) a.ctas = a.ctas / VEC * VEC > 0 ? a.ctas / VEC * VEC : VEC;  // whole periods of kinds of rows
         auto launch = [&](auto kernel, int arrays) {
-            launch_ring(kernel, a, static_cast<unsigned>(a.ctas), group_threads<G>(), ring_bytes<G, NP>(arrays), st);
+            launch_ring(kernel, a, static_cast<unsigned>(a.ctas), group_threads<G>(), ring_bytes<G, NP>(arrays, backward_ctas<G, ODD>()), st);
         };
-        if constexpr (VEC > 1 && G * NP <= kRingPacks) passed ? launch(norm_grad_ring<T, VEC, G, NP, true>, 3) : launch(norm_grad_ring<T, VEC, G, NP, false>, 2);
-        else passed ? launch(norm_grad_held<T, VEC, G, NP, true>, 0) : launch(norm_grad_held<T, VEC, G, NP, false>, 0);
+        if constexpr (VEC > 1 && G * NP <= kRingPacks) passed ? launch(norm_grad_ring<T, VEC, G, NP, true, ODD>, 3) : launch(norm_grad_ring<T, VEC, G, NP, false, ODD>, 2);
+        else if constexpr (!ODD) passed ? launch(norm_grad_held<T, VEC, G, NP, true>, 0) : launch(norm_grad_held<T, VEC, G, NP, false>, 0);
     });
 }
 
 template <class T> void run_grad(NormGradArgs& a, cudaStream_t st) {
     constexpr int kVec = 16 / sizeof(T);
     const int vec = pack_of(a.v, {kNgUp, kNgSummed, kNgPassed, kNgGradX});
-    const bool held = vec == kVec ? run_grad_held<T, kVec>(a, st) : vec == 1 && run_grad_held<T, 1>(a, st);
+    const bool held = vec == kVec ? run_grad_held<T, kVec, false>(a, st)
+                                  : vec == 1 && ((alike(a.v, {kNgUp, kNgSummed, kNgPassed, kNgGradX}) && run_grad_held<T, kVec, true>(a, st)) ||
+                                                 run_grad_held<T, 1, false>(a, st));
     if (!held) launch_dependent(norm_grad_any<T>, static_cast<unsigned>(a.ctas), kAnyThreads, 0, st, a);
     count_launch();
 }
