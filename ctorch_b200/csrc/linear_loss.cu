@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kOrderThreads) linear_order(LinearArgs a) {
         const double w = row_weight(a, r);
         if (w != 0.0) {
             ++mine;
-            top = fmaxf(top, static_cast<float>(fabs(w)));
+            top = fmaxf(top, fminf(fmaxf(static_cast<float>(fabs(w)), 1.17549435e-38f), 3.4e38f));  // a divisor in any case
         }
     }
     counts[threadIdx.x] = mine;

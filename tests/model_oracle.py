@@ -107,8 +107,9 @@ def head(hidden, weight, targets, weights, z_coef=0.0, temperature=1.0, grad=Tru
         sums = (rows / 16 + 1) * 4 * U if half_g else (rows + 1) * U
         bw = half(hidden.dtype) * gw.abs() + math.sqrt(alike) * spread * torch.sqrt((g * g).T @ (h * h)) + \
             ((rel[:, None] * mag).T @ h.abs() + sums * (mag.T @ h.abs()) + (least * h.abs()).sum(0))
-        out["grad_hidden"] = (gh.view(hidden.shape), bh.view(hidden.shape))
-        out["grad_weight"] = (gw, bw)
+        # what is too small for the results' own type: half of bfloat16's least number (float32's is smaller)
+        out["grad_hidden"] = (gh.view(hidden.shape), bh.view(hidden.shape) + 2.0 ** -134)
+        out["grad_weight"] = (gw, bw + 2.0 ** -134)
         # the norm of both if every logit's gradient were its row's weight at the target
         out["unit_grad_hidden"] = float(((hot @ w) * torch.where(on, share, 0.0)[:, None]).norm()) / temperature
         out["unit_grad_weight"] = float((h * torch.where(on, share, 0.0)[:, None]).norm()) / temperature

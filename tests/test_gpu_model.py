@@ -308,6 +308,58 @@ def test_head_bad_targets_and_values(kind):
     check_head(cb().linear_cross_entropy(far, w, t), O.head(far, w, t, None), kind)
 
 
+@pytest.mark.parametrize("kind", list(KIND))
+def test_head_weights_of_any_size(kind):
+    """float64 weights far below float32's numbers count, and add nothing that a float32 could hold."""
+    g = gen(14)
+    h, w, t = head_inputs(g, 90, 64, 301, kind)
+    tiny = torch.full((90,), 1e-50, dtype=torch.float64, device="cuda")
+    r = cb().linear_cross_entropy(h, w, t, weights=tiny)
+    assert float(r.loss) == 0 and (r.grad_hidden == 0).all() and (r.grad_weight == 0).all() and torch.isfinite(r.row_loss).all()
+    tiny[::3] = 0.5
+    check_head(cb().linear_cross_entropy(h, w, t, weights=tiny), O.head(h, w, t, tiny), kind)
+    signs = torch.where(torch.arange(90, device="cuda") % 2 == 0, 1.0, -0.25)
+    check_head(cb().linear_cross_entropy(h, w, t, weights=signs), O.head(h, w, t, signs), kind)
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+def test_a_single_row_without_leading_dims(kind):
+    g = gen(15)
+    h, w, t = head_inputs(g, 1, 72, 301, kind)
+    r = cb().linear_cross_entropy(h[0], w, t[0])
+    assert r.row_loss.shape == () and r.grad_hidden.shape == (72,)
+    check_head(r, O.head(h[0], w, t[0], None), kind)
+    for quant in (None, "row", "block"):
+        n = cb().rms_norm(h[0], w[0], residual=w[1], quant=quant)
+        assert n.rstd.shape == () and n.out.shape == (72,)
+        check_norm(n, h[0], w[1], w[0], 1e-6, quant, KIND[kind])
+    one = cb().balance_loss(h[0], torch.tensor([3, 5], device="cuda"))
+    check_balance(one, O.balance(h, torch.tensor([[3, 5]], device="cuda"), None, 1, 0.01, 0.0) | {"grad": tuple(
+        v[0] for v in O.balance(h, torch.tensor([[3, 5]], device="cuda"), None, 1, 0.01, 0.0)["grad"])})
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("rows,dim", [(2000, 255), (700, 1001), (300, 4093), (40, 8191), (30, 16383)])
+def test_norm_every_row_of_odd_ones(rows, dim, kind):
+    """Rows that start anywhere, many to a group of threads, next to rows of NaN: packs of memory that two rows share."""
+    g, t = gen(rows), KIND[kind]
+    x, res, up, passed = (normal(g, rows, dim, dtype=t) for _ in range(4))
+    w = (1 + 0.3 * normal(g, dim)).to(t)
+    x[5::7] = NAN
+    fine = ~torch.isnan(x[:, 0])
+    for quant in (None, "row", "block"):
+        r = cb().rms_norm(x, w, residual=res, quant=quant)
+        assert torch.isnan(r.out[~fine].float()).all() and torch.isnan(r.rstd[~fine]).all()
+        check_norm(type(r)(r.out[fine], r.summed[fine], r.rstd[fine], None if quant is None else r.scales[fine]), x[fine], res[fine], w,
+                   1e-6, quant, t)
+    x = torch.where(fine[:, None], x, 1.0).to(t)
+    f = cb().rms_norm(x, w)
+    b = cb().rms_norm_backward(up, x, w, f.rstd, grad_summed=passed)
+    gx, bx, gw, bw = O.norm_grad(up, x, w, 1e-6, passed)
+    near(b.grad_x, (gx, bx + O.half(t) * gx.abs() + 1e-38), "grad_x")
+    near(b.grad_weight, (gw, bw + O.half(w.dtype) * gw.abs() + 1e-38), "grad_weight")
+
+
 def test_head_against_differences():
     g = gen(9)
     h, w, t = normal(g, 5, 6, dtype=torch.float64), normal(g, 11, 6, dtype=torch.float64), torch.tensor([0, 10, 3, 3, 7], device="cuda")
@@ -498,6 +550,27 @@ def test_a_step(kind):
     graph.replay()
     for k in out:
         assert torch.equal(out[k], got[k]), k
+
+
+def test_python_front_refusals():
+    c = cb()
+    g = gen(40)
+    x, w = normal(g, 6, 16), normal(g, 16)
+    W, t = normal(g, 9, 16), torch.zeros(6, dtype=torch.int64, device="cuda")
+    for error, f in ((c.DTypeError, lambda: c.rms_norm(x.double(), w)), (c.DTypeError, lambda: c.rms_norm(x.int(), w)),
+                     (c.ShapeError, lambda: c.rms_norm(x[0, 0], w)), (ValueError, lambda: c.rms_norm(x, w, quant="rows")),
+                     (ValueError, lambda: c.rms_norm(x, w, out_summed=x)), (ValueError, lambda: c.rms_norm(x, w, quant="row", out=x)),
+                     (c.AliasError, lambda: c.rms_norm(x[:, :8], w[:8], out=x[:, 4:12])), (c.AliasError, lambda: c.rms_norm(x, w, residual=W[:6], out=W[:6])),
+                     (c.DeviceError, lambda: c.rms_norm(x, w.cpu())), (c.DTypeError, lambda: c.linear_cross_entropy(x, W.bfloat16(), t)),
+                     (c.AliasError, lambda: c.linear_cross_entropy(x, W, t, out_grad_hidden=x)),
+                     (c.AliasError, lambda: c.linear_cross_entropy(x, W, t, out_grad_weight=W)),
+                     (c.ShapeError, lambda: c.linear_cross_entropy(x, W, t, out_grad_weight=W[:8].clone())),
+                     (c.ShapeError, lambda: c.linear_cross_entropy(x, W[:, :8], t)), (ValueError, lambda: c.linear_cross_entropy(x, W, t, temperature=0.0)),
+                     (c.ShapeError, lambda: c.balance_loss(x, t[:, None], groups=4)), (ValueError, lambda: c.balance_loss(x, t[:, None], groups=0)),
+                     (c.DTypeError, lambda: c.balance_loss(x, t[:, None].float())), (c.AliasError, lambda: c.balance_loss(x[:, :8], t[:, None], out_grad=x[:, 4:12])),
+                     (c.DTypeError, lambda: c.add(c.rms_norm(x, w, quant="row").out, x)), (TypeError, lambda: c.rms_norm(x, 1.0))):
+        with pytest.raises(error):
+            f()
 
 
 def test_streams():
