@@ -495,6 +495,7 @@ __global__ void __launch_bounds__(group_threads<G>(), forward_ctas<G>()) norm_ro
     int turns = 0;
     if (ODD && QUANT == 2) {
         for (int k = threadIdx.x % G; k <= v.cols / kScaleBlock; k += G) block_tops[0][threadIdx.x / G][k] = 0u;
+        __syncwarp();  // a group of one warp meets nowhere else before its first row's maxima
     }
     constexpr int kGroups = group_threads<G>() / G, kArrays = RES ? 2 : 1, kRing = ring_stages<G, NP>(kArrays, forward_ctas<G>());
     const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
