@@ -114,6 +114,7 @@ def _load() -> ctypes.CDLL:
                                            ctypes.POINTER(ctypes.c_int64)]),
         "ctb_debug_last_reduction_kernel": (i32, [ctypes.c_char_p, i32]),
         "ctb_debug_noalloc_fits": (i32, [sz]),
+        "ctb_debug_norm_reads": (i32, [i64, i32, i64, i32, i32, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)]),
         "ctb_wait_timeouts": (i32, [ctypes.POINTER(ctypes.c_uint64)]),
         "ctb_debug_wait_timeout": (i32, [u64, ctypes.POINTER(ctypes.c_int)]),
     }

@@ -7,6 +7,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "ctb/ctb_debug.h"
 #include "rows.cuh"
 
 namespace ctb {
@@ -382,15 +383,15 @@ template <class T, int VEC> __device__ __forceinline__ Pack<T, VEC> ring_pack(ui
 }
 
 // The rows and columns of a group of threads. ODD: rows start anywhere, all matrices' alike; packs are those of memory, so
-// the first and the last one of a row may be in part its neighbours': they are read whole, but for the first row's first
-// and the last row's last one, which might reach out of the matrix, and written element by element. How far a row
-// starts behind a pack repeats every `period` rows (a power of two), and a group takes rows of one kind: its columns,
-// and with them its weights and sums of grad_weight, stay the same.
-template <int VEC, int G, bool ODD> struct Share {
+// the first and the last one of a row may be in part its neighbours': they are read whole where they lie inside the
+// matrix (pack_inside: of rows narrower than a pack those of several rows reach out of it), else, and when they are
+// written, element by element. How far a row starts behind a pack repeats every `period` rows (a power of two), and a
+// group takes rows of one kind: its columns, and with them its weights and sums of grad_weight, stay the same.
+template <int VEC, bool ODD> struct Share {
     int64_t lo, hi, first, period;  // rows first + period * [lo, hi)
     int behind;                     // elements from a pack's start to the row's
 
-    __device__ __forceinline__ Share(int64_t rows, int64_t group, int64_t groups, int base, int64_t stride) {
+    __host__ __device__ __forceinline__ Share(int64_t rows, int64_t group, int64_t groups, int base, int64_t stride) {
         first = 0;
         period = 1;
         behind = 0;
@@ -407,21 +408,25 @@ template <int VEC, int G, bool ODD> struct Share {
         lo = rows * group / groups;
         hi = rows * (group + 1) / groups;
     }
-    __device__ __forceinline__ int64_t row(int64_t i) const { return ODD ? first + period * i : i; }
-    __device__ __forceinline__ int column(int pack) const { return pack * VEC - behind; }
+    __host__ __device__ __forceinline__ int64_t row(int64_t i) const { return ODD ? first + period * i : i; }
+    __host__ __device__ __forceinline__ int column(int pack) const { return pack * VEC - behind; }
     // 2: all of the pack is the row's, 1: a part, 0: nothing
-    __device__ __forceinline__ int kind(int j, int cols) const {
+    __host__ __device__ __forceinline__ int kind(int j, int cols) const {
         if (!ODD) return j < cols ? 2 : 0;
         return j >= 0 && j + VEC <= cols ? 2 : j + VEC > 0 && j < cols ? 1 : 0;
     }
 };
 
-// A thread's pack of a row on its way into its place in the ring. What may reach out of the matrix (before its first row,
-// behind its last one) is read element by element at once.
+// Whether `vec` elements from the `at`-th on belong to a matrix whose last element is the `last`-th, gaps between its rows
+// counted in.
+__host__ __device__ __forceinline__ bool pack_inside(int64_t at, int vec, int64_t last) { return at >= 0 && at + vec - 1 <= last; }
+
+// A thread's pack of a row on its way into its place in the ring; `row` starts `at` elements into its matrix. What is in part
+// the row's and reaches out of the matrix is read element by element at once.
 template <class T, int VEC, bool ODD>
-__device__ __forceinline__ void fetch_pack(uint32_t to, const T* row, int kind, int j, int cols, int64_t r, int64_t rows) {
+__device__ __forceinline__ void fetch_pack(uint32_t to, const T* row, int kind, int j, int cols, int64_t at, int64_t last) {
     if (!kind) return;
-    if (!ODD || kind == 2 || ((j >= 0 || r > 0) && (j + VEC <= cols || r + 1 < rows))) {
+    if (!ODD || kind == 2 || pack_inside(at + j, VEC, last)) {
         copy16(to, row + j);
         return;
     }
@@ -500,20 +505,23 @@ __global__ void __launch_bounds__(group_threads<G>(), forward_ctas<G>()) norm_ro
     constexpr int kGroups = group_threads<G>() / G, kArrays = RES ? 2 : 1, kRing = ring_stages<G, NP>(kArrays, forward_ctas<G>());
     const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
     const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, group = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
-    const Share<VEC, G, ODD> share(v.rows, group, groups, elements_behind<T, VEC>(v.ptr[kNmX]), v.stride[kNmX][0]);
+    const Share<VEC, ODD> share(v.rows, group, groups, elements_behind<T, VEC>(v.ptr[kNmX]), v.stride[kNmX][0]);
     const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
     constexpr uint32_t kStep = group_threads<G>() * 16;  // from one pack of a thread to its next
     auto fetch = [&](int64_t i, int stage) {
         if (i < share.hi) {
             const int64_t r = share.row(i);
-            const T* const x = static_cast<const T*>(v.ptr[kNmX]) + row_offset(v, kNmX, r);
-            const T* const res = RES ? static_cast<const T*>(v.ptr[kNmResidual]) + row_offset(v, kNmResidual, r) : nullptr;
+            auto matrix = [&](int slot, int array) {
+                const int64_t at = row_offset(v, slot, r), last = ODD ? row_offset(v, slot, v.rows - 1) + cols - 1 : 0;
 #pragma unroll
-            for (int q = 0; q < NP; ++q) {
-                const int j = share.column(q * G + t), kind = share.kind(j, cols);
-                fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + q) * kStep, x, kind, j, cols, r, v.rows);
-                if (RES) fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + NP + q) * kStep, res, kind, j, cols, r, v.rows);
-            }
+                for (int q = 0; q < NP; ++q) {
+                    const int j = share.column(q * G + t);
+                    fetch_pack<T, VEC, ODD>(mine + ((stage * kArrays + array) * NP + q) * kStep, static_cast<const T*>(v.ptr[slot]) + at, share.kind(j, cols), j,
+                                            cols, at, last);
+                }
+            };
+            matrix(kNmX, 0);
+            if (RES) matrix(kNmResidual, 1);
         }
         copies_commit();
     };
@@ -749,23 +757,24 @@ __global__ void __launch_bounds__(group_threads<G>(), backward_ctas<G, ODD>()) n
     constexpr int kGroups = group_threads<G>() / G, kArrays = PASSED ? 3 : 2, kRing = ring_stages<G, NP>(kArrays, backward_ctas<G, ODD>());
     const int t = threadIdx.x % G, cols = static_cast<int>(v.cols);
     const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, group = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
-    const Share<VEC, G, ODD> share(v.rows, group, groups, elements_behind<T, VEC>(v.ptr[kNgUp]), v.stride[kNgUp][0]);
+    const Share<VEC, ODD> share(v.rows, group, groups, elements_behind<T, VEC>(v.ptr[kNgUp]), v.stride[kNgUp][0]);
     const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
     constexpr uint32_t kStep = group_threads<G>() * 16;
-    auto row_of = [&](int slot, int64_t r) { return static_cast<const T*>(v.ptr[slot]) + row_offset(v, slot, r); };
     auto fetch = [&](int64_t i, int stage) {
         if (i < share.hi) {
             const int64_t r = share.row(i);
-            const T* const up = row_of(kNgUp, r);
-            const T* const x = row_of(kNgSummed, r);
-            const T* const p = PASSED ? row_of(kNgPassed, r) : nullptr;
+            auto matrix = [&](int slot, int array) {
+                const int64_t at = row_offset(v, slot, r), last = ODD ? row_offset(v, slot, v.rows - 1) + cols - 1 : 0;
 #pragma unroll
-            for (int q = 0; q < NP; ++q) {
-                const int j = share.column(q * G + t), kind = share.kind(j, cols);
-                fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + q) * kStep, up, kind, j, cols, r, v.rows);
-                fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + NP + q) * kStep, x, kind, j, cols, r, v.rows);
-                if (PASSED) fetch_pack<T, VEC, ODD>(mine + (stage * kArrays * NP + 2 * NP + q) * kStep, p, kind, j, cols, r, v.rows);
-            }
+                for (int q = 0; q < NP; ++q) {
+                    const int j = share.column(q * G + t);
+                    fetch_pack<T, VEC, ODD>(mine + ((stage * kArrays + array) * NP + q) * kStep, static_cast<const T*>(v.ptr[slot]) + at, share.kind(j, cols), j,
+                                            cols, at, last);
+                }
+            };
+            matrix(kNgUp, 0);
+            matrix(kNgSummed, 1);
+            if (PASSED) matrix(kNgPassed, 2);
         }
         copies_commit();
     };
@@ -971,6 +980,25 @@ template <class T> void run_grad(NormGradArgs& a, cudaStream_t st) {
     count_launch();
 }
 
+// The elements that the ring's packs read of a matrix, by the kernels' own arithmetic: the first and the last one that is part of
+// a pack read whole.
+template <int VEC> void packs_read(int64_t rows, int cols, int64_t stride, int base, int64_t& lowest, int64_t& highest) {
+    const int64_t last = (rows - 1) * stride + cols - 1, groups = VEC;
+    lowest = highest = 0;
+    for (int64_t group = 0; group < groups; ++group) {
+        const Share<VEC, true> share(rows, group, groups, base, stride);
+        for (int64_t i = share.lo; i < share.hi; ++i)
+            for (int pack = 0; pack <= (cols + 2 * VEC - 2) / VEC; ++pack) {
+                const int j = share.column(pack), kind = share.kind(j, cols);
+                const int64_t at = share.row(i) * stride + j;
+                if (kind == 2 || (kind == 1 && pack_inside(at, VEC, last))) {
+                    lowest = std::min(lowest, at);
+                    highest = std::max(highest, at + VEC - 1);
+                }
+            }
+    }
+}
+
 }  // namespace
 }  // namespace ctb
 
@@ -1065,6 +1093,14 @@ int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summed, cons
         }
         return CTB_OK;
     });
+}
+
+int ctb_debug_norm_reads(int64_t rows, int cols, int64_t stride, int base, int elem_bytes, int64_t* lowest, int64_t* highest) {
+    if (rows < 1 || cols < 1 || (rows > 1 && stride < cols) || base < 0 || !lowest || !highest) return CTB_ERR_ARGUMENT;
+    if (elem_bytes == 4) packs_read<4>(rows, cols, stride, base, *lowest, *highest);
+    else if (elem_bytes == 2) packs_read<8>(rows, cols, stride, base, *lowest, *highest);
+    else return CTB_ERR_ARGUMENT;
+    return CTB_OK;
 }
 
 }  // extern "C"

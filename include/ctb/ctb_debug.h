@@ -41,6 +41,13 @@ CTB_API uint64_t ctb_debug_fastdiv(uint64_t n, uint64_t d);
  * point gives (ctb_last_error). */
 CTB_API int ctb_debug_noalloc_fits(size_t need);
 
+/* The norm's reads of rows that start anywhere, without a device: of a [rows, cols] matrix of 4- or 2-byte elements with
+ * `stride` elements from row to row, whose first one lies `base` elements behind a 16-byte boundary, the first and the
+ * last element (counted from the matrix's first) that a 16-byte read covers; 0 where there is none. Reads inside the
+ * matrix stay within 0 and (rows - 1) * stride + cols - 1. */
+CTB_API int ctb_debug_norm_reads(int64_t rows, int cols, int64_t stride, int base, int elem_bytes, int64_t* lowest,
+                                 int64_t* highest);
+
 /* Self-test of the bounded wait (needs a GPU, unlike the functions above): one thread waits on a
  * shared-memory barrier that nothing arrives at, for limit_ns (at most 100 ms), then returns.
  * *completed is 0 when the wait timed out, as it must; the timeout is also counted by
