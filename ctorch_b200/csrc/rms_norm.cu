@@ -384,9 +384,9 @@ template <class T, int VEC> __device__ __forceinline__ Pack<T, VEC> ring_pack(ui
 
 // The rows and columns of a group of threads. ODD: rows start anywhere, all matrices' alike; packs are those of memory, so
 // the first and the last one of a row may be in part its neighbours': they are read whole where they lie inside the
-// matrix (pack_inside: of rows narrower than a pack those of several rows reach out of it), else, and when they are
-// written, element by element. How far a row starts behind a pack repeats every `period` rows (a power of two), and a
-// group takes rows of one kind: its columns, and with them its weights and sums of grad_weight, stay the same.
+// matrix (pack_inside), else, and when they are written, element by element. How far a row starts behind a pack repeats
+// every `period` rows (a power of two), and a group takes rows of one kind: its columns, and with them its weights and
+// sums of grad_weight, stay the same.
 template <int VEC, bool ODD> struct Share {
     int64_t lo, hi, first, period;  // rows first + period * [lo, hi)
     int behind;                     // elements from a pack's start to the row's
@@ -417,16 +417,18 @@ template <int VEC, bool ODD> struct Share {
     }
 };
 
-// Whether `vec` elements from the `at`-th on belong to a matrix whose last element is the `last`-th, gaps between its rows
-// counted in.
-__host__ __device__ __forceinline__ bool pack_inside(int64_t at, int vec, int64_t last) { return at >= 0 && at + vec - 1 <= last; }
+// Whether a pack that has columns j to j + VEC - 1 in or next to row r lies inside the matrix, gaps between rows counted in: all
+// but the first row's first and the last row's last one, as rows have VEC - 1 elements at least (alike()).
+template <int VEC> __host__ __device__ __forceinline__ bool pack_inside(int j, int cols, int64_t r, int64_t rows) {
+    return (j >= 0 || r > 0) && (j + VEC <= cols || r + 1 < rows);
+}
 
-// A thread's pack of a row on its way into its place in the ring; `row` starts `at` elements into its matrix. What is in part
-// the row's and reaches out of the matrix is read element by element at once.
+// A thread's pack of a row on its way into its place in the ring. What is in part the row's and reaches out of the matrix is
+// read element by element at once.
 template <class T, int VEC, bool ODD>
-__device__ __forceinline__ void fetch_pack(uint32_t to, const T* row, int kind, int j, int cols, int64_t at, int64_t last) {
+__device__ __forceinline__ void fetch_pack(uint32_t to, const T* row, int kind, int j, int cols, int64_t r, int64_t rows) {
     if (!kind) return;
-    if (!ODD || kind == 2 || pack_inside(at + j, VEC, last)) {
+    if (!ODD || kind == 2 || pack_inside<VEC>(j, cols, r, rows)) {
         copy16(to, row + j);
         return;
     }
@@ -512,12 +514,11 @@ __global__ void __launch_bounds__(group_threads<G>(), forward_ctas<G>()) norm_ro
         if (i < share.hi) {
             const int64_t r = share.row(i);
             auto matrix = [&](int slot, int array) {
-                const int64_t at = row_offset(v, slot, r), last = ODD ? row_offset(v, slot, v.rows - 1) + cols - 1 : 0;
+                const T* const row = static_cast<const T*>(v.ptr[slot]) + row_offset(v, slot, r);
 #pragma unroll
                 for (int q = 0; q < NP; ++q) {
                     const int j = share.column(q * G + t);
-                    fetch_pack<T, VEC, ODD>(mine + ((stage * kArrays + array) * NP + q) * kStep, static_cast<const T*>(v.ptr[slot]) + at, share.kind(j, cols), j,
-                                            cols, at, last);
+                    fetch_pack<T, VEC, ODD>(mine + ((stage * kArrays + array) * NP + q) * kStep, row, share.kind(j, cols), j, cols, r, v.rows);
                 }
             };
             matrix(kNmX, 0);
@@ -764,12 +765,11 @@ __global__ void __launch_bounds__(group_threads<G>(), backward_ctas<G, ODD>()) n
         if (i < share.hi) {
             const int64_t r = share.row(i);
             auto matrix = [&](int slot, int array) {
-                const int64_t at = row_offset(v, slot, r), last = ODD ? row_offset(v, slot, v.rows - 1) + cols - 1 : 0;
+                const T* const row = static_cast<const T*>(v.ptr[slot]) + row_offset(v, slot, r);
 #pragma unroll
                 for (int q = 0; q < NP; ++q) {
                     const int j = share.column(q * G + t);
-                    fetch_pack<T, VEC, ODD>(mine + ((stage * kArrays + array) * NP + q) * kStep, static_cast<const T*>(v.ptr[slot]) + at, share.kind(j, cols), j,
-                                            cols, at, last);
+                    fetch_pack<T, VEC, ODD>(mine + ((stage * kArrays + array) * NP + q) * kStep, row, share.kind(j, cols), j, cols, r, v.rows);
                 }
             };
             matrix(kNgUp, 0);
@@ -865,11 +865,14 @@ template <int N> int pack_of(const RowViews<N>& v, std::initializer_list<int> sl
     return vec;
 }
 
+// Whether rows fill a pack but for one element, so that a pack of memory touches two of them at most.
+constexpr bool wide_rows(int64_t cols, int vec) { return cols >= vec - 1; }
+
 // Whether all rows of the given matrices start equally far behind a pack (16 bytes of the rows' type), with unit strides along
-// and one stride across: packs of memory then serve all of them.
+// and one stride across, and are wide enough: packs of memory then serve all of them.
 template <int N> bool alike(const RowViews<N>& v, std::initializer_list<int> slots) {
-    if (v.rank != 1) return false;
     const int64_t size = static_cast<int64_t>(dtype_size(v.dtype[0])), vec = 16 / size;
+    if (v.rank != 1 || !wide_rows(v.cols, static_cast<int>(vec))) return false;
     const int64_t base = reinterpret_cast<uintptr_t>(v.ptr[0]) / size % vec;
     for (int s : slots) {
         if (!v.ptr[s]) continue;
@@ -983,19 +986,20 @@ template <class T> void run_grad(NormGradArgs& a, cudaStream_t st) {
 // The elements that the ring's packs read of a matrix, by the kernels' own arithmetic: the first and the last one that is part of
 // a pack read whole.
 template <int VEC> void packs_read(int64_t rows, int cols, int64_t stride, int base, int64_t& lowest, int64_t& highest) {
-    const int64_t last = (rows - 1) * stride + cols - 1, groups = VEC;
     lowest = highest = 0;
-    for (int64_t group = 0; group < groups; ++group) {
-        const Share<VEC, true> share(rows, group, groups, base, stride);
-        for (int64_t i = share.lo; i < share.hi; ++i)
+    if (!wide_rows(cols, VEC)) return;  // such rows are read element by element
+    for (int64_t group = 0; group < VEC; ++group) {
+        const Share<VEC, true> share(rows, group, VEC, base, stride);
+        for (int64_t i = share.lo; i < share.hi; ++i) {
+            const int64_t r = share.row(i);
             for (int pack = 0; pack <= (cols + 2 * VEC - 2) / VEC; ++pack) {
                 const int j = share.column(pack), kind = share.kind(j, cols);
-                const int64_t at = share.row(i) * stride + j;
-                if (kind == 2 || (kind == 1 && pack_inside(at, VEC, last))) {
-                    lowest = std::min(lowest, at);
-                    highest = std::max(highest, at + VEC - 1);
+                if (kind == 2 || (kind == 1 && pack_inside<VEC>(j, cols, r, rows))) {
+                    lowest = std::min(lowest, r * stride + j);
+                    highest = std::max(highest, r * stride + j + VEC - 1);
                 }
             }
+        }
     }
 }
 

@@ -14,8 +14,8 @@ def reads(C, rows, cols, stride, base, size):
 
 @pytest.mark.parametrize("size", [4, 2])
 def test_norm_reads_stay_inside_the_matrix(size):
-    """Rows that start anywhere are read in packs of 16 bytes of memory; of rows narrower than a pack one reaches over several
-    rows, and must not reach out of the matrix on either side."""
+    """Rows that start anywhere are read in packs of 16 bytes of memory, which must not reach out of the matrix on either side: of
+    rows narrower than a pack one would reach over several rows."""
     C, vec = _lib(), 16 // size
     for rows in (1, 2, 3, 4, 5, 9, 17):
         for cols in (1, 2, 3, 5, 6, 7, 8, 9, 15, 16, 17, 33):
@@ -27,8 +27,8 @@ def test_norm_reads_stay_inside_the_matrix(size):
 
 def test_norm_reads_whole_packs_where_it_can():
     C = _lib()
-    assert reads(C, 3, 2, 2, 0, 2) == (0, 0)  # six elements hold no pack of eight
-    assert reads(C, 5, 2, 2, 0, 2) == (0, 7)
+    assert reads(C, 3, 2, 2, 0, 2) == (0, 0)  # rows narrower than a pack are read element by element
+    assert reads(C, 9, 7, 7, 0, 2) == (0, 55)
     assert reads(C, 4, 16, 17, 0, 2) == (0, 63)  # a gap between rows belongs to the matrix, what follows the last row does not
     assert reads(C, 4, 16, 17, 3, 2) == (0, 60)
 
