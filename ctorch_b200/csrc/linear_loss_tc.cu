@@ -31,6 +31,7 @@ constexpr int kStageBytes = 2 * kHalf * kK * 2;  // of one CTA: its halves of bo
 constexpr int kEpilogueWarps = 8, kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kBoxBytes = 32 * 128;  // of results on their way out, one a warp
 constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;
+constexpr int kLogitsStretch = 12, kGradStretch = 256;  // stages summed in tensor memory at a time
 constexpr int kGroup = 8;  // tiles of rows walked together, so that both operands are met again in L2 (2 to 32: within 5%)
 
 enum Product : int { kLogits = 0, kLogitsOnly = 1, kGradHidden = 2, kGradWeight = 3 };
@@ -97,13 +98,14 @@ __device__ __forceinline__ uint32_t two_bf16(float x, float y) {
     return r;
 }
 
-// The tensor cores truncate a float32 sum at every step of 16 products, so what comes out is short by a share of itself that
-// grows with the steps. Measured on B200 for logits of 64 to 4096 columns, random and leaning ones: 1.5e-8 to 1.7e-8 a
-// step (a sum that grows evenly loses 2^-24 of 0.7 of half of itself a step at most). Given back on average: the
-// log-sum-exp of 4096 columns was 1.3e-6 off one way.
-constexpr double kTruncated = 1.6e-8;
-
-__device__ __forceinline__ float given_back(int64_t kblocks) { return static_cast<float>(1.0 + kTruncated * (kK / 16) * static_cast<double>(kblocks)); }
+// The tensor cores truncate a float32 sum at every step of 16 products, so a long one comes out short by a share of itself (one
+// that grows evenly by about 1.6e-8 a step; an exact one by nothing). So they sum a stretch of stages, and the stretches are
+// added in registers, rounded to nearest: a logit loses 8e-7 of itself at most on average, however long, and an exact one
+// nothing. Short stretches wait for the rows' exponentials, which take as long as the products of about 20 stages. B200,
+// 3686 x 2048 x 32768 (32 stages), z and the log-sum-exp's error: one stretch 349 us and 1.3e-6 at twice the columns, 16
+// stages 356 and 3.6e-7, 12 stages 362 and 2.4e-7, 8 stages 379 and 1.7e-7. Gradients are rounded to 16 bits or of such
+// terms, and 1.6e-5 of a stretch is far below that.
+template <int P> constexpr int stretch() { return P == kLogits || P == kLogitsOnly ? kLogitsStretch : kGradStretch; }
 
 // 128 columns of a row of logits: their maximum and the sum of exp((z - max) / T), the target's z, and with HOLD
 // 2^15 exp((z - max) / T) in 16 bits: 11 bits of precision down to 2^-29 of the largest, nothing below 2^-40.
@@ -125,7 +127,7 @@ __device__ __forceinline__ void box_free() {
 }
 
 template <bool HOLD>
-__device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf], int64_t i, int64_t col, int64_t target, bool live, float back,
+__device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf], int64_t i, int64_t col, int64_t target, bool live,
                                            const Out& out) {
     const int64_t left = a.vocab - col;
     if (left < kHalf) {
@@ -140,19 +142,19 @@ __device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf
 #pragma unroll
         for (int j = 0; j < kHalf; ++j)
             if (j == t) zt = z[j];
-        if (here) a.target_z[i] = zt * back;
+        if (here) a.target_z[i] = zt;
     }
     float m = z[0];
 #pragma unroll
     for (int j = 1; j < kHalf; ++j) m = fmaxf(m, z[j]);
-    const float at = m == -INFINITY ? 0.0f : m, c2 = a.c2 * back;
+    const float at = m == -INFINITY ? 0.0f : m;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < kHalf; ++j) {
-        z[j] = exp2_approx(fmaf(z[j] - at, c2, 15.0f));
+        z[j] = exp2_approx(fmaf(z[j] - at, a.c2, 15.0f));
         s[j & 3] += z[j];
     }
-    if (live) a.stats[i * a.tiles + col / kHalf] = make_float2(m * back, ((s[0] + s[1]) + (s[2] + s[3])) * 3.0517578125e-05f);
+    if (live) a.stats[i * a.tiles + col / kHalf] = make_float2(m, ((s[0] + s[1]) + (s[2] + s[3])) * 3.0517578125e-05f);
     if (!HOLD) return;
     const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -171,7 +173,7 @@ __device__ __forceinline__ void logits_row(const LinearArgs& a, float (&z)[kHalf
 
 constexpr int kChunk = 32;  // columns of a gradient that a thread has in hand at a time
 
-__device__ __forceinline__ void grad_hidden_rows(const float (&x)[kChunk], int64_t col, const Out& out) {
+__device__ __forceinline__ void grad_hidden_rows(const float* x, int64_t col, const Out& out) {
     box_free();
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -181,7 +183,7 @@ __device__ __forceinline__ void grad_hidden_rows(const float (&x)[kChunk], int64
 }
 
 // 32 columns of dW into half of the warp's box, which leaves with every second piece.
-__device__ __forceinline__ void grad_weight_rows(const float (&x)[kChunk], int64_t col, float factor, int piece, const Out& out) {
+__device__ __forceinline__ void grad_weight_rows(const float* x, int64_t col, float factor, int piece, const Out& out) {
     if ((piece & 1) == 0) box_free();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -193,7 +195,7 @@ __device__ __forceinline__ void grad_weight_rows(const float (&x)[kChunk], int64
 }
 
 // The same for any layout of dW, and where the blocks before are added.
-__device__ __forceinline__ void grad_weight_row(const LinearArgs& a, const ProductArgs& p, float (&x)[kChunk], int64_t v, int64_t col,
+__device__ __forceinline__ void grad_weight_row(const LinearArgs& a, const ProductArgs& p, float* x, int64_t v, int64_t col,
                                                 int64_t cols, float factor) {
     if (a.acc) {
         float* const acc = a.acc + v * a.acc_pitch + col;
@@ -307,33 +309,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t acc_phase = 0;
             for (int64_t w = pair; ok && w < plan.total; w += pairs) {
                 const Work o = plan.at(w);
-                if (o.kbs == 0) continue;
-                if (!mbar_wait(&bars.free[acc], acc_phase ^ 1u)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem + acc * kTile;
-                for (int64_t kb = 0; kb < o.kbs; ++kb) {
-                    if (!mbar_wait(&bars.full[stage], phase)) {
+                for (int64_t left = o.kbs; ok && left > 0; left -= stretch<P>()) {
+                    if (!mbar_wait(&bars.free[acc], acc_phase ^ 1u)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_addr(smem + stage * kStageBytes), sb = sa + kStageBytes / 2;
+                    const uint32_t d = tmem + acc * kTile;
+                    const int stages = static_cast<int>(min(left, static_cast<int64_t>(stretch<P>())));
+                    for (int kb = 0; kb < stages; ++kb) {
+                        if (!mbar_wait(&bars.full[stage], phase)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t sa = smem_addr(smem + stage * kStageBytes), sb = sa + kStageBytes / 2;
 #pragma unroll
-                    for (int k = 0; k < kK / 16; ++k)
-                        mma_pair(d, matrix_descriptor(sa + k * kAStep, 8192, 1024), matrix_descriptor(sb + k * kBStep, 8192, 1024),
-                                 kInstruction, kb > 0 || k > 0);
-                    mma_commit_pair(&bars.empty[stage]);
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1u;
+                        for (int k = 0; k < kK / 16; ++k)
+                            mma_pair(d, matrix_descriptor(sa + k * kAStep, 8192, 1024), matrix_descriptor(sb + k * kBStep, 8192, 1024),
+                                     kInstruction, kb > 0 || k > 0);
+                        mma_commit_pair(&bars.empty[stage]);
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
+                    mma_commit_pair(&bars.done[acc]);
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1u;
                 }
-                mma_commit_pair(&bars.done[acc]);
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1u;
             }
         }
     } else {
@@ -352,48 +356,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int64_t r = a.order ? a.order[p.first + i] : p.first + i;
                 target = index_at(a.v.ptr[kLnTarget], a.v.dtype[kLnTarget], row_offset(a.v, kLnTarget, r));
             }
-            if (o.kbs != 0) {
+            float x[kHalf];
+            for (int64_t kb = 0; kb < o.kbs; kb += stretch<P>()) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&bars.done[acc], acc_phase));
                 if (!ok) break;
                 tc_fence_after();
-            }
-            const uint32_t from = tmem + acc * kTile + half * kHalf + (static_cast<uint32_t>(quarter * 32) << 16);
-            // gives the sums back to the products once they are in registers
-            auto release = [&] {
+                const uint32_t from = tmem + acc * kTile + half * kHalf + (static_cast<uint32_t>(quarter * 32) << 16);
+                if (kb == 0) {
+#pragma unroll
+                    for (int c = 0; c < kHalf / 32; ++c) tmem_load32(x + c * 32, from + c * 32);
+                    tmem_load_wait();
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kHalf / 16; ++c) {
+                        float y[16];
+                        tmem_load16(y, from + c * 16);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[c * 16 + j] += y[j];
+                    }
+                }
+                // the sums are in registers: the tensor memory goes back to the products
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(in_first_cta(&bars.free[acc]));
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
-            };
+            }
+            if (!ok) break;
+            if (o.kbs == 0) {
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j) x[j] = 0.0f;
+            }
             if constexpr (P == kLogits || P == kLogitsOnly) {
-                float z[kHalf];
-#pragma unroll
-                for (int c = 0; c < kHalf / 32; ++c) tmem_load32(z + c * 32, from + c * 32);
-                tmem_load_wait();
-                release();
-                if (col < p.n && i0 < m) logits_row<P == kLogits>(a, z, i, col, target, i < m, given_back(o.kbs), out);
+                if (col < p.n && i0 < m) logits_row<P == kLogits>(a, x, i, col, target, i < m, out);
             } else {
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < kHalf / kChunk; ++c) {
-                    float x[kChunk];
-                    if (o.kbs == 0) {
-#pragma unroll
-                        for (int j = 0; j < kChunk; ++j) x[j] = 0.0f;
-                    } else {
-                        tmem_load32(x, from + c * kChunk);
-                        tmem_load_wait();
-                    }
-                    if (c == kHalf / kChunk - 1 && o.kbs != 0) release();
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) x[j] *= given_back(o.kbs);
                     const int64_t at = col + c * kChunk;
                     if (P == kGradHidden) {
-                        if (i0 < m && at < p.n) grad_hidden_rows(x, at, out);
+                        if (i0 < m && at < p.n) grad_hidden_rows(x + c * kChunk, at, out);
                     } else if (p.boxes) {
-                        if (i0 < m && col + (c & ~1) * kChunk < p.n) grad_weight_rows(x, at, factor, c, out);
+                        if (i0 < m && col + (c & ~1) * kChunk < p.n) grad_weight_rows(x + c * kChunk, at, factor, c, out);
                     } else if (i < m && at < p.n) {
-                        grad_weight_row(a, p, x, i, at, p.n, factor);
+                        grad_weight_row(a, p, x + c * kChunk, i, at, p.n, factor);
                     }
                 }
             }

@@ -1,0 +1,84 @@
+"""GPU checks of what stands around the losses where it can go wrong without the bounds of test_gpu_model.py seeing it: logits
+that are exact."""
+import pytest
+import torch
+
+import model_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+KIND = {"f32": torch.float32, "bf16": torch.bfloat16}
+NAN = float("nan")
+
+
+def cb():
+    import ctorch_b200
+
+    return ctorch_b200
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def whole(g, low, high, *shape):
+    return torch.randint(low, high + 1, shape, generator=g, device="cuda").double()
+
+
+def check_exact_logits(h, w, t, dtype):
+    """Every product and every partial sum of the logits is a float32, so only the softmax errs: an exponential by 2^-22, its
+    argument's two roundings (2^-24 of at most 40, in powers of 2, before the exponential vanishes against the sum) and the
+    sum's additions (32 of a tile's quarter, the tiles by fours and lanes) by 2^-24 each; then a log's result is rounded."""
+    z = h @ w.T
+    lse = torch.logsumexp(z, 1)
+    loss = lse - z.gather(1, t[:, None])[:, 0]
+    r = cb().linear_cross_entropy(h.to(dtype), w.to(dtype), t, grad=False)
+    bound = (4 + 2 * 40 + 64) * O.U
+    for name, got, want in (("lse", r.lse, lse), ("row_loss", r.row_loss, loss)):
+        off = (got.double() - want).abs() - (bound + 2 * O.U * want.abs())
+        k = int(off.argmax())
+        assert off[k] <= 0, (name, float(got[k]), float(want[k]))
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("dim", [64, 100, 768, 4096, 16384])
+def test_logits_of_one_column_are_exact(dim, kind):
+    """Rows with one entry that is not 0, in the first column, the last one and others."""
+    g = gen(dim)
+    rows, vocab = 70, 600
+    w = whole(g, -64, 64, vocab, dim)
+    at = torch.randint(dim, (rows,), generator=g, device="cuda")
+    at[0], at[1], at[2], at[3] = 0, dim - 1, min(dim - 1, 767), min(dim - 1, 768)
+    h = torch.zeros(rows, dim, dtype=torch.float64, device="cuda").scatter_(1, at[:, None], 1.0)
+    check_exact_logits(h, w, torch.randint(vocab, (rows,), generator=g, device="cuda"), KIND[kind])
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("dim", [64, 1000, 4096, 16384])
+def test_logits_of_whole_numbers_are_exact(dim, kind):
+    """Sums of whole numbers below 2^24."""
+    g = gen(dim + 1)
+    rows, vocab = 70, 600
+    check_exact_logits(whole(g, -2, 2, rows, dim), whole(g, -8, 8, vocab, dim), torch.randint(vocab, (rows,), generator=g, device="cuda"), KIND[kind])
+
+
+@pytest.mark.parametrize("rows,dim,vocab", [(64, 256, 70000), (40000, 256, 64)])
+def test_gradients_of_long_sums(rows, dim, vocab):
+    """One way sums of many terms, along the vocabulary and along the rows: what truncated sums lose shows in their mean. The
+    results' rounding to bfloat16 (2^-8 at most, independent) averages to 2^-8 / sqrt(3 n) over n of them, six of which are
+    allowed, beside what a stretch loses (below 2e-5) and the truth's own share of G's rounding, likewise averaged."""
+    g = gen(rows)
+    h = (1 + torch.rand(rows, dim, generator=g, device="cuda")).bfloat16()
+    w = (torch.rand(vocab, dim, generator=g, device="cuda") / dim).bfloat16()
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    r = cb().linear_cross_entropy(h, w, t)
+    want = O.head(h, w, t, None)
+    for name, got in (("grad_hidden", r.grad_hidden), ("grad_weight", r.grad_weight[1:])):
+        value = want[name][0] if name == "grad_hidden" else want[name][0][1:]
+        big = value.abs() > 0.1 * value.abs().mean()
+        n = int(big.sum())
+        bias = float((got.double() / value - 1)[big].mean())
+        terms = vocab if name == "grad_hidden" else rows
+        assert abs(bias) <= 6 * 2.0 ** -8 * (1 / (3 * n)) ** 0.5 + 6 * 2.0 ** -8 * (1 / (3 * terms)) ** 0.5 + 2e-5, (name, bias)
