@@ -82,3 +82,27 @@ def test_gradients_of_long_sums(rows, dim, vocab):
         bias = float((got.double() / value - 1)[big].mean())
         terms = vocab if name == "grad_hidden" else rows
         assert abs(bias) <= 6 * 2.0 ** -8 * (1 / (3 * n)) ** 0.5 + 6 * 2.0 ** -8 * (1 / (3 * terms)) ** 0.5 + 2e-5, (name, bias)
+
+
+# ------------------------------------------------------------------------------------- 8 bits
+
+
+@pytest.mark.parametrize("quant", ["row", "block"])
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("rows,dim", [(1, 1), (64, 64), (40, 129), (300, 4096), (37, 5003), (5, 20008), (3, 40000), (400, 640)])
+def test_8_bits_are_the_quotients_rounded_to_nearest(rows, dim, kind, quant):
+    """y and its largest are the float32 numbers that the kernel has too (the rows' own rstd, two products), so the scale and
+    the quotient rounded to 8 bits are known to the bit. Whole numbers and weights of few bits bring many quotients next to a
+    tie."""
+    g, t = gen(rows + dim), KIND[kind]
+    x = whole(g, -60, 60, rows, dim).to(t)
+    w = (whole(g, 1, 8, dim) / 4).to(t)
+    for view in (x, torch.cat([x, x[:, :1]], 1)[:, :dim], x.t().contiguous().t()):  # packs, rows that start anywhere, columns
+        r = cb().rms_norm(view, w, quant=quant)
+        y = x.float() * r.rstd[:, None] * w.float()
+        width = dim if quant == "row" else O.BLOCK
+        top = torch.stack([p.abs().amax(-1) for p in y.split(width, -1)], -1)
+        scale = torch.where(top == 0, 1.0, top / torch.tensor(448.0, device="cuda"))
+        assert torch.equal(r.scales, scale[:, 0] if quant == "row" else scale)
+        want = (y / scale.repeat_interleave(width, -1)[:, :dim]).to(torch.float8_e4m3fn)
+        assert torch.equal(r.out.view(torch.uint8), want.view(torch.uint8))
