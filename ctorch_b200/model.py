@@ -88,7 +88,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, quant: str | None = No
 
     With quant="row" or "block", out is float8_e4m3fn and stands for out * scales: a float32 scale a row, or one for
     every 128 columns ([..., ceil(columns / 128)]). scales is None without quant. `out` (not with quant) and
-    `out_summed` may be given; out may be x's own view, out_summed x's or the residual's."""
+    `out_summed` may be given; out may be x's own view, out_summed x's or the residual's. Without a residual an out in
+    x's place leaves nothing of x to differentiate: summed is None then."""
     name = "rms_norm"
     dev = _matrices(name, x, weight, residual)
     if quant not in _QUANT:
@@ -117,7 +118,9 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, quant: str | None = No
     rstd = _new(rows, torch.float32, dev)
     _run(name, dev, C.lib.ctb_rms_norm, _view(x), _view(weight), _view(residual), eps, _QUANT[quant], vout, vsum,
          _view(rstd), vscales)
-    return RmsNorm(y, x if summed is None else summed, rstd, scales)
+    if summed is None and (out is None or not may_overlap(out, x)):
+        summed = x
+    return RmsNorm(y, summed, rstd, scales)
 
 
 def rms_norm_backward(grad_out, summed, weight, rstd, grad_summed=None, out=None) -> RmsNormGrad:
@@ -125,6 +128,8 @@ def rms_norm_backward(grad_out, summed, weight, rstd, grad_summed=None, out=None
     grad_x, of x and of the residual alike, and grad_weight in weight's type. summed and rstd are rms_norm's. grad_x
     is written to `out` when given, which may be the view of grad_out, summed or grad_summed."""
     name = "rms_norm_backward"
+    if summed is None:
+        raise ValueError(f"ctorch::{name}: summed is needed (rms_norm wrote over x where out was x's own view)")
     dev = _matrices(name, grad_out, summed, weight, rstd, grad_summed)
     grad_x = _new(grad_out.shape, grad_out.dtype, dev) if out is None else \
         _output(name, "out", out, grad_out, dev, same=(grad_out, summed, grad_summed), apart=(weight, rstd))

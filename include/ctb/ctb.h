@@ -402,7 +402,7 @@ CTB_API size_t ctb_rms_norm_backward_scratch_bytes(const ctb_view* summed);
 
 /* Its backward pass. With h = summed * rstd and g = grad_out * weight:
  *     grad_x = rstd * (g - h * mean(g h)) + grad_summed,   grad_weight = sum over rows of grad_out * h
- * summed and rstd are the forward call's (x itself without a residual); grad_summed is what comes back to `summed`
+ * summed and rstd are the forward call's (without a residual x as it was: an out in x's place leaves none); grad_summed is what comes back to `summed`
  * from elsewhere (NULL: nothing). grad_x is the gradient of x and of the residual alike; it may be grad_out's,
  * summed's or grad_summed's own view. grad_weight has weight's type and may be NULL. */
 CTB_API int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summed, const ctb_view* weight,

@@ -106,3 +106,27 @@ def test_8_bits_are_the_quotients_rounded_to_nearest(rows, dim, kind, quant):
         assert torch.equal(r.scales, scale[:, 0] if quant == "row" else scale)
         want = (y / scale.repeat_interleave(width, -1)[:, :dim]).to(torch.float8_e4m3fn)
         assert torch.equal(r.out.view(torch.uint8), want.view(torch.uint8))
+
+
+# ------------------------------------------------------------------------------------- the norm's summed
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+def test_norm_in_the_place_of_x_has_no_summed(kind):
+    """Without a residual the backward pass needs x, which an out in its place has written over."""
+    g, t = gen(5), KIND[kind]
+    x, up, w = whole(g, -9, 9, 6, 40).to(t), whole(g, -9, 9, 6, 40).to(t), torch.ones(40, device="cuda")
+    want = cb().rms_norm(x, w)
+    assert want.summed is x
+    apart = cb().rms_norm(x, w, out=torch.empty_like(x))
+    assert apart.summed is x and torch.equal(apart.out, want.out)
+    for y in (x.clone(), x.clone().view(2, 3, 40)):
+        r = cb().rms_norm(y, w, out=y.view(y.shape))
+        assert r.summed is None and torch.equal(r.out.view(6, 40), want.out)
+        with pytest.raises(ValueError, match="summed"):
+            cb().rms_norm_backward(up.view(y.shape), r.summed, w, r.rstd)
+    y = x.clone()
+    r = cb().rms_norm(y, w, residual=up, out=y)  # with a residual the sum is kept apart
+    b = cb().rms_norm_backward(up, r.summed, w, r.rstd)
+    gx, bx, _, _ = O.norm_grad(up, (x.double() + up.double()).to(t), w, 1e-6, None)
+    assert ((b.grad_x.double() - gx).abs() <= bx + O.half(t) * gx.abs()).all()
