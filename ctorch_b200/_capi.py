@@ -99,6 +99,7 @@ def _load() -> ctypes.CDLL:
         "ctb_rms_norm_backward_scratch_bytes": (sz, [V]),
         "ctb_rms_norm_backward": (i32, [V, V, V, V, V, V, V, vp, sz, vp]),
         "ctb_linear_loss_scratch_bytes": (sz, [V, V, i32, i32]),
+        "ctb_linear_loss_forward_scratch_bytes": (sz, [V, V, i32]),
         "ctb_linear_cross_entropy": (i32, [V, V, V, V, f64, f64, f64, V, V, V, V, V, vp, vp, sz, vp]),
         "ctb_balance_loss_scratch_bytes": (sz, [V, i64]),
         "ctb_balance_loss": (i32, [V, V, V, i64, f64, f64, V, V, V, V, vp, vp, sz, vp]),

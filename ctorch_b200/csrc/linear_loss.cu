@@ -16,6 +16,7 @@ unsigned long long* wait_timeout_counter();  // async.cu
 namespace {
 
 constexpr int64_t kHeldBytes = int64_t(2) << 30;  // of a block's logits or exponentials: 8192 rows of 131072 in 16 bits
+constexpr int64_t kStatsBytes = int64_t(256) << 20;  // of a block's statistics where nothing is held: 32768 rows of 131072
 constexpr int kOrderThreads = 1024;
 
 __device__ __forceinline__ double row_weight(const LinearArgs& a, int64_t row) {
@@ -425,8 +426,12 @@ int splits_of(bool tc, int64_t rows, int64_t dim, int64_t vocab) {
     return static_cast<int>(best);
 }
 
-// The sizes of a call's pieces. Everything here follows from shapes, strides and alignment alone.
-void lay_out(LinearPlan& p) {
+// Rows of a block whose rows take `each` of at most `bytes`.
+int64_t block_rows(int64_t rows, int64_t bytes, int64_t each) { return std::min(rows, std::max<int64_t>(256, bytes / each / 256 * 256)); }
+
+// The sizes of a call's pieces. Everything here follows from shapes, strides and alignment alone. Without gradients bfloat16
+// needs its pieces' statistics alone; `held`: room for the exponentials all the same.
+void lay_out(LinearPlan& p, bool held = false) {
     LinearArgs& a = p.a;
     const int64_t rows = a.v.rows, dim = a.v.cols, vocab = a.vocab;
     p.work = a.v.dtype[kLnHidden];
@@ -435,8 +440,8 @@ void lay_out(LinearPlan& p) {
     const int64_t pitch = round_up(dim, pack);
     a.held_pitch = round_up(vocab, 64);
     a.tiles = (vocab + kLinearPiece - 1) / kLinearPiece;
-    a.block = std::max<int64_t>(256, kHeldBytes / (a.held_pitch * size) / 256 * 256);
-    a.block = std::min(a.block, rows);
+    held = held || p.grad || !tc;
+    a.block = block_rows(rows, held ? kHeldBytes : kStatsBytes, held ? a.held_pitch * size : a.tiles * 8);
     p.blocks = (rows + a.block - 1) / a.block;
     p.pack_h = p.weighted || p.h_row < 0 ||
                !in_place(a.v.ptr[kLnHidden], p.h_row, a.v.inner[kLnHidden], rows, dim, a.v.dtype[kLnHidden], p.work);
@@ -452,7 +457,7 @@ void lay_out(LinearPlan& p) {
     p.target_z = l.add(a.block, 4);
     p.factors = l.add(tc ? a.block : 0, sizeof(LinearRowFactor));
     p.stats = l.add(tc ? a.block * a.tiles : 0, 8);
-    p.held = l.add(a.block * a.held_pitch, size);
+    p.held = l.add(held ? a.block * a.held_pitch : 0, size);
     p.partial = l.add(p.grad ? a.splits * a.part_rows * a.part_pitch : 0, 4);
     p.acc = l.add(p.grad && p.blocks > 1 ? vocab * a.acc_pitch : 0, 4);
     p.h = l.add(p.pack_h ? rows * pitch : 0, size);
@@ -565,11 +570,7 @@ int begin_plan(LinearPlan& p, RowBuilder<kLnViews>& b, const ctb_view* hidden, c
     return CTB_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad) {
+size_t scratch_of(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad, bool held) {
     size_t need = 0;
     c_entry([&]() -> int {
         LinearPlan p;
@@ -579,11 +580,24 @@ size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* wei
         p.a.v = b.v;
         p.weighted = weighted != 0;
         p.grad = grad != 0;
-        if (b.v.rows) lay_out(p);
+        if (!b.v.rows) return CTB_OK;
+        lay_out(p, held);
         need = p.bytes;
         return CTB_OK;
     });
     return need;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad) {
+    return scratch_of(hidden, weight, weighted, grad, true);
+}
+
+size_t ctb_linear_loss_forward_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted) {
+    return scratch_of(hidden, weight, weighted, 0, false);
 }
 
 int ctb_linear_cross_entropy(const ctb_view* hidden, const ctb_view* weight, const ctb_view* targets,

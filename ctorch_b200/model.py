@@ -164,7 +164,10 @@ def linear_cross_entropy(hidden, weight, targets, weights=None, temperature: flo
         gh = _output(name, "out_grad_hidden", out_grad_hidden, hidden, dev, apart=operands)
         gw = _output(name, "out_grad_weight", out_grad_weight, weight, dev, apart=(*operands, out_grad_hidden))
     vh, vw = _view(hidden), _view(weight)
-    need = C.lib.ctb_linear_loss_scratch_bytes(vh, vw, weights is not None, grad)
+    if grad:
+        need = C.lib.ctb_linear_loss_scratch_bytes(vh, vw, weights is not None, True)
+    else:
+        need = C.lib.ctb_linear_loss_forward_scratch_bytes(vh, vw, weights is not None)
     scratch = _scratch(need, dev)
     row_loss, lse = _new(rows, torch.float32, dev), _new(rows, torch.float32, dev)
     loss = _new((), torch.float32, dev)

@@ -414,6 +414,10 @@ CTB_API int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summ
  * cannot be read in place. Depends on the views' strides and alignment too. */
 CTB_API size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad);
 
+/* What a call without gradients needs: in bfloat16 nothing of the logits is held then, and up to 256 MiB of statistics take
+ * its place (the query above, which counts both, is enough as well). */
+CTB_API size_t ctb_linear_loss_forward_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted);
+
 /* Cross entropy of the projection of hidden [..., D] to a vocabulary, weight [V, D] of the same type, without the
  * logits z = hidden weight^T / temperature as a matrix: with lse = log sum exp z of a row,
  *     row_loss = lse - z[target] + z_coef lse^2,    loss = sum of weight_scale * weights * row_loss (weights NULL: 1)

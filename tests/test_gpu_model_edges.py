@@ -130,3 +130,29 @@ def test_norm_in_the_place_of_x_has_no_summed(kind):
     b = cb().rms_norm_backward(up, r.summed, w, r.rstd)
     gx, bx, _, _ = O.norm_grad(up, (x.double() + up.double()).to(t), w, 1e-6, None)
     assert ((b.grad_x.double() - gx).abs() <= bx + O.half(t) * gx.abs()).all()
+
+
+# ------------------------------------------------------------------------------------- a projection without gradients
+
+
+def test_scores_of_many_rows():
+    """More rows than a block of statistics holds, in little memory; the same numbers as with gradients."""
+    g = gen(33)
+    rows, dim, vocab = 33_000, 8, 131_072
+    h, w = torch.randn(rows, dim, generator=g, device="cuda").bfloat16(), torch.randn(vocab, dim, generator=g, device="cuda").bfloat16()
+    t = torch.randint(vocab, (rows,), generator=g, device="cuda")
+    share = (torch.rand(rows, generator=g, device="cuda") < 0.99).float()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for weights in (None, share):
+        r = cb().linear_cross_entropy(h, w, t, weights=weights, grad=False)
+        assert torch.cuda.max_memory_allocated() - before < 300 << 20
+        for s in (slice(0, 300), slice(32_700, 33_000)):
+            some = cb().linear_cross_entropy(h[s], w, t[s], weights=None if weights is None else weights[s])
+            assert torch.equal(r.row_loss[s], some.row_loss) and torch.equal(r.lse[s], some.lse)
+        total = (r.row_loss.double() * (1 / rows if weights is None else weights.double())).sum()
+        assert abs(float(r.loss) - float(total)) <= 4 * O.U * float(total)
+        del some
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
