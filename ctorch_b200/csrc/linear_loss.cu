@@ -42,7 +42,9 @@ __global__ void __launch_bounds__(kOrderThreads) linear_order(LinearArgs a) {
         const double w = row_weight(a, r);
         if (w != 0.0) {
             ++mine;
-            top = fmaxf(top, fminf(fmaxf(static_cast<float>(fabs(w)), 1.17549435e-38f), 3.4e38f));  // a divisor in any case
+            // a divisor in any case; a weight that no float32 holds spoils its own row alone, not what the others are relative to
+            const float size = static_cast<float>(fabs(w));
+            if (size < INFINITY) top = fmaxf(top, fmaxf(size, 1.17549435e-38f));
         }
     }
     counts[threadIdx.x] = mine;

@@ -17,7 +17,7 @@ enum LinearRow : int { kLnHidden = 0, kLnGrad, kLnTarget, kLnWeight, kLnRowLoss,
 // Device-side facts of a call, written by linear_order (or known before it).
 struct LinearFacts {
     int32_t count;   // rows that count
-    float wmax;      // the largest |weight| among them; 1 without weights
+    float wmax;      // the largest finite |weight| among them, 0 without any
 };
 
 struct LinearRowFactor {  // what turns a row's held exponentials into its G (bfloat16)

@@ -156,3 +156,26 @@ def test_scores_of_many_rows():
         del some
         torch.cuda.empty_cache()
         torch.cuda.reset_peak_memory_stats()
+
+
+# ------------------------------------------------------------------------------------- weights without a value
+
+
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("odd", [float("inf"), -float("inf"), NAN, 1e300])
+def test_a_weight_without_a_value_spoils_its_own_row_alone(odd, kind):
+    g, t = gen(44), KIND[kind]
+    h, w = torch.randn(50, 64, generator=g, device="cuda").to(t), torch.randn(300, 64, generator=g, device="cuda").to(t)
+    targets = torch.randint(300, (50,), generator=g, device="cuda")
+    share = (torch.rand(50, generator=g, device="cuda") + 0.5).double()
+    share[5] = share[6] = share.max()  # the largest stays when the odd row's is gone
+    share[9] = 0
+    usual = cb().linear_cross_entropy(h, w, targets, weights=share)
+    share[5] = odd
+    r = cb().linear_cross_entropy(h, w, targets, weights=share)
+    others = torch.arange(50, device="cuda") != 5
+    assert torch.equal(r.row_loss, usual.row_loss) and torch.equal(r.lse, usual.lse)
+    assert torch.equal(r.grad_hidden[others], usual.grad_hidden[others])
+    assert not torch.isfinite(r.grad_hidden[5]).any() and not torch.isfinite(r.loss)
+    alone = cb().linear_cross_entropy(h[5:6], w, targets[5:6], weights=share[5:6])
+    assert not torch.isfinite(alone.grad_hidden).any() and torch.equal(alone.row_loss, usual.row_loss[5:6])
