@@ -55,6 +55,11 @@ def _matrices(name, first, *others):
     return _check(name, first, *others)
 
 
+def _overlap(a, b):
+    """Nothing overlaps a tensor of no elements (whose storage may have no address, like another's)."""
+    return a.numel() > 0 and b.numel() > 0 and may_overlap(a, b)
+
+
 def _output(name, what, out, like, dev, same=(), apart=()):
     """A new tensor like `like`, or `out` checked: `same` are operands whose own view it may be, `apart` those that it
     must not overlap."""
@@ -65,10 +70,10 @@ def _output(name, what, out, like, dev, same=(), apart=()):
         raise (DTypeError if out.dtype != like.dtype else ShapeError)(
             f"ctorch::{name}: {what} must be {like.dtype} {list(like.shape)}")
     for t in same:
-        if t is not None and may_overlap(out, t) and not _same_view(out, t):
+        if t is not None and _overlap(out, t) and not _same_view(out, t):
             raise AliasError(f"ctorch::{name}: {what} overlaps an operand without being the same view")
     for t in apart:
-        if t is not None and may_overlap(out, t):
+        if t is not None and _overlap(out, t):
             raise AliasError(f"ctorch::{name}: {what} overlaps an operand")
     return out
 
@@ -105,7 +110,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, quant: str | None = No
     if quant is None:
         y = _new(shape, x.dtype, dev) if out is None else \
             _output(name, "out", out, x, dev, same=(x,), apart=(weight, residual))
-        if out is not None and summed is not None and may_overlap(out, summed):
+        if out is not None and summed is not None and _overlap(out, summed):
             raise AliasError(f"ctorch::{name}: out overlaps summed")
         vout = _view(y)
     else:
@@ -118,7 +123,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, quant: str | None = No
     rstd = _new(rows, torch.float32, dev)
     _run(name, dev, C.lib.ctb_rms_norm, _view(x), _view(weight), _view(residual), eps, _QUANT[quant], vout, vsum,
          _view(rstd), vscales)
-    if summed is None and (out is None or not may_overlap(out, x)):
+    if summed is None and (out is None or not _overlap(out, x)):
         summed = x
     return RmsNorm(y, summed, rstd, scales)
 

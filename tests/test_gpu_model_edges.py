@@ -179,3 +179,21 @@ def test_a_weight_without_a_value_spoils_its_own_row_alone(odd, kind):
     assert not torch.isfinite(r.grad_hidden[5]).any() and not torch.isfinite(r.loss)
     alone = cb().linear_cross_entropy(h[5:6], w, targets[5:6], weights=share[5:6])
     assert not torch.isfinite(alone.grad_hidden).any() and torch.equal(alone.row_loss, usual.row_loss[5:6])
+
+
+# ------------------------------------------------------------------------------------- calls refused, and not
+
+
+def test_outputs_of_no_rows_overlap_nothing():
+    c, none = cb(), lambda *shape: torch.empty(shape, device="cuda")
+    w, W, t = torch.ones(16, device="cuda"), torch.ones(9, 16, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    out, summed = none(0, 16), none(0, 16)
+    r = c.rms_norm(none(0, 16), w, residual=none(0, 16), out=out, out_summed=summed)
+    assert r.out is out and r.summed is summed
+    b = c.rms_norm_backward(none(0, 16), none(0, 16), w, none(0), out=none(0, 16))
+    assert b.grad_x.shape == (0, 16) and not b.grad_weight.any()
+    gw = torch.ones(9, 16, device="cuda")
+    h = c.linear_cross_entropy(none(0, 16), W, t, out_grad_hidden=none(0, 16), out_grad_weight=gw)
+    assert h.grad_weight is gw and not gw.any() and float(h.loss) == 0
+    a = c.balance_loss(none(0, 16), t[:, None], out_grad=none(0, 16))
+    assert a.grad.shape == (0, 16) and float(a.loss) == 0
