@@ -24,6 +24,7 @@ LinearCrossEntropy = namedtuple("LinearCrossEntropy", ["loss", "row_loss", "lse"
 BalanceLoss = namedtuple("BalanceLoss", ["loss", "counts", "probs", "grad"])
 
 SCALE_BLOCK = 128  # columns that share a scale with quant="block"
+MAX_GROUPS = 1 << 20  # of the balance loss
 _QUANT = {None: 0, "row": 1, "block": 2}
 _MATRIX = (torch.float32, torch.bfloat16)
 _FLOAT8 = torch.float8_e4m3fn
@@ -198,12 +199,14 @@ def balance_loss(logits, experts, mask=None, groups: int = 1, coef: float = 0.01
     g = None
     if grad or out_grad is not None:
         g = _output(name, "out_grad", out_grad, logits, dev, same=(logits,), apart=(experts, mask))
-    if groups < 1:
-        raise ValueError(f"ctorch::{name}: groups must be at least 1")
+    n = logits.shape[-1]
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"ctorch::{name}: groups must be 1 to {MAX_GROUPS}")
+    if n and logits.numel() // n % groups:  # before anything a group is allocated
+        raise ShapeError(f"ctorch::{name}: the rows do not divide into {groups} groups")
     vx = _view(logits)
     need = C.lib.ctb_balance_loss_scratch_bytes(vx, groups)
     scratch = _scratch(need, dev)
-    n = logits.shape[-1]
     counts = _new((groups, n), torch.int64, dev)
     probs = _new((groups, n), torch.float32, dev)
     loss = _new((), torch.float32, dev)

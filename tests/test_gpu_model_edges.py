@@ -197,3 +197,13 @@ def test_outputs_of_no_rows_overlap_nothing():
     assert h.grad_weight is gw and not gw.any() and float(h.loss) == 0
     a = c.balance_loss(none(0, 16), t[:, None], out_grad=none(0, 16))
     assert a.grad.shape == (0, 16) and float(a.loss) == 0
+
+
+def test_groups_are_refused_before_their_tables_are_made():
+    x, e = torch.randn(6, 4096, device="cuda"), torch.zeros(6, 1, dtype=torch.int64, device="cuda")
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for error, groups in ((ValueError, 0), (ValueError, (1 << 20) + 1), (ValueError, 1 << 50), (cb().ShapeError, 1 << 20), (cb().ShapeError, 4)):
+        with pytest.raises(error):
+            cb().balance_loss(x, e, groups=groups, grad=False)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
