@@ -82,6 +82,8 @@ def _output(name, what, out, like, dev, same=(), apart=()):
 def _view8(t):
     """The view of a float8 output, a type that no other operator takes."""
     shape = t.shape
+    if len(shape) > C.MAX_DIMS:
+        raise ShapeError(f"ctorch: tensor rank exceeds kMaxRank (got {len(shape)})")
     return _PACK[len(shape)](t.data_ptr(), C.F8E4M3, len(shape), *shape, *t.stride())
 
 

@@ -68,3 +68,16 @@ def test_a_projection_without_gradients_refuses_less_scratch(dtype):
     d.update(h=view(C, [2, 3, 8], dtype=dtype), w=view(C, [11, 8], dtype=dtype), gh=None, gw=None)
     d["nbytes"] = C.lib.ctb_linear_loss_forward_scratch_bytes(P(d["h"]), P(d["w"]), 0) - 1
     assert head(C, d) == C.ERR_SCRATCH
+
+
+def test_views_of_too_many_dims_are_refused():
+    """By the error that other operands of that rank get."""
+    import torch
+
+    import ctorch_b200 as cb
+    from ctorch_b200 import losses, model
+
+    for f, dtype in ((losses._view, torch.float32), (model._view8, torch.float8_e4m3fn)):
+        f(torch.empty([1] * 16, dtype=dtype))
+        with pytest.raises(cb.ShapeError, match="rank"):
+            f(torch.empty([1] * 17, dtype=dtype))
