@@ -59,7 +59,7 @@ __device__ __forceinline__ float scale_of(float amax) { return amax == 0.0f ? 1.
 // Quotients by a scale, rounded to nearest: what is left of y after the quotient by the rounded reciprocal, which a fused
 // multiply-add gives exactly, corrects it (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
 // processor", 1990). By the reciprocal alone quotients next to a tie of e4m3 fell to its other side. B200, 8192 x 8192
-// bfloat16, a scale for 128 columns: 83.2 us by the reciprocal, 84.4 so in pairs, 86.4 one at a time, 114 with a division.
+// bfloat16, a scale for 128 columns: 83.2 us by the reciprocal, 85.9 so in pairs, 114 with a division.
 struct Divisor {
     float minus, inverse;  // of the scale; by an infinite one quotients are 0, by NaN and of an infinite y NaN
     __device__ __forceinline__ explicit Divisor(float scale) : minus(scale < INFINITY ? -scale : 0.0f), inverse(1.0f / scale) {}
@@ -964,15 +964,16 @@ template <class T, int VEC, bool ODD> bool run_norm_held(const NormArgs& a, cuda
         const bool res = a.v.ptr[kNmResidual] != nullptr;
         unsigned grid = grid_for((a.v.rows + groups - 1) / groups, VEC > 1 && G * NP <= kRingPacks ? norm_grid(forward_ctas<G>(), a.quant, a.v.rows) : 64);
         if (ODD) grid = grid < VEC ? VEC : grid / VEC * VEC;  // whole periods of kinds of rows
-        auto launch = [&](auto kernel, int arrays) { launch_ring(kernel, a, grid, threads, ring_bytes<G, NP>(arrays, forward_ctas<G>()), st); };
         if constexpr (VEC > 1 && G * NP <= kRingPacks) {
+            auto launch = [&](auto kernel, int arrays) { launch_ring(kernel, a, grid, threads, ring_bytes<G, NP>(arrays, forward_ctas<G>()), st); };
             if (a.quant == 0) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 0, ODD>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 0, ODD>, 1);
             else if (a.quant == 1) res ? launch(norm_rows_ring<T, VEC, G, NP, true, 1, ODD>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 1, ODD>, 1);
             else res ? launch(norm_rows_ring<T, VEC, G, NP, true, 2, ODD>, 2) : launch(norm_rows_ring<T, VEC, G, NP, false, 2, ODD>, 1);
         } else if constexpr (!ODD) {
-            if (a.quant == 0) res ? launch(norm_rows_held<T, VEC, G, NP, true, 0>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 0>, 0);
-            else if (a.quant == 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 1>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 1>, 0);
-            else if constexpr (VEC > 1) res ? launch(norm_rows_held<T, VEC, G, NP, true, 2>, 0) : launch(norm_rows_held<T, VEC, G, NP, false, 2>, 0);
+            auto plain = [&](auto kernel) { launch_dependent(kernel, grid, threads, 0, st, a); };
+            if (a.quant == 0) res ? plain(norm_rows_held<T, VEC, G, NP, true, 0>) : plain(norm_rows_held<T, VEC, G, NP, false, 0>);
+            else if (a.quant == 1) res ? plain(norm_rows_held<T, VEC, G, NP, true, 1>) : plain(norm_rows_held<T, VEC, G, NP, false, 1>);
+            else if constexpr (VEC > 1) res ? plain(norm_rows_held<T, VEC, G, NP, true, 2>) : plain(norm_rows_held<T, VEC, G, NP, false, 2>);
         }
     });
 }
@@ -1001,11 +1002,14 @@ template <class T, int VEC, bool ODD> bool run_grad_held(NormGradArgs& a, cudaSt
         constexpr int groups = group_threads<G>() / G, per_sm = backward_ctas<G, ODD>();
         a.ctas = static_cast<int>(std::min<int64_t>({a.ctas, (a.v.rows + groups - 1) / groups, static_cast<int64_t>(sm_count()) * per_sm}));
         if (ODD) a.ctas = a.ctas / VEC * VEC > 0 ? a.ctas / VEC * VEC : VEC;  // whole periods of kinds of rows
-        auto launch = [&](auto kernel, int arrays) {
-            launch_ring(kernel, a, static_cast<unsigned>(a.ctas), group_threads<G>(), ring_bytes<G, NP>(arrays, backward_ctas<G, ODD>()), st);
-        };
-        if constexpr (VEC > 1 && G * NP <= kRingPacks) passed ? launch(norm_grad_ring<T, VEC, G, NP, true, ODD>, 3) : launch(norm_grad_ring<T, VEC, G, NP, false, ODD>, 2);
-        else if constexpr (!ODD) passed ? launch(norm_grad_held<T, VEC, G, NP, true>, 0) : launch(norm_grad_held<T, VEC, G, NP, false>, 0);
+        const unsigned grid = static_cast<unsigned>(a.ctas);
+        if constexpr (VEC > 1 && G * NP <= kRingPacks) {
+            auto launch = [&](auto kernel, int arrays) { launch_ring(kernel, a, grid, group_threads<G>(), ring_bytes<G, NP>(arrays, backward_ctas<G, ODD>()), st); };
+            passed ? launch(norm_grad_ring<T, VEC, G, NP, true, ODD>, 3) : launch(norm_grad_ring<T, VEC, G, NP, false, ODD>, 2);
+        } else if constexpr (!ODD) {
+            auto plain = [&](auto kernel) { launch_dependent(kernel, grid, group_threads<G>(), 0, st, a); };
+            passed ? plain(norm_grad_held<T, VEC, G, NP, true>) : plain(norm_grad_held<T, VEC, G, NP, false>);
+        }
     });
 }
 
