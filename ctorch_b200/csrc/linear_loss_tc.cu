@@ -31,7 +31,7 @@ constexpr int kStageBytes = 2 * kHalf * kK * 2;  // of one CTA: its halves of bo
 constexpr int kEpilogueWarps = 8, kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kBoxBytes = 32 * 128;  // of results on their way out, one a warp
 constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;
-constexpr int kLogitsStretch = 12, kGradStretch = 256;  // stages summed in tensor memory at a time
+constexpr int kLogitsStretch = 12, kFewRows = 8, kFewStretch = 4, kGradStretch = 256;  // stages summed in tensor memory at a time
 constexpr int kGroup = 8;  // tiles of rows walked together, so that both operands are met again in L2 (2 to 32: within 5%)
 
 enum Product : int { kLogits = 0, kLogitsOnly = 1, kGradHidden = 2, kGradWeight = 3 };
@@ -41,6 +41,7 @@ struct ProductArgs {
     int64_t first;    // the block's first row
     int last;         // the last block
     int boxes;        // dW leaves as boxes
+    int stretch;      // stages that tensor memory sums at a time
 };
 
 struct Bars {
@@ -101,11 +102,13 @@ __device__ __forceinline__ uint32_t two_bf16(float x, float y) {
 // The tensor cores truncate a float32 sum at every step of 16 products, so a long one comes out short by a share of itself (one
 // that grows evenly by about 1.6e-8 a step; an exact one by nothing). So they sum a stretch of stages, and the stretches are
 // added in registers, rounded to nearest: a logit loses 8e-7 of itself at most on average, however long, and an exact one
-// nothing. Short stretches wait for the rows' exponentials, which take as long as the products of about 20 stages. B200,
-// 3686 x 2048 x 32768 (32 stages), z and the log-sum-exp's error: one stretch 349 us and 1.3e-6 at twice the columns, 16
-// stages 356 and 3.6e-7, 12 stages 362 and 2.4e-7, 8 stages 379 and 1.7e-7. Gradients are rounded to 16 bits or of such
-// terms, and 1.6e-5 of a stretch is far below that.
-template <int P> constexpr int stretch() { return P == kLogits || P == kLogitsOnly ? kLogitsStretch : kGradStretch; }
+// nothing. Every stretch costs the products about half a microsecond, and short ones wait for the rows' exponentials. B200,
+// 3686 x 2048 x 32768 (32 stages), z and the log-sum-exp's error: one stretch 349 us and 1.3e-6 (at twice the columns), 16
+// stages 356 and 3.6e-7, 12 stages 363 and 2.4e-7, 8 stages 380 and 1.7e-7, 4 stages 450 and 8e-8. A few rows' losses have
+// no others to average with: their stretches are of 4 stages (1 row: 46.7 -> 51.8 us, the loss's error 3.0e-7 -> 1.0e-7 at the
+// median, 2.6e-6 -> 4.2e-7 at most; 4 rows 44.2 -> 46.5). Gradients are rounded to 16 bits or of such terms, and 1.6e-5 of a
+// stretch is far below that.
+int logits_stretch(const LinearArgs& a) { return a.v.rows <= kFewRows ? kFewStretch : kLogitsStretch; }
 
 // 128 columns of a row of logits: their maximum and the sum of exp((z - max) / T), the target's z, and with HOLD
 // 2^15 exp((z - max) / T) in 16 bits: 11 bits of precision down to 2^-29 of the largest, nothing below 2^-40.
@@ -309,14 +312,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t acc_phase = 0;
             for (int64_t w = pair; ok && w < plan.total; w += pairs) {
                 const Work o = plan.at(w);
-                for (int64_t left = o.kbs; ok && left > 0; left -= stretch<P>()) {
+                for (int64_t left = o.kbs; ok && left > 0; left -= p.stretch) {
                     if (!mbar_wait(&bars.free[acc], acc_phase ^ 1u)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t d = tmem + acc * kTile;
-                    const int stages = static_cast<int>(min(left, static_cast<int64_t>(stretch<P>())));
+                    const int stages = static_cast<int>(min(left, static_cast<int64_t>(p.stretch)));
                     for (int kb = 0; kb < stages; ++kb) {
                         if (!mbar_wait(&bars.full[stage], phase)) {
                             ok = false;
@@ -357,12 +360,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 target = index_at(a.v.ptr[kLnTarget], a.v.dtype[kLnTarget], row_offset(a.v, kLnTarget, r));
             }
             float x[kHalf];
-            for (int64_t kb = 0; kb < o.kbs; kb += stretch<P>()) {
+            for (int64_t kb = 0; kb < o.kbs; kb += p.stretch) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&bars.done[acc], acc_phase));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t from = tmem + acc * kTile + half * kHalf + (static_cast<uint32_t>(quarter * 32) << 16);
-                if (kb == 0) {
+                if (i0 >= m) {
+                    // no rows here: the sums stay where they are (loads of tensor memory take the products' time at it)
+                } else if (kb == 0) {
 #pragma unroll
                     for (int c = 0; c < kHalf / 32; ++c) tmem_load32(x + c * 32, from + c * 32);
                     tmem_load_wait();
@@ -448,7 +453,7 @@ int linear_logits_tc(const LinearArgs& a, int64_t first, int64_t rows, bool hold
         !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kHalf) ||
         !encode_matrix_map(&e, hold ? a.held : a.h.ptr, rows, hold ? a.vocab : 1, hold ? a.held_pitch : a.h.row, 32))
         return no_map();
-    const ProductArgs p{rows, a.vocab, a.v.cols, first, 0, 0};
+    const ProductArgs p{rows, a.vocab, a.v.cols, first, 0, 0, logits_stretch(a)};
     return hold ? launch<kLogits>(a, p, h, w, e, st) : launch<kLogitsOnly>(a, p, h, w, e, st);
 }
 
@@ -458,7 +463,7 @@ int linear_grad_hidden_tc(const LinearArgs& a, int64_t first, int64_t rows, cuda
         !encode_matrix_map(&w, a.w.ptr, a.vocab, a.v.cols, a.w.row, kK) ||
         !encode_matrix_map(&out, a.partial, a.splits * a.part_rows, a.v.cols, a.part_pitch, 32, 4))
         return no_map();
-    return launch<kGradHidden>(a, ProductArgs{rows, a.v.cols, a.vocab, first, 0, 0}, g, w, out, st);
+    return launch<kGradHidden>(a, ProductArgs{rows, a.v.cols, a.vocab, first, 0, 0, kGradStretch}, g, w, out, st);
 }
 
 int linear_grad_weight_tc(const LinearArgs& a, int64_t first, int64_t rows, bool last, cudaStream_t st) {
@@ -470,7 +475,7 @@ int linear_grad_weight_tc(const LinearArgs& a, int64_t first, int64_t rows, bool
         !encode_matrix_map(&h, a.h.ptr, a.v.rows, a.v.cols, a.h.row, kK) ||
         !(boxes ? encode_matrix_map(&out, d.ptr, a.vocab, a.v.cols, d.row, 32) : encode_matrix_map(&out, a.held, rows, a.vocab, a.held_pitch, 32)))
         return no_map();
-    return launch<kGradWeight>(a, ProductArgs{a.vocab, a.v.cols, rows, first, last ? 1 : 0, boxes ? 1 : 0}, g, h, out, st);
+    return launch<kGradWeight>(a, ProductArgs{a.vocab, a.v.cols, rows, first, last ? 1 : 0, boxes ? 1 : 0, kGradStretch}, g, h, out, st);
 }
 
 }  // namespace ctb

@@ -207,3 +207,26 @@ def test_groups_are_refused_before_their_tables_are_made():
         with pytest.raises(error):
             cb().balance_loss(x, e, groups=groups, grad=False)
     assert torch.cuda.max_memory_allocated() - before < 1 << 20
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 40])
+def test_a_few_rows_losses(rows):
+    """Rows that lean towards their targets: losses far below the logits. What a row's loss errs by: its log-sum-exp and its
+    target's logit, each within a stretch's truncation (2^-23 of the partial sums that one of 16 products at most reaches, by a
+    step, one way), which a stretch of 4 stages holds to 16 steps and one of 12 to 48; as a mean square over the rows."""
+    g = gen(rows)
+    dim, vocab = 2048, 20_000
+    w = (torch.randn(vocab, dim, generator=g, device="cuda") * (2 / dim ** 0.5)).bfloat16()
+    steps = 16 if rows <= 8 else 48
+    for _ in range(4):
+        t = torch.randint(vocab, (rows,), generator=g, device="cuda")
+        h = (torch.randn(rows, dim, generator=g, device="cuda") + 2 * w[t].float()).bfloat16()
+        z = h.double() @ w.double().T
+        lse = torch.logsumexp(z, 1)
+        zt = z.gather(1, t[:, None])[:, 0]
+        r = cb().linear_cross_entropy(h, w, t, grad=False)
+        # a logit's partial sums stay below its own size and six deviations of a sum of such products, 2 |h| / sqrt(dim)
+        reach = zt.abs() + 6 * 2 * h.double().norm(dim=1) / dim ** 0.5
+        bound = 2 * steps * 2 * O.U * reach + 60 * O.U + 2 * O.U * lse.abs()
+        assert ((r.row_loss.double() - (lse - zt)).abs() <= bound).all()
+        assert ((r.lse.double() - lse).abs() <= bound).all()
