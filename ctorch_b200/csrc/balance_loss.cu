@@ -4,8 +4,9 @@
 // For a group of rows of which n count, with p = softmax(x) of a row, its k chosen experts and lse = log sum exp x:
 //     f_e = (times e was chosen) / (n k),  P_e = mean p_e,  loss = coef E sum_e f_e P_e + z_coef mean lse^2
 //     dloss/dx_j = p_j / n (a_j - sum_e a_e p_e + 2 z_coef lse),  a_e = coef E f_e
-// A row's gradient needs the whole group's counts, so the rows are read twice: balance_rows sums a run of rows of one
-// group per CTA, balance_join adds the runs in their order, balance_grad writes the gradient.
+// A row's gradient needs the whole group's counts. They are taken in the same pass as the sums of p, so the logits are read
+// twice: balance_rows sums a run of rows of one group per CTA, balance_join adds the runs in their order, balance_grad writes
+// the gradient. (The counts need experts and mask alone: counted first, one read of the logits would do.)
 #include <algorithm>
 #include <cmath>
 

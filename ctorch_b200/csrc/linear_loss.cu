@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(kJoinThreads) linear_rows_tc(LinearArgs a, int
     }
 }
 
-// Turns the held exponentials into G, rounded once to bfloat16, in their place; rows behind the last one, up to a stage of
-// the products, become zeros. Bound by reading and writing 2 bytes an element, which run at the copy rate only if
+// Turns the held exponentials (16-bit floats) into G, rounded to bfloat16, in their place; rows behind the last one, up to a
+// stage of the products, become zeros. Bound by reading and writing 2 bytes an element, which run at the copy rate only if
 // reads stay on their way while results are written: a CTA walks its share of spans of a row (16 KiB each) in order and
 // has the next span's vectors under way before it writes this one's. B200, 8192 x 131072 (4.3 GB): 781 us with 16 CTAs
 // an SM, four times what is resident (853 with 8, 1119 with 4: the SMs do not all stream alike); without the next span

@@ -1,7 +1,7 @@
 // linear_loss_f32.cu — the three products of the projection with its cross entropy in float32.
 //
-// The tensor cores take float32 operands with 10 bits (tf32), which is not what a float32 caller asks for, so these
-// run on the FMA pipe: 128 x 128 tiles, 16 of the inner dimension a step through double-buffered shared memory, 8 x 8
+// The tensor cores take float32 operands with 10 bits (tf32), which is not what a float32 caller asks for (operands split
+// into three bfloat16 parts each, six products of parts, would keep 23 bits; not built), so these run on the FMA pipe: 128 x 128 tiles, 16 of the inner dimension a step through double-buffered shared memory, 8 x 8
 // sums a thread as packed pairs (fma.rn.f32x2: half the instructions of single ones, so the shared-memory loads fit
 // beside them). Sums are float32, one rounding a step. B200, 509 x 517 x 10007: 160, 143 and 160 us, 33 to 37 TFLOP/s, about
 // half of the pipe's rate; with single FMA instructions 8% slower.

@@ -13,10 +13,9 @@
 //
 // Why these tiles: a pair's 256 x 256 tile needs 64 bytes of operands a clock and SM at the tensor cores' full rate, half of what
 // a 128 x 256 tile of one CTA would, and two of them fit tensor memory, so a tile's results leave while the next one is
-// computed. Bound by the tensor cores and, in long runs, by power: B200, 3686 x 2048 x 32768: 355 (z, with the
-// exponentials written), 364 (dH, in four splits) and 326 us (dW), 1.36 to 1.52 PFLOP/s, the tensor pipe 79 to 82% busy; 8192 x 4096
-// x 131072 6.8 to 7.4 ms each, 1.2 to 1.3 PFLOP/s. Results as 16-byte stores of a thread took 364, 353 and 328 us, and
-// 7.4 to 7.8 ms.
+// computed. Bound by the tensor cores and, in long runs, by power: B200, 3686 x 2048 x 32768: 365 (z, with the
+// exponentials written), 356 (dH, in four splits) and 319 us (dW), 1.36 to 1.55 PFLOP/s, the tensor pipe 74 to 84% busy; 8192 x 4096 x 131072 6.8 to 7.6 ms each,
+// 1.15 to 1.3 PFLOP/s. Results as 16-byte stores of a thread took 364, 353 and 328 us, and 7.4 to 7.8 ms (z in one stretch).
 #include <cuda_fp16.h>
 
 #include "linear_loss.cuh"

@@ -382,8 +382,10 @@ CTB_API int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets,
 /* Common to the entry points of this section. Matrices are [..., columns]: any leading dims and strides, float32 or
  * bfloat16; a "row" is one position of the leading dims of the first matrix, further matrices have the same leading
  * shape, numbers a row broadcast (right-aligned) to it, results a row have exactly it and float32 elements.
- * Statistics, sums and products are float32 or more, each result is rounded once, no sum's order changes: equal calls
- * give equal bits. Nothing is kept between calls, so any of them may be captured into a graph and replayed; calls
+ * Statistics, sums and products are float32 or more, each result is rounded once (but see the projection's gradients), no
+ * sum's order changes: equal calls give equal bits. The sums of the bfloat16 products are truncated at every 16 terms inside
+ * stretches of 768 terms (256 where there are 8 rows or fewer; gradients 16384), which are added rounded to nearest; a sum
+ * that is exact stays so. Nothing is kept between calls, so any of them may be captured into a graph and replayed; calls
  * that may run at the same time need scratch of their own. d_status as in the losses. No ctorch counterpart. */
 
 /* The root-mean-square norm of rows, with the residual's addition:
@@ -392,7 +394,8 @@ CTB_API int ctb_preference_loss(const ctb_view* logits, const ctb_view* targets,
  * summed = s (given exactly when residual is; it may be x's or residual's own view), out = y in x's type (it may be
  * x's own view), or with quant 1 or 2 in 8 bits: out = y / scale as CTB_FLOAT8_E4M3 (rounded to nearest), one scale
  * a row (1) or one for every 128 columns, [..., ceil(columns / 128)] (2); scale = the largest |y| / 448, and 1 where
- * that is 0. weight is [columns], float32 or bfloat16. rstd may be NULL. Otherwise outputs must not overlap inputs. */
+ * that is 0 (never below float32's least normal number, 2^-126). weight is [columns], float32 or bfloat16. rstd may be NULL.
+ * The sum of s^2 is a float32: beyond 3.4e38 a row comes out as 0. Otherwise outputs must not overlap inputs. */
 CTB_API int ctb_rms_norm(const ctb_view* x, const ctb_view* weight, const ctb_view* residual, double eps, int quant,
                          const ctb_view* out, const ctb_view* summed, const ctb_view* rstd, const ctb_view* scales,
                          ctb_stream stream);
@@ -410,8 +413,10 @@ CTB_API int ctb_rms_norm_backward(const ctb_view* grad_out, const ctb_view* summ
                                   const ctb_view* grad_weight, void* scratch, size_t scratch_bytes, ctb_stream stream);
 
 /* Scratch bytes of ctb_linear_cross_entropy (256-byte aligned); weighted: whether weights are given, grad: whether
- * gradients are wanted. Up to 2 GiB for the pieces of the logits that are held at a time, beside copies of what
- * cannot be read in place. Depends on the views' strides and alignment too. */
+ * gradients are wanted. Up to 2 GiB for the pieces of the logits that are held at a time (rows are taken in blocks of that
+ * size, 256 rows at least); with gradients also float32 sums, [splits][a block's rows][D] of grad_hidden (1 split or more,
+ * 64 at most where there are few rows) and, where there are several blocks, [V][D] of grad_weight; and copies of
+ * what cannot be read in place. Depends on the views' strides and alignment too. */
 CTB_API size_t ctb_linear_loss_scratch_bytes(const ctb_view* hidden, const ctb_view* weight, int weighted, int grad);
 
 /* What a call without gradients needs: in bfloat16 nothing of the logits is held then, and up to 256 MiB of statistics take
@@ -425,8 +430,10 @@ CTB_API size_t ctb_linear_loss_forward_scratch_bytes(const ctb_view* hidden, con
  * A row whose weight is 0 does not count: its hidden state and target are not looked at, its results and its row of
  * grad_hidden are 0. A target outside [0, V) in a row that counts makes that row's results, its row of grad_hidden
  * and all of grad_weight NaN. loss, row_loss and lse may each be NULL. Gradients must not overlap each other or the
- * operands. Without rows loss and grad_weight are 0. In bfloat16 the gradient of a logit is rounded once to bfloat16
- * (relative to its row's weight) before the products with weight and hidden, which sum in float32. */
+ * operands. Without rows loss and grad_weight are 0. In bfloat16 the gradient of a logit is rounded to bfloat16 (relative to
+ * its row's weight) before the products with weight and hidden; but for the target's own, its exponential was held as a
+ * 16-bit float relative to the largest of its 128 columns before that (11 bits, fewer below 2^-29 of the largest, 0 below
+ * 2^-40). */
 CTB_API int ctb_linear_cross_entropy(const ctb_view* hidden, const ctb_view* weight, const ctb_view* targets,
                                      const ctb_view* weights, double weight_scale, double temperature, double z_coef,
                                      const ctb_view* loss, const ctb_view* row_loss, const ctb_view* lse,
