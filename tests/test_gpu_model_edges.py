@@ -230,3 +230,26 @@ def test_a_few_rows_losses(rows):
         bound = 2 * steps * 2 * O.U * reach + 60 * O.U + 2 * O.U * lse.abs()
         assert ((r.row_loss.double() - (lse - zt)).abs() <= bound).all()
         assert ((r.lse.double() - lse).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("quant", ["row", "block"])
+@pytest.mark.parametrize("kind", list(KIND))
+@pytest.mark.parametrize("dim", [300, 640, 5003, 40000])
+def test_8_bits_beside_infinities_and_the_smallest_numbers(dim, kind, quant):
+    """By an infinite scale: 0, and NaN of the infinity; scales that would be below float32's normal numbers stay at the least."""
+    g, t = gen(dim), KIND[kind]
+    x = whole(g, 1, 60, 6, dim).to(t)
+    x[4] = 0.0
+    w = torch.ones(dim, device="cuda")
+    w[200] = float("inf")
+    r = cb().rms_norm(x, w, quant=quant)
+    rows = [0, 1, 2, 3, 5]
+    hit = torch.zeros(dim, dtype=torch.bool, device="cuda")
+    hit[slice(None) if quant == "row" else slice(128, 256)] = True
+    out = r.out.float()
+    assert torch.isnan(out[:, 200]).all()  # infinity over infinity, and 0 times infinity
+    hit[200] = False
+    assert (out[rows][:, hit] == 0).all() and torch.isnan(out[4, hit]).all()
+    assert torch.isfinite(out[:, ~hit & (torch.arange(dim, device="cuda") != 200)]).all()
+    small = cb().rms_norm(x, torch.full((dim,), 2.0 ** -126, device="cuda"), quant=quant)
+    assert torch.isfinite(small.out.float()).all() and (small.scales[rows] == 2.0 ** -126).all() and (small.scales[4] == 1).all()
