@@ -1,5 +1,6 @@
 """GPU checks of what stands around the losses where it can go wrong without the bounds of test_gpu_model.py seeing it: logits
-that are exact."""
+that are exact and long sums, quotients to 8 bits, what the norm returns of x, scores without gradients, weights without a
+value, calls of no rows and refused ones."""
 import pytest
 import torch
 
